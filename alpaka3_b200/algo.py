@@ -13,6 +13,13 @@ Device buffers are torch CUDA tensors (plumbing only: allocation, streams); ever
 * :func:`nbody_step`, :func:`nbody_update_velocities`, :func:`nbody_update_positions`  (example/nBody)
 * :func:`heat_step`, :func:`heat_init`  (example/heatEquation2D)
 
+Reductions of a language model's training and decoding steps, which alpaka3 does not have:
+
+* :func:`token_logprobs`, :func:`token_logprobs_backward`  per row of logits: the log probability of its token, entropy,
+                              log-sum-exp and most likely alternatives, and their gradient
+* :class:`TensorList`, :func:`grad_norm`, :func:`clip_grads`, :func:`clip_grad_norm`  norm and clipping of a list of
+                              gradients
+
 Errors raise :class:`alpaka3_b200.capi.A3BError` (the reference throws std::runtime_error on backend errors).
 """
 import ctypes
@@ -30,6 +37,10 @@ REDUCE = {"plus": capi.PLUS, "min": capi.MIN, "max": capi.MAX}
 XFORM = {"identity": capi.IDENTITY, "square": capi.SQUARE, "product": capi.PRODUCT}
 STREAM = {"init": capi.INIT, "copy": capi.COPY, "mul": capi.MUL, "add": capi.ADD, "triad": capi.TRIAD,
           "nstream": capi.NSTREAM}
+NORM = {"l2": capi.NORM_L2, "l1": capi.NORM_L1, "max": capi.NORM_MAX}
+_LOGITS_DT = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
+_GRAD_DT = {**_LOGITS_DT, torch.float64: capi.F64}
+_INDEX_DT = {torch.int64: capi.I64, torch.int32: capi.I32}
 MAP = {"copy": capi.MAP_COPY, "scale": capi.MAP_SCALE, "add": capi.MAP_ADD, "mul": capi.MAP_MUL,
        "axpy": capi.MAP_AXPY, "square": capi.MAP_SQUARE}
 
@@ -199,6 +210,246 @@ def inclusive_scan_in_place(data, buffer=None, stream=None):
 
 def exclusive_scan_in_place(data, buffer=None, stream=None):
     return _scan(False, data, data, buffer, None, stream)
+
+
+# ------------------------------------------------------------------------------------- token log probabilities
+def _call_on(device, stream, name, *args):
+    """capi.call on `stream` (default: the device's current stream) with `device` current."""
+    if stream is not None and stream.device_index != device.index:
+        raise ValueError(f"the stream belongs to device {stream.device_index}, the tensors to {device}")
+    if torch.cuda.current_device() == device.index:
+        return capi.call(name, stream_handle(stream), *args)
+    with torch.cuda.device(device):
+        return capi.call(name, stream_handle(stream), *args)
+
+
+def _rows(t, name):
+    """(outer, inner, outer stride, inner stride) of the rows (last dimension) of t: all other dimensions together must
+    step through memory with at most two strides, as those of logits[:, :-1] do."""
+    if t.dim() < 1 or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{name}: rows must be contiguous in the last dimension")
+    levels = []
+    for size, stride in zip(t.shape[:-1], t.stride()[:-1]):
+        if size == 1:
+            continue
+        if levels and levels[-1][1] == size * stride:
+            levels[-1] = (levels[-1][0] * size, stride)
+        else:
+            levels.append((size, stride))
+    if t.numel() == 0:
+        levels = [(t.numel(), 0)]
+    if len(levels) > 2:
+        raise ValueError(f"{name}: the dimensions before the last do not collapse to two strides")
+    (outer, so), (inner, si) = [(1, 0)] * (2 - len(levels)) + levels
+    return outer, inner, so, si
+
+
+def _per_row(t, name, rows, device, dtypes, width=None):
+    """Address of a dense per-row array (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name}: unsupported dtype {t.dtype}")
+    if t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor on {device}")
+    if t.numel() != rows * (1 if width is None else width):
+        raise ValueError(f"{name}: expected {rows * (1 if width is None else width)} elements, got {t.numel()}")
+    return ctypes.c_void_p(t.data_ptr())
+
+
+def _logits_code(logits):
+    if logits.dtype not in _LOGITS_DT:
+        raise TypeError(f"unsupported logits dtype {logits.dtype}")
+    if not logits.is_cuda:
+        raise ValueError("expected a CUDA tensor")
+    return _LOGITS_DT[logits.dtype]
+
+
+_F32 = (torch.float32,)
+
+
+def token_logprobs(logp, logits, targets, entropy=None, lse=None, top_logp=None, top_index=None, scale=1.0,
+                   stream=None):
+    """Per row of logits (..., vocab), float32 / float16 / bfloat16, z = scale * logits: writes the log probability of
+    the row's token to `logp`, the entropy of its distribution to `entropy`, ln sum e^z to `lse` (float32, one per row,
+    each optional; logp may be None) and the k most likely alternatives to `top_logp` and `top_index` (k = their last
+    dimension, up to 32; largest first, a tie to the lower index). One launch, one pass over the logits.
+
+    targets: int64 or int32, one per row (None without logp); outside [0, vocab) there is no token: logp 0. top_index:
+    dtype of targets, or int64 / int32 without them. The logits' rows may be strided (logits[:, :-1], a padded
+    vocabulary); the other tensors are contiguous. Infinities and NaN: see a3b_token_logprobs. Returns logp."""
+    code = _logits_code(logits)
+    outer, inner, so, si = _rows(logits, "logits")
+    rows, vocab, dev = outer * inner, logits.shape[-1], logits.device
+    if (top_logp is None) != (top_index is None):
+        raise ValueError("top_logp and top_index belong together")
+    if logp is not None and targets is None:
+        raise ValueError("logp needs targets")
+    top = 0 if top_logp is None else top_logp.shape[-1]
+    ints = targets if targets is not None else top_index
+    if targets is not None and top_index is not None and top_index.dtype != targets.dtype:
+        raise TypeError("top_index and targets must have the same dtype")
+    index = capi.I64 if ints is None else _INDEX_DT.get(ints.dtype, -1)
+    _call_on(dev, stream, "a3b_token_logprobs", code, ctypes.c_void_p(logits.data_ptr()), outer, inner, vocab, so, si,
+             float(scale), index, _per_row(targets, "targets", rows, dev, _INDEX_DT),
+             _per_row(logp, "logp", rows, dev, _F32), _per_row(entropy, "entropy", rows, dev, _F32),
+             _per_row(lse, "lse", rows, dev, _F32), top, _per_row(top_logp, "top_logp", rows, dev, _F32, top),
+             _per_row(top_index, "top_index", rows, dev, _INDEX_DT, top))
+    return logp
+
+
+def token_logprobs_backward(grad_logits, logits, targets, lse, entropy=None, grad_logp=None, grad_entropy=None,
+                            grad_lse=None, scale=1.0, stream=None):
+    """Gradient of token_logprobs' logp, entropy and lse with respect to the logits: given lse (and entropy, for
+    grad_entropy) as token_logprobs wrote them and the gradients of a loss with respect to them (float32, one per row;
+    None is zero), writes that with respect to the logits to `grad_logits` (shape and dtype of logits; any row strides;
+    may be `logits` itself). Rows without a token get nothing from grad_logp. Returns grad_logits."""
+    code = _logits_code(logits)
+    outer, inner, so, si = _rows(logits, "logits")
+    if grad_logits.shape != logits.shape or grad_logits.dtype != logits.dtype or grad_logits.device != logits.device:
+        raise ValueError("grad_logits must have the shape, dtype and device of logits")
+    go, gi, gso, gsi = _rows(grad_logits, "grad_logits")
+    if (go, gi) != (outer, inner):  # one of the two collapses further than the other
+        if outer == 1 and go > 1:
+            outer, inner, so = go, gi, si * gi
+        elif go == 1 and outer > 1:
+            gso = gsi * inner
+        else:
+            raise ValueError("logits and grad_logits do not collapse to the same two dimensions")
+    rows, dev = outer * inner, logits.device
+    if lse is None:
+        raise ValueError("lse is needed")
+    index = capi.I64 if targets is None else _INDEX_DT.get(targets.dtype, -1)
+    _call_on(dev, stream, "a3b_token_logprobs_backward", code, ctypes.c_void_p(logits.data_ptr()), outer, inner,
+             logits.shape[-1], so, si, float(scale), index, _per_row(targets, "targets", rows, dev, _INDEX_DT),
+             _per_row(lse, "lse", rows, dev, _F32), _per_row(entropy, "entropy", rows, dev, _F32),
+             _per_row(grad_logp, "grad_logp", rows, dev, _F32),
+             _per_row(grad_entropy, "grad_entropy", rows, dev, _F32),
+             _per_row(grad_lse, "grad_lse", rows, dev, _F32), ctypes.c_void_p(grad_logits.data_ptr()), gso, gsi)
+    return grad_logits
+
+
+# ------------------------------------------------------------------------------------ norm and clipping of a list
+def _is_dense(t):
+    """Whether t's elements fill one stretch of memory, in any order of the dimensions."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, sz) for sz, st in zip(t.shape, t.stride()) if sz != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+class TensorList:
+    """A list of CUDA tensors (float32, float64, float16, bfloat16, mixed as needed, of one device) for grad_norm,
+    clip_grads and clip_grad_norm, with the tensors that receive the clipped values: `outputs`, with the dtypes, shapes
+    and strides of `inputs`, or the inputs themselves (in place). Each tensor must be dense (its elements fill one
+    stretch of memory, in any order of dimensions).
+
+    Making one costs the host about a microsecond per tensor; a program whose gradients stay where they are makes it
+    once. It holds the addresses of the tensors as they are now, and keeps those tensors alive."""
+
+    def __init__(self, inputs, outputs=None):
+        self.inputs = list(inputs)
+        self.outputs = self.inputs if outputs is None else list(outputs)
+        self._handle = None
+        n = len(self.inputs)
+        if len(self.outputs) != n:
+            raise ValueError("inputs and outputs must be equally many")
+        self.device = self.inputs[0].device if n else None
+        for t in self.inputs:
+            if t.dtype not in _GRAD_DT:
+                raise TypeError(f"unsupported dtype {t.dtype}")
+            if not t.is_cuda or t.device != self.device:
+                raise ValueError("expected CUDA tensors of one device")
+            if not _is_dense(t):
+                raise ValueError("expected dense tensors")
+        for t, o in zip(self.inputs, self.outputs):
+            if o is not t and (o.dtype != t.dtype or o.device != t.device or o.shape != t.shape
+                               or (o.stride() != t.stride() and t.numel() > 1)):
+                raise ValueError("an output must have the dtype, device, shape and strides of its input")
+        handle = ctypes.c_void_p()
+        capi.call("a3b_tensor_list_create", (ctypes.c_void_p * n)(*[t.data_ptr() for t in self.inputs]),
+                  (ctypes.c_void_p * n)(*[t.data_ptr() for t in self.outputs]),
+                  (ctypes.c_uint64 * n)(*[t.numel() for t in self.inputs]),
+                  (ctypes.c_int * n)(*[_GRAD_DT[t.dtype] for t in self.inputs]), n, ctypes.byref(handle))
+        self._handle = handle
+        self._storages = [t.untyped_storage() for t in self.inputs + self.outputs]  # alive even if a tensor moves on
+        self._workspace = None
+
+    def __del__(self):
+        if getattr(self, "_handle", None) is not None and capi is not None:
+            capi.lib().a3b_tensor_list_destroy(self._handle)
+            self._handle = None
+
+    def __len__(self):
+        return len(self.inputs)
+
+    def workspace(self, device, stream):
+        """Scratch for one call, from torch's allocator in the order of the call's stream."""
+        if self._workspace is None:
+            with torch.cuda.device(device):
+                self._workspace = capi.lib().a3b_grad_norm_workspace(self._handle) // 8
+        if stream is None:
+            return torch.empty(self._workspace, dtype=torch.float64, device=device)
+        with torch.cuda.stream(stream):
+            return torch.empty(self._workspace, dtype=torch.float64, device=device)
+
+
+def _list_args(norm, tensors, kind, *more):
+    """(TensorList, device, kind code, norm's dtype code, norm's address)"""
+    if kind not in NORM:
+        raise ValueError(f"unknown norm {kind!r}: one of {', '.join(NORM)}")
+    if not isinstance(tensors, TensorList):
+        tensors = TensorList(tensors)
+    some = next((t for t in (norm, *more) if t is not None), None)
+    if some is None:
+        raise ValueError("nothing to compute: no output is given")
+    dev = tensors.device if tensors.device is not None else some.device
+    for t in (norm, *more):
+        if t is not None and (t.device != dev or not t.is_cuda or t.numel() != 1):
+            raise ValueError(f"expected a tensor of one element on {dev}")
+    for t in more:
+        if t is not None and t.dtype != torch.float64:
+            raise TypeError("partial must be float64")
+    if norm is not None and norm.dtype not in (torch.float32, torch.float64):
+        raise TypeError(f"unsupported dtype {norm.dtype} of the norm")
+    code = capi.F32 if norm is None else _DT[norm.dtype]
+    return tensors, dev, NORM[kind], code, None if norm is None else ctypes.c_void_p(norm.data_ptr())
+
+
+def grad_norm(norm, tensors, kind="l2", partial=None, stream=None):
+    """Norm over all elements of a list of tensors ("l2", "l1" or "max"; a TensorList or any sequence of tensors) into
+    `norm`, one float32 or float64 element on the device. partial: one float64 element that receives the sum of squares,
+    the sum of magnitudes or the largest magnitude unrounded, for combination across ranks; either may be None."""
+    tensors, dev, k, code, p = _list_args(norm, tensors, kind, partial)
+    ws = tensors.workspace(dev, stream)
+    _call_on(dev, stream, "a3b_grad_norm", tensors._handle, k, ctypes.c_void_p(ws.data_ptr()), ws.numel() * 8,
+             None if partial is None else ctypes.c_void_p(partial.data_ptr()), code, p)
+    return norm
+
+
+def clip_grads(norm, tensors, partial, max_norm, kind="l2", stream=None):
+    """Multiplies every tensor of the list by min(1, max_norm / (norm + 1e-6)), with the norm that `partial` stands for
+    (as grad_norm wrote it, or combined across ranks), and writes that norm to `norm` (None: not written)."""
+    tensors, dev, k, code, p = _list_args(norm, tensors, kind, partial)
+    if partial is None:
+        raise ValueError("partial is needed")
+    _call_on(dev, stream, "a3b_clip_grads", tensors._handle, k, ctypes.c_void_p(partial.data_ptr()), float(max_norm),
+             code, p)
+    return norm
+
+
+def clip_grad_norm(norm, tensors, max_norm, kind="l2", stream=None):
+    """grad_norm and clip_grads in one call: the tensors of the list scaled down so that their common norm is at most
+    `max_norm`, written to the list's outputs (a plain sequence: in place); the norm before goes to `norm`."""
+    tensors, dev, k, code, p = _list_args(norm, tensors, kind)
+    ws = tensors.workspace(dev, stream)
+    _call_on(dev, stream, "a3b_clip_grad_norm", tensors._handle, k, float(max_norm), ctypes.c_void_p(ws.data_ptr()),
+             ws.numel() * 8, code, p)
+    return norm
 
 
 # ------------------------------------------------------------------------------------------------------- nBody

@@ -15,7 +15,9 @@ LIB_PATH = os.environ.get("A3B_LIBRARY") or os.path.join(_HERE, "lib", "libalpak
 # status codes
 OK, ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED, ERR_TIMEOUT, ERR_NOMEM, ERR_TOO_LARGE = range(7)
 # dtypes
-I32, U32, I64, U64, F32, F64 = range(6)
+I32, U32, I64, U64, F32, F64, F16, BF16 = range(8)
+# norms over a tensor list
+NORM_L2, NORM_L1, NORM_MAX = range(3)
 # reduce / transform functors
 PLUS, MIN, MAX = range(3)
 IDENTITY, SQUARE, PRODUCT = range(3)
@@ -31,6 +33,8 @@ _U64 = ctypes.c_uint64
 _I = ctypes.c_int
 _D = ctypes.c_double
 _F = ctypes.c_float
+_I64 = ctypes.c_int64
+_U32 = ctypes.c_uint32
 
 # name -> argtypes (all return int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -66,6 +70,15 @@ SIGNATURES = {
     "a3b_reduce_lower_ranks": [_P, _P, _I, _P, _U64, _P],
     "a3b_scan_buffer_size": [_I, _U64],
     "a3b_scan": [_P, _I, _I, _P, _P, _U64, _P, _P, ctypes.c_size_t],
+    "a3b_token_logprobs": [_P, _I, _P, _U64, _U64, _U64, _I64, _I64, _D, _I, _P, _P, _P, _P, _U32, _P, _P],
+    "a3b_token_logprobs_backward": [_P, _I, _P, _U64, _U64, _U64, _I64, _I64, _D, _I, _P, _P, _P, _P, _P, _P, _P,
+                                    _I64, _I64],
+    "a3b_tensor_list_create": [_P, _P, _P, _P, _U64, _P],
+    "a3b_tensor_list_destroy": [_P],
+    "a3b_grad_norm_workspace": [_P],
+    "a3b_grad_norm": [_P, _P, _I, _P, ctypes.c_size_t, _P, _I, _P],
+    "a3b_clip_grads": [_P, _P, _I, _P, _D, _I, _P],
+    "a3b_clip_grad_norm": [_P, _P, _I, _D, _P, ctypes.c_size_t, _I, _P],
     "a3b_nbody_update_velocities": [_P, _P, _P, _P, _P, _U64, _U64, _U64, _P, _P, _P, _F, _F],
     "a3b_nbody_step": [_P, _P, _P, _P, _P, _U64, _U64, _U64, _P, _P, _P, _F, _F],
     "a3b_haccmk_step10": [_P, _P, _P, _P, _P, _I, _I, _F, _F, _F, _P, _P, _P],
@@ -84,7 +97,8 @@ SIGNATURES = {
     "a3b_debug_early_start_probe": [_I, _P, _P, _P, _U64, _P, _P],
 }
 _RESTYPES = {"a3b_last_error": ctypes.c_char_p, "a3b_scan_buffer_size": ctypes.c_size_t,
-             "a3b_ipc_handle_size": ctypes.c_size_t, "a3b_halo_bytes": ctypes.c_size_t}
+             "a3b_grad_norm_workspace": ctypes.c_size_t, "a3b_ipc_handle_size": ctypes.c_size_t,
+             "a3b_halo_bytes": ctypes.c_size_t}
 
 
 class LibraryNotBuilt(RuntimeError):

@@ -7,6 +7,8 @@ smallest data that has to move:
 * :func:`allreduce_partial`        reduce/dot/transformReduce: one 8-byte partial per rank, NCCL all-reduce, then the
                                    final rounding to the output dtype (same op order on every rank)
 * :func:`scan_carry`               scan: all-gather of the per-rank totals, carry = sum of the totals of lower ranks
+* :func:`clip_grad_norm`           gradients sharded over the ranks: all-gather of one 8-byte partial per rank, then every
+                                   rank scales its shards by the same factor
 * :func:`nbody_allgather`          nBody: all-gather of the x/y/z shards into the full position arrays
 * :func:`heat_exchange_halos`      heat: one boundary row to each neighbour (send/recv), into the neighbour's ghost row
 * :class:`HeatSlab`                heat time steps on row slabs: fused stencil + halo exchange over NVLink (HaloMailbox)
@@ -126,6 +128,32 @@ def transform_reduce(neutral, reduce_fn, transform_fn, in0_local, in1_local=None
         out.copy_(res)
         return out
     return res
+
+
+def combine_norm(partial, kind="l2"):
+    """Combines the ranks' norm partials (algo.grad_norm: sums, or largest magnitudes for "max") in place, in rank order
+    on every rank, so that all get the same bits; a NaN of any rank stays."""
+    if dist.is_initialized() and dist.get_world_size() > 1:
+        world = dist.get_world_size()
+        gathered = torch.empty(world, dtype=partial.dtype, device=partial.device)
+        if dist.get_backend() == "nccl":
+            dist.all_gather_into_tensor(gathered, partial)
+        else:
+            dist.all_gather(list(gathered.chunk(world)), partial)
+        partial.copy_((gathered.amax(0) if kind == "max" else gathered.sum(0)).reshape(1))
+    return partial
+
+
+def clip_grad_norm(norm, tensors, max_norm, kind="l2"):
+    """algo.clip_grad_norm for gradients sharded over the ranks (every element on one rank): the norm over all ranks'
+    tensors, each rank's own scaled by the factor that follows from it."""
+    from . import algo
+    if not isinstance(tensors, algo.TensorList):
+        tensors = algo.TensorList(tensors)
+    partial = torch.empty(1, dtype=torch.float64, device=norm.device)
+    algo.grad_norm(None, tensors, kind, partial=partial)
+    combine_norm(partial, kind)
+    return algo.clip_grads(norm, tensors, partial, max_norm, kind)
 
 
 def carry_to_dtype(carry, dtype):

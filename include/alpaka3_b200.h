@@ -46,7 +46,9 @@ enum a3b_dtype
     A3B_I64 = 2,
     A3B_U64 = 3,
     A3B_F32 = 4,
-    A3B_F64 = 5
+    A3B_F64 = 5,
+    A3B_F16 = 6, /* IEEE half and bfloat16: only for the entry points over logits and gradients that name them */
+    A3B_BF16 = 7
 };
 
 /* binary reduce functors: std::plus, ScalarFunc{min}, ScalarFunc{max} (test/unit/algorithm/reduce.cpp:22-56) */
@@ -254,6 +256,88 @@ A3B_API size_t a3b_scan_buffer_size(int dtype, uint64_t n);
  *         scan is split across GPUs); null means 0. Integer arithmetic wraps (two's complement). */
 A3B_API int a3b_scan(a3b_stream_t stream, int dtype, int inclusive, void const* in, void* out, uint64_t n,
              void const* carry_in, void* buffer, size_t buffer_bytes);
+
+/* ---------------------------------------------------------------------------- token log probabilities (rows) */
+
+/* Reductions over every row of logits (vocab values each): with z = scale * x,
+ *   lse = ln sum_v e^(z_v),  logp = z_t - lse for the row's token t,  entropy = -sum_v p_v ln p_v, p_v = e^(z_v - lse),
+ * and the `top` largest logits of the row, largest first, a tie to the lower index (-0 equals 0; NaN counts as larger
+ * than +infinity): their log probabilities and their indices. One launch, every logit read once; the sums are held in
+ * fp32. No counterpart in alpaka3, whose reductions give one value for a whole buffer.
+ *
+ * Rows: logits of dtype A3B_F32, A3B_F16 or A3B_BF16; row r = o * inner + i (o < outer, i < inner) starts at element
+ * o * outer_stride + i * inner_stride and is contiguous; any strides, also ones that make rows overlap. The other
+ * arrays are dense in row order: targets (index_dtype A3B_I32 or A3B_I64), logp, entropy, lse (fp32), top_logp (fp32)
+ * and top_index (index_dtype), `top` of each per row. logp, entropy and lse may be null (not computed); targets may be
+ * null if logp is. top: 0 .. 32, at most vocab. scale: positive and finite (the inverse temperature).
+ *
+ * A target outside [0, vocab) marks a row without a token: its logp is 0. Logits of -infinity have probability 0 (logp
+ * -infinity); a row of nothing else has lse -infinity, entropy 0 and logp -infinity for every token. A NaN in a row
+ * makes its lse, logp and entropy NaN. With +infinity in a row its lse is +infinity, its entropy NaN, the logp of a
+ * finite logit -infinity and that of +infinity NaN.
+ * At most 2^31 - 1 rows of at most 2^31 - 65 logits (A3B_ERR_TOO_LARGE). */
+A3B_API int a3b_token_logprobs(a3b_stream_t stream, int dtype, void const* logits, uint64_t outer, uint64_t inner,
+                               uint64_t vocab, int64_t outer_stride, int64_t inner_stride, double scale, int index_dtype,
+                               void const* targets, float* logp, float* entropy, float* lse, uint32_t top,
+                               float* top_logp, void* top_index);
+
+/* Gradient of the outputs of a3b_token_logprobs with respect to the logits, one launch:
+ *   grad_v = scale * (grad_logp * ([v == t] - p_v) + grad_lse * p_v - grad_entropy * p_v * (ln p_v + entropy)).
+ * lse and entropy: as a3b_token_logprobs wrote them for the same logits, targets and scale. grad_logp, grad_entropy,
+ * grad_lse: one fp32 value per row, each may be null (zero); targets may be null if grad_logp is, entropy if
+ * grad_entropy is. A row without a token (target outside [0, vocab)) gets nothing from grad_logp; a row with lse
+ * -infinity gets zeros. The alternatives have no gradient. grad_logits has the logits' dtype, rounded once, and its
+ * own strides; its rows may not overlap. It may be the logits themselves (same address and strides: in place) or must
+ * lie wholly before or behind them. */
+A3B_API int a3b_token_logprobs_backward(a3b_stream_t stream, int dtype, void const* logits, uint64_t outer, uint64_t inner,
+                                        uint64_t vocab, int64_t outer_stride, int64_t inner_stride, double scale,
+                                        int index_dtype, void const* targets, float const* lse, float const* entropy,
+                                        float const* grad_logp, float const* grad_entropy, float const* grad_lse,
+                                        void* grad_logits, int64_t grad_outer_stride, int64_t grad_inner_stride);
+
+/* --------------------------------------------------------------------- norm and clipping of a list of gradients */
+
+/* A list of dense device tensors on the device that is current when it is used: count pairs of an input and an output
+ * address with the number of elements (0 is allowed) and dtype (A3B_F32, A3B_F64, A3B_F16 or A3B_BF16, mixed within a
+ * list as needed). `out` may be null (every tensor in place), as may single entries of it. The list holds addresses
+ * and sizes only: the caller keeps the memory alive while calls on it are pending, and makes a new list when an
+ * address changes. It may be destroyed as soon as the calls that use it have returned, and used by several streams
+ * and threads at once. No counterpart in alpaka3, whose algorithms take one buffer each. */
+typedef struct a3b_tensor_list a3b_tensor_list;
+A3B_API int a3b_tensor_list_create(void const* const* in, void* const* out, uint64_t const* n, int const* dtype,
+                                   uint64_t count, a3b_tensor_list** list);
+A3B_API int a3b_tensor_list_destroy(a3b_tensor_list* list);
+
+/* norm over all elements x of a list: sqrt(sum x^2), sum |x|, max |x| (NaN if any element is) */
+enum a3b_norm_kind
+{
+    A3B_NORM_L2 = 0,
+    A3B_NORM_L1 = 1,
+    A3B_NORM_MAX = 2
+};
+
+/* Bytes of device scratch that a3b_grad_norm and a3b_clip_grad_norm need for this list on the current device (any
+ * contents; nothing is kept in it between calls). Calls that overlap on the GPU need one each. 0 on failure. */
+A3B_API size_t a3b_grad_norm_workspace(a3b_tensor_list const* list);
+
+/* Norm of the whole list, held in fp64 and rounded once to norm (one element of norm_dtype, A3B_F32 or A3B_F64).
+ * partial: null, or one double that receives sum x^2, sum |x| or max |x| unrounded, to be combined across ranks (sum,
+ * sum, max) before a3b_clip_grads. Either of norm and partial may be null. Squares that leave fp32's range are formed
+ * in fp64. The order of the sum depends on the list and the device alone: repeated calls give the same bits. */
+A3B_API int a3b_grad_norm(a3b_stream_t stream, a3b_tensor_list const* list, int kind, void* workspace,
+                          size_t workspace_bytes, double* partial, int norm_dtype, void* norm);
+
+/* out = in * min(1, max_norm / (norm + 1e-6)) for every tensor of the list, with the norm that `partial` (one double on
+ * the device, as a3b_grad_norm leaves it or combined over ranks) stands for; the product is formed in fp32 (fp64 for
+ * A3B_F64) and rounded once. Tensors in place are not touched where the factor is 1. norm: null, or one element that
+ * receives the norm. A NaN norm makes every output NaN. The outputs may not overlap one another, and each must be its
+ * own input or overlap no input (A3B_ERR_INVALID). max_norm: not negative, not NaN. */
+A3B_API int a3b_clip_grads(a3b_stream_t stream, a3b_tensor_list const* list, int kind, double const* partial,
+                           double max_norm, int norm_dtype, void* norm);
+
+/* a3b_grad_norm and a3b_clip_grads in one call. */
+A3B_API int a3b_clip_grad_norm(a3b_stream_t stream, a3b_tensor_list const* list, int kind, double max_norm,
+                               void* workspace, size_t workspace_bytes, int norm_dtype, void* norm);
 
 /* ----------------------------------------------------------------------------------------------------- nBody */
 
