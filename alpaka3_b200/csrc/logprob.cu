@@ -8,8 +8,10 @@
 //     entropy = -sum p logp  = ln s - (sum (z - m) e^(z - m)) / s
 // evaluated in one pass with a running maximum: when a larger m' arrives, the sums kept so far are rescaled by
 // e^(m - m') (and the second one by what the shift of the exponents adds to it).
+#include <algorithm>
 #include <cfloat>
 #include <climits>
+#include <type_traits>
 
 #include "rows.cuh"
 
@@ -25,13 +27,13 @@ namespace a3b
         // The rows of a logits-like tensor: row r starts at (r / inner) * outerStride + (r % inner) * innerStride.
         struct RowLayout
         {
-            uint64_t inner;
+            uint32_t inner;
             int64_t outerStride;
             int64_t innerStride;
 
-            __device__ __forceinline__ int64_t at(uint64_t r) const
+            __device__ __forceinline__ int64_t at(uint32_t r) const
             {
-                uint64_t const o = r / inner;
+                uint32_t const o = r / inner;
                 return static_cast<int64_t>(o) * outerStride + static_cast<int64_t>(r - o * inner) * innerStride;
             }
         };
@@ -40,6 +42,8 @@ namespace a3b
         {
             void const* logits;
             RowLayout layout;
+            uint64_t rows;
+            uint32_t tiles; // of a row, or of its slice
             uint32_t vocab;
             uint32_t top;
             float scale;
@@ -102,53 +106,62 @@ namespace a3b
         }
 
         constexpr int kBlock = 256;
-        constexpr int kWarps = kBlock / 32;
-        constexpr int kCandidates = kBlock + kMaxTop;
+        constexpr int kMaxCluster = 8;
 
-        struct SelectSmem
+        // A row's team is W warps: a block, or (W = 1) one warp of a block of kBlock threads.
+        template<int W>
+        __device__ __forceinline__ void teamSync()
         {
-            unsigned long long keys[kCandidates];
-            unsigned long long kept[kMaxTop]; // the best so far, in order
-            unsigned bound[kWarps];
-            unsigned count;
-            unsigned floor; // an element below this order cannot enter `kept`
-            unsigned tally[3];
+            if constexpr(W == 1)
+                __syncwarp();
+            else
+                __syncthreads();
+        }
+
+        template<int W>
+        __device__ __forceinline__ unsigned teamThread()
+        {
+            return W == 1 ? threadIdx.x & 31u : threadIdx.x;
+        }
+
+        // A row: `head` elements up to the first 16-byte boundary, `packs` 16-byte packs, `tail` elements behind them.
+        template<typename T>
+        struct Row
+        {
+            static constexpr uint32_t E = PackOf<T>::E;
+            T const* p;
+            uint32_t head, packs, tail;
+
+            __device__ __forceinline__ Row(LogprobArgs const& a, uint64_t r) : p(static_cast<T const*>(a.logits) + a.layout.at(static_cast<uint32_t>(r)))
+            {
+                head = min(a.vocab, static_cast<uint32_t>((16u - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / static_cast<uint32_t>(sizeof(T)));
+                packs = (a.vocab - head) / E;
+                tail = a.vocab - head - packs * E;
+            }
         };
 
-        // One tile of a row in the registers of a block: pack p of thread t is pack base + p * kBlock + t of the row,
-        // counted from the 16-byte boundary at or below the row's first element (`lead` elements before it).
-        template<typename T>
+        // A tile of a row: P packs of every thread of the team, pack p of thread t being pack base + p * team + t of the
+        // row.
+        template<typename T, int W, int P>
         struct Tile
         {
             static constexpr int E = PackOf<T>::E;
-            unsigned q[kPacks][4];
+            static constexpr uint32_t team = W * 32;
+            unsigned q[P][4];
 
-            // Packs outside [.., end) and the elements outside the row read as -infinity; a pack that the row fills
-            // only partly is read element by element.
-            __device__ __forceinline__ void load(T const* row, uint32_t vocab, int lead, uint32_t base, uint32_t end)
+            // packs outside [.., end) read as -infinity
+            __device__ __forceinline__ void load(Row<T> const& row, uint32_t base, uint32_t end)
             {
-                T const* const origin = row - lead;
+                auto const* const from = reinterpret_cast<uint4 const*>(row.p + row.head);
 #pragma unroll
-                for(int p = 0; p < kPacks; ++p)
+                for(int p = 0; p < P; ++p)
                 {
-                    uint32_t const k = base + p * kBlock + threadIdx.x;
-                    int64_t const first = static_cast<int64_t>(k) * E - lead;
-                    if(k < end && first >= 0 && first + E <= static_cast<int64_t>(vocab))
-                    {
-                        uint4 const v = __ldcs(reinterpret_cast<uint4 const*>(origin) + k);
-                        q[p][0] = v.x, q[p][1] = v.y, q[p][2] = v.z, q[p][3] = v.w;
-                    }
-                    else
-                    {
-                        q[p][0] = q[p][1] = q[p][2] = q[p][3] = PackOf<T>::negInfWord();
-                        if(k < end)
-                        {
-#pragma unroll
-                            for(int e = 0; e < E; ++e)
-                                if(first + e >= 0 && first + e < static_cast<int64_t>(vocab))
-                                    PackOf<T>::setRaw(q[p], e, row + first + e);
-                        }
-                    }
+                    uint32_t const k = base + p * team + teamThread<W>();
+                    unsigned const n = PackOf<T>::negInfWord();
+                    uint4 v = make_uint4(n, n, n, n);
+                    if(k < end)
+                        v = __ldcs(from + k);
+                    q[p][0] = v.x, q[p][1] = v.y, q[p][2] = v.z, q[p][3] = v.w;
                 }
             }
 
@@ -157,205 +170,263 @@ namespace a3b
             __device__ __forceinline__ void fence()
             {
 #pragma unroll
-                for(int p = 0; p < kPacks; ++p)
+                for(int p = 0; p < P; ++p)
                     asm volatile("" : "+r"(q[p][0]), "+r"(q[p][1]), "+r"(q[p][2]), "+r"(q[p][3]));
-            }
-
-            // f(value, index) for every element of the row that this thread holds
-            template<typename F>
-            __device__ __forceinline__ void each(uint32_t vocab, int lead, uint32_t base, uint32_t end, F&& f) const
-            {
-#pragma unroll
-                for(int p = 0; p < kPacks; ++p)
-                {
-                    uint32_t const k = base + p * kBlock + threadIdx.x;
-                    if(k >= end)
-                        continue;
-                    int64_t const first = static_cast<int64_t>(k) * E - lead;
-#pragma unroll
-                    for(int w = 0; w < PackOf<T>::pairs; ++w)
-                    {
-                        float2 const v = PackOf<T>::pair(q[p], w);
-                        int64_t const i = first + 2 * w;
-                        if(i >= 0 && i < static_cast<int64_t>(vocab))
-                            f(v.x, static_cast<uint32_t>(i));
-                        if(i + 1 >= 0 && i + 1 < static_cast<int64_t>(vocab))
-                            f(v.y, static_cast<uint32_t>(i + 1));
-                    }
-                }
             }
         };
 
-        // how many elements of the tile satisfy `f`, over the block; `turn` counts the calls of one selection
-        template<typename T, typename F>
-        __device__ __forceinline__ unsigned countIf(
-            Tile<T>& t, uint32_t vocab, int lead, uint32_t base, uint32_t end, SelectSmem& s, int& turn, F&& f)
-        {
-            unsigned n = 0;
-            t.fence();
-            t.each(vocab, lead, base, end, [&](float x, uint32_t i) { n += f(orderOf(x), i) ? 1u : 0u; });
-            n = __reduce_add_sync(kFullMask, n);
-            if((threadIdx.x & 31) == 0)
-                atomicAdd(&s.tally[turn % 3], n);
-            if(threadIdx.x == 0)
-                s.tally[(turn + 1) % 3] = 0u; // nobody reads it any more: the last reads were two calls ago
-            __syncthreads();
-            unsigned const total = s.tally[turn % 3];
-            ++turn;
-            return total;
-        }
+        // ------------------------------------------------------------------------------------------ selection
+        constexpr unsigned kOrderNegInf = 0x007fffffu; // orderOf(-infinity), below every other one
 
-        // Adds the tile to the selection of the row's `top` largest elements (ties to the lower index). s.kept holds
-        // `kept` keys in order before and the returned number after; the block is synchronised on return.
-        //
-        // Every warp's need-th largest thread maximum, need = ceil(top / warps), is reached by `need` elements of that
-        // warp; so at least `top` elements of the tile reach the smallest of these bounds, and no element below it can
-        // be among the `top` largest. For logits in no particular order a few dozen elements of a tile pass. They are
-        // collected in shared memory (their order there does not matter: the keys are distinct) and ranked by
-        // counting. Where more pass than there is room for (many equal values), the tile's `top` are found by
-        // bisection over the values, then over the index among equal ones.
-        template<typename T>
-        __device__ __forceinline__ unsigned selectTile(
-            Tile<T>& t,
-            float threadMax,
-            uint32_t vocab,
-            int lead,
-            uint32_t base,
-            uint32_t end,
-            unsigned top,
-            unsigned kept,
-            SelectSmem& s)
+        // Candidates for a row's `top` largest elements. Two buffers take turns: one starts with the keys kept so far, in
+        // order, and collects more; ranking them writes the new kept ones to the start of the other.
+        template<int W>
+        struct Select
         {
-            int const lane = threadIdx.x & 31;
-            unsigned const mine = orderOf(threadMax);
-            unsigned bound = 0, left = mine;
-            for(unsigned i = 0; i < (top + kWarps - 1) / kWarps; ++i)
+            // the kept keys and one element of each thread always fit
+            static constexpr unsigned room = W * 32 + 2 * kMaxTop;
+            unsigned long long keys[2][room];
+            unsigned long long kth; // the last of `top` kept keys
+            unsigned count[2];
+            unsigned bound[W];
+
+            __device__ __forceinline__ void push(unsigned buffer, unsigned order, uint32_t index)
             {
-                bound = __reduce_max_sync(kFullMask, left);
-                if(lane == __ffs(static_cast<int>(__ballot_sync(kFullMask, left == bound))) - 1)
-                    left = 0u;
+                unsigned const at = atomicAdd(&count[buffer], 1u);
+                if(at < room)
+                    keys[buffer][at] = keyOf(order, index);
             }
-            if(lane == 0)
-                s.bound[threadIdx.x >> 5] = bound;
-            if(threadIdx.x < kept)
-                s.keys[threadIdx.x] = s.kept[threadIdx.x];
-            if(threadIdx.x == 0)
-                s.count = kept;
-            __syncthreads();
+
+            // Ranks the first m candidates of `buffer` by counting (their order there does not matter: the keys are
+            // distinct) and keeps the `top` best in the other one.
+            __device__ __forceinline__ void rank(unsigned buffer, unsigned m, unsigned top)
+            {
+                unsigned const thread = teamThread<W>();
+                for(unsigned i = thread; i < m; i += W * 32)
+                {
+                    unsigned long long const key = keys[buffer][i];
+                    unsigned above = 0;
+                    for(unsigned j = 0; j < m; ++j)
+                        above += keys[buffer][j] > key ? 1u : 0u;
+                    if(above < top)
+                        keys[buffer ^ 1u][above] = key;
+                    if(above == top - 1)
+                        kth = key;
+                }
+                if(thread == 0)
+                    count[buffer ^ 1u] = min(m, top);
+            }
+
+            // The order from which an element behind those kept can enter: it has a higher index, so an equal one cannot.
+            // 0: none can (the kept ones are all NaN).
+            __device__ __forceinline__ unsigned from(unsigned kept, unsigned top) const
+            {
+                return kept == top ? static_cast<unsigned>(kth >> 32) + 1u : kOrderNegInf + 1u;
+            }
+
+            // Every warp's need-th largest thread maximum, need = ceil(top / W), is reached by `need` elements of that
+            // warp; so at least `top` elements of the tile reach the smallest of these bounds, and no element below it
+            // can be among the `top` largest. For logits in no particular order a few dozen elements of a tile pass.
+            __device__ __forceinline__ unsigned boundOf(unsigned mine, unsigned top)
+            {
+                int const lane = threadIdx.x & 31;
+                unsigned least = 0, left = mine;
+                for(unsigned i = 0; i < (top + W - 1) / W; ++i)
+                {
+                    least = __reduce_max_sync(kFullMask, left);
+                    if(lane == __ffs(static_cast<int>(__ballot_sync(kFullMask, left == least))) - 1)
+                        left = 0u;
+                }
+                if(W > 1 && lane == 0)
+                    bound[threadIdx.x >> 5] = least;
+                teamSync<W>();
+                if constexpr(W > 1)
+                {
 #pragma unroll
-            for(int w = 0; w < kWarps; ++w)
-                bound = min(bound, s.bound[w]);
-            if(kept == top)
-                bound = max(bound, s.floor);
-
-            auto push = [&](float x, uint32_t i)
-            {
-                unsigned const at = atomicAdd(&s.count, 1u);
-                if(at < kCandidates)
-                    s.keys[at] = keyOf(orderOf(x), i);
-            };
-            if(mine >= bound)
-                t.each(vocab, lead, base, end, [&](float x, uint32_t i) {
-                    if(orderOf(x) >= bound)
-                        push(x, i);
-                });
-            __syncthreads();
-            t.fence();
-            unsigned n = s.count;
-            if(n > kCandidates)
-            {
-                // more than `top` elements reach `bound`: the largest value that `top` of them reach
-                __syncthreads(); // every thread has read the count
-                if(threadIdx.x == 0)
-                {
-                    s.count = kept;
-                    s.tally[0] = 0u;
+                    for(int w = 0; w < W; ++w)
+                        least = min(least, bound[w]);
                 }
-                __syncthreads();
-                int turn = 0;
-                auto count = [&](auto&& f) { return countIf(t, vocab, lead, base, end, s, turn, f); };
-                unsigned long long lo = bound, hi = 0x100000000ull; // reached by `top` elements / by fewer
-                if(count([&](unsigned o, uint32_t) { return o > bound; }) < top)
-                    hi = lo + 1;
-                while(hi - lo > 1)
-                {
-                    unsigned long long const mid = lo + (hi - lo) / 2;
-                    if(count([&](unsigned o, uint32_t) { return o >= mid; }) >= top)
-                        lo = mid;
-                    else
-                        hi = mid;
-                }
-                // of the elements with that value, the first ones, up to the index that makes `top` in all
-                unsigned const value = static_cast<unsigned>(lo);
-                unsigned const above = count([&](unsigned o, uint32_t) { return o > value; });
-                uint32_t a = 0, b = vocab - 1;
-                while(a < b)
-                {
-                    uint32_t const mid = a + (b - a) / 2;
-                    if(above + count([&](unsigned o, uint32_t i) { return o == value && i <= mid; }) >= top)
-                        b = mid;
-                    else
-                        a = mid + 1;
-                }
-                t.each(vocab, lead, base, end, [&](float x, uint32_t i) {
-                    unsigned const o = orderOf(x);
-                    if(o > value || (o == value && i <= a))
-                        push(x, i);
-                });
-                __syncthreads();
-                n = s.count;
+                return max(least, kOrderNegInf + 1u);
             }
-            if(n == kept)
-                return kept; // nothing new (a thread already in the next tile stores this same number in s.count)
-            for(unsigned i = threadIdx.x; i < n; i += kBlock)
-            {
-                unsigned long long const key = s.keys[i];
-                unsigned rank = 0;
-                for(unsigned j = 0; j < n; ++j)
-                    rank += s.keys[j] > key ? 1u : 0u;
-                if(rank < top)
-                    s.kept[rank] = key;
-                if(rank == top - 1)
-                {
-                    unsigned const o = static_cast<unsigned>(key >> 32);
-                    s.floor = o == 0xffffffffu ? o : o + 1u; // later tiles have higher indices: equal is not enough
-                }
-            }
-            __syncthreads();
-            return min(n, top);
-        }
 
-        template<typename T, bool TOP, bool ENT>
-        __global__ void __launch_bounds__(kBlock) logprobKernel(LogprobArgs a)
-        {
-            __shared__ Stats stats[kWarps];
-            __shared__ SelectSmem sel;
-            uint64_t const r = blockIdx.x;
-            T const* const row = static_cast<T const*>(a.logits) + a.layout.at(r);
-            int const lead = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
-            uint32_t const packs
-                = static_cast<uint32_t>((static_cast<uint64_t>(lead) + a.vocab + Tile<T>::E - 1) / Tile<T>::E);
-            float const c = a.scale * kLog2e;
-            int64_t const target = a.logp ? loadIndex(a.targets, r, a.index64) : -1;
-            bool const counts = target >= 0 && target < static_cast<int64_t>(a.vocab);
-            float const xt = counts ? toFloat(row[target]) : 0.0f;
-
-            float high = -INFINITY;
-            float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
-            unsigned kept = 0;
-            for(uint32_t base = 0; base < packs; base += kBlock * kPacks)
+            // Collects the tile's elements with an order of `least` or more. Where a warp has any, every thread picks its
+            // packs that hold one, one pack a turn, and looks at that pack's elements: mostly one turn, and code that
+            // is short (a search unrolled over all packs did not fit the instruction cache).
+            template<typename T, int P>
+            __device__ __forceinline__ void collect(
+                Tile<T, W, P> const& t, unsigned least, unsigned mine, uint32_t head, uint32_t base, unsigned buffer)
             {
-                Tile<T> t;
-                t.load(row, a.vocab, lead, base, packs);
-                float threadMax = -INFINITY;
+                bool const has = mine >= least && least != 0u;
+                if(!__any_sync(kFullMask, has))
+                    return;
+                float const value = valueOf(least); // NaN where `least` is: then every pack is looked at
+                unsigned packs = 0;
 #pragma unroll
-                for(int p = 0; p < kPacks; ++p)
+                for(int p = 0; p < P; ++p)
+                    packs |= PackOf<T>::max(t.q[p]) < value ? 0u : 1u << p;
+                packs = has ? packs : 0u;
+                while(packs != 0u)
+                {
+                    int const p = __ffs(static_cast<int>(packs)) - 1;
+                    packs &= packs - 1u;
+                    unsigned word[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                    for(int i = 0; i < P; ++i)
+#pragma unroll
+                        for(int w = 0; w < 4; ++w)
+                            word[w] = i == p ? t.q[i][w] : word[w];
+                    uint32_t const index
+                        = head + (base + p * Tile<T, W, P>::team + teamThread<W>()) * Tile<T, W, P>::E;
 #pragma unroll
                     for(int w = 0; w < PackOf<T>::pairs; ++w)
                     {
-                        float2 const v = PackOf<T>::pair(t.q[p], w);
-                        threadMax = maxNan(threadMax, maxNan(v.x, v.y));
+                        float2 const v = PackOf<T>::pair(word, w);
+                        unsigned const o = orderOf(v.x), o1 = orderOf(v.y);
+                        if(o >= least)
+                            push(buffer, o, index + 2 * w);
+                        if(o1 >= least)
+                            push(buffer, o1, index + 2 * w + 1);
                     }
+                }
+                __syncwarp();
+            }
+
+            // The same selection for the elements [first, last) of a row, whatever they are, in steps that always fit: an
+            // element of every thread, or eight where few of them enter. For tiles of which too many elements passed:
+            // many equal ones (constant rows, masks of one low value), rows in rising order. `buffer` starts with `kept`
+            // keys in order, those of lower indices, and its count is `kept`.
+            template<typename T>
+            __device__ __noinline__ uint2 careful(
+                T const* row, uint32_t first, uint32_t last, unsigned top, unsigned kept, unsigned buffer)
+            {
+                constexpr unsigned per = 8;
+                unsigned const thread = teamThread<W>();
+                for(uint32_t base = first; base < last; base += W * 32 * per)
+                {
+                    unsigned order[per];
+                    bool any = false;
+                    unsigned const least = from(kept, top);
+#pragma unroll
+                    for(unsigned k = 0; k < per; ++k)
+                    {
+                        uint32_t const i = base + k * W * 32 + thread;
+                        order[k] = i < last ? orderOf(toFloat(row[i])) : 0u;
+                        any |= order[k] >= least && least != 0u;
+                    }
+                    bool some;
+                    if constexpr(W == 1)
+                        some = __any_sync(kFullMask, any);
+                    else
+                        some = __syncthreads_or(any);
+                    if(!some)
+                        continue;
+                    for(unsigned k = 0; k < per; ++k)
+                    {
+                        unsigned o = 0;
+#pragma unroll
+                        for(unsigned j = 0; j < per; ++j)
+                            o = j == k ? order[j] : o;
+                        unsigned const enters = from(kept, top);
+                        if(o >= enters && enters != 0u)
+                            push(buffer, o, base + k * W * 32 + thread);
+                        teamSync<W>();
+                        unsigned const n = count[buffer];
+                        if(n > kept)
+                        {
+                            rank(buffer, n, top);
+                            kept = min(n, top);
+                            buffer ^= 1u;
+                        }
+                        teamSync<W>();
+                    }
+                }
+                return make_uint2(kept, buffer);
+            }
+        };
+
+        // Fills `kept` up to `top` keys with the row's first elements of -infinity, by one warp. All others are among the
+        // kept ones, so the first 2 top elements of the row hold enough of them.
+        template<typename T>
+        __device__ __forceinline__ void fillWithNegInf(
+            T const* row, uint32_t vocab, unsigned top, unsigned kept, unsigned long long* keys)
+        {
+            unsigned const lane = threadIdx.x & 31u;
+            for(uint32_t i0 = 0; kept < top && i0 < vocab; i0 += 32)
+            {
+                uint32_t const i = i0 + lane;
+                bool const hit = i < vocab && toFloat(row[i]) == -INFINITY;
+                unsigned const hits = __ballot_sync(kFullMask, hit);
+                unsigned const at = kept + __popc(hits & ((1u << lane) - 1u));
+                if(hit && at < top)
+                    keys[at] = keyOf(kOrderNegInf, i);
+                kept = min(top, kept + __popc(hits));
+            }
+            __syncwarp();
+        }
+
+        // What the blocks of a cluster leave in the first one's shared memory.
+        template<bool TOP>
+        struct Gather
+        {
+            Stats stats[kMaxCluster];
+            unsigned long long keys[TOP ? kMaxCluster * kMaxTop : 1];
+        };
+
+        // W > 1: the team is a block of W warps; in a launch with clusters, slice b of a row is the tiles of the cluster's
+        // block b, and the first block joins the slices. W = 1: warp w of block b takes row kBlock / 32 * b + w.
+        template<typename T, int W, int P, bool TOP, bool ENT>
+        __global__ void __launch_bounds__(W == 1 ? kBlock : W * 32, (W == 1 ? 1 : 8 / W) * (TOP ? 3 : 4))
+            logprobKernel(LogprobArgs a)
+        {
+            constexpr int teams = W == 1 ? kBlock / 32 : 1;
+            __shared__ Stats stats[W];
+            __shared__ Select<W> select[TOP ? teams : 1];
+            __shared__ Gather<TOP> gather;
+            Select<W>& sel = select[TOP && W == 1 ? threadIdx.x >> 5 : 0];
+            unsigned const thread = teamThread<W>();
+            unsigned slice = 0, slices = 1;
+            uint64_t r = W == 1 ? static_cast<uint64_t>(blockIdx.x) * teams + (threadIdx.x >> 5) : blockIdx.x;
+            if constexpr(W > 1)
+            {
+                slices = clusterBlocks();
+                if(slices > 1)
+                {
+                    clusterArrive(); // waited for before the first block's shared memory is written
+                    slice = clusterRank();
+                    r = blockIdx.x / slices;
+                }
+            }
+            else if(r >= a.rows)
+                return;
+            Row<T> const row(a, r);
+            float const c = a.scale * kLog2e;
+            uint32_t const span = P * W * 32; // packs of a tile
+            uint32_t const firstTile = slice * a.tiles;
+            int64_t const target = a.logp ? loadIndex(a.targets, r, a.index64) : -1;
+            // What lies outside the packs, one element a lane of the first warp: the head is taken with the first tile,
+            // in front of it, the tail with the last one.
+            uint32_t const aside = thread < 16 ? (thread < 8 ? thread : a.vocab - row.tail + thread - 8) : 0;
+            bool const inHead = thread < row.head && slice == 0;
+            bool const inTail = thread >= 8 && thread < 8 + row.tail && slice == slices - 1;
+            float const asideValue = inHead || inTail ? toFloat(row.p[aside]) : -INFINITY;
+            float xt = 0.0f;
+
+            float high = -INFINITY;
+            float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
+            unsigned kept = 0, buffer = 0;
+            uint32_t ranked = 0; // tiles whose candidates have been ranked
+            if(TOP && thread == 0)
+                sel.count[0] = 0u;
+            for(uint32_t tile = 0; tile < a.tiles; ++tile)
+            {
+                uint32_t const base = (firstTile + tile) * span;
+                bool const last = tile + 1 == a.tiles;
+                Tile<T, W, P> t;
+                t.load(row, base, row.packs);
+                if(tile == 0 && target >= 0 && target < static_cast<int64_t>(a.vocab))
+                    xt = toFloat(row.p[target]);
+                float const more = (inHead && tile == 0) || (inTail && last) ? asideValue : -INFINITY;
+                float const threadMax = maxNan(more, PackOf<T>::template max<P>(t.q));
                 t.fence();
                 // the warp's running maximum, and its sums moved there
                 float const to = maxNan(high, warpMaxNan(threadMax));
@@ -369,55 +440,144 @@ namespace a3b
                 }
                 float const off = -finiteOrZero(high);
                 float2 const off2 = make_float2(off, off), c2 = make_float2(c, c);
+                auto add = [&](float2 x)
+                {
+                    float2 d = mul2(add2(x, off2), c2);
+                    if constexpr(ENT)
+                    {
+                        // -infinity times the zero that it gives would be NaN; 2^-200 is zero in fp32
+                        d.x = maxNan(d.x, -200.0f);
+                        d.y = maxNan(d.y, -200.0f);
+                    }
+                    float2 const e = make_float2(exp2Approx(d.x), exp2Approx(d.y));
+                    s2 = add2(s2, e);
+                    if constexpr(ENT)
+                        u2 = fma2(d, e, u2);
+                };
 #pragma unroll
-                for(int p = 0; p < kPacks; ++p)
+                for(int p = 0; p < P; ++p)
+                {
+                    // a short tile's packs in the second half: none, for the whole team
+                    if(p == P / 2 && base + p * W * 32 >= row.packs)
+                        break;
 #pragma unroll
                     for(int w = 0; w < PackOf<T>::pairs; ++w)
-                    {
-                        float2 d = mul2(add2(PackOf<T>::pair(t.q[p], w), off2), c2);
-                        if constexpr(ENT)
-                        {
-                            // -infinity times the zero that it gives would be NaN; 2^-200 is zero in fp32
-                            d.x = maxNan(d.x, -200.0f);
-                            d.y = maxNan(d.y, -200.0f);
-                        }
-                        float2 const e = make_float2(exp2Approx(d.x), exp2Approx(d.y));
-                        s2 = add2(s2, e);
-                        if constexpr(ENT)
-                            u2 = fma2(d, e, u2);
-                    }
-                t.fence();
+                        add(PackOf<T>::pair(t.q[p], w));
+                }
+                if((tile == 0 || last) && (W == 1 || threadIdx.x < 32))
+                    add(make_float2(more, -INFINITY));
                 if constexpr(TOP)
-                    kept = selectTile(t, threadMax, a.vocab, lead, base, packs, a.top, kept, sel);
+                {
+                    // The first tile's candidates are ranked at once, later ones are collected without a barrier,
+                    // against what was kept when they were last ranked: after tiles 1, 2, 4, ..., so that about `top`
+                    // elements pass in between.
+                    t.fence();
+                    unsigned const mine = orderOf(threadMax);
+                    unsigned const least = tile == 0 ? sel.boundOf(mine, a.top) : sel.from(kept, a.top);
+                    sel.collect(t, least, mine, row.head, base, buffer);
+                    if(orderOf(more) >= least && least != 0u)
+                        sel.push(buffer, orderOf(more), aside);
+                    if(last || (tile & (tile + 1)) == 0)
+                    {
+                        teamSync<W>();
+                        unsigned const n = sel.count[buffer];
+                        if(n > sel.room)
+                        {
+                            teamSync<W>(); // every thread has read the count
+                            if(thread == 0)
+                                sel.count[buffer] = kept;
+                            teamSync<W>();
+                            uint32_t const perTile = span * PackOf<T>::E;
+                            uint32_t const from = ranked == 0 && slice == 0 ? 0 : row.head + (firstTile + ranked) * perTile;
+                            uint64_t const upTo = row.head + static_cast<uint64_t>(firstTile + tile + 1) * perTile;
+                            bool const end = last && slice == slices - 1;
+                            uint2 const got = sel.careful(
+                                row.p, from,
+                                static_cast<uint32_t>(end ? a.vocab : min(upTo, uint64_t{row.head} + row.packs * PackOf<T>::E)),
+                                a.top, kept, buffer);
+                            kept = got.x;
+                            buffer = got.y;
+                        }
+                        else
+                        {
+                            if(n > kept)
+                            {
+                                sel.rank(buffer, n, a.top);
+                                kept = min(n, a.top);
+                                buffer ^= 1u;
+                            }
+                            teamSync<W>(); // ranked, and every thread has read the count before anyone collects more
+                        }
+                        ranked = tile + 1;
+                    }
+                }
             }
             float s = s2.x + s2.y, u = u2.x + u2.y;
 #pragma unroll
             for(int m = 16; m > 0; m >>= 1)
             {
                 s += __shfl_xor_sync(kFullMask, s, m);
-                u += __shfl_xor_sync(kFullMask, u, m);
+                if constexpr(ENT)
+                    u += __shfl_xor_sync(kFullMask, u, m);
             }
-            if((threadIdx.x & 31) == 0)
-                stats[threadIdx.x >> 5] = Stats{high, s, u};
-            __syncthreads();
-            if(threadIdx.x >= 32)
-                return;
-            high = stats[0].high;
-#pragma unroll
-            for(int w = 1; w < kWarps; ++w)
-                high = maxNan(high, stats[w].high);
-            s = u = 0.0f;
-#pragma unroll
-            for(int w = 0; w < kWarps; ++w)
-                addStats(high, c, stats[w], s, u);
+            unsigned long long* const best = sel.keys[buffer];
+            if constexpr(W > 1)
+            {
+                if((threadIdx.x & 31) == 0)
+                    stats[threadIdx.x >> 5] = Stats{high, s, u};
+                __syncthreads();
+                if(slices == 1 && threadIdx.x >= 32)
+                    return;
+                auto join = [&](Stats const* all, unsigned n)
+                {
+                    high = all[0].high;
+                    for(unsigned k = 1; k < n; ++k)
+                        high = maxNan(high, all[k].high);
+                    s = u = 0.0f;
+                    for(unsigned k = 0; k < n; ++k)
+                        addStats(high, c, all[k], s, u);
+                };
+                join(stats, W);
+                if(slices > 1)
+                {
+                    clusterWait();
+                    if(threadIdx.x == 0)
+                        *inFirstBlock(&gather.stats[slice]) = Stats{high, s, u};
+                    if constexpr(TOP)
+                        if(threadIdx.x < a.top)
+                            *inFirstBlock(&gather.keys[slice * a.top + threadIdx.x])
+                                = threadIdx.x < kept ? best[threadIdx.x] : 0ull;
+                    clusterArrive();
+                    clusterWait();
+                    if(slice != 0)
+                        return;
+                    join(gather.stats, slices);
+                    if constexpr(TOP)
+                    {
+                        unsigned const n = slices * a.top;
+                        unsigned long long const key = threadIdx.x < n ? gather.keys[threadIdx.x] : 0ull;
+                        if(key != 0ull)
+                        {
+                            unsigned above = 0;
+                            for(unsigned j = 0; j < n; ++j)
+                                above += gather.keys[j] > key ? 1u : 0u;
+                            if(above < a.top)
+                                best[above] = key;
+                        }
+                        kept = min(a.top, static_cast<unsigned>(__syncthreads_count(key != 0ull)));
+                    }
+                    if(threadIdx.x >= 32)
+                        return;
+                }
+            }
 
             bool const nothing = high == -INFINITY;
             float const lnS = high == INFINITY ? 0.0f : logf(s);
             auto logpOf = [&](float x) { return nothing ? -INFINITY : fmaf(x - high, a.scale, -lnS); };
-            if(threadIdx.x == 0)
+            if(thread == 0)
             {
                 if(a.logp)
-                    a.logp[r] = counts ? logpOf(xt) : 0.0f;
+                    a.logp[r] = target >= 0 && target < static_cast<int64_t>(a.vocab) ? logpOf(xt) : 0.0f;
                 if(a.lse)
                     a.lse[r] = nothing ? -INFINITY : fmaf(high, a.scale, lnS);
                 if constexpr(ENT)
@@ -427,10 +587,12 @@ namespace a3b
                 }
             }
             if constexpr(TOP)
-                if(threadIdx.x < a.top)
+            {
+                fillWithNegInf(row.p, a.vocab, a.top, kept, best);
+                if(thread < a.top)
                 {
-                    unsigned long long const key = sel.kept[threadIdx.x];
-                    uint64_t const at = r * a.top + threadIdx.x;
+                    unsigned long long const key = best[thread];
+                    uint64_t const at = r * a.top + thread;
                     unsigned const index = ~static_cast<unsigned>(key);
                     a.topLogp[at] = logpOf(valueOf(static_cast<unsigned>(key >> 32)));
                     if(a.index64)
@@ -438,25 +600,68 @@ namespace a3b
                     else
                         static_cast<int32_t*>(a.topIndex)[at] = static_cast<int32_t>(index);
                 }
+            }
         }
 
-        template<typename T>
-        int launchLogprob(cudaStream_t stream, uint64_t rows, LogprobArgs const& a)
+        template<typename T, int W, int P, bool TOP, bool ENT>
+        int launchRows(cudaStream_t stream, unsigned cluster, LogprobArgs const& a)
         {
-            auto const grid = static_cast<unsigned>(rows);
-            if(a.top > 0)
-            {
-                if(a.entropy)
-                    logprobKernel<T, true, true><<<grid, kBlock, 0, stream>>>(a);
-                else
-                    logprobKernel<T, true, false><<<grid, kBlock, 0, stream>>>(a);
-            }
-            else if(a.entropy)
-                logprobKernel<T, false, true><<<grid, kBlock, 0, stream>>>(a);
-            else
-                logprobKernel<T, false, false><<<grid, kBlock, 0, stream>>>(a);
-            A3B_CHECK_LAUNCH("logprobKernel");
+            uint64_t const teams = W == 1 ? kBlock / 32 : 1;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = cluster;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(static_cast<unsigned>((a.rows + teams - 1) / teams) * cluster);
+            cfg.blockDim = dim3(W == 1 ? kBlock : W * 32);
+            cfg.stream = stream;
+            cfg.attrs = attr;
+            cfg.numAttrs = cluster > 1 ? 1 : 0;
+            A3B_CUDA(cudaLaunchKernelEx(&cfg, logprobKernel<T, W, P, TOP, ENT>, a));
             return A3B_OK;
+        }
+
+        // The team of a row. Warps that need no barrier are best as long as there are enough of them: W is the smallest
+        // that makes kEnoughWarps of all rows, but not more than a row fills with one tile. Measured on a B200, bf16,
+        // W = 1 / 2 / 4 / 8 in microseconds: 8192 rows of 8192 logits 26 / 28 / 30 / 42; 4096 x 16384 28 / 27 / 28 / 30;
+        // 2048 x 50257 46 / 40 / 40 / 43, with 20 alternatives 87 / 77 / 72 / 80. Rows of up to 64 packs take tiles of
+        // two packs a thread, whose kernel has fewer registers and more warps: 32768 x 257 with 2 alternatives 34
+        // against 42. Few long rows are cut into slices over a cluster, as many as the GPU holds at once (a second
+        // wave costs more than a slice gains): 1 / 2 / 4 / 8 slices of 16 rows of 131072 with 20 alternatives
+        // 20 / 15 / 11 / 10, of 64 fp32 rows with 5 28 / 19 / 15 / 19.
+        constexpr uint64_t kEnoughWarps = 8192;
+
+        template<typename T>
+        int launchLogprob(cudaStream_t stream, DeviceProps const* props, LogprobArgs a)
+        {
+            uint64_t const packs = a.vocab / PackOf<T>::E;
+            auto go = [&](auto w, auto p, unsigned cluster)
+            {
+                constexpr int W = decltype(w)::value, P = decltype(p)::value;
+                uint64_t const tiles = (packs + uint64_t{W} * 32 * P * cluster - 1) / (uint64_t{W} * 32 * P * cluster);
+                a.tiles = static_cast<uint32_t>(std::max<uint64_t>(tiles, 1));
+                if(a.top > 0)
+                    return a.entropy ? launchRows<T, W, P, true, true>(stream, cluster, a)
+                                     : launchRows<T, W, P, true, false>(stream, cluster, a);
+                return a.entropy ? launchRows<T, W, P, false, true>(stream, cluster, a)
+                                 : launchRows<T, W, P, false, false>(stream, cluster, a);
+            };
+            using std::integral_constant;
+            constexpr integral_constant<int, kPacks> full;
+            uint64_t const oneTile = 32 * kPacks; // packs of a warp's tile
+            if(packs <= 64)
+                return go(integral_constant<int, 1>{}, integral_constant<int, 2>{}, 1u);
+            if(a.rows >= kEnoughWarps || packs <= oneTile)
+                return go(integral_constant<int, 1>{}, full, 1u);
+            if(a.rows >= kEnoughWarps / 2 || packs <= 2 * oneTile)
+                return go(integral_constant<int, 2>{}, full, 1u);
+            if(a.rows >= kEnoughWarps / 4 || packs <= 4 * oneTile)
+                return go(integral_constant<int, 4>{}, full, 1u);
+            uint64_t const held = static_cast<uint64_t>(props->smCount) * 3; // blocks
+            unsigned cluster = 1;
+            while(cluster < kMaxCluster && a.rows * cluster * 2 <= held && packs > cluster * 8 * oneTile)
+                cluster *= 2;
+            return go(integral_constant<int, 8>{}, full, cluster);
         }
 
         // ------------------------------------------------------------------------------------------- gradient
@@ -488,8 +693,8 @@ namespace a3b
             constexpr int E = PackOf<T>::E;
             uint64_t const r = blockIdx.x / a.chunks;
             uint32_t const chunk = blockIdx.x - static_cast<uint32_t>(r * a.chunks);
-            T const* const row = static_cast<T const*>(a.logits) + a.layout.at(r);
-            T* const out = static_cast<T*>(a.grad) + a.gradLayout.at(r);
+            T const* const row = static_cast<T const*>(a.logits) + a.layout.at(static_cast<uint32_t>(r));
+            T* const out = static_cast<T*>(a.grad) + a.gradLayout.at(static_cast<uint32_t>(r));
             // packs on the 16-byte boundaries of the output row; the input row may lie differently
             int const lead = static_cast<int>((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T));
             bool const alike = (reinterpret_cast<uintptr_t>(row) & 15u) == (reinterpret_cast<uintptr_t>(out) & 15u);
@@ -671,15 +876,14 @@ extern "C"
         int const rd = currentDevice(&props);
         if(rd != A3B_OK)
             return rd;
-        LogprobArgs a{logits, {inner, outer_stride, inner_stride}, static_cast<uint32_t>(vocab), top,
-                      static_cast<float>(scale), index_dtype == A3B_I64, targets, logp, entropy, lse, top_logp,
-                      top_index};
+        LogprobArgs a{logits, {static_cast<uint32_t>(inner), outer_stride, inner_stride}, rows, 1u, static_cast<uint32_t>(vocab), top, static_cast<float>(scale), index_dtype == A3B_I64,
+                      targets, logp, entropy, lse, top_logp, top_index};
         auto s = static_cast<cudaStream_t>(stream);
         if(dtype == A3B_F32)
-            return launchLogprob<float>(s, rows, a);
+            return launchLogprob<float>(s, props, a);
         if(dtype == A3B_F16)
-            return launchLogprob<__half>(s, rows, a);
-        return launchLogprob<__nv_bfloat16>(s, rows, a);
+            return launchLogprob<__half>(s, props, a);
+        return launchLogprob<__nv_bfloat16>(s, props, a);
     }
 
     int a3b_token_logprobs_backward(
@@ -736,8 +940,8 @@ extern "C"
         int const rd = currentDevice(&props);
         if(rd != A3B_OK)
             return rd;
-        BackwardArgs a{logits, grad_logits, {inner, outer_stride, inner_stride},
-                       {inner, grad_outer_stride, grad_inner_stride}, static_cast<uint32_t>(vocab), 1u,
+        BackwardArgs a{logits, grad_logits, {static_cast<uint32_t>(inner), outer_stride, inner_stride},
+                       {static_cast<uint32_t>(inner), grad_outer_stride, grad_inner_stride}, static_cast<uint32_t>(vocab), 1u,
                        static_cast<float>(scale), index_dtype == A3B_I64, targets, lse, entropy, grad_logp,
                        grad_entropy, grad_lse};
         auto s = static_cast<cudaStream_t>(stream);

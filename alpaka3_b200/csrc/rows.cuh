@@ -36,6 +36,40 @@ namespace a3b
         return r;
     }
 
+    // ------------------------------------------------------------------------------------- thread-block clusters
+    __device__ __forceinline__ unsigned clusterRank()
+    {
+        unsigned r;
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+        return r;
+    }
+
+    __device__ __forceinline__ unsigned clusterBlocks()
+    {
+        unsigned r;
+        asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+        return r;
+    }
+
+    __device__ __forceinline__ void clusterArrive()
+    {
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    }
+
+    __device__ __forceinline__ void clusterWait()
+    {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+
+    // the address of the same shared variable in the cluster's first block
+    template<typename V>
+    __device__ __forceinline__ V* inFirstBlock(V* p)
+    {
+        V* r;
+        asm("mapa.u64 %0, %1, 0;" : "=l"(r) : "l"(p));
+        return r;
+    }
+
     // Elements of one 16-byte pack (E of them, W = 4 words) as 32-bit floats, two at a time: element 2w and 2w + 1 of
     // a 16-bit type come from word w, of a 32-bit type from words 2w and 2w + 1.
     template<typename T>
@@ -76,6 +110,56 @@ namespace a3b
                 __half2 const h = __float22half2_rn(v);
                 memcpy(word + w, &h, 4);
             }
+        }
+
+        // largest element of one pack, or of N packs (NaN if any is one); 16-bit types two at a time
+        template<int N>
+        static __device__ __forceinline__ float max(unsigned const (&word)[N][4])
+        {
+            if constexpr(std::is_same_v<T, float>)
+            {
+                float m = -INFINITY;
+#pragma unroll
+                for(int p = 0; p < N; ++p)
+                    m = maxNan(m, max(word[p]));
+                return m;
+            }
+            else
+            {
+                unsigned m = word[0][0];
+#pragma unroll
+                for(int p = 0; p < N; ++p)
+#pragma unroll
+                    for(int w = 0; w < 4; ++w)
+                        m = maxWord(m, word[p][w]);
+                return halves(m);
+            }
+        }
+
+        static __device__ __forceinline__ float max(unsigned const* word)
+        {
+            if constexpr(std::is_same_v<T, float>)
+                return maxNan(maxNan(__uint_as_float(word[0]), __uint_as_float(word[1])),
+                              maxNan(__uint_as_float(word[2]), __uint_as_float(word[3])));
+            else
+                return halves(maxWord(maxWord(word[0], word[1]), maxWord(word[2], word[3])));
+        }
+
+        // of two elements in one word each
+        static __device__ __forceinline__ unsigned maxWord(unsigned a, unsigned b)
+        {
+            unsigned r;
+            if constexpr(std::is_same_v<T, __nv_bfloat16>)
+                asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+            else
+                asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+            return r;
+        }
+
+        static __device__ __forceinline__ float halves(unsigned w)
+        {
+            float2 const v = pair(&w, 0);
+            return maxNan(v.x, v.y);
         }
 
         static __device__ __forceinline__ unsigned negInfWord()
