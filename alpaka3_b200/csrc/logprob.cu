@@ -81,7 +81,8 @@ namespace a3b
             return (static_cast<unsigned long long>(order) << 32) | static_cast<unsigned>(~index);
         }
 
-        // Sums of one share of a row: e^(z - m) and (z - m) / ln 2 * e^(z - m), m = scale * high.
+        // Sums of one share of a row whose largest logit is `high`: s = sum 2^t and u = sum t 2^t over its logits x, with
+        // t = c x + offset, one fused operation. c = scale / ln 2, and offset = -(c high) as it is rounded.
         struct Stats
         {
             float high;
@@ -89,20 +90,35 @@ namespace a3b
             float u;
         };
 
-        __device__ __forceinline__ float finiteOrZero(float high)
+        // Logits next to one beyond 2^80 differ from it by 2^56 or more, so only those equal to it count: any factor does
+        // that keeps c x in range and takes every other t below -2^16. u is 0 then (and not computed: `u` holds NaN if
+        // there are logits of -infinity, which no clamp separates from a maximum of fp32's lowest value).
+        __device__ __forceinline__ bool isBig(float high)
         {
-            return high == -INFINITY ? 0.0f : high;
+            return !(fabsf(high) <= 0x1p80f);
         }
 
-        // the sums of `b` moved to the maximum `high` (not below b's) and added to s, u; c = scale / ln 2
+        __device__ __forceinline__ float factorOf(float high, float c)
+        {
+            return isBig(high) && high != -INFINITY ? 0x1p-40f : c;
+        }
+
+        __device__ __forceinline__ float offsetOf(float high, float c)
+        {
+            // rounded on its own wherever it is used: fused into a difference of offsets it would be another number
+            return high == -INFINITY ? 0.0f : -__fmul_rn(high, factorOf(high, c));
+        }
+
+        // the sums of `b` moved to the maximum `high` (not below b's) and added to s, u
         __device__ __forceinline__ void addStats(float high, float c, Stats const& b, float& s, float& u)
         {
             if(b.high == -INFINITY)
                 return; // nothing in that share
-            float const d = (b.high - finiteOrZero(high)) * c;
+            bool const big = isBig(high) || isBig(b.high);
+            float const d = b.high == high ? 0.0f : big ? -200.0f : fmaxf(offsetOf(high, c) - offsetOf(b.high, c), -200.0f);
             float const f = exp2Approx(d);
             s += f * b.s;
-            u += f * fmaf(fmaxf(d, -200.0f), b.s, b.u);
+            u += big ? 0.0f : f * fmaf(d, b.s, b.u);
         }
 
         constexpr int kBlock = 256;
@@ -152,16 +168,27 @@ namespace a3b
             // packs outside [.., end) read as -infinity
             __device__ __forceinline__ void load(Row<T> const& row, uint32_t base, uint32_t end)
             {
-                auto const* const from = reinterpret_cast<uint4 const*>(row.p + row.head);
-#pragma unroll
-                for(int p = 0; p < P; ++p)
+                auto const* const from = reinterpret_cast<uint4 const*>(row.p + row.head) + base + teamThread<W>();
+                unsigned const n = PackOf<T>::negInfWord();
+                if(base + P * team <= end)
                 {
-                    uint32_t const k = base + p * team + teamThread<W>();
-                    unsigned const n = PackOf<T>::negInfWord();
-                    uint4 v = make_uint4(n, n, n, n);
-                    if(k < end)
-                        v = __ldcs(from + k);
-                    q[p][0] = v.x, q[p][1] = v.y, q[p][2] = v.z, q[p][3] = v.w;
+#pragma unroll
+                    for(int p = 0; p < P; ++p)
+                    {
+                        uint4 const v = __ldcs(from + p * team);
+                        q[p][0] = v.x, q[p][1] = v.y, q[p][2] = v.z, q[p][3] = v.w;
+                    }
+                }
+                else
+                {
+#pragma unroll
+                    for(int p = 0; p < P; ++p)
+                    {
+                        uint4 v = make_uint4(n, n, n, n);
+                        if(base + p * team + teamThread<W>() < end)
+                            v = __ldcs(from + p * team);
+                        q[p][0] = v.x, q[p][1] = v.y, q[p][2] = v.z, q[p][3] = v.w;
+                    }
                 }
             }
 
@@ -411,7 +438,8 @@ namespace a3b
             float const asideValue = inHead || inTail ? toFloat(row.p[aside]) : -INFINITY;
             float xt = 0.0f;
 
-            float high = -INFINITY;
+            float high = -INFINITY, factor = c, offset = 0.0f;
+            unsigned low = PackOf<T>::negInfWord();
             float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
             unsigned kept = 0, buffer = 0;
             uint32_t ranked = 0; // tiles whose candidates have been ranked
@@ -430,20 +458,25 @@ namespace a3b
                 t.fence();
                 // the warp's running maximum, and its sums moved there
                 float const to = maxNan(high, warpMaxNan(threadMax));
-                if(to != high)
+                if(tile == 0 || to != high)
                 {
-                    Stats const x{high, s2.x, u2.x}, y{high, s2.y, u2.y};
-                    s2 = u2 = make_float2(0.0f, 0.0f);
-                    addStats(to, c, x, s2.x, u2.x);
-                    addStats(to, c, y, s2.y, u2.y);
+                    if(tile > 0)
+                    {
+                        Stats const before{high, s2.x + s2.y, u2.x + u2.y};
+                        s2 = u2 = make_float2(0.0f, 0.0f);
+                        addStats(to, c, before, s2.x, u2.x);
+                    }
                     high = to;
+                    factor = factorOf(high, c);
+                    offset = offsetOf(high, c);
+                    // far below what counts (t < -200), for logits of -infinity: see below
+                    low = PackOf<T>::twice(high - fmaf(fabsf(high), 0x1p-6f, 256.0f / c));
                 }
-                float const off = -finiteOrZero(high);
-                float2 const off2 = make_float2(off, off), c2 = make_float2(c, c);
+                float2 const offset2 = make_float2(offset, offset), factor2 = make_float2(factor, factor);
                 auto add = [&](float2 x)
                 {
-                    float2 d = mul2(add2(x, off2), c2);
-                    if constexpr(ENT)
+                    float2 d = fma2(x, factor2, offset2);
+                    if constexpr(ENT && !std::is_same_v<T, __nv_bfloat16>)
                     {
                         // -infinity times the zero that it gives would be NaN; 2^-200 is zero in fp32
                         d.x = maxNan(d.x, -200.0f);
@@ -462,10 +495,19 @@ namespace a3b
                         break;
 #pragma unroll
                     for(int w = 0; w < PackOf<T>::pairs; ++w)
-                        add(PackOf<T>::pair(t.q[p], w));
+                    {
+                        // bf16: the same bound in front of the conversion, for two elements at once
+                        unsigned word[4] = {t.q[p][0], t.q[p][1], t.q[p][2], t.q[p][3]};
+                        if constexpr(ENT && std::is_same_v<T, __nv_bfloat16>)
+                            word[w] = PackOf<T>::maxWord(word[w], low);
+                        add(PackOf<T>::pair(word, w));
+                    }
                 }
                 if((tile == 0 || last) && (W == 1 || threadIdx.x < 32))
-                    add(make_float2(more, -INFINITY));
+                {
+                    float const least = high - fmaf(fabsf(high), 0x1p-6f, 256.0f / c);
+                    add(make_float2(maxNan(more, least), least));
+                }
                 if constexpr(TOP)
                 {
                     // The first tile's candidates are ranked at once, later ones are collected without a barrier,
@@ -571,8 +613,11 @@ namespace a3b
                 }
             }
 
-            bool const nothing = high == -INFINITY;
-            float const lnS = high == INFINITY ? 0.0f : logf(s);
+            // The largest logit's own t is what the rounding of the offset left (not quite 0): s over its 2^t is the sum
+            // of e^(z - m), 1 in a row with one logit left.
+            bool const nothing = high == -INFINITY, big = isBig(high);
+            float const rest = big ? 0.0f : fmaf(high, c, offsetOf(high, c));
+            float const lnS = high == INFINITY ? 0.0f : logf(s / exp2Approx(rest));
             auto logpOf = [&](float x) { return nothing ? -INFINITY : fmaf(x - high, a.scale, -lnS); };
             if(thread == 0)
             {
@@ -582,8 +627,8 @@ namespace a3b
                     a.lse[r] = nothing ? -INFINITY : fmaf(high, a.scale, lnS);
                 if constexpr(ENT)
                 {
-                    float const h = lnS - kLn2 * (u / s);
-                    a.entropy[r] = nothing ? 0.0f : (high == INFINITY ? NAN : (h < 0.0f ? 0.0f : h));
+                    float const h = lnS - (big ? 0.0f : kLn2 * (u / s - rest));
+                    a.entropy[r] = nothing ? 0.0f : !(high < INFINITY) ? NAN : (h < 0.0f ? 0.0f : h);
                 }
             }
             if constexpr(TOP)
@@ -804,8 +849,7 @@ namespace a3b
             A3B_REQUIRE(dtype == A3B_F32 || dtype == A3B_F16 || dtype == A3B_BF16, "logits must be f32, f16 or bf16");
             A3B_REQUIRE(indexDtype == A3B_I32 || indexDtype == A3B_I64, "token indices must be i32 or i64");
             A3B_REQUIRE(vocab > 0, "a row needs at least one logit");
-            A3B_REQUIRE(scale > 0.0 && scale <= static_cast<double>(FLT_MAX), "scale must be positive and finite");
-            A3B_REQUIRE(static_cast<float>(scale) > 0.0f, "scale is too small for fp32");
+            A3B_REQUIRE(scale >= 0x1p-20 && scale <= 0x1p20, "scale must lie between 2^-20 and 2^20");
             A3B_REQUIRE(outer == 0 || inner <= UINT64_MAX / outer, "rows overflow");
             if(vocab > static_cast<uint64_t>(INT_MAX) - 64 || outer * inner > static_cast<uint64_t>(INT_MAX))
             {

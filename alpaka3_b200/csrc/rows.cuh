@@ -156,6 +156,15 @@ namespace a3b
             return r;
         }
 
+        // a word of `v` rounded to T, twice for 16-bit types
+        static __device__ __forceinline__ unsigned twice(float v)
+        {
+            unsigned word[4] = {__float_as_uint(v), 0u, 0u, 0u};
+            if constexpr(!std::is_same_v<T, float>)
+                setPair(word, 0, make_float2(v, v));
+            return word[0];
+        }
+
         static __device__ __forceinline__ float halves(unsigned w)
         {
             float2 const v = pair(&w, 0);

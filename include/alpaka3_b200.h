@@ -269,7 +269,7 @@ A3B_API int a3b_scan(a3b_stream_t stream, int dtype, int inclusive, void const* 
  * o * outer_stride + i * inner_stride and is contiguous; any strides, also ones that make rows overlap. The other
  * arrays are dense in row order: targets (index_dtype A3B_I32 or A3B_I64), logp, entropy, lse (fp32), top_logp (fp32)
  * and top_index (index_dtype), `top` of each per row. logp, entropy and lse may be null (not computed); targets may be
- * null if logp is. top: 0 .. 32, at most vocab. scale: positive and finite (the inverse temperature).
+ * null if logp is. top: 0 .. 32, at most vocab. scale (the inverse temperature): between 2^-20 and 2^20.
  *
  * A target outside [0, vocab) marks a row without a token: its logp is 0. Logits of -infinity have probability 0 (logp
  * -infinity); a row of nothing else has lse -infinity, entropy 0 and logp -infinity for every token. A NaN in a row
