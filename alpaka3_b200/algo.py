@@ -213,14 +213,21 @@ def exclusive_scan_in_place(data, buffer=None, stream=None):
 
 
 # ------------------------------------------------------------------------------------- token log probabilities
-def _call_on(device, stream, name, *args):
-    """capi.call on `stream` (default: the device's current stream) with `device` current."""
-    if stream is not None and stream.device_index != device.index:
-        raise ValueError(f"the stream belongs to device {stream.device_index}, the tensors to {device}")
-    if torch.cuda.current_device() == device.index:
-        return capi.call(name, stream_handle(stream), *args)
-    with torch.cuda.device(device):
-        return capi.call(name, stream_handle(stream), *args)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the address alone, without a Stream object
+
+
+def _call_on(index, stream, name, *args):
+    """capi.call on `stream` (default: the current stream of device `index`) with that device current."""
+    if stream is None:
+        handle = _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream
+    elif stream.device_index != index:
+        raise ValueError(f"the stream belongs to device {stream.device_index}, the tensors to device {index}")
+    else:
+        handle = stream.cuda_stream
+    if torch.cuda.current_device() == index:
+        return capi.call(name, handle, *args)
+    with torch.cuda.device(index):
+        return capi.call(name, handle, *args)
 
 
 def _rows(t, name):
@@ -244,25 +251,32 @@ def _rows(t, name):
     return outer, inner, so, si
 
 
-def _per_row(t, name, rows, device, dtypes, width=None):
-    """Address of a dense per-row array (None stays None)."""
+def _per_row(t, name, count, index, dtypes):
+    """Address of a dense array of `count` elements on device `index` (None stays None)."""
     if t is None:
         return None
     if t.dtype not in dtypes:
         raise TypeError(f"{name}: unsupported dtype {t.dtype}")
-    if t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous tensor on {device}")
-    if t.numel() != rows * (1 if width is None else width):
-        raise ValueError(f"{name}: expected {rows * (1 if width is None else width)} elements, got {t.numel()}")
-    return ctypes.c_void_p(t.data_ptr())
+    if t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor on CUDA device {index}")
+    if t.numel() != count:
+        raise ValueError(f"{name}: expected {count} elements, got {t.numel()}")
+    return t.data_ptr()
 
 
-def _logits_code(logits):
-    if logits.dtype not in _LOGITS_DT:
-        raise TypeError(f"unsupported logits dtype {logits.dtype}")
-    if not logits.is_cuda:
-        raise ValueError("expected a CUDA tensor")
-    return _LOGITS_DT[logits.dtype]
+def _logits(t, name="logits"):
+    """(dtype code, device index, outer, inner, vocab, outer stride, inner stride)"""
+    code = _LOGITS_DT.get(t.dtype)
+    if code is None:
+        raise TypeError(f"unsupported {name} dtype {t.dtype}")
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"{name}: expected a CUDA tensor")
+    if t.dim() > 0 and t.is_contiguous():
+        vocab = t.shape[-1]
+        return code, index, 1, t.numel() // max(vocab, 1), vocab, 0, vocab
+    outer, inner, so, si = _rows(t, name)
+    return code, index, outer, inner, t.shape[-1], so, si
 
 
 _F32 = (torch.float32,)
@@ -278,23 +292,25 @@ def token_logprobs(logp, logits, targets, entropy=None, lse=None, top_logp=None,
     targets: int64 or int32, one per row (None without logp); outside [0, vocab) there is no token: logp 0. top_index:
     dtype of targets, or int64 / int32 without them. The logits' rows may be strided (logits[:, :-1], a padded
     vocabulary); the other tensors are contiguous. Infinities and NaN: see a3b_token_logprobs. Returns logp."""
-    code = _logits_code(logits)
-    outer, inner, so, si = _rows(logits, "logits")
-    rows, vocab, dev = outer * inner, logits.shape[-1], logits.device
-    if (top_logp is None) != (top_index is None):
-        raise ValueError("top_logp and top_index belong together")
-    if logp is not None and targets is None:
+    code, dev, outer, inner, vocab, so, si = _logits(logits)
+    rows = outer * inner
+    top, index = 0, capi.I64
+    if top_logp is not None or top_index is not None:
+        if top_logp is None or top_index is None:
+            raise ValueError("top_logp and top_index belong together")
+        top = top_logp.shape[-1]
+        index = _INDEX_DT.get(top_index.dtype, -1)
+    if targets is not None:
+        if top and top_index.dtype != targets.dtype:
+            raise TypeError("top_index and targets must have the same dtype")
+        index = _INDEX_DT.get(targets.dtype, -1)
+    elif logp is not None:
         raise ValueError("logp needs targets")
-    top = 0 if top_logp is None else top_logp.shape[-1]
-    ints = targets if targets is not None else top_index
-    if targets is not None and top_index is not None and top_index.dtype != targets.dtype:
-        raise TypeError("top_index and targets must have the same dtype")
-    index = capi.I64 if ints is None else _INDEX_DT.get(ints.dtype, -1)
-    _call_on(dev, stream, "a3b_token_logprobs", code, ctypes.c_void_p(logits.data_ptr()), outer, inner, vocab, so, si,
-             float(scale), index, _per_row(targets, "targets", rows, dev, _INDEX_DT),
-             _per_row(logp, "logp", rows, dev, _F32), _per_row(entropy, "entropy", rows, dev, _F32),
-             _per_row(lse, "lse", rows, dev, _F32), top, _per_row(top_logp, "top_logp", rows, dev, _F32, top),
-             _per_row(top_index, "top_index", rows, dev, _INDEX_DT, top))
+    _call_on(dev, stream, "a3b_token_logprobs", code, logits.data_ptr(), outer, inner, vocab, so, si, scale, index,
+             _per_row(targets, "targets", rows, dev, _INDEX_DT), _per_row(logp, "logp", rows, dev, _F32),
+             _per_row(entropy, "entropy", rows, dev, _F32), _per_row(lse, "lse", rows, dev, _F32), top,
+             _per_row(top_logp, "top_logp", rows * top, dev, _F32),
+             _per_row(top_index, "top_index", rows * top, dev, _INDEX_DT))
     return logp
 
 
@@ -304,28 +320,26 @@ def token_logprobs_backward(grad_logits, logits, targets, lse, entropy=None, gra
     grad_entropy) as token_logprobs wrote them and the gradients of a loss with respect to them (float32, one per row;
     None is zero), writes that with respect to the logits to `grad_logits` (shape and dtype of logits; any row strides;
     may be `logits` itself). Rows without a token get nothing from grad_logp. Returns grad_logits."""
-    code = _logits_code(logits)
-    outer, inner, so, si = _rows(logits, "logits")
-    if grad_logits.shape != logits.shape or grad_logits.dtype != logits.dtype or grad_logits.device != logits.device:
+    code, dev, outer, inner, vocab, so, si = _logits(logits)
+    if grad_logits.shape != logits.shape or grad_logits.dtype != logits.dtype or grad_logits.get_device() != dev:
         raise ValueError("grad_logits must have the shape, dtype and device of logits")
-    go, gi, gso, gsi = _rows(grad_logits, "grad_logits")
-    if (go, gi) != (outer, inner):  # one of the two collapses further than the other
-        if outer == 1 and go > 1:
+    _, _, go, gi, _, gso, gsi = _logits(grad_logits, "grad_logits")
+    if go != outer:  # one of the two collapses further than the other
+        if outer == 1:
             outer, inner, so = go, gi, si * gi
-        elif go == 1 and outer > 1:
+        elif go == 1:
             gso = gsi * inner
-        else:
-            raise ValueError("logits and grad_logits do not collapse to the same two dimensions")
-    rows, dev = outer * inner, logits.device
+    if go * gi != outer * inner or (go != 1 and gi != inner):
+        raise ValueError("logits and grad_logits do not collapse to the same two dimensions")
+    rows = outer * inner
     if lse is None:
         raise ValueError("lse is needed")
     index = capi.I64 if targets is None else _INDEX_DT.get(targets.dtype, -1)
-    _call_on(dev, stream, "a3b_token_logprobs_backward", code, ctypes.c_void_p(logits.data_ptr()), outer, inner,
-             logits.shape[-1], so, si, float(scale), index, _per_row(targets, "targets", rows, dev, _INDEX_DT),
-             _per_row(lse, "lse", rows, dev, _F32), _per_row(entropy, "entropy", rows, dev, _F32),
-             _per_row(grad_logp, "grad_logp", rows, dev, _F32),
-             _per_row(grad_entropy, "grad_entropy", rows, dev, _F32),
-             _per_row(grad_lse, "grad_lse", rows, dev, _F32), ctypes.c_void_p(grad_logits.data_ptr()), gso, gsi)
+    _call_on(dev, stream, "a3b_token_logprobs_backward", code, logits.data_ptr(), outer, inner, vocab, so, si, scale,
+             index, _per_row(targets, "targets", rows, dev, _INDEX_DT), _per_row(lse, "lse", rows, dev, _F32),
+             _per_row(entropy, "entropy", rows, dev, _F32), _per_row(grad_logp, "grad_logp", rows, dev, _F32),
+             _per_row(grad_entropy, "grad_entropy", rows, dev, _F32), _per_row(grad_lse, "grad_lse", rows, dev, _F32),
+             grad_logits.data_ptr(), gso, gsi)
     return grad_logits
 
 
@@ -387,68 +401,78 @@ class TensorList:
     def __len__(self):
         return len(self.inputs)
 
-    def workspace(self, device, stream):
+    def _scratch(self, index, stream):
         """Scratch for one call, from torch's allocator in the order of the call's stream."""
         if self._workspace is None:
-            with torch.cuda.device(device):
-                self._workspace = capi.lib().a3b_grad_norm_workspace(self._handle) // 8
+            with torch.cuda.device(index):
+                self._workspace = capi.lib().a3b_grad_norm_workspace(self._handle)
         if stream is None:
-            return torch.empty(self._workspace, dtype=torch.float64, device=device)
+            return torch.empty(self._workspace, dtype=torch.uint8, device=torch.device("cuda", index))
         with torch.cuda.stream(stream):
-            return torch.empty(self._workspace, dtype=torch.float64, device=device)
+            return torch.empty(self._workspace, dtype=torch.uint8, device=torch.device("cuda", index))
 
 
-def _list_args(norm, tensors, kind, *more):
-    """(TensorList, device, kind code, norm's dtype code, norm's address)"""
+def _scalar(t, name, index, dtypes):
+    """Address of one element on device `index` (None stays None)."""
+    if t is None:
+        return None
+    if t.dtype not in dtypes:
+        raise TypeError(f"unsupported dtype {t.dtype} of {name}")
+    if t.get_device() != index or t.numel() != 1:
+        raise ValueError(f"{name}: expected a tensor of one element on CUDA device {index}")
+    return t.data_ptr()
+
+
+_NORM_DT = {torch.float32: capi.F32, torch.float64: capi.F64}
+
+
+def _list_args(norm, tensors, kind, partial=None):
+    """(TensorList, device index, kind code, address of partial, norm's dtype code, norm's address)"""
     if kind not in NORM:
         raise ValueError(f"unknown norm {kind!r}: one of {', '.join(NORM)}")
     if not isinstance(tensors, TensorList):
         tensors = TensorList(tensors)
-    some = next((t for t in (norm, *more) if t is not None), None)
-    if some is None:
-        raise ValueError("nothing to compute: no output is given")
-    dev = tensors.device if tensors.device is not None else some.device
-    for t in (norm, *more):
-        if t is not None and (t.device != dev or not t.is_cuda or t.numel() != 1):
-            raise ValueError(f"expected a tensor of one element on {dev}")
-    for t in more:
-        if t is not None and t.dtype != torch.float64:
-            raise TypeError("partial must be float64")
-    if norm is not None and norm.dtype not in (torch.float32, torch.float64):
-        raise TypeError(f"unsupported dtype {norm.dtype} of the norm")
-    code = capi.F32 if norm is None else _DT[norm.dtype]
-    return tensors, dev, NORM[kind], code, None if norm is None else ctypes.c_void_p(norm.data_ptr())
+    index = tensors.device.index if tensors.device is not None else -1
+    for t in (norm, partial):
+        if index < 0 and t is not None:
+            index = t.get_device()
+    if index < 0:
+        raise ValueError("expected CUDA tensors")
+    p = _scalar(partial, "partial", index, (torch.float64,))
+    if norm is None:
+        return tensors, index, NORM[kind], p, capi.F32, None
+    n = _scalar(norm, "norm", index, _NORM_DT)
+    return tensors, index, NORM[kind], p, _NORM_DT[norm.dtype], n
 
 
 def grad_norm(norm, tensors, kind="l2", partial=None, stream=None):
     """Norm over all elements of a list of tensors ("l2", "l1" or "max"; a TensorList or any sequence of tensors) into
     `norm`, one float32 or float64 element on the device. partial: one float64 element that receives the sum of squares,
     the sum of magnitudes or the largest magnitude unrounded, for combination across ranks; either may be None."""
-    tensors, dev, k, code, p = _list_args(norm, tensors, kind, partial)
-    ws = tensors.workspace(dev, stream)
-    _call_on(dev, stream, "a3b_grad_norm", tensors._handle, k, ctypes.c_void_p(ws.data_ptr()), ws.numel() * 8,
-             None if partial is None else ctypes.c_void_p(partial.data_ptr()), code, p)
+    if norm is None and partial is None:
+        raise ValueError("nothing to compute: no output is given")
+    tensors, dev, k, p, code, n = _list_args(norm, tensors, kind, partial)
+    ws = tensors._scratch(dev, stream)
+    _call_on(dev, stream, "a3b_grad_norm", tensors._handle, k, ws.data_ptr(), ws.numel(), p, code, n)
     return norm
 
 
 def clip_grads(norm, tensors, partial, max_norm, kind="l2", stream=None):
     """Multiplies every tensor of the list by min(1, max_norm / (norm + 1e-6)), with the norm that `partial` stands for
     (as grad_norm wrote it, or combined across ranks), and writes that norm to `norm` (None: not written)."""
-    tensors, dev, k, code, p = _list_args(norm, tensors, kind, partial)
     if partial is None:
         raise ValueError("partial is needed")
-    _call_on(dev, stream, "a3b_clip_grads", tensors._handle, k, ctypes.c_void_p(partial.data_ptr()), float(max_norm),
-             code, p)
+    tensors, dev, k, p, code, n = _list_args(norm, tensors, kind, partial)
+    _call_on(dev, stream, "a3b_clip_grads", tensors._handle, k, p, max_norm, code, n)
     return norm
 
 
 def clip_grad_norm(norm, tensors, max_norm, kind="l2", stream=None):
     """grad_norm and clip_grads in one call: the tensors of the list scaled down so that their common norm is at most
     `max_norm`, written to the list's outputs (a plain sequence: in place); the norm before goes to `norm`."""
-    tensors, dev, k, code, p = _list_args(norm, tensors, kind)
-    ws = tensors.workspace(dev, stream)
-    _call_on(dev, stream, "a3b_clip_grad_norm", tensors._handle, k, float(max_norm), ctypes.c_void_p(ws.data_ptr()),
-             ws.numel() * 8, code, p)
+    tensors, dev, k, _, code, n = _list_args(norm, tensors, kind)
+    ws = tensors._scratch(dev, stream)
+    _call_on(dev, stream, "a3b_clip_grad_norm", tensors._handle, k, max_norm, ws.data_ptr(), ws.numel(), code, n)
     return norm
 
 

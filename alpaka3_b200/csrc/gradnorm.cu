@@ -4,11 +4,15 @@
 //
 // The list travels in the kernels' parameters (addresses and sizes by value, up to kEntries tensors a launch), so a call
 // copies nothing to the device and can be captured in a graph. The tensors are cut into chunks of kChunkPacks 16-byte
-// packs; a block finds the tensor of a chunk by bisection over the chunks' running count.
-//   * normKernel: every block folds its chunks into one fp64 partial in the workspace;
-//   * clipKernel: every block folds all partials in the same order, then scales its chunks.
-// The workspace holds nothing between calls (no tickets), and no block waits for another: captured graphs and streams
-// only need a workspace each.
+// packs, numbered through the list; a block finds the tensor of a chunk by bisection over the chunks' running count.
+//   * normKernel: resident blocks, each folds a run of consecutive chunks into one fp64 partial in the workspace
+//     (7.1 TB/s on a B200 over 2.1 GB);
+//   * finishKernel: one block folds the partials in their order;
+//   * clipKernel: a block for every chunk, handed out in order (copies at 6.5 TB/s; resident blocks reached 5.9).
+//     It and finishKernel are launched while the kernel before drains (programmatic dependent launch);
+//   * clipSmallKernel: both for a short list, one launch of one cluster.
+// The workspace holds nothing between calls (no tickets), and no block waits for another one's progress in memory:
+// captured graphs and streams only need a workspace each.
 #include <algorithm>
 #include <cfloat>
 #include <climits>
@@ -27,8 +31,11 @@ namespace a3b
         constexpr int kWarps = kBlock / 32;
         constexpr int kPacks = 4;                                // packs of a chunk per thread
         constexpr uint64_t kChunkPacks = uint64_t{kBlock} * kPacks; // 16 KB
-        constexpr int kEntries = 960;                            // tensors a launch: 32 bytes each, of 32764
-        constexpr int kBlocksPerSm = 4;
+        constexpr int kEntries = 960;     // tensors a launch: 32 bytes each, of 32764
+        constexpr int kFewEntries = 32;   // parameters of 1 KB: 30 KB cost the host 2 us a launch
+        constexpr int kBlocksPerSm = 6;
+        constexpr uint32_t kSmallChunks = 32; // up to here one cluster does it all
+        constexpr unsigned kSmallCluster = 8;
 
         struct Entry
         {
@@ -39,12 +46,14 @@ namespace a3b
             int32_t dtype;
         };
 
-        struct Batch
+        template<int N>
+        struct BatchOf
         {
             uint32_t count;
             uint32_t chunks;
-            Entry e[kEntries];
+            Entry e[N];
         };
+        using Batch = BatchOf<kEntries>;
         static_assert(sizeof(Batch) <= 32000, "kernel parameters hold 32764 bytes");
 
         int sizeOf(int dtype)
@@ -186,7 +195,7 @@ namespace a3b
                     int64_t i;
                     if(whole(n, lead, c, p, i) && aligned)
                     {
-                        uint4 const v = __ldg(reinterpret_cast<uint4 const*>(in + i));
+                        uint4 const v = __ldcs(reinterpret_cast<uint4 const*>(in + i));
                         q[p][0] = v.x, q[p][1] = v.y, q[p][2] = v.z, q[p][3] = v.w;
                     }
                     else
@@ -219,7 +228,9 @@ namespace a3b
             }
         };
 
-        __device__ __forceinline__ Entry const& entryOf(Batch const& b, uint32_t chunk)
+        // index of the tensor that chunk `chunk` of the list belongs to
+        template<int N>
+        __device__ __forceinline__ uint32_t entryOf(BatchOf<N> const& b, uint32_t chunk)
         {
             uint32_t lo = 0, hi = b.count; // e[lo].firstChunk <= chunk < e[hi].firstChunk
             while(hi - lo > 1)
@@ -230,7 +241,14 @@ namespace a3b
                 else
                     hi = mid;
             }
-            return b.e[lo];
+            return lo;
+        }
+
+        // the run of chunks that block `block` of `blocks` takes
+        __device__ __forceinline__ uint2 runOf(uint32_t chunks, uint32_t block, uint32_t blocks)
+        {
+            return make_uint2(static_cast<uint32_t>(uint64_t{chunks} * block / blocks),
+                              static_cast<uint32_t>(uint64_t{chunks} * (block + 1u) / blocks));
         }
 
         __device__ __forceinline__ int leadOf(void const* p, int size)
@@ -267,14 +285,17 @@ namespace a3b
             return r;
         }
 
-        template<int KIND>
-        __global__ void __launch_bounds__(kBlock) normKernel(__grid_constant__ Batch const b, double* partials)
+        // this block's share of the norm: the chunks [run.x, run.y), in order
+        template<int KIND, int N>
+        __device__ __forceinline__ double runNorm(BatchOf<N> const& b, uint2 run)
         {
-            __shared__ double smem[kWarps];
             double r = 0.0;
-            for(uint32_t c = blockIdx.x; c < b.chunks; c += gridDim.x)
+            uint32_t k = run.x < run.y ? entryOf(b, run.x) : 0;
+            for(uint32_t c = run.x; c < run.y; ++c)
             {
-                Entry const& e = entryOf(b, c);
+                while(k + 1 < b.count && b.e[k + 1].firstChunk <= c)
+                    ++k;
+                Entry const& e = b.e[k];
                 uint64_t const at = c - e.firstChunk;
                 switch(e.dtype)
                 {
@@ -291,7 +312,16 @@ namespace a3b
                     r = fold<KIND>(r, chunkNorm<KIND, __nv_bfloat16>(e, at));
                 }
             }
-            r = blockFold<KIND>(r, smem);
+            return r;
+        }
+
+        template<int KIND, int N>
+        __global__ void __launch_bounds__(kBlock, kBlocksPerSm)
+            normKernel(__grid_constant__ BatchOf<N> const b, double* partials)
+        {
+            asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); // they wait before they read `partials`
+            __shared__ double smem[kWarps];
+            double const r = blockFold<KIND>(runNorm<KIND>(b, runOf(b.chunks, blockIdx.x, gridDim.x)), smem);
             if(threadIdx.x == 0)
                 partials[blockIdx.x] = r;
         }
@@ -324,9 +354,13 @@ namespace a3b
 
         template<int KIND>
         __global__ void __launch_bounds__(kBlock)
-            finishKernel(double const* partials, uint32_t count, double* partial, int dtype, void* norm)
+            finishKernel(double const* partials, uint32_t count, double* partial, int dtype, void* norm, bool clips)
         {
             __shared__ double smem[kWarps];
+            // clipKernel waits before it reads the result; whatever else comes next on the stream may not
+            if(clips)
+                asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+            asm volatile("griddepcontrol.wait;" ::: "memory");
             double const t = total<KIND>(partials, count, smem);
             if(threadIdx.x == 0)
             {
@@ -336,22 +370,54 @@ namespace a3b
             }
         }
 
-        template<typename T, typename F>
-        __device__ __forceinline__ void clipChunk(Entry const& e, uint64_t c, F factor)
+        // min(1, maxNorm / (norm + 1e-6)), NaN stays
+        __device__ __forceinline__ double factorOf(double norm, double maxNorm)
+        {
+            double const ratio = maxNorm / (norm + 1e-6);
+            return ratio > 1.0 ? 1.0 : ratio;
+        }
+
+        template<typename T>
+        __device__ __forceinline__ void clipChunk(Entry const& e, uint64_t c, double factor)
         {
             // packs on the output's boundaries; the input is read by elements where it lies differently
             Chunk<T> x;
             int const lead = leadOf(e.out, sizeof(T));
             x.load(static_cast<T const*>(e.in), e.n, lead, c, lead == leadOf(e.in, sizeof(T)));
+            using S = std::conditional_t<std::is_same_v<T, double>, double, float>;
 #pragma unroll
             for(int p = 0; p < kPacks; ++p)
-                scalePack<T>(x.q[p], factor);
+                scalePack<T>(x.q[p], static_cast<S>(factor));
             x.store(static_cast<T*>(e.out), e.n, lead, c);
         }
 
-        template<int KIND>
-        __global__ void __launch_bounds__(kBlock) clipKernel(
-            __grid_constant__ Batch const b,
+        template<int N>
+        __device__ __forceinline__ void clipOne(BatchOf<N> const& b, uint32_t c, double factor)
+        {
+            Entry const& e = b.e[entryOf(b, c)];
+            uint64_t const at = c - e.firstChunk;
+            if(factor == 1.0 && e.in == e.out)
+                return;
+            switch(e.dtype)
+            {
+            case A3B_F32:
+                clipChunk<float>(e, at, factor);
+                break;
+            case A3B_F64:
+                clipChunk<double>(e, at, factor);
+                break;
+            case A3B_F16:
+                clipChunk<__half>(e, at, factor);
+                break;
+            default:
+                clipChunk<__nv_bfloat16>(e, at, factor);
+            }
+        }
+
+        // Block b scales chunk b. `partials`: those of normKernel, or (count = 1) their fold.
+        template<int KIND, int N>
+        __global__ void __launch_bounds__(kBlock, kBlocksPerSm) clipKernel(
+            __grid_constant__ BatchOf<N> const b,
             double const* partials,
             uint32_t count,
             double maxNorm,
@@ -359,32 +425,39 @@ namespace a3b
             void* normOut)
         {
             __shared__ double smem[kWarps];
-            double const norm = normOf<KIND>(total<KIND>(partials, count, smem));
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            double const norm
+                = normOf<KIND>(count == 1u ? __ldcg(partials) : total<KIND>(partials, count, smem));
             if(blockIdx.x == 0 && threadIdx.x == 0)
                 writeNorm(norm, dtype, normOut);
-            double const ratio = maxNorm / (norm + 1e-6);
-            double const factor = ratio > 1.0 ? 1.0 : ratio; // NaN stays
-            for(uint32_t c = blockIdx.x; c < b.chunks; c += gridDim.x)
-            {
-                Entry const& e = entryOf(b, c);
-                uint64_t const at = c - e.firstChunk;
-                if(factor == 1.0 && e.in == e.out)
-                    continue;
-                switch(e.dtype)
-                {
-                case A3B_F32:
-                    clipChunk<float>(e, at, static_cast<float>(factor));
-                    break;
-                case A3B_F64:
-                    clipChunk<double>(e, at, factor);
-                    break;
-                case A3B_F16:
-                    clipChunk<__half>(e, at, static_cast<float>(factor));
-                    break;
-                default:
-                    clipChunk<__nv_bfloat16>(e, at, static_cast<float>(factor));
-                }
-            }
+            clipOne(b, blockIdx.x, factorOf(norm, maxNorm));
+        }
+
+        // Norm and clipping of a list of up to kSmallChunks chunks by one cluster: the blocks leave their partials in one
+        // another's shared memory. One launch instead of two, and nothing in the workspace.
+        template<int KIND, int N>
+        __global__ void __launch_bounds__(kBlock) __cluster_dims__(kSmallCluster, 1, 1)
+            clipSmallKernel(__grid_constant__ BatchOf<N> const b, double maxNorm, int dtype, void* normOut)
+        {
+            __shared__ double smem[kWarps];
+            __shared__ double all[kSmallCluster];
+            clusterArrive();
+            uint2 const run = runOf(b.chunks, blockIdx.x, kSmallCluster);
+            double const r = blockFold<KIND>(runNorm<KIND>(b, run), smem);
+            clusterWait(); // every block has started
+            if(threadIdx.x < kSmallCluster)
+                *inBlock(all + blockIdx.x, threadIdx.x) = r;
+            clusterArrive();
+            clusterWait();
+            double t = all[0];
+#pragma unroll
+            for(unsigned k = 1; k < kSmallCluster; ++k)
+                t = fold<KIND>(t, all[k]);
+            double const norm = normOf<KIND>(t);
+            if(blockIdx.x == 0 && threadIdx.x == 0)
+                writeNorm(norm, dtype, normOut);
+            for(uint32_t c = run.x; c < run.y; ++c)
+                clipOne(b, c, factorOf(norm, maxNorm));
         }
     } // namespace
 } // namespace a3b
@@ -466,6 +539,36 @@ namespace a3b
             return n * sizeof(double);
         }
 
+        // f(the batch as kernel parameters): few tensors as the short form
+        template<typename F>
+        int withBatch(Batch const& b, F&& f)
+        {
+            if(b.count > static_cast<uint32_t>(kFewEntries))
+                return f(b);
+            BatchOf<kFewEntries> few;
+            few.count = b.count;
+            few.chunks = b.chunks;
+            std::copy(b.e, b.e + b.count, few.e);
+            return f(few);
+        }
+
+        // Launches `kernel` so that it may start while the kernel before it drains; it waits by itself.
+        template<typename... P, typename... A>
+        int launchAfter(cudaStream_t s, uint32_t grid, void (*kernel)(P...), A const&... args)
+        {
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[0].val.programmaticStreamSerializationAllowed = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(grid);
+            cfg.blockDim = dim3(kBlock);
+            cfg.stream = s;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            A3B_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+            return A3B_OK;
+        }
+
         template<int KIND>
         int launchNorm(cudaStream_t s, a3b_tensor_list const* list, DeviceProps const* props, double* partials, uint32_t* count)
         {
@@ -473,7 +576,10 @@ namespace a3b
             for(Batch const& b : list->batches)
             {
                 uint32_t const grid = gridOf(b, props);
-                normKernel<KIND><<<grid, kBlock, 0, s>>>(b, partials + *count);
+                withBatch(b, [&](auto const& p) {
+                    normKernel<KIND><<<grid, kBlock, 0, s>>>(p, partials + *count);
+                    return A3B_OK;
+                });
                 A3B_CHECK_LAUNCH("normKernel");
                 *count += grid;
             }
@@ -481,33 +587,72 @@ namespace a3b
         }
 
         template<int KIND>
-        int launchFinish(cudaStream_t s, double const* partials, uint32_t count, double* partial, int dtype, void* norm)
+        int launchFinish(cudaStream_t s, double const* partials, uint32_t count, double* partial, int dtype, void* norm, bool clips)
         {
-            finishKernel<KIND><<<1, kBlock, 0, s>>>(partials, count, partial, dtype, norm);
-            A3B_CHECK_LAUNCH("finishKernel");
-            return A3B_OK;
+            return launchAfter(s, 1, finishKernel<KIND>, partials, count, partial, dtype, norm, clips);
         }
 
+        // `early`: the kernel right before on the stream is normKernel or finishKernel
         template<int KIND>
         int launchClip(
             cudaStream_t s,
             a3b_tensor_list const* list,
-            DeviceProps const* props,
             double const* partials,
             uint32_t count,
             double maxNorm,
             int dtype,
+            void* norm,
+            bool early)
+        {
+            for(Batch const& b : list->batches)
+            {
+                int const rc = withBatch(b, [&](auto const& p) {
+                    constexpr int N = sizeof(p.e) / sizeof(Entry);
+                    if(early)
+                        return launchAfter(s, b.chunks, clipKernel<KIND, N>, p, partials, count, maxNorm, dtype, norm);
+                    clipKernel<KIND, N><<<b.chunks, kBlock, 0, s>>>(p, partials, count, maxNorm, dtype, norm);
+                    A3B_CHECK_LAUNCH("clipKernel");
+                    return static_cast<int>(A3B_OK);
+                });
+                if(rc != A3B_OK)
+                    return rc;
+                norm = nullptr;
+                early = false;
+            }
+            return A3B_OK;
+        }
+
+        // Norm, then clipping. Lists of one wave of blocks: every block folds the partials. Longer ones: one block does, in
+        // a launch of its own, and a block for every chunk reads the result (162 tensors, 2.1 GB of bf16 on a B200:
+        // 958 us; resident blocks that walk runs of chunks 1042).
+        template<int KIND>
+        int launchBoth(
+            cudaStream_t s,
+            a3b_tensor_list const* list,
+            DeviceProps const* props,
+            double maxNorm,
+            double* workspace,
+            int dtype,
             void* norm)
         {
             if(list->batches.empty())
-                return norm ? launchFinish<KIND>(s, partials, count, nullptr, dtype, norm) : A3B_OK;
-            for(Batch const& b : list->batches)
-            {
-                clipKernel<KIND><<<gridOf(b, props), kBlock, 0, s>>>(b, partials, count, maxNorm, dtype, norm);
-                A3B_CHECK_LAUNCH("clipKernel");
-                norm = nullptr;
-            }
-            return A3B_OK;
+                return norm ? launchFinish<KIND>(s, workspace, 0u, nullptr, dtype, norm, false) : A3B_OK;
+            Batch const& first = list->batches[0];
+            if(list->batches.size() == 1 && first.chunks <= kSmallChunks)
+                return withBatch(first, [&](auto const& p) {
+                    clipSmallKernel<KIND><<<kSmallCluster, kBlock, 0, s>>>(p, maxNorm, dtype, norm);
+                    A3B_CHECK_LAUNCH("clipSmallKernel");
+                    return static_cast<int>(A3B_OK);
+                });
+            double* const partials = workspace + 1;
+            uint32_t count = 0;
+            int const rc = launchNorm<KIND>(s, list, props, partials, &count);
+            if(rc != A3B_OK)
+                return rc;
+            if(list->batches.size() == 1 && first.chunks <= gridOf(first, props))
+                return launchClip<KIND>(s, list, partials, count, maxNorm, dtype, norm, true);
+            int const rf = launchFinish<KIND>(s, partials, count, workspace, dtype, norm, true);
+            return rf != A3B_OK ? rf : launchClip<KIND>(s, list, workspace, 1u, maxNorm, dtype, nullptr, true);
         }
 
         // f(std::integral_constant<int, kind>)
@@ -547,9 +692,9 @@ namespace a3b
                 uint64_t const perPack = 16 / size;
                 uint64_t const own = ((n[k] + most + perPack - 1) / perPack + kChunkPacks - 1) / kChunkPacks;
                 if(list->batches.empty() || list->batches.back().count == static_cast<uint32_t>(kEntries)
-                   || chunks + own > static_cast<uint64_t>(UINT32_MAX))
+                   || chunks + own > static_cast<uint64_t>(INT_MAX))
                 {
-                    A3B_REQUIRE(own <= static_cast<uint64_t>(UINT32_MAX), "a tensor is larger than any device");
+                    A3B_REQUIRE(own <= static_cast<uint64_t>(INT_MAX), "a tensor is larger than any device");
                     list->batches.emplace_back();
                     list->batches.back().count = 0;
                     chunks = 0;
@@ -641,7 +786,7 @@ extern "C"
             auto* const partials = static_cast<double*>(workspace);
             uint32_t count = 0;
             int const e = launchNorm<k()>(s, list, props, partials, &count);
-            return e != A3B_OK ? e : launchFinish<k()>(s, partials, count, partial, norm_dtype, norm);
+            return e != A3B_OK ? e : launchFinish<k()>(s, partials, count, partial, norm_dtype, norm, false);
         });
     }
 
@@ -666,7 +811,9 @@ extern "C"
             return rd;
         auto s = static_cast<cudaStream_t>(stream);
         return withKind(kind, [&](auto k) {
-            return launchClip<k()>(s, list, props, partial, 1u, max_norm, norm_dtype, norm);
+            if(list->batches.empty())
+                return norm ? launchFinish<k()>(s, partial, 1u, nullptr, norm_dtype, norm, false) : static_cast<int>(A3B_OK);
+            return launchClip<k()>(s, list, partial, 1u, max_norm, norm_dtype, norm, false);
         });
     }
 
@@ -693,10 +840,7 @@ extern "C"
         A3B_REQUIRE(workspace_bytes >= workspaceOf(list, props), "workspace is too small");
         auto s = static_cast<cudaStream_t>(stream);
         return withKind(kind, [&](auto k) {
-            auto* const partials = static_cast<double*>(workspace);
-            uint32_t count = 0;
-            int const e = launchNorm<k()>(s, list, props, partials, &count);
-            return e != A3B_OK ? e : launchClip<k()>(s, list, props, partials, count, max_norm, norm_dtype, norm);
+            return launchBoth<k()>(s, list, props, max_norm, static_cast<double*>(workspace), norm_dtype, norm);
         });
     }
 }

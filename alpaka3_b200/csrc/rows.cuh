@@ -61,12 +61,12 @@ namespace a3b
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
 
-    // the address of the same shared variable in the cluster's first block
+    // the address of the same shared variable in block `rank` of the cluster
     template<typename V>
-    __device__ __forceinline__ V* inFirstBlock(V* p)
+    __device__ __forceinline__ V* inBlock(V* p, unsigned rank)
     {
         V* r;
-        asm("mapa.u64 %0, %1, 0;" : "=l"(r) : "l"(p));
+        asm("mapa.u64 %0, %1, %2;" : "=l"(r) : "l"(p), "r"(rank));
         return r;
     }
 
@@ -212,6 +212,18 @@ namespace a3b
             return __bfloat162float(v);
         else
             return __half2float(v);
+    }
+
+    // rounded to the nearest value of T
+    template<typename T>
+    __device__ __forceinline__ T fromFloat(float v)
+    {
+        if constexpr(std::is_same_v<T, float>)
+            return v;
+        else if constexpr(std::is_same_v<T, __nv_bfloat16>)
+            return __float2bfloat16_rn(v);
+        else
+            return __float2half_rn(v);
     }
 
     // Two fp32 operations in one instruction (sm_100's packed fp32 pipe), each rounded on its own.

@@ -260,6 +260,10 @@ def check_backward(x, t, scale=1.0, use=("logp", "entropy", "lse"), out=None, se
     type_step = torch.finfo(x.dtype).eps / 2
     # p's error grows with |t| = |q| / ln 2; under the smallest normal number a type loses a fixed amount
     tol = scale * p * mag * (2.0**-21 + 2.0**-21 * q.abs().nan_to_num(posinf=0)) + want.abs() * (type_step + 2 * U)
+    # The kernel forms ln p / ln 2 as a fused c x - lse / ln 2, both factors rounded to fp32, plus a rest that carries
+    # what the two roundings left: |rest| <= 2 * 2^-24 |lse| / ln 2 < 2^-22 |lse|. The rest is rounded too, and the sum of
+    # two terms that cancel: 2^-24 |rest| each, 2^-44 |lse| with room for both. It counts where q itself is 0.
+    tol = tol + scale * p * gh.abs()[:, None] * torch.where(some, lse.abs(), zero)[:, None] * 2.0**-44
     tol = tol.nan_to_num(0.0) + gp.abs()[:, None] * scale * 2 * U + torch.finfo(x.dtype).tiny * max(type_step * 2, 2.0**-8)
     close(res.reshape(-1, v), want, tol)
     return res
