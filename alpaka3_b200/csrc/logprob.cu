@@ -192,6 +192,16 @@ namespace a3b
                 }
             }
 
+            // pack p from `from`, or (for the whole team) left as it is
+            __device__ __forceinline__ void reload(int p, uint4 const* from, bool really)
+            {
+                asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+                             "@p ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                             : "+r"(q[p][0]), "+r"(q[p][1]), "+r"(q[p][2]), "+r"(q[p][3])
+                             : "l"(from), "r"(really ? 1u : 0u)
+                             : "memory");
+            }
+
             // Keeps the compiler from carrying unpacked elements from one use of the tile to the next: unpacking again
             // is an instruction or less an element, the floats of a whole tile are 64 registers.
             __device__ __forceinline__ void fence()
@@ -204,6 +214,25 @@ namespace a3b
 
         // ------------------------------------------------------------------------------------------ selection
         constexpr unsigned kOrderNegInf = 0x007fffffu; // orderOf(-infinity), below every other one
+
+        // how many of m keys in shared memory are larger than `key`; independent loads, eight at a time
+        __device__ __forceinline__ unsigned countAbove(unsigned long long const* keys, unsigned m, unsigned long long key)
+        {
+            unsigned above = 0, j = 0;
+            for(; j + 8 <= m; j += 8)
+            {
+                unsigned long long k[8];
+#pragma unroll
+                for(int i = 0; i < 8; ++i)
+                    k[i] = keys[j + i];
+#pragma unroll
+                for(int i = 0; i < 8; ++i)
+                    above += k[i] > key ? 1u : 0u;
+            }
+            for(; j < m; ++j)
+                above += keys[j] > key ? 1u : 0u;
+            return above;
+        }
 
         // Candidates for a row's `top` largest elements. Two buffers take turns: one starts with the keys kept so far, in
         // order, and collects more; ranking them writes the new kept ones to the start of the other.
@@ -232,9 +261,7 @@ namespace a3b
                 for(unsigned i = thread; i < m; i += W * 32)
                 {
                     unsigned long long const key = keys[buffer][i];
-                    unsigned above = 0;
-                    for(unsigned j = 0; j < m; ++j)
-                        above += keys[buffer][j] > key ? 1u : 0u;
+                    unsigned const above = countAbove(keys[buffer], m, key);
                     if(above < top)
                         keys[buffer ^ 1u][above] = key;
                     if(above == top - 1)
@@ -442,17 +469,17 @@ namespace a3b
             unsigned low = PackOf<T>::negInfWord();
             float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
             unsigned kept = 0, buffer = 0;
-            uint32_t ranked = 0; // tiles whose candidates have been ranked
+            uint32_t ranked = 0, rankAfter = 1; // tiles whose candidates have been ranked, or will be next
             if(TOP && thread == 0)
                 sel.count[0] = 0u;
+            Tile<T, W, P> t;
+            t.load(row, firstTile * span, row.packs);
+            if(target >= 0 && target < static_cast<int64_t>(a.vocab))
+                xt = toFloat(row.p[target]);
             for(uint32_t tile = 0; tile < a.tiles; ++tile)
             {
                 uint32_t const base = (firstTile + tile) * span;
                 bool const last = tile + 1 == a.tiles;
-                Tile<T, W, P> t;
-                t.load(row, base, row.packs);
-                if(tile == 0 && target >= 0 && target < static_cast<int64_t>(a.vocab))
-                    xt = toFloat(row.p[target]);
                 float const more = (inHead && tile == 0) || (inTail && last) ? asideValue : -INFINITY;
                 float const threadMax = maxNan(more, PackOf<T>::template max<P>(t.q));
                 t.fence();
@@ -472,6 +499,17 @@ namespace a3b
                     // far below what counts (t < -200), for logits of -infinity: see below
                     low = PackOf<T>::twice(high - fmaf(fabsf(high), 0x1p-6f, 256.0f / c));
                 }
+                if constexpr(TOP)
+                {
+                    // The first tile's candidates are ranked at once, later ones are collected without a barrier,
+                    // against what was kept when they were last ranked.
+                    unsigned const mine = orderOf(threadMax);
+                    unsigned const least = tile == 0 ? sel.boundOf(mine, a.top) : sel.from(kept, a.top);
+                    sel.collect(t, least, mine, row.head, base, buffer);
+                    if(orderOf(more) >= least && least != 0u)
+                        sel.push(buffer, orderOf(more), aside);
+                    t.fence();
+                }
                 float2 const offset2 = make_float2(offset, offset), factor2 = make_float2(factor, factor);
                 auto add = [&](float2 x)
                 {
@@ -487,6 +525,10 @@ namespace a3b
                     if constexpr(ENT)
                         u2 = fma2(d, e, u2);
                 };
+                // The registers of a pack that is done take the same pack of the next tile, if that is a full one: its
+                // loads run under the rest of this tile.
+                bool const nextFull = !last && base + 2 * span <= row.packs;
+                auto const* const next = reinterpret_cast<uint4 const*>(row.p + row.head) + base + span + thread;
 #pragma unroll
                 for(int p = 0; p < P; ++p)
                 {
@@ -502,24 +544,18 @@ namespace a3b
                             word[w] = PackOf<T>::maxWord(word[w], low);
                         add(PackOf<T>::pair(word, w));
                     }
+                    t.reload(p, next + p * W * 32, nextFull);
                 }
                 if((tile == 0 || last) && (W == 1 || threadIdx.x < 32))
                 {
                     float const least = high - fmaf(fabsf(high), 0x1p-6f, 256.0f / c);
                     add(make_float2(maxNan(more, least), least));
                 }
+                if(!last && !nextFull)
+                    t.load(row, base + span, row.packs);
                 if constexpr(TOP)
                 {
-                    // The first tile's candidates are ranked at once, later ones are collected without a barrier,
-                    // against what was kept when they were last ranked: after tiles 1, 2, 4, ..., so that about `top`
-                    // elements pass in between.
-                    t.fence();
-                    unsigned const mine = orderOf(threadMax);
-                    unsigned const least = tile == 0 ? sel.boundOf(mine, a.top) : sel.from(kept, a.top);
-                    sel.collect(t, least, mine, row.head, base, buffer);
-                    if(orderOf(more) >= least && least != 0u)
-                        sel.push(buffer, orderOf(more), aside);
-                    if(last || (tile & (tile + 1)) == 0)
+                    if(last || tile + 1 == rankAfter)
                     {
                         teamSync<W>();
                         unsigned const n = sel.count[buffer];
@@ -551,6 +587,9 @@ namespace a3b
                             teamSync<W>(); // ranked, and every thread has read the count before anyone collects more
                         }
                         ranked = tile + 1;
+                        // Between ranking at n tiles and at k n about (k - 1) top elements pass: k = 4 as long as they fit
+                        // with room to spare.
+                        rankAfter = ranked * (8u * a.top <= sel.room ? 4u : 2u);
                     }
                 }
             }
@@ -570,15 +609,24 @@ namespace a3b
                 __syncthreads();
                 if(slices == 1 && threadIdx.x >= 32)
                     return;
+                // one share a lane, for every warp that is still here alike
                 auto join = [&](Stats const* all, unsigned n)
                 {
-                    high = all[0].high;
-                    for(unsigned k = 1; k < n; ++k)
-                        high = maxNan(high, all[k].high);
+                    unsigned const lane = threadIdx.x & 31u;
+                    Stats const mine = lane < n ? all[lane] : Stats{-INFINITY, 0.0f, 0.0f};
+                    high = warpMaxNan(mine.high);
                     s = u = 0.0f;
-                    for(unsigned k = 0; k < n; ++k)
-                        addStats(high, c, all[k], s, u);
+                    addStats(high, c, mine, s, u);
+#pragma unroll
+                    for(int m = 4; m > 0; m >>= 1)
+                    {
+                        s += __shfl_xor_sync(kFullMask, s, m);
+                        u += __shfl_xor_sync(kFullMask, u, m);
+                    }
+                    s = __shfl_sync(kFullMask, s, 0);
+                    u = __shfl_sync(kFullMask, u, 0);
                 };
+                static_assert(W <= 8 && kMaxCluster <= 8, "join() sums eight lanes");
                 join(stats, W);
                 if(slices > 1)
                 {
@@ -600,9 +648,7 @@ namespace a3b
                         unsigned long long const key = threadIdx.x < n ? gather.keys[threadIdx.x] : 0ull;
                         if(key != 0ull)
                         {
-                            unsigned above = 0;
-                            for(unsigned j = 0; j < n; ++j)
-                                above += gather.keys[j] > key ? 1u : 0u;
+                            unsigned const above = countAbove(gather.keys, n, key);
                             if(above < a.top)
                                 best[above] = key;
                         }
