@@ -32,7 +32,7 @@ namespace a3b
         constexpr int kPacks = 4;                                // packs of a chunk per thread
         constexpr uint64_t kChunkPacks = uint64_t{kBlock} * kPacks; // 16 KB
         constexpr int kEntries = 960;     // tensors a launch: 32 bytes each, of 32764
-        constexpr int kFewEntries = 32;   // parameters of 1 KB: 30 KB cost the host 2 us a launch
+        constexpr int kFewEntries = 120;  // parameters under 4 KB: 30 KB cost the host 2 us a launch
         constexpr int kBlocksPerSm = 6;
         constexpr uint32_t kSmallChunks = 32; // up to here one cluster does it all
         constexpr unsigned kSmallCluster = 8;

@@ -25,9 +25,9 @@ def tol_sum(v):
     return (v / 256 + 84 + 3 * math.log(v + 1) + 4) * U
 
 
-def oracle(x, scale=1.0):
+def oracle(x, scale=1.0, where="cpu"):
     """q (log probabilities), lse and entropy of 2-D logits in 64 bits, by the documented rules."""
-    z = x.double().cpu() * scale
+    z = x.double().to(where) * scale
     m = z.amax(-1, keepdim=True)
     safe = torch.where(torch.isinf(m), torch.zeros_like(m), m)
     ln_s = torch.log(torch.exp(z - safe).sum(-1, keepdim=True))
@@ -40,9 +40,9 @@ def oracle(x, scale=1.0):
     return q, lse[:, 0], h
 
 
-def ranks(x, k):
+def ranks(x, k, where="cpu"):
     """indices of the k largest per row: NaN above all, -0 equal to 0, ties to the lower index"""
-    return torch.sort(x.float().cpu() + 0.0, dim=-1, descending=True, stable=True)[1][:, :k]
+    return torch.sort(x.float().to(where) + 0.0, dim=-1, descending=True, stable=True)[1][:, :k]
 
 
 def close(got, want, tol):
@@ -220,6 +220,57 @@ def test_rows_do_not_touch_neighbours(cuda):
     outs = torch.full((8, 3), 9.0, device="cuda")
     algo.token_logprobs(outs[1:7].reshape(-1)[:6], x, t)
     assert (outs.reshape(-1)[9:] == 9).all() and (outs.reshape(-1)[:3] == 9).all()
+
+
+# many rows: a warp a row with several tiles, two and four warps a row, and rows that leave the last tile nearly empty
+MANY = [(8192, 5003), (8200, 2060), (4100, 9001), (2048, 17011), (2051, 33000), (8192, 700), (20000, 65), (65537, 3)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,v", MANY)
+def test_many_rows(cuda, dtype, rows, v):
+    """Every kind of row among ordinary ones: constant, rising, falling, few left, none left, two values, low masks."""
+    x, t = make(rows, v, dtype)
+    x[0::97] = 0.0
+    x[1::97] = torch.linspace(-30, 30, v, device="cuda").to(dtype)
+    x[2::97] = torch.linspace(30, -30, v, device="cuda").to(dtype)
+    x[3::97, 2:] = -INF
+    x[4::97] = -INF
+    x[5::97] = (torch.arange(v, device="cuda") % 7 == 0).to(dtype)
+    x[6::97, 1:] = torch.finfo(dtype).min
+    x[7::97, v // 2:] = 40.0
+    x[8::97, -1] = 50.0
+    x[9::97, v // 3] = math.nan
+    top = min(v, 32)
+    for k in (top, min(v, 5)):
+        got = forward(x, t, k)
+        q, lse, h = oracle(x, where="cuda")
+        tl = tol_sum(32 * v)  # one warp: 8 times the additions of a block, and the lanes' halves
+        picked = q.gather(1, t[:, None])[:, 0]
+        size = 4 * U * (picked.abs().nan_to_num(0.0, posinf=0.0) + lse.abs().nan_to_num(0.0, posinf=0.0) + 1)
+        close(got["logp"], picked, tl + size)
+        close(got["lse"], lse, tl + size)
+        close(got["entropy"], h, 3 * tl * (1 + math.log(v + 1)))
+        order = ranks(x, k, where="cuda")
+        assert torch.equal(got["top_index"], order)
+        best = q.gather(1, order)
+        close(got["top_logp"], best, tl + 4 * U * (best.abs().nan_to_num(0.0, posinf=0.0) + 1))
+
+
+def test_many_rows_gradient(cuda):
+    """Rows of many chunks and rows of a part of one, in one launch of more than 2^16 warps."""
+    from alpaka3_b200 import algo
+    for rows, v, dtype in ((20011, 65, torch.bfloat16), (3000, 4099, torch.float32)):
+        x, t = make(rows, v, dtype)
+        f = forward(x, t)
+        g = torch.randn(rows, device="cuda")
+        res = torch.empty_like(x)
+        algo.token_logprobs_backward(res, x, t, f["lse"], grad_logp=g)
+        p = torch.exp(x.double() - f["lse"].double()[:, None])
+        want = -g.double()[:, None] * p
+        want.scatter_add_(1, t[:, None], g.double()[:, None])
+        tol = g.abs().double()[:, None] * p * 2.0**-19 + want.abs() * torch.finfo(dtype).eps / 2 + g.abs()[:, None] * 2 * U
+        assert ((res.double() - want).abs() <= tol).all()
 
 
 def test_repeated_calls_give_the_same_bits(cuda):
