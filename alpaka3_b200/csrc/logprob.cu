@@ -47,6 +47,7 @@ namespace a3b
             uint32_t vocab;
             uint32_t top;
             float scale;
+            float reach; // 256 / (scale / ln 2): logits this far below the largest one do not count
             int index64; // targets and topIndex hold 64-bit (else 32-bit) integers
             void const* targets;
             float* logp;
@@ -124,21 +125,52 @@ namespace a3b
         constexpr int kBlock = 256;
         constexpr int kMaxCluster = 8;
 
-        // A row's team is W warps: a block, or (W = 1) one warp of a block of kBlock threads.
-        template<int W>
-        __device__ __forceinline__ void teamSync()
+        // A row's team is S threads: a block (S = 64, 128, 256), a warp or a quarter of one in a block of kBlock.
+        template<int S>
+        struct Team
         {
-            if constexpr(W == 1)
-                __syncwarp();
-            else
-                __syncthreads();
-        }
+            static constexpr int warps = S > 32 ? S / 32 : 1;
+            static constexpr int perBlock = S > 32 ? 1 : kBlock / S;
+            static constexpr int block = S > 32 ? S : kBlock;
+            static constexpr int width = S < 32 ? S : 32; // threads of the team in one warp
 
-        template<int W>
-        __device__ __forceinline__ unsigned teamThread()
-        {
-            return W == 1 ? threadIdx.x & 31u : threadIdx.x;
-        }
+            static __device__ __forceinline__ unsigned thread()
+            {
+                return threadIdx.x & (S - 1);
+            }
+            // the team's part of this warp
+            static __device__ __forceinline__ unsigned mask()
+            {
+                return S >= 32 ? kFullMask : ((1u << (S & 31)) - 1u) << (threadIdx.x & 31u & ~(S - 1u));
+            }
+            static __device__ __forceinline__ void sync()
+            {
+                if constexpr(S > 32)
+                    __syncthreads();
+                else
+                    __syncwarp(mask());
+            }
+            // the largest value of the team's part of this warp (NaN if there is one)
+            static __device__ __forceinline__ float max(float v)
+            {
+                if constexpr(S >= 32)
+                    return warpMaxNan(v);
+                else
+                {
+#pragma unroll
+                    for(int m = width / 2; m > 0; m >>= 1)
+                        v = maxNan(v, __shfl_xor_sync(mask(), v, m));
+                    return v;
+                }
+            }
+            static __device__ __forceinline__ float sum(float v)
+            {
+#pragma unroll
+                for(int m = width / 2; m > 0; m >>= 1)
+                    v += __shfl_xor_sync(mask(), v, m);
+                return v;
+            }
+        };
 
         // A row: `head` elements up to the first 16-byte boundary, `packs` 16-byte packs, `tail` elements behind them.
         template<typename T>
@@ -158,17 +190,17 @@ namespace a3b
 
         // A tile of a row: P packs of every thread of the team, pack p of thread t being pack base + p * team + t of the
         // row.
-        template<typename T, int W, int P>
+        template<typename T, int S, int P>
         struct Tile
         {
             static constexpr int E = PackOf<T>::E;
-            static constexpr uint32_t team = W * 32;
+            static constexpr uint32_t team = S;
             unsigned q[P][4];
 
             // packs outside [.., end) read as -infinity
             __device__ __forceinline__ void load(Row<T> const& row, uint32_t base, uint32_t end)
             {
-                auto const* const from = reinterpret_cast<uint4 const*>(row.p + row.head) + base + teamThread<W>();
+                auto const* const from = reinterpret_cast<uint4 const*>(row.p + row.head) + base + Team<S>::thread();
                 unsigned const n = PackOf<T>::negInfWord();
                 if(base + P * team <= end)
                 {
@@ -185,7 +217,7 @@ namespace a3b
                     for(int p = 0; p < P; ++p)
                     {
                         uint4 v = make_uint4(n, n, n, n);
-                        if(base + p * team + teamThread<W>() < end)
+                        if(base + p * team + Team<S>::thread() < end)
                             v = __ldcs(from + p * team);
                         q[p][0] = v.x, q[p][1] = v.y, q[p][2] = v.z, q[p][3] = v.w;
                     }
@@ -237,15 +269,15 @@ namespace a3b
 
         // Candidates for a row's `top` largest elements. Two buffers take turns: one starts with the keys kept so far, in
         // order, and collects more; ranking them writes the new kept ones to the start of the other.
-        template<int W>
+        template<int S>
         struct Select
         {
             // the kept keys and one element of each thread always fit
-            static constexpr unsigned room = W * 32 + 2 * kMaxTop;
+            static constexpr unsigned room = S + 2 * kMaxTop;
             unsigned long long keys[2][room];
             unsigned long long kth; // the last of `top` kept keys
             unsigned count[2];
-            unsigned bound[W];
+            unsigned bound[Team<S>::warps];
 
             __device__ __forceinline__ void push(unsigned buffer, unsigned order, uint32_t index)
             {
@@ -258,8 +290,8 @@ namespace a3b
             // distinct) and keeps the `top` best in the other one.
             __device__ __forceinline__ void rank(unsigned buffer, unsigned m, unsigned top)
             {
-                unsigned const thread = teamThread<W>();
-                for(unsigned i = thread; i < m; i += W * 32)
+                unsigned const thread = Team<S>::thread();
+                for(unsigned i = thread; i < m; i += S)
                 {
                     unsigned long long const key = keys[buffer][i];
                     unsigned const above = countAbove(keys[buffer], m, key);
@@ -279,26 +311,26 @@ namespace a3b
                 return kept == top ? static_cast<unsigned>(kth >> 32) + 1u : kOrderNegInf + 1u;
             }
 
-            // Every warp's need-th largest thread maximum, need = ceil(top / W), is reached by `need` elements of that
+            // Every warp's need-th largest thread maximum, need = ceil(top / warps), is reached by `need` elements of that
             // warp; so at least `top` elements of the tile reach the smallest of these bounds, and no element below it
             // can be among the `top` largest. For logits in no particular order a few dozen elements of a tile pass.
             __device__ __forceinline__ unsigned boundOf(unsigned mine, unsigned top)
             {
                 int const lane = threadIdx.x & 31;
                 unsigned least = 0, left = mine;
-                for(unsigned i = 0; i < (top + W - 1) / W; ++i)
+                for(unsigned i = 0; i < (top + Team<S>::warps - 1) / Team<S>::warps; ++i)
                 {
-                    least = __reduce_max_sync(kFullMask, left);
-                    if(lane == __ffs(static_cast<int>(__ballot_sync(kFullMask, left == least))) - 1)
+                    least = __reduce_max_sync(Team<S>::mask(), left);
+                    if(lane == __ffs(static_cast<int>(__ballot_sync(Team<S>::mask(), left == least))) - 1)
                         left = 0u;
                 }
-                if(W > 1 && lane == 0)
+                if(S > 32 && lane == 0)
                     bound[threadIdx.x >> 5] = least;
-                teamSync<W>();
-                if constexpr(W > 1)
+                Team<S>::sync();
+                if constexpr(S > 32)
                 {
 #pragma unroll
-                    for(int w = 0; w < W; ++w)
+                    for(int w = 0; w < Team<S>::warps; ++w)
                         least = min(least, bound[w]);
                 }
                 return max(least, kOrderNegInf + 1u);
@@ -309,10 +341,10 @@ namespace a3b
             // is short (a search unrolled over all packs did not fit the instruction cache).
             template<typename T, int P>
             __device__ __forceinline__ void collect(
-                Tile<T, W, P> const& t, unsigned least, unsigned mine, uint32_t head, uint32_t base, unsigned buffer)
+                Tile<T, S, P> const& t, unsigned least, unsigned mine, uint32_t head, uint32_t base, unsigned buffer)
             {
                 bool const has = mine >= least && least != 0u;
-                if(!__any_sync(kFullMask, has))
+                if(!__any_sync(Team<S>::mask(), has))
                     return;
                 float const value = valueOf(least); // NaN where `least` is: then every pack is looked at
                 unsigned packs = 0;
@@ -331,7 +363,7 @@ namespace a3b
                         for(int w = 0; w < 4; ++w)
                             word[w] = i == p ? t.q[i][w] : word[w];
                     uint32_t const index
-                        = head + (base + p * Tile<T, W, P>::team + teamThread<W>()) * Tile<T, W, P>::E;
+                        = head + (base + p * Tile<T, S, P>::team + Team<S>::thread()) * Tile<T, S, P>::E;
 #pragma unroll
                     for(int w = 0; w < PackOf<T>::pairs; ++w)
                     {
@@ -348,7 +380,7 @@ namespace a3b
                             consider(v.y, index + 2 * w + 1);
                     }
                 }
-                __syncwarp();
+                __syncwarp(Team<S>::mask());
             }
 
             // The same selection for the elements [first, last) of a row, whatever they are, in steps that always fit: an
@@ -360,8 +392,8 @@ namespace a3b
                 T const* row, uint32_t first, uint32_t last, unsigned top, unsigned kept, unsigned buffer)
             {
                 constexpr unsigned per = 8;
-                unsigned const thread = teamThread<W>();
-                for(uint32_t base = first; base < last; base += W * 32 * per)
+                unsigned const thread = Team<S>::thread();
+                for(uint32_t base = first; base < last; base += S * per)
                 {
                     unsigned order[per];
                     bool any = false;
@@ -369,13 +401,13 @@ namespace a3b
 #pragma unroll
                     for(unsigned k = 0; k < per; ++k)
                     {
-                        uint32_t const i = base + k * W * 32 + thread;
+                        uint32_t const i = base + k * S + thread;
                         order[k] = i < last ? orderOf(toFloat(row[i])) : 0u;
                         any |= order[k] >= least && least != 0u;
                     }
                     bool some;
-                    if constexpr(W == 1)
-                        some = __any_sync(kFullMask, any);
+                    if constexpr(S <= 32)
+                        some = __any_sync(Team<S>::mask(), any);
                     else
                         some = __syncthreads_or(any);
                     if(!some)
@@ -388,8 +420,8 @@ namespace a3b
                             o = j == k ? order[j] : o;
                         unsigned const enters = from(kept, top);
                         if(o >= enters && enters != 0u)
-                            push(buffer, o, base + k * W * 32 + thread);
-                        teamSync<W>();
+                            push(buffer, o, base + k * S + thread);
+                        Team<S>::sync();
                         unsigned const n = count[buffer];
                         if(n > kept)
                         {
@@ -397,31 +429,32 @@ namespace a3b
                             kept = min(n, top);
                             buffer ^= 1u;
                         }
-                        teamSync<W>();
+                        Team<S>::sync();
                     }
                 }
                 return make_uint2(kept, buffer);
             }
         };
 
-        // Fills `kept` up to `top` keys with the row's first elements of -infinity, by one warp. All others are among the
-        // kept ones, so the first 2 top elements of the row hold enough of them.
-        template<typename T>
+        // Fills `kept` up to `top` keys with the row's first elements of -infinity, by the team's (first) warp. All others
+        // are among the kept ones, so the first 2 top elements of the row hold enough of them.
+        template<int S, typename T>
         __device__ __forceinline__ void fillWithNegInf(
             T const* row, uint32_t vocab, unsigned top, unsigned kept, unsigned long long* keys)
         {
-            unsigned const lane = threadIdx.x & 31u;
-            for(uint32_t i0 = 0; kept < top && i0 < vocab; i0 += 32)
+            constexpr uint32_t width = Team<S>::width;
+            unsigned const lane = threadIdx.x & (width - 1u), below = (1u << (threadIdx.x & 31u)) - 1u;
+            for(uint32_t i0 = 0; kept < top && i0 < vocab; i0 += width)
             {
                 uint32_t const i = i0 + lane;
                 bool const hit = i < vocab && toFloat(row[i]) == -INFINITY;
-                unsigned const hits = __ballot_sync(kFullMask, hit);
-                unsigned const at = kept + __popc(hits & ((1u << lane) - 1u));
+                unsigned const hits = __ballot_sync(Team<S>::mask(), hit);
+                unsigned const at = kept + __popc(hits & below);
                 if(hit && at < top)
                     keys[at] = keyOf(kOrderNegInf, i);
                 kept = min(top, kept + __popc(hits));
             }
-            __syncwarp();
+            __syncwarp(Team<S>::mask());
         }
 
         // What the blocks of a cluster leave in the first one's shared memory.
@@ -433,28 +466,28 @@ namespace a3b
         };
 
         // Blocks of kBlock threads an SM that the registers are bounded to. Measured on a B200 with 3 / 4 for the
-        // alternatives: 32768 x 257 fp16 34 / 30 us (two packs a thread), but 64 x 131072 fp32 15 / 17 us (eight: spills).
+        // alternatives: 32768 x 257 fp16 20 / 18 us (four packs a thread), but 64 x 131072 fp32 15 / 17 us (eight: spills).
         template<int P, bool TOP>
         constexpr int residentBlocks()
         {
-            return P == 2 ? (TOP ? 4 : 6) : (TOP ? 3 : 4);
+            return P == 2 ? (TOP ? 4 : 6) : P == 4 ? 4 : (TOP ? 3 : 4);
         }
 
-        // W > 1: the team is a block of W warps; in a launch with clusters, slice b of a row is the tiles of the cluster's
-        // block b, and the first block joins the slices. W = 1: warp w of block b takes row kBlock / 32 * b + w.
-        template<typename T, int W, int P, bool TOP, bool ENT>
-        __global__ void __launch_bounds__(W == 1 ? kBlock : W * 32, (W == 1 ? 1 : 8 / W) * residentBlocks<P, TOP>())
+        // One row a team. In a launch with clusters, slice b of a row is the tiles of the cluster's block b, and the first
+        // block joins the slices.
+        template<typename T, int S, int P, bool TOP, bool ENT>
+        __global__ void __launch_bounds__(Team<S>::block, kBlock / Team<S>::block * residentBlocks<P, TOP>())
             logprobKernel(LogprobArgs a)
         {
-            constexpr int teams = W == 1 ? kBlock / 32 : 1;
-            __shared__ Stats stats[W];
-            __shared__ Select<W> select[TOP ? teams : 1];
+            constexpr int teams = Team<S>::perBlock;
+            __shared__ Stats stats[Team<S>::warps];
+            __shared__ Select<S> select[TOP ? teams : 1];
             __shared__ Gather<TOP> gather;
-            Select<W>& sel = select[TOP && W == 1 ? threadIdx.x >> 5 : 0];
-            unsigned const thread = teamThread<W>();
+            Select<S>& sel = select[TOP && S <= 32 ? threadIdx.x / S : 0];
+            unsigned const thread = Team<S>::thread();
             unsigned slice = 0, slices = 1;
-            uint64_t r = W == 1 ? static_cast<uint64_t>(blockIdx.x) * teams + (threadIdx.x >> 5) : blockIdx.x;
-            if constexpr(W > 1)
+            uint64_t r = S <= 32 ? static_cast<uint64_t>(blockIdx.x) * teams + threadIdx.x / S : blockIdx.x;
+            if constexpr(S > 32)
             {
                 slices = clusterBlocks();
                 if(slices > 1)
@@ -468,15 +501,14 @@ namespace a3b
                 return;
             Row<T> const row(a, r);
             float const c = a.scale * kLog2e;
-            uint32_t const span = P * W * 32; // packs of a tile
+            uint32_t const span = P * S; // packs of a tile
             uint32_t const firstTile = slice * a.tiles;
             int64_t const target = a.logp ? loadIndex(a.targets, r, a.index64) : -1;
-            // What lies outside the packs, one element a lane of the first warp: the head is taken with the first tile,
-            // in front of it, the tail with the last one.
-            uint32_t const aside = thread < 16 ? (thread < 8 ? thread : a.vocab - row.tail + thread - 8) : 0;
-            bool const inHead = thread < row.head && slice == 0;
-            bool const inTail = thread >= 8 && thread < 8 + row.tail && slice == slices - 1;
-            float const asideValue = inHead || inTail ? toFloat(row.p[aside]) : -INFINITY;
+            // What lies outside the packs, one element each of the first eight threads: the head is taken with the first
+            // tile, in front of it, the tail with the last one.
+            float const inHead = thread < row.head && slice == 0 ? toFloat(row.p[thread]) : -INFINITY;
+            uint32_t const tailIndex = a.vocab - row.tail + thread;
+            float const inTail = thread < row.tail && slice == slices - 1 ? toFloat(row.p[tailIndex]) : -INFINITY;
             float xt = 0.0f;
 
             float high = -INFINITY, factor = c, offset = 0.0f;
@@ -486,7 +518,7 @@ namespace a3b
             uint32_t ranked = 0, rankAfter = 1; // tiles whose candidates have been ranked, or will be next
             if(TOP && thread == 0)
                 sel.count[0] = 0u;
-            Tile<T, W, P> t;
+            Tile<T, S, P> t;
             t.load(row, firstTile * span, row.packs);
             if(target >= 0 && target < static_cast<int64_t>(a.vocab))
                 xt = toFloat(row.p[target]);
@@ -494,11 +526,11 @@ namespace a3b
             {
                 uint32_t const base = (firstTile + tile) * span;
                 bool const last = tile + 1 == a.tiles;
-                float const more = (inHead && tile == 0) || (inTail && last) ? asideValue : -INFINITY;
-                float const threadMax = maxNan(more, PackOf<T>::template max<P>(t.q));
+                float const front = tile == 0 ? inHead : -INFINITY, behind = last ? inTail : -INFINITY;
+                float const threadMax = maxNan(maxNan(front, behind), PackOf<T>::template max<P>(t.q));
                 t.fence();
                 // the warp's running maximum, and its sums moved there
-                float const to = maxNan(high, warpMaxNan(threadMax));
+                float const to = maxNan(high, Team<S>::max(threadMax));
                 if(tile == 0 || to != high)
                 {
                     if(tile > 0)
@@ -511,7 +543,7 @@ namespace a3b
                     factor = factorOf(high, c);
                     offset = offsetOf(high, c);
                     // far below what counts (t < -200), for logits of -infinity: see below
-                    low = PackOf<T>::twice(high - fmaf(fabsf(high), 0x1p-6f, 256.0f / c));
+                    low = PackOf<T>::twice(high - fmaf(fabsf(high), 0x1p-6f, a.reach));
                 }
                 if constexpr(TOP)
                 {
@@ -520,8 +552,13 @@ namespace a3b
                     unsigned const mine = orderOf(threadMax);
                     unsigned const least = tile == 0 ? sel.boundOf(mine, a.top) : sel.from(kept, a.top);
                     sel.collect(t, least, mine, row.head, base, buffer);
-                    if(orderOf(more) >= least && least != 0u)
-                        sel.push(buffer, orderOf(more), aside);
+                    if((tile == 0 || last) && least != 0u)
+                    {
+                        if(orderOf(front) >= least)
+                            sel.push(buffer, orderOf(front), thread);
+                        if(orderOf(behind) >= least)
+                            sel.push(buffer, orderOf(behind), tailIndex);
+                    }
                     t.fence();
                 }
                 float2 const offset2 = make_float2(offset, offset), factor2 = make_float2(factor, factor);
@@ -547,7 +584,7 @@ namespace a3b
                 for(int p = 0; p < P; ++p)
                 {
                     // a short tile's packs in the second half: none, for the whole team
-                    if(p == P / 2 && base + p * W * 32 >= row.packs)
+                    if(p == P / 2 && base + p * S >= row.packs)
                         break;
 #pragma unroll
                     for(int w = 0; w < PackOf<T>::pairs; ++w)
@@ -558,12 +595,12 @@ namespace a3b
                             word[w] = PackOf<T>::maxWord(word[w], low);
                         add(PackOf<T>::pair(word, w));
                     }
-                    t.reload(p, next + p * W * 32, nextFull);
+                    t.reload(p, next + p * S, nextFull);
                 }
-                if((tile == 0 || last) && (W == 1 || threadIdx.x < 32))
+                if((tile == 0 || last) && (S <= 32 || threadIdx.x < 32))
                 {
-                    float const least = high - fmaf(fabsf(high), 0x1p-6f, 256.0f / c);
-                    add(make_float2(maxNan(more, least), least));
+                    float const least = high - fmaf(fabsf(high), 0x1p-6f, a.reach);
+                    add(make_float2(maxNan(front, least), maxNan(behind, least)));
                 }
                 if(!last && !nextFull)
                     t.load(row, base + span, row.packs);
@@ -571,14 +608,14 @@ namespace a3b
                 {
                     if(last || tile + 1 == rankAfter)
                     {
-                        teamSync<W>();
+                        Team<S>::sync();
                         unsigned const n = sel.count[buffer];
                         if(n > sel.room)
                         {
-                            teamSync<W>(); // every thread has read the count
+                            Team<S>::sync(); // every thread has read the count
                             if(thread == 0)
                                 sel.count[buffer] = kept;
-                            teamSync<W>();
+                            Team<S>::sync();
                             uint32_t const perTile = span * PackOf<T>::E;
                             uint32_t const from = ranked == 0 && slice == 0 ? 0 : row.head + (firstTile + ranked) * perTile;
                             uint64_t const upTo = row.head + static_cast<uint64_t>(firstTile + tile + 1) * perTile;
@@ -598,7 +635,7 @@ namespace a3b
                                 kept = min(n, a.top);
                                 buffer ^= 1u;
                             }
-                            teamSync<W>(); // ranked, and every thread has read the count before anyone collects more
+                            Team<S>::sync(); // ranked, and every thread has read the count before anyone collects more
                         }
                         ranked = tile + 1;
                         // Between ranking at n tiles and at k n about (k - 1) top elements pass: k = 4 as long as they fit
@@ -607,16 +644,9 @@ namespace a3b
                     }
                 }
             }
-            float s = s2.x + s2.y, u = u2.x + u2.y;
-#pragma unroll
-            for(int m = 16; m > 0; m >>= 1)
-            {
-                s += __shfl_xor_sync(kFullMask, s, m);
-                if constexpr(ENT)
-                    u += __shfl_xor_sync(kFullMask, u, m);
-            }
+            float s = Team<S>::sum(s2.x + s2.y), u = ENT ? Team<S>::sum(u2.x + u2.y) : 0.0f;
             unsigned long long* const best = sel.keys[buffer];
-            if constexpr(W > 1)
+            if constexpr(S > 32)
             {
                 if((threadIdx.x & 31) == 0)
                     stats[threadIdx.x >> 5] = Stats{high, s, u};
@@ -640,8 +670,8 @@ namespace a3b
                     s = __shfl_sync(kFullMask, s, 0);
                     u = __shfl_sync(kFullMask, u, 0);
                 };
-                static_assert(W <= 8 && kMaxCluster <= 8, "join() sums eight lanes");
-                join(stats, W);
+                static_assert(Team<S>::warps <= 8 && kMaxCluster <= 8, "join() sums eight lanes");
+                join(stats, Team<S>::warps);
                 if(slices > 1)
                 {
                     clusterWait();
@@ -693,7 +723,7 @@ namespace a3b
             }
             if constexpr(TOP)
             {
-                fillWithNegInf(row.p, a.vocab, a.top, kept, best);
+                fillWithNegInf<S>(row.p, a.vocab, a.top, kept, best);
                 if(thread < a.top)
                 {
                     unsigned long long const key = best[thread];
@@ -708,65 +738,75 @@ namespace a3b
             }
         }
 
-        template<typename T, int W, int P, bool TOP, bool ENT>
+        template<typename T, int S, int P, bool TOP, bool ENT>
         int launchRows(cudaStream_t stream, unsigned cluster, LogprobArgs const& a)
         {
-            uint64_t const teams = W == 1 ? kBlock / 32 : 1;
+            uint64_t const teams = Team<S>::perBlock;
             cudaLaunchAttribute attr[1];
             attr[0].id = cudaLaunchAttributeClusterDimension;
             attr[0].val.clusterDim.x = cluster;
             attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
             cudaLaunchConfig_t cfg = {};
             cfg.gridDim = dim3(static_cast<unsigned>((a.rows + teams - 1) / teams) * cluster);
-            cfg.blockDim = dim3(W == 1 ? kBlock : W * 32);
+            cfg.blockDim = dim3(Team<S>::block);
             cfg.stream = stream;
             cfg.attrs = attr;
             cfg.numAttrs = cluster > 1 ? 1 : 0;
-            A3B_CUDA(cudaLaunchKernelEx(&cfg, logprobKernel<T, W, P, TOP, ENT>, a));
+            A3B_CUDA(cudaLaunchKernelEx(&cfg, logprobKernel<T, S, P, TOP, ENT>, a));
             return A3B_OK;
         }
 
-        // The team of a row. Warps that need no barrier are best as long as there are enough of them: W is the smallest
-        // that makes kEnoughWarps of all rows, but not more than a row fills with one tile. Measured on a B200, bf16,
-        // W = 1 / 2 / 4 / 8 in microseconds: 8192 rows of 8192 logits 26 / 28 / 30 / 42; 4096 x 16384 28 / 27 / 28 / 30;
-        // 2048 x 50257 46 / 40 / 40 / 43, with 20 alternatives 87 / 77 / 72 / 80. Rows of up to 64 packs take tiles of
-        // two packs a thread, whose kernel has fewer registers and more warps: 32768 x 257 with 2 alternatives 34
-        // against 42. Few long rows are cut into slices over a cluster, as many as the GPU holds at once (a second
-        // wave costs more than a slice gains): 1 / 2 / 4 / 8 slices of 16 rows of 131072 with 20 alternatives
-        // 20 / 15 / 11 / 10, of 64 fp32 rows with 5 28 / 19 / 15 / 19.
+        // The team of a row. Warps that need no barrier are best as long as there are enough of them: it has the fewest
+        // warps that make kEnoughWarps of all rows, but not more than a row fills with one tile. Measured on a B200,
+        // bf16, 1 / 2 / 4 / 8 warps, in microseconds: 8192 rows of 8192 logits 26 / 28 / 30 / 42; 4096 x 16384
+        // 28 / 27 / 28 / 30; 2048 x 50257 46 / 40 / 40 / 43, with 20 alternatives 87 / 77 / 72 / 80.
+        // Short rows in great number take a quarter or half of a warp, which spreads what a row costs besides its logits
+        // over four or two rows (32768 rows of 257 fp16 with 2 alternatives 18 us, one warp each 31; 500 fp16 24 / 33;
+        // 1000 bf16 with 3 38 / 49; but 100 rows of 500 6.9 / 4.2). More alternatives than half the team's threads are
+        // badly bounded by its thread maxima. Other rows of up to 64 packs take tiles of two packs a thread, whose kernel
+        // has fewer registers (16 / 18 us for 32768 x 257).
+        // Few long rows are cut into slices over a cluster, as many as the GPU holds at once (a second wave costs more
+        // than a slice gains): 1 / 2 / 4 / 8 slices of 16 rows of 131072 with 20 alternatives 20 / 15 / 11 / 10, of 64
+        // fp32 rows with 5 28 / 19 / 15 / 19.
         constexpr uint64_t kEnoughWarps = 8192;
 
         template<typename T>
         int launchLogprob(cudaStream_t stream, DeviceProps const* props, LogprobArgs a)
         {
             uint64_t const packs = a.vocab / PackOf<T>::E;
-            auto go = [&](auto w, auto p, unsigned cluster)
+            auto go = [&](auto size, auto p, unsigned cluster)
             {
-                constexpr int W = decltype(w)::value, P = decltype(p)::value;
-                uint64_t const tiles = (packs + uint64_t{W} * 32 * P * cluster - 1) / (uint64_t{W} * 32 * P * cluster);
-                a.tiles = static_cast<uint32_t>(std::max<uint64_t>(tiles, 1));
+                constexpr int S = decltype(size)::value, P = decltype(p)::value;
+                uint64_t const tile = uint64_t{S} * P * cluster;
+                a.tiles = static_cast<uint32_t>(std::max<uint64_t>((packs + tile - 1) / tile, 1));
                 if(a.top > 0)
-                    return a.entropy ? launchRows<T, W, P, true, true>(stream, cluster, a)
-                                     : launchRows<T, W, P, true, false>(stream, cluster, a);
-                return a.entropy ? launchRows<T, W, P, false, true>(stream, cluster, a)
-                                 : launchRows<T, W, P, false, false>(stream, cluster, a);
+                    return a.entropy ? launchRows<T, S, P, true, true>(stream, cluster, a)
+                                     : launchRows<T, S, P, true, false>(stream, cluster, a);
+                return a.entropy ? launchRows<T, S, P, false, true>(stream, cluster, a)
+                                 : launchRows<T, S, P, false, false>(stream, cluster, a);
             };
             using std::integral_constant;
             constexpr integral_constant<int, kPacks> full;
             uint64_t const oneTile = 32 * kPacks; // packs of a warp's tile
+            if(a.rows >= kEnoughWarps && packs <= 128 && a.top <= (packs <= 64 ? 4u : 8u))
+            {
+                if(packs <= 32)
+                    return go(integral_constant<int, 8>{}, integral_constant<int, 4>{}, 1u);
+                return packs <= 64 ? go(integral_constant<int, 8>{}, full, 1u) : go(integral_constant<int, 16>{}, full, 1u);
+            }
             if(packs <= 64)
-                return go(integral_constant<int, 1>{}, integral_constant<int, 2>{}, 1u);
+                return go(integral_constant<int, 32>{}, integral_constant<int, 2>{}, 1u);
             if(a.rows >= kEnoughWarps || packs <= oneTile)
-                return go(integral_constant<int, 1>{}, full, 1u);
+                return go(integral_constant<int, 32>{}, full, 1u);
             if(a.rows >= kEnoughWarps / 2 || packs <= 2 * oneTile)
-                return go(integral_constant<int, 2>{}, full, 1u);
+                return go(integral_constant<int, 64>{}, full, 1u);
             if(a.rows >= kEnoughWarps / 4 || packs <= 4 * oneTile)
-                return go(integral_constant<int, 4>{}, full, 1u);
+                return go(integral_constant<int, 128>{}, full, 1u);
             uint64_t const held = static_cast<uint64_t>(props->smCount) * 3; // blocks
             unsigned cluster = 1;
             while(cluster < kMaxCluster && a.rows * cluster * 2 <= held && packs > cluster * 8 * oneTile)
                 cluster *= 2;
-            return go(integral_constant<int, 8>{}, full, cluster);
+            return go(integral_constant<int, 256>{}, full, cluster);
         }
 
         // ------------------------------------------------------------------------------------------- gradient
@@ -1018,8 +1058,8 @@ extern "C"
         int const rd = currentDevice(&props);
         if(rd != A3B_OK)
             return rd;
-        LogprobArgs a{logits, {static_cast<uint32_t>(inner), outer_stride, inner_stride}, rows, 1u, static_cast<uint32_t>(vocab), top, static_cast<float>(scale), index_dtype == A3B_I64,
-                      targets, logp, entropy, lse, top_logp, top_index};
+        LogprobArgs a{logits, {static_cast<uint32_t>(inner), outer_stride, inner_stride}, rows, 1u, static_cast<uint32_t>(vocab), top, static_cast<float>(scale),
+                      static_cast<float>(256.0 / (scale * 1.4426950408889634074)), index_dtype == A3B_I64, targets, logp, entropy, lse, top_logp, top_index};
         auto s = static_cast<cudaStream_t>(stream);
         if(dtype == A3B_F32)
             return launchLogprob<float>(s, props, a);

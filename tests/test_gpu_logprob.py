@@ -222,8 +222,9 @@ def test_rows_do_not_touch_neighbours(cuda):
     assert (outs.reshape(-1)[9:] == 9).all() and (outs.reshape(-1)[:3] == 9).all()
 
 
-# many rows: a warp a row with several tiles, two and four warps a row, and rows that leave the last tile nearly empty
-MANY = [(8192, 5003), (8200, 2060), (4100, 9001), (2048, 17011), (2051, 33000), (8192, 700), (20000, 65), (65537, 3)]
+# many rows: a quarter, half or whole warp a row, a warp with several tiles, two and four warps, last tiles nearly empty
+MANY = [(8192, 5003), (8200, 2060), (4100, 9001), (2048, 17011), (2051, 33000), (8192, 700), (8192, 1031),
+        (20000, 65), (9001, 130), (8193, 262), (9000, 300), (8300, 517), (65537, 3)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -242,7 +243,7 @@ def test_many_rows(cuda, dtype, rows, v):
     x[8::97, -1] = 50.0
     x[9::97, v // 3] = math.nan
     top = min(v, 32)
-    for k in (top, min(v, 5)):
+    for k in (top, min(v, 8), min(v, 4)):
         got = forward(x, t, k)
         q, lse, h = oracle(x, where="cuda")
         tl = tol_sum(32 * v)  # one warp: 8 times the additions of a block, and the lanes' halves
