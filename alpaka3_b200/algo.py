@@ -23,6 +23,7 @@ Reductions of a language model's training and decoding steps, which alpaka3 does
 Errors raise :class:`alpaka3_b200.capi.A3BError` (the reference throws std::runtime_error on backend errors).
 """
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -216,18 +217,31 @@ def exclusive_scan_in_place(data, buffer=None, stream=None):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the address alone, without a Stream object
 
 
+@functools.cache
+def _entry(name):
+    return getattr(capi.lib(), name)
+
+
+@functools.cache
+def _one_device():
+    return torch.cuda.device_count() == 1
+
+
 def _call_on(index, stream, name, *args):
-    """capi.call on `stream` (default: the current stream of device `index`) with that device current."""
+    """Entry point `name` on `stream` (default: the current stream of device `index`) with that device current."""
     if stream is None:
         handle = _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream
     elif stream.device_index != index:
         raise ValueError(f"the stream belongs to device {stream.device_index}, the tensors to device {index}")
     else:
         handle = stream.cuda_stream
-    if torch.cuda.current_device() == index:
-        return capi.call(name, handle, *args)
-    with torch.cuda.device(index):
-        return capi.call(name, handle, *args)
+    if _one_device() or torch.cuda.current_device() == index:
+        rc = _entry(name)(handle, *args)
+    else:
+        with torch.cuda.device(index):
+            rc = _entry(name)(handle, *args)
+    if rc:
+        capi.check(rc, name)
 
 
 def _rows(t, name):
