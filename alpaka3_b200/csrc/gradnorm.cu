@@ -8,7 +8,7 @@
 //   * normKernel: resident blocks, each folds a run of consecutive chunks into one fp64 partial in the workspace
 //     (7.1 TB/s on a B200 over 2.1 GB);
 //   * finishKernel: one block folds the partials in their order;
-//   * clipKernel: a block for every chunk, handed out in order (copies at 6.5 TB/s; resident blocks reached 5.9).
+//   * clipKernel: a block for every chunk, handed out in order (6.8 TB/s read and written; resident blocks reached 5.9).
 //     It and finishKernel are launched while the kernel before drains (programmatic dependent launch);
 //   * clipSmallKernel: both for a short list, one launch of one cluster.
 // The workspace holds nothing between calls (no tickets), and no block waits for another one's progress in memory:
@@ -523,11 +523,14 @@ namespace a3b
             return std::min<uint32_t>(b.chunks, static_cast<uint32_t>(props->smCount) * kBlocksPerSm);
         }
 
-        int checkCall(a3b_tensor_list const* list, int kind, int normDtype)
+        int checkCall(a3b_tensor_list const* list, int kind, double const* partial, int normDtype, void const* norm)
         {
             A3B_REQUIRE(list, "null tensor list");
             A3B_REQUIRE(kind == A3B_NORM_L2 || kind == A3B_NORM_L1 || kind == A3B_NORM_MAX, "unknown norm kind");
             A3B_REQUIRE(normDtype == A3B_F32 || normDtype == A3B_F64, "the norm is f32 or f64");
+            A3B_REQUIRE(reinterpret_cast<uintptr_t>(norm) % (normDtype == A3B_F64 ? 8u : 4u) == 0u
+                            && reinterpret_cast<uintptr_t>(partial) % 8u == 0u,
+                        "norm or partial is not aligned to its type");
             return A3B_OK;
         }
 
@@ -624,7 +627,7 @@ namespace a3b
 
         // Norm, then clipping. Lists of one wave of blocks: every block folds the partials. Longer ones: one block does, in
         // a launch of its own, and a block for every chunk reads the result (162 tensors, 2.1 GB of bf16 on a B200:
-        // 958 us; resident blocks that walk runs of chunks 1042).
+        // 938 us; resident blocks that walk runs of chunks 1042).
         template<int KIND>
         int launchBoth(
             cudaStream_t s,
@@ -771,7 +774,7 @@ extern "C"
         int norm_dtype,
         void* norm)
     {
-        int const rc = checkCall(list, kind, norm_dtype);
+        int const rc = checkCall(list, kind, partial, norm_dtype, norm);
         if(rc != A3B_OK)
             return rc;
         A3B_REQUIRE(partial || norm, "nothing to compute: no output is given");
@@ -799,7 +802,7 @@ extern "C"
         int norm_dtype,
         void* norm)
     {
-        int const rc = checkCall(list, kind, norm_dtype);
+        int const rc = checkCall(list, kind, partial, norm_dtype, norm);
         if(rc != A3B_OK)
             return rc;
         A3B_REQUIRE(partial, "null partial");
@@ -827,7 +830,7 @@ extern "C"
         int norm_dtype,
         void* norm)
     {
-        int const rc = checkCall(list, kind, norm_dtype);
+        int const rc = checkCall(list, kind, nullptr, norm_dtype, norm);
         if(rc != A3B_OK)
             return rc;
         A3B_REQUIRE(!list->notClippable, list->notClippable);

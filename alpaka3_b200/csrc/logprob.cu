@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <climits>
+#include <initializer_list>
 #include <type_traits>
 
 #include "rows.cuh"
@@ -836,8 +837,8 @@ namespace a3b
         // and lse / ln 2 leave is one number for a row (where p counts, x is near lse / scale): 2^ of it goes into a and b.
         //
         // One warp takes a chunk of kBackPacks packs a lane and needs no other: chunks are handed out in the order of
-        // memory. 40 registers, 6 blocks of 8 warps an SM (measured on a B200: 4096 x 131072 fp32 645 us, 2048 x 50257
-        // bf16 78 us; without the bound on registers 3 blocks and 744 / 148 us).
+        // memory. Measured on a B200: 4096 x 131072 fp32 643 us, 2048 x 50257 bf16 63 us, HBM-bound. The bound of 40
+        // registers (6 blocks of 8 warps an SM) is what took the second one from 148 to 78, the fused exponents the rest.
         constexpr int kBackPacks = 4;
 
         template<typename T>
@@ -1000,6 +1001,14 @@ namespace a3b
             return A3B_OK;
         }
 
+        bool alignedTo(uintptr_t size, std::initializer_list<void const*> pointers)
+        {
+            for(void const* p : pointers)
+                if(reinterpret_cast<uintptr_t>(p) % size != 0u)
+                    return false;
+            return true;
+        }
+
         // In 128 bits: strides come from the caller and may be anything.
         using Wide = __int128;
 
@@ -1054,12 +1063,17 @@ extern "C"
         A3B_REQUIRE(logp || entropy || lse || top > 0, "nothing to compute: no output is given");
         A3B_REQUIRE(!logp || targets, "log probabilities need targets");
         A3B_REQUIRE(top == 0 || (top_logp && top_index), "null output for the alternatives");
+        A3B_REQUIRE(alignedTo(4, {logp, entropy, lse, top_logp})
+                        && alignedTo(index_dtype == A3B_I64 ? 8 : 4, {targets, top_index}),
+                    "an array is not aligned to its type");
         DeviceProps const* props = nullptr;
         int const rd = currentDevice(&props);
         if(rd != A3B_OK)
             return rd;
-        LogprobArgs a{logits, {static_cast<uint32_t>(inner), outer_stride, inner_stride}, rows, 1u, static_cast<uint32_t>(vocab), top, static_cast<float>(scale),
-                      static_cast<float>(256.0 / (scale * 1.4426950408889634074)), index_dtype == A3B_I64, targets, logp, entropy, lse, top_logp, top_index};
+        LogprobArgs a{logits, {static_cast<uint32_t>(inner), outer_stride, inner_stride}, rows, 1u,
+                      static_cast<uint32_t>(vocab), top, static_cast<float>(scale),
+                      static_cast<float>(256.0 / (scale * 1.4426950408889634074)), index_dtype == A3B_I64, targets, logp,
+                      entropy, lse, top_logp, top_index};
         auto s = static_cast<cudaStream_t>(stream);
         if(dtype == A3B_F32)
             return launchLogprob<float>(s, props, a);
@@ -1098,6 +1112,9 @@ extern "C"
         A3B_REQUIRE(lse && grad_logits, "null lse or grad_logits");
         A3B_REQUIRE(!grad_logp || targets, "a gradient of the log probabilities needs targets");
         A3B_REQUIRE(!grad_entropy || entropy, "a gradient of the entropy needs the entropy");
+        A3B_REQUIRE(alignedTo(4, {lse, entropy, grad_logp, grad_entropy, grad_lse})
+                        && alignedTo(index_dtype == A3B_I64 ? 8 : 4, {targets}),
+                    "an array is not aligned to its type");
         int const es = dtype == A3B_F32 ? 4 : 2;
         A3B_REQUIRE((reinterpret_cast<uintptr_t>(grad_logits) & static_cast<uintptr_t>(es - 1)) == 0,
                     "grad_logits is not aligned to its type");

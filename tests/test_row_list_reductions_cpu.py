@@ -16,6 +16,7 @@ def L():
 
 
 P = ctypes.c_void_p(0x10000000)  # stands for a device address: nothing below may use it
+ODD = ctypes.c_void_p(0x10000001)
 
 
 def forward(L, **kw):
@@ -41,7 +42,9 @@ def test_forward_refusals(L):
                dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(scale=1e-60),
                dict(logits=None), dict(logits=ctypes.c_void_p(0x10000002)), dict(logp=None), dict(targets=None),
                dict(top=33, top_logp=P, top_index=P), dict(top=5), dict(top=5, top_logp=P),
-               dict(vocab=3, top=4, top_logp=P, top_index=P), dict(outer=1 << 63, inner=4)):
+               dict(vocab=3, top=4, top_logp=P, top_index=P), dict(outer=1 << 63, inner=4), dict(targets=ODD),
+               dict(logp=ODD), dict(entropy=ODD), dict(lse=ODD), dict(top=5, top_logp=ODD, top_index=P),
+               dict(top=5, top_logp=P, top_index=ODD), dict(index=capi.I32, targets=ctypes.c_void_p(0x10000002))):
         assert forward(L, **kw) == capi.ERR_INVALID, kw
         assert capi.last_error()
     for kw in (dict(vocab=(1 << 31) - 64), dict(inner=1 << 31), dict(outer=1 << 16, inner=1 << 16)):
@@ -55,7 +58,8 @@ def test_backward_refusals(L):
                dict(grad=ctypes.c_void_p(0x20000001)), dict(gsi=99), dict(gsi=0), dict(gsi=-50),
                dict(outer=3, gso=399, gsi=100), dict(outer=3, gso=0), dict(grad=ctypes.c_void_p(0x10000004)),
                dict(grad=P, gsi=101), dict(grad=ctypes.c_void_p(0x10000000 + 1596)),
-               dict(grad=ctypes.c_void_p(0x10000000 - 1596)), dict(si=1 << 62)):
+               dict(grad=ctypes.c_void_p(0x10000000 - 1596)), dict(si=1 << 62), dict(lse=ODD), dict(entropy=ODD),
+               dict(grad_logp=ODD), dict(grad_entropy=ODD, entropy=P), dict(grad_lse=ODD), dict(targets=ODD)):
         rc = backward(L, **kw)
         assert rc == capi.ERR_INVALID, (kw, rc)
     assert backward(L, inner=0) == capi.OK
@@ -89,6 +93,10 @@ def test_list_refusals(L):
     assert L.a3b_grad_norm(None, h, 0, None, 8, P, F, None) == capi.ERR_INVALID
     assert L.a3b_grad_norm(None, h, 0, ctypes.c_void_p(0x10004), 8, P, F, None) == capi.ERR_INVALID
     assert L.a3b_clip_grad_norm(None, h, 0, 1.0, None, 0, F, P) == capi.ERR_INVALID
+    assert L.a3b_clip_grad_norm(None, h, 0, 1.0, P, 64, F, ODD) == capi.ERR_INVALID
+    assert L.a3b_clip_grad_norm(None, h, 0, 1.0, P, 64, D, ctypes.c_void_p(0x10004)) == capi.ERR_INVALID
+    assert L.a3b_grad_norm(None, h, 0, P, 64, ctypes.c_void_p(0x10004), F, P) == capi.ERR_INVALID
+    assert L.a3b_clip_grads(None, h, 0, ctypes.c_void_p(0x10004), 1.0, F, P) == capi.ERR_INVALID
     assert L.a3b_tensor_list_destroy(h) == capi.OK
 
 
