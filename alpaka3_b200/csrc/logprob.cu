@@ -45,6 +45,7 @@ namespace a3b
             RowLayout layout;
             uint64_t rows;
             uint32_t tiles; // of a row, or of its slice
+            uint32_t share; // packs of a slice (the last one takes what is left)
             uint32_t vocab;
             uint32_t top;
             float scale;
@@ -466,18 +467,19 @@ namespace a3b
             unsigned long long keys[TOP ? kMaxCluster * kMaxTop : 1];
         };
 
-        // Blocks of kBlock threads an SM that the registers are bounded to. Measured on a B200 with 3 / 4 for the
-        // alternatives: 32768 x 257 fp16 20 / 18 us (four packs a thread), but 64 x 131072 fp32 15 / 17 us (eight: spills).
-        template<int P, bool TOP>
+        // Blocks of kBlock threads an SM that the registers are bounded to. Measured on a B200 with 3 / 4 for tiles of eight
+        // packs and alternatives: 2048 x 50257 bf16 on teams of 128 threads 55 / 50 us; on single warps (which spill at
+        // 64 registers) 16384 x 2048 31 / 34 us; the few long rows of teams of 256 leave most of an SM free anyway.
+        template<int S, int P, bool TOP>
         constexpr int residentBlocks()
         {
-            return P == 2 ? (TOP ? 4 : 6) : P == 4 ? 4 : (TOP ? 3 : 4);
+            return P == 2 ? (TOP ? 4 : 6) : P == 8 && TOP && (S <= 32 || S == 256) ? 3 : 4;
         }
 
         // One row a team. In a launch with clusters, slice b of a row is the tiles of the cluster's block b, and the first
         // block joins the slices.
         template<typename T, int S, int P, bool TOP, bool ENT>
-        __global__ void __launch_bounds__(Team<S>::block, kBlock / Team<S>::block * residentBlocks<P, TOP>())
+        __global__ void __launch_bounds__(Team<S>::block, kBlock / Team<S>::block * residentBlocks<S, P, TOP>())
             logprobKernel(LogprobArgs a)
         {
             constexpr int teams = Team<S>::perBlock;
@@ -503,7 +505,8 @@ namespace a3b
             Row<T> const row(a, r);
             float const c = a.scale * kLog2e;
             uint32_t const span = P * S; // packs of a tile
-            uint32_t const firstTile = slice * a.tiles;
+            uint32_t const begin = min(row.packs, slice * a.share);
+            uint32_t const end = slice == slices - 1 ? row.packs : min(row.packs, begin + a.share);
             int64_t const target = a.logp ? loadIndex(a.targets, r, a.index64) : -1;
             // What lies outside the packs, one element each of the first eight threads: the head is taken with the first
             // tile, in front of it, the tail with the last one.
@@ -517,15 +520,19 @@ namespace a3b
             float2 s2 = make_float2(0.0f, 0.0f), u2 = make_float2(0.0f, 0.0f);
             unsigned kept = 0, buffer = 0;
             uint32_t ranked = 0, rankAfter = 1; // tiles whose candidates have been ranked, or will be next
+            // The first of the tiles whose candidates were too many: from there the row is selected again at the end (a call
+            // in the loop would keep the tile's registers from being all there is).
+            constexpr uint32_t kNever = UINT32_MAX;
+            uint32_t again = kNever;
             if(TOP && thread == 0)
                 sel.count[0] = 0u;
             Tile<T, S, P> t;
-            t.load(row, firstTile * span, row.packs);
+            t.load(row, begin, end);
             if(target >= 0 && target < static_cast<int64_t>(a.vocab))
                 xt = toFloat(row.p[target]);
             for(uint32_t tile = 0; tile < a.tiles; ++tile)
             {
-                uint32_t const base = (firstTile + tile) * span;
+                uint32_t const base = begin + tile * span;
                 bool const last = tile + 1 == a.tiles;
                 float const front = tile == 0 ? inHead : -INFINITY, behind = last ? inTail : -INFINITY;
                 float const threadMax = maxNan(maxNan(front, behind), PackOf<T>::template max<P>(t.q));
@@ -551,7 +558,8 @@ namespace a3b
                     // The first tile's candidates are ranked at once, later ones are collected without a barrier,
                     // against what was kept when they were last ranked.
                     unsigned const mine = orderOf(threadMax);
-                    unsigned const least = tile == 0 ? sel.boundOf(mine, a.top) : sel.from(kept, a.top);
+                    unsigned const least
+                        = tile == 0 ? sel.boundOf(mine, a.top) : again == kNever ? sel.from(kept, a.top) : 0u;
                     sel.collect(t, least, mine, row.head, base, buffer);
                     if((tile == 0 || last) && least != 0u)
                     {
@@ -579,13 +587,13 @@ namespace a3b
                 };
                 // The registers of a pack that is done take the same pack of the next tile, if that is a full one: its
                 // loads run under the rest of this tile.
-                bool const nextFull = !last && base + 2 * span <= row.packs;
+                bool const nextFull = !last && base + 2 * span <= end;
                 auto const* const next = reinterpret_cast<uint4 const*>(row.p + row.head) + base + span + thread;
 #pragma unroll
                 for(int p = 0; p < P; ++p)
                 {
                     // a short tile's packs in the second half: none, for the whole team
-                    if(p == P / 2 && base + p * S >= row.packs)
+                    if(p == P / 2 && base + p * S >= end)
                         break;
 #pragma unroll
                     for(int w = 0; w < PackOf<T>::pairs; ++w)
@@ -604,40 +612,22 @@ namespace a3b
                     add(make_float2(maxNan(front, least), maxNan(behind, least)));
                 }
                 if(!last && !nextFull)
-                    t.load(row, base + span, row.packs);
+                    t.load(row, base + span, end);
                 if constexpr(TOP)
                 {
-                    if(last || tile + 1 == rankAfter)
+                    if((last || tile + 1 == rankAfter) && again == kNever)
                     {
                         Team<S>::sync();
                         unsigned const n = sel.count[buffer];
                         if(n > sel.room)
+                            again = ranked;
+                        else if(n > kept)
                         {
-                            Team<S>::sync(); // every thread has read the count
-                            if(thread == 0)
-                                sel.count[buffer] = kept;
-                            Team<S>::sync();
-                            uint32_t const perTile = span * PackOf<T>::E;
-                            uint32_t const from = ranked == 0 && slice == 0 ? 0 : row.head + (firstTile + ranked) * perTile;
-                            uint64_t const upTo = row.head + static_cast<uint64_t>(firstTile + tile + 1) * perTile;
-                            bool const end = last && slice == slices - 1;
-                            uint2 const got = sel.careful(
-                                row.p, from,
-                                static_cast<uint32_t>(end ? a.vocab : min(upTo, uint64_t{row.head} + row.packs * PackOf<T>::E)),
-                                a.top, kept, buffer);
-                            kept = got.x;
-                            buffer = got.y;
+                            sel.rank(buffer, n, a.top);
+                            kept = min(n, a.top);
+                            buffer ^= 1u;
                         }
-                        else
-                        {
-                            if(n > kept)
-                            {
-                                sel.rank(buffer, n, a.top);
-                                kept = min(n, a.top);
-                                buffer ^= 1u;
-                            }
-                            Team<S>::sync(); // ranked, and every thread has read the count before anyone collects more
-                        }
+                        Team<S>::sync(); // ranked, and every thread has read the count before anyone collects more
                         ranked = tile + 1;
                         // Between ranking at n tiles and at k n about (k - 1) top elements pass: k = 4 as long as they fit
                         // with room to spare.
@@ -645,6 +635,19 @@ namespace a3b
                     }
                 }
             }
+            if constexpr(TOP)
+                if(again != kNever)
+                {
+                    if(thread == 0)
+                        sel.count[buffer] = kept;
+                    Team<S>::sync();
+                    uint64_t const body = begin + uint64_t{again} * span;
+                    uint64_t const from = again == 0 && slice == 0 ? 0 : row.head + min(uint64_t{end}, body) * PackOf<T>::E;
+                    uint64_t const to = slice == slices - 1 ? a.vocab : row.head + uint64_t{end} * PackOf<T>::E;
+                    uint2 const got = sel.careful(row.p, static_cast<uint32_t>(from), static_cast<uint32_t>(to), a.top, kept, buffer);
+                    kept = got.x;
+                    buffer = got.y;
+                }
             float s = Team<S>::sum(s2.x + s2.y), u = ENT ? Team<S>::sum(u2.x + u2.y) : 0.0f;
             unsigned long long* const best = sel.keys[buffer];
             if constexpr(S > 32)
@@ -778,8 +781,13 @@ namespace a3b
             auto go = [&](auto size, auto p, unsigned cluster)
             {
                 constexpr int S = decltype(size)::value, P = decltype(p)::value;
-                uint64_t const tile = uint64_t{S} * P * cluster;
-                a.tiles = static_cast<uint32_t>(std::max<uint64_t>((packs + tile - 1) / tile, 1));
+                // Whole tiles, if the last slice keeps a quarter of one; else equal shares: a slice of a few packs leaves
+                // warps without a maximum, and the bound of its alternatives with it (8 rows of 50257 bf16 with 20
+                // alternatives 14 us with 138 packs in the last of four slices, 9 with equal ones).
+                uint64_t const tile = uint64_t{S} * P, whole = ((packs + cluster - 1) / cluster + tile - 1) / tile * tile;
+                uint64_t const share = (cluster - 1) * whole + tile / 4 <= packs ? whole : (packs + cluster - 1) / cluster;
+                a.share = static_cast<uint32_t>(share);
+                a.tiles = static_cast<uint32_t>(std::max<uint64_t>((share + tile - 1) / tile, 1));
                 if(a.top > 0)
                     return a.entropy ? launchRows<T, S, P, true, true>(stream, cluster, a)
                                      : launchRows<T, S, P, true, false>(stream, cluster, a);
@@ -1070,7 +1078,7 @@ extern "C"
         int const rd = currentDevice(&props);
         if(rd != A3B_OK)
             return rd;
-        LogprobArgs a{logits, {static_cast<uint32_t>(inner), outer_stride, inner_stride}, rows, 1u,
+        LogprobArgs a{logits, {static_cast<uint32_t>(inner), outer_stride, inner_stride}, rows, 1u, 0u,
                       static_cast<uint32_t>(vocab), top, static_cast<float>(scale),
                       static_cast<float>(256.0 / (scale * 1.4426950408889634074)), index_dtype == A3B_I64, targets, logp,
                       entropy, lse, top_logp, top_index};
