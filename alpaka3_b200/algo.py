@@ -380,31 +380,38 @@ class TensorList:
     once. It holds the addresses of the tensors as they are now, and keeps those tensors alive."""
 
     def __init__(self, inputs, outputs=None):
-        self.inputs = list(inputs)
-        self.outputs = self.inputs if outputs is None else list(outputs)
         self._handle = None
-        n = len(self.inputs)
-        if len(self.outputs) != n:
+        ins = self.inputs = list(inputs)
+        outs = self.outputs = ins if outputs is None else list(outputs)
+        n = len(ins)
+        if len(outs) != n:
             raise ValueError("inputs and outputs must be equally many")
-        self.device = self.inputs[0].device if n else None
-        for t in self.inputs:
-            if t.dtype not in _GRAD_DT:
-                raise TypeError(f"unsupported dtype {t.dtype}")
-            if not t.is_cuda or t.device != self.device:
-                raise ValueError("expected CUDA tensors of one device")
-            if not _is_dense(t):
-                raise ValueError("expected dense tensors")
-        for t, o in zip(self.inputs, self.outputs):
-            if o is not t and (o.dtype != t.dtype or o.device != t.device or o.shape != t.shape
-                               or (o.stride() != t.stride() and t.numel() > 1)):
-                raise ValueError("an output must have the dtype, device, shape and strides of its input")
+        self.device = ins[0].device if n else None
+        index = ins[0].get_device() if n else -1
+        codes = [_GRAD_DT.get(t.dtype, -1) for t in ins]
+        if -1 in codes:
+            raise TypeError(f"unsupported dtype {ins[codes.index(-1)].dtype}")
+        if n and (index < 0 or any(t.get_device() != index for t in ins)):
+            raise ValueError("expected CUDA tensors of one device")
+        if not all(t.is_contiguous() or _is_dense(t) for t in ins):
+            raise ValueError("expected dense tensors")
+        sizes = [t.numel() for t in ins]
+        addresses = [t.data_ptr() for t in ins]
+        keep = [t.untyped_storage() for t in ins]  # alive even if a tensor moves on
+        if outs is ins:
+            targets = None
+        else:
+            for t, o in zip(ins, outs):
+                if (o.dtype != t.dtype or o.get_device() != index or o.shape != t.shape
+                        or not (o.is_contiguous() and t.is_contiguous() or o.stride() == t.stride())):
+                    raise ValueError("an output must have the dtype, device, shape and strides of its input")
+            targets = (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs])
+            keep += [o.untyped_storage() for o in outs]
         handle = ctypes.c_void_p()
-        capi.call("a3b_tensor_list_create", (ctypes.c_void_p * n)(*[t.data_ptr() for t in self.inputs]),
-                  (ctypes.c_void_p * n)(*[t.data_ptr() for t in self.outputs]),
-                  (ctypes.c_uint64 * n)(*[t.numel() for t in self.inputs]),
-                  (ctypes.c_int * n)(*[_GRAD_DT[t.dtype] for t in self.inputs]), n, ctypes.byref(handle))
+        capi.call("a3b_tensor_list_create", (ctypes.c_void_p * n)(*addresses), targets, (ctypes.c_uint64 * n)(*sizes),
+                  (ctypes.c_int * n)(*codes), n, ctypes.byref(handle))
         self._handle = handle
-        self._storages = [t.untyped_storage() for t in self.inputs + self.outputs]  # alive even if a tensor moves on
+        self._storages = keep
         self._workspace = None
 
     def __del__(self):
