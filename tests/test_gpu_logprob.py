@@ -258,6 +258,17 @@ def test_many_rows(cuda, dtype, rows, v):
         close(got["top_logp"], best, tl + 4 * U * (best.abs().nan_to_num(0.0, posinf=0.0) + 1))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_very_long_rows(cuda, dtype):
+    """Millions of logits a row: many tiles a slice; one row with its best at the very end."""
+    v = 5_000_003
+    x, t = make(2, v, dtype)
+    x[1, -40:] = torch.linspace(20, 30, 40, device="cuda").to(dtype)
+    t[1] = v - 1
+    check_forward(x, t, 32)
+    check_backward(x, t)
+
+
 def test_many_rows_gradient(cuda):
     """Rows of many chunks and rows of a part of one, in one launch of more than 2^16 warps."""
     from alpaka3_b200 import algo
