@@ -468,12 +468,12 @@ namespace a3b
         };
 
         // Blocks of kBlock threads an SM that the registers are bounded to. Measured on a B200 with 3 / 4 for tiles of eight
-        // packs and alternatives: 2048 x 50257 bf16 on teams of 128 threads 55 / 50 us; on single warps (which spill at
-        // 64 registers) 16384 x 2048 31 / 34 us; the few long rows of teams of 256 leave most of an SM free anyway.
+        // packs and alternatives: 2048 x 50257 bf16 on teams of 128 threads 55 / 50 us, 300 x 131072 fp32 on 256 35 / 33;
+        // on single warps, which spill at 64 registers, 16384 x 2048 bf16 31 / 34 us.
         template<int S, int P, bool TOP>
         constexpr int residentBlocks()
         {
-            return P == 2 ? (TOP ? 4 : 6) : P == 8 && TOP && (S <= 32 || S == 256) ? 3 : 4;
+            return P == 2 ? (TOP ? 4 : 6) : P == 8 && TOP && S <= 32 ? 3 : 4;
         }
 
         // One row a team. In a launch with clusters, slice b of a row is the tiles of the cluster's block b, and the first

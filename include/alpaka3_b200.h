@@ -274,7 +274,8 @@ A3B_API int a3b_scan(a3b_stream_t stream, int dtype, int inclusive, void const* 
  * A target outside [0, vocab) marks a row without a token: its logp is 0. Logits of -infinity have probability 0 (logp
  * -infinity); a row of nothing else has lse -infinity, entropy 0 and logp -infinity for every token. A NaN in a row
  * makes its lse, logp and entropy NaN. With +infinity in a row its lse is +infinity, its entropy NaN, the logp of a
- * finite logit -infinity and that of +infinity NaN.
+ * finite logit -infinity and that of +infinity NaN. Repeated calls give the same bits; the order of a row's sums follows
+ * from the number of rows, their length and alignment.
  * At most 2^31 - 1 rows of at most 2^31 - 65 logits (A3B_ERR_TOO_LARGE). */
 A3B_API int a3b_token_logprobs(a3b_stream_t stream, int dtype, void const* logits, uint64_t outer, uint64_t inner,
                                uint64_t vocab, int64_t outer_stride, int64_t inner_stride, double scale, int index_dtype,
