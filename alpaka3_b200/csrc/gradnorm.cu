@@ -573,7 +573,8 @@ namespace a3b
         }
 
         template<int KIND>
-        int launchNorm(cudaStream_t s, a3b_tensor_list const* list, DeviceProps const* props, double* partials, uint32_t* count)
+        int launchNorm(
+            cudaStream_t s, a3b_tensor_list const* list, DeviceProps const* props, double* partials, uint32_t* count)
         {
             *count = 0;
             for(Batch const& b : list->batches)
@@ -590,7 +591,8 @@ namespace a3b
         }
 
         template<int KIND>
-        int launchFinish(cudaStream_t s, double const* partials, uint32_t count, double* partial, int dtype, void* norm, bool clips)
+        int launchFinish(
+            cudaStream_t s, double const* partials, uint32_t count, double* partial, int dtype, void* norm, bool clips)
         {
             return launchAfter(s, 1, finishKernel<KIND>, partials, count, partial, dtype, norm, clips);
         }

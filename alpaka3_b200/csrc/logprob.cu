@@ -174,6 +174,14 @@ namespace a3b
             }
         };
 
+        // elements from p to the next 16-byte boundary
+        template<typename T>
+        __device__ __forceinline__ uint32_t toBoundary(T const* p)
+        {
+            auto const past = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15u);
+            return ((16u - past) & 15u) / static_cast<uint32_t>(sizeof(T));
+        }
+
         // A row: `head` elements up to the first 16-byte boundary, `packs` 16-byte packs, `tail` elements behind them.
         template<typename T>
         struct Row
@@ -182,9 +190,10 @@ namespace a3b
             T const* p;
             uint32_t head, packs, tail;
 
-            __device__ __forceinline__ Row(LogprobArgs const& a, uint64_t r) : p(static_cast<T const*>(a.logits) + a.layout.at(static_cast<uint32_t>(r)))
+            __device__ __forceinline__ Row(LogprobArgs const& a, uint64_t r)
+                : p(static_cast<T const*>(a.logits) + a.layout.at(static_cast<uint32_t>(r)))
             {
-                head = min(a.vocab, static_cast<uint32_t>((16u - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / static_cast<uint32_t>(sizeof(T)));
+                head = min(a.vocab, toBoundary(p));
                 packs = (a.vocab - head) / E;
                 tail = a.vocab - head - packs * E;
             }
@@ -647,7 +656,8 @@ namespace a3b
                     uint64_t const body = begin + uint64_t{again} * span;
                     uint64_t const from = again == 0 && slice == 0 ? 0 : row.head + min(uint64_t{end}, body) * PackOf<T>::E;
                     uint64_t const to = slice == slices - 1 ? a.vocab : row.head + uint64_t{end} * PackOf<T>::E;
-                    uint2 const got = sel.careful(row.p, static_cast<uint32_t>(from), static_cast<uint32_t>(to), a.top, kept, buffer);
+                    uint2 const got = sel.careful(
+                        row.p, static_cast<uint32_t>(from), static_cast<uint32_t>(to), a.top, kept, buffer);
                     kept = got.x;
                     buffer = got.y;
                 }
@@ -865,8 +875,7 @@ namespace a3b
             T const* const row = static_cast<T const*>(a.logits) + a.layout.at(r);
             T* const out = static_cast<T*>(a.grad) + a.gradLayout.at(r);
             // packs on the 16-byte boundaries of the output row, as in the forward pass; the input row may lie differently
-            uint32_t const head
-                = min(a.vocab, static_cast<uint32_t>((16u - (reinterpret_cast<uintptr_t>(out) & 15u)) & 15u) / static_cast<uint32_t>(sizeof(T)));
+            uint32_t const head = min(a.vocab, toBoundary(out));
             uint32_t const packs = (a.vocab - head) / E, tail = a.vocab - head - packs * E;
             bool const alike = (reinterpret_cast<uintptr_t>(row) & 15u) == (reinterpret_cast<uintptr_t>(out) & 15u);
 
