@@ -56,7 +56,7 @@ def close(got, want, tol):
     assert not bad.any(), ((got[fine] - want[fine]).abs().max(), tol[fine].max())
 
 
-def forward(x, t, top=0, scale=1.0, want=("logp", "entropy", "lse"), stream=None):
+def forward(x, t, top=0, scale=1.0, want=("logp", "entropy", "lse")):
     from alpaka3_b200 import algo
     shape, dev = x.shape[:-1], x.device
     out = {k: torch.full(shape, 77.0, device=dev) for k in want}
@@ -64,8 +64,7 @@ def forward(x, t, top=0, scale=1.0, want=("logp", "entropy", "lse"), stream=None
     if top:
         tops = {"top_logp": torch.full((*shape, top), 77.0, device=dev),
                 "top_index": torch.full((*shape, top), -7, dtype=t.dtype if t is not None else torch.int64, device=dev)}
-    algo.token_logprobs(out.get("logp"), x, t, entropy=out.get("entropy"), lse=out.get("lse"), scale=scale,
-                        stream=stream, **tops)
+    algo.token_logprobs(out.get("logp"), x, t, entropy=out.get("entropy"), lse=out.get("lse"), scale=scale, **tops)
     return {**out, **tops}
 
 
@@ -256,6 +255,13 @@ def test_many_rows(cuda, dtype, rows, v):
         assert torch.equal(got["top_index"], order)
         best = q.gather(1, order)
         close(got["top_logp"], best, tl + 4 * U * (best.abs().nan_to_num(0.0, posinf=0.0) + 1))
+        # without the entropy another kernel runs; without alternatives a third
+        plain = forward(x, t, k, want=("logp", "lse"))
+        assert torch.equal(plain["top_index"], order)
+        bare = forward(x, t, want=("logp", "lse"))
+        for some in (plain, bare, forward(x, t)):
+            close(some["logp"], picked, tl + size)
+            close(some["lse"], lse, tl + size)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -400,8 +406,10 @@ def test_other_stream_and_captured_graphs(cuda):
     want = forward(x, t, 8)
     ones = torch.ones(33, device="cuda")
     side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
-    got = forward(x, t, 8, stream=side)  # outputs are made on the current stream before
+    got = {k: torch.zeros_like(w) for k, w in want.items()}
+    side.wait_stream(torch.cuda.current_stream())  # what the outputs were filled with is in place by then
+    algo.token_logprobs(got["logp"], x, t, entropy=got["entropy"], lse=got["lse"], top_logp=got["top_logp"],
+                        top_index=got["top_index"], stream=side)
     side.synchronize()
     assert all(torch.equal(got[k], want[k]) for k in want)
 
