@@ -127,6 +127,14 @@ namespace a3b
         constexpr int kBlock = 256;
         constexpr int kMaxCluster = 8;
 
+        // elements from p to the next 16-byte boundary
+        template<typename T>
+        __device__ __forceinline__ uint32_t toBoundary(T const* p)
+        {
+            auto const past = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15u);
+            return ((16u - past) & 15u) / static_cast<uint32_t>(sizeof(T));
+        }
+
         // A row's team is S threads: a block (S = 64, 128, 256), a warp or a quarter of one in a block of kBlock.
         template<int S>
         struct Team
@@ -173,14 +181,6 @@ namespace a3b
                 return v;
             }
         };
-
-        // elements from p to the next 16-byte boundary
-        template<typename T>
-        __device__ __forceinline__ uint32_t toBoundary(T const* p)
-        {
-            auto const past = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15u);
-            return ((16u - past) & 15u) / static_cast<uint32_t>(sizeof(T));
-        }
 
         // A row: `head` elements up to the first 16-byte boundary, `packs` 16-byte packs, `tail` elements behind them.
         template<typename T>
@@ -394,54 +394,81 @@ namespace a3b
                 __syncwarp(Team<S>::mask());
             }
 
-            // The same selection for the elements [first, last) of a row, whatever they are, in steps that always fit: an
-            // element of every thread, or eight where few of them enter. For tiles of which too many elements passed:
-            // many equal ones (constant rows, masks of one low value), rows in rising order. `buffer` starts with `kept`
-            // keys in order, those of lower indices, and its count is `kept`.
+            // whether any thread of the team says so (the team is synchronised)
+            static __device__ __forceinline__ bool anyOf(bool b)
+            {
+                if constexpr(S <= 32)
+                    return __any_sync(Team<S>::mask(), b);
+                else
+                    return __syncthreads_or(b);
+            }
+
+            // The same selection for the elements [first, last) of a row, whatever they are: where too many passed (many
+            // equal ones: constant rows, masks of one low value; rows in rising order). Eight packs a thread are skipped
+            // where nothing enters; else the elements are taken in steps that always fit, one of every thread. `buffer`
+            // starts with `kept` keys in order, those of lower indices, and its count is `kept`.
             template<typename T>
             __device__ __noinline__ uint2 careful(
                 T const* row, uint32_t first, uint32_t last, unsigned top, unsigned kept, unsigned buffer)
             {
-                constexpr unsigned per = 8;
+                constexpr unsigned per = 8, E = PackOf<T>::E, stride = S * per * E;
                 unsigned const thread = Team<S>::thread();
-                for(uint32_t base = first; base < last; base += S * per)
+                while(first < last)
                 {
-                    unsigned order[per];
-                    bool any = false;
-                    unsigned const least = from(kept, top);
-#pragma unroll
-                    for(unsigned k = 0; k < per; ++k)
+                    uint32_t const edge = toBoundary(row + first);
+                    uint32_t upTo = edge != 0u && edge < last - first ? first + edge : last;
+                    if(edge == 0u && stride <= last - first)
                     {
-                        uint32_t const i = base + k * S + thread;
-                        order[k] = i < last ? orderOf(toFloat(row[i])) : 0u;
-                        any |= order[k] >= least && least != 0u;
-                    }
-                    bool some;
-                    if constexpr(S <= 32)
-                        some = __any_sync(Team<S>::mask(), any);
-                    else
-                        some = __syncthreads_or(any);
-                    if(!some)
-                        continue;
-                    for(unsigned k = 0; k < per; ++k)
-                    {
-                        unsigned o = 0;
+                        unsigned q[per][4];
 #pragma unroll
-                        for(unsigned j = 0; j < per; ++j)
-                            o = j == k ? order[j] : o;
-                        unsigned const enters = from(kept, top);
-                        if(o >= enters && enters != 0u)
-                            push(buffer, o, base + k * S + thread);
-                        Team<S>::sync();
-                        unsigned const n = count[buffer];
-                        if(n > kept)
+                        for(unsigned k = 0; k < per; ++k)
                         {
-                            rank(buffer, n, top);
-                            kept = min(n, top);
-                            buffer ^= 1u;
+                            uint4 const v = __ldcs(reinterpret_cast<uint4 const*>(row + first) + k * S + thread);
+                            q[k][0] = v.x, q[k][1] = v.y, q[k][2] = v.z, q[k][3] = v.w;
                         }
-                        Team<S>::sync();
+                        unsigned const least = from(kept, top);
+                        upTo = first + stride;
+                        if(!anyOf(least != 0u && orderOf(PackOf<T>::template max<per>(q)) >= least))
+                        {
+                            first = upTo;
+                            continue;
+                        }
                     }
+                    for(; first < upTo; first += S * per)
+                    {
+                        unsigned order[per];
+                        bool enters = false;
+                        unsigned const least = from(kept, top);
+#pragma unroll
+                        for(unsigned k = 0; k < per; ++k)
+                        {
+                            uint32_t const i = first + k * S + thread;
+                            order[k] = i < upTo ? orderOf(toFloat(row[i])) : 0u;
+                            enters |= order[k] >= least && least != 0u;
+                        }
+                        if(!anyOf(enters))
+                            continue;
+                        for(unsigned k = 0; k < per; ++k)
+                        {
+                            unsigned o = 0;
+#pragma unroll
+                            for(unsigned j = 0; j < per; ++j)
+                                o = j == k ? order[j] : o;
+                            unsigned const now = from(kept, top);
+                            if(o >= now && now != 0u)
+                                push(buffer, o, first + k * S + thread);
+                            Team<S>::sync();
+                            unsigned const n = count[buffer];
+                            if(n > kept)
+                            {
+                                rank(buffer, n, top);
+                                kept = min(n, top);
+                                buffer ^= 1u;
+                            }
+                            Team<S>::sync();
+                        }
+                    }
+                    first = upTo;
                 }
                 return make_uint2(kept, buffer);
             }
