@@ -885,17 +885,17 @@ namespace a3b
         // fused operation, it is 2^t (a + b t), a = scale (g_lse - g - g_H H), b = -scale g_H ln 2. What the roundings of c
         // and lse / ln 2 leave is one number for a row (where p counts, x is near lse / scale): 2^ of it goes into a and b.
         //
-        // One warp takes a chunk of kBackPacks packs a lane and needs no other: chunks are handed out in the order of
+        // L threads take a chunk of kBackPacks packs each and need no others: chunks are handed out in the order of
         // memory. Measured on a B200: 4096 x 131072 fp32 643 us, 2048 x 50257 bf16 63 us, HBM-bound. The bound of 40
         // registers (6 blocks of 8 warps an SM) is what took the second one from 148 to 78, the fused exponents the rest.
         constexpr int kBackPacks = 4;
 
-        template<typename T>
+        template<typename T, int L>
         __global__ void __launch_bounds__(kBlock, 6) logprobBackwardKernel(BackwardArgs a)
         {
             constexpr int E = PackOf<T>::E;
-            constexpr uint32_t span = 32 * kBackPacks;
-            uint32_t const id = blockIdx.x * (kBlock / 32) + threadIdx.x / 32, lane = threadIdx.x & 31u;
+            constexpr uint32_t span = L * kBackPacks;
+            uint32_t const id = blockIdx.x * (kBlock / L) + threadIdx.x / L, lane = threadIdx.x & (L - 1u);
             if(id >= a.total)
                 return;
             uint32_t const r = id / a.chunks, base = (id - r * a.chunks) * span;
@@ -920,7 +920,7 @@ namespace a3b
                 // element. The product is rounded on its own, as lse is: the largest logit is exactly at 0 then.
                 uint64_t const from = base == 0 ? 0 : head + static_cast<uint64_t>(base) * E;
                 uint64_t const to = base + span >= packs ? a.vocab : head + static_cast<uint64_t>(base + span) * E;
-                for(uint64_t i = from + lane; i < to; i += 32)
+                for(uint64_t i = from + lane; i < to; i += L)
                 {
                     float const t = __fmul_rn(toFloat(row[i]), a.scale) - lse, p = expf(t);
                     float const d = p == 0.0f ? 0.0f : p * ((gl - g) - gh * (t + h));
@@ -935,7 +935,7 @@ namespace a3b
 #pragma unroll
                 for(int p = 0; p < kBackPacks; ++p)
                 {
-                    uint4 const v = __ldcs(from + p * 32);
+                    uint4 const v = __ldcs(from + p * L);
                     q[p][0] = v.x, q[p][1] = v.y, q[p][2] = v.z, q[p][3] = v.w;
                 }
             }
@@ -944,7 +944,7 @@ namespace a3b
 #pragma unroll
                 for(int p = 0; p < kBackPacks; ++p)
                 {
-                    uint32_t const k = base + p * 32 + lane;
+                    uint32_t const k = base + p * L + lane;
                     uint4 v = make_uint4(0u, 0u, 0u, 0u);
                     T const* const from = row + head + static_cast<uint64_t>(k) * E;
                     if(k < packs && alike)
@@ -956,15 +956,24 @@ namespace a3b
                             PackOf<T>::setRaw(q[p], e, from + e);
                 }
             }
-            // the elements in front of and behind the packs, one a lane of the row's first warp
-            uint32_t const aside = lane < 8 ? lane : a.vocab - tail + lane - 8;
-            bool const isAside = base == 0 && (lane < 8 ? lane < head : lane < 8 + tail);
-            float const asideValue = isAside ? toFloat(row[aside]) : 0.0f;
+            // the elements in front of and behind the packs, up to eight each, by the threads of the row's first chunk
+            constexpr int asides = L < 16 ? 16 / L : 1;
+            uint32_t aside[asides];
+            bool isAside[asides];
+            float asideValue[asides];
+#pragma unroll
+            for(int i = 0; i < asides; ++i)
+            {
+                uint32_t const j = lane + i * L;
+                aside[i] = j < 8 ? j : a.vocab - tail + j - 8;
+                isAside[i] = base == 0 && (j < 8 ? j < head : j < 8 + tail);
+                asideValue[i] = isAside[i] ? toFloat(row[aside[i]]) : 0.0f;
+            }
 
-            // where the target is in this warp's packs
+            // where the target is in this chunk's packs
             uint32_t const place = static_cast<uint32_t>(target) - head, hitPack = place / E - base;
             bool const hit = counts && static_cast<uint32_t>(target) >= head && hitPack < span && place / E < packs
-                             && hitPack % 32u == lane;
+                             && hitPack % L == lane;
             float const hitValue = hit ? toFloat(row[target]) : 0.0f;
 
             constexpr float log2eRest = 1.92596299e-8f; // 1 / ln 2 - kLog2e
@@ -987,7 +996,7 @@ namespace a3b
 #pragma unroll
             for(int p = 0; p < kBackPacks; ++p)
             {
-                uint32_t const k = base + p * 32 + lane;
+                uint32_t const k = base + p * L + lane;
                 unsigned o[4];
 #pragma unroll
                 for(int w = 0; w < PackOf<T>::pairs; ++w)
@@ -997,19 +1006,26 @@ namespace a3b
             }
             if(hit)
                 out[target] = fromFloat<T>(gradOf(make_float2(hitValue, 0.0f)).x + a.scale * g);
-            if(isAside)
-            {
-                float const d = gradOf(make_float2(asideValue, 0.0f)).x;
-                out[aside] = fromFloat<T>(counts && target == static_cast<int64_t>(aside) ? d + a.scale * g : d);
-            }
+#pragma unroll
+            for(int i = 0; i < asides; ++i)
+                if(isAside[i])
+                {
+                    float const d = gradOf(make_float2(asideValue[i], 0.0f)).x;
+                    bool const isTarget = counts && target == static_cast<int64_t>(aside[i]);
+                    out[aside[i]] = fromFloat<T>(isTarget ? d + a.scale * g : d);
+                }
         }
 
         template<typename T>
         int launchBackward(cudaStream_t stream, uint64_t rows, BackwardArgs a)
         {
-            uint64_t const packs = a.vocab / PackOf<T>::E, span = 32 * kBackPacks;
+            // Short rows in great number take a quarter of a warp each, as in the forward pass (a whole one / a quarter on
+            // a B200: 32768 x 257 fp16 22 / 12 us, 65536 x 64 fp32 31 / 12, 100 x 257 3.4 / 4.0).
+            uint64_t const packs = a.vocab / PackOf<T>::E;
+            bool const quarter = rows >= kEnoughWarps / 4 && packs <= 8 * kBackPacks;
+            uint64_t const span = (quarter ? 8 : 32) * kBackPacks, perBlock = kBlock / (quarter ? 8 : 32);
             uint64_t const chunks = std::max<uint64_t>((packs + span - 1) / span, 1);
-            if(rows * chunks > static_cast<uint64_t>(UINT32_MAX) - 8)
+            if(rows * chunks > static_cast<uint64_t>(UINT32_MAX) - perBlock)
             {
                 setError("%llu rows of %u logits are more than one launch holds",
                          static_cast<unsigned long long>(rows), a.vocab);
@@ -1017,8 +1033,11 @@ namespace a3b
             }
             a.total = static_cast<uint32_t>(rows * chunks);
             a.chunks = static_cast<uint32_t>(chunks);
-            unsigned const grid = (a.total + kBlock / 32 - 1) / (kBlock / 32);
-            logprobBackwardKernel<T><<<grid, kBlock, 0, stream>>>(a);
+            auto const grid = static_cast<unsigned>((a.total + perBlock - 1) / perBlock);
+            if(quarter)
+                logprobBackwardKernel<T, 8><<<grid, kBlock, 0, stream>>>(a);
+            else
+                logprobBackwardKernel<T, 32><<<grid, kBlock, 0, stream>>>(a);
             A3B_CHECK_LAUNCH("logprobBackwardKernel");
             return A3B_OK;
         }

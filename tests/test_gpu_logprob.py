@@ -320,7 +320,12 @@ def check_backward(x, t, scale=1.0, use=("logp", "entropy", "lse"), out=None, se
     counts, some = ((t2 >= 0) & (t2 < v)), lse != -INF
     gp = torch.where(counts & some, gp, zero)
     gh, gl = torch.where(some, gh, zero), torch.where(some, gl, zero)
-    q = x2 * scale - torch.where(some, lse, zero)[:, None]
+    lse = torch.where(some, lse, zero)
+    # Next to 2^100 a step of lse's fp32 is 2^76: the difference from a product in 64 bits would be that rounding alone. The
+    # product is rounded as lse was (the scale to fp32, then the product), so that a row of one value is at 0, not -ln V.
+    rounded = (x2 * torch.tensor(scale, dtype=torch.float32).double().item()).float().double()
+    product = torch.where((lse.abs() > 2.0**80)[:, None], rounded, x2 * scale)
+    q = product - lse[:, None]
     p = q.exp()
     pq = torch.where(p == 0, torch.zeros_like(p), p * (q + ent[:, None]))
     want = p * (gl - gp)[:, None] - gh[:, None] * pq
@@ -380,6 +385,25 @@ def test_gradient_strides_alignment_in_place(cuda, dtype):
     want = check_backward(buf[:, :-1, 1:1004], t)
     x = buf[:, :-1, 1:1004]
     assert torch.equal(check_backward(x, t, out=x), want)  # in place
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [1, 3, 15, 64, 130, 135, 255, 257, 263, 519])
+def test_gradient_many_short_rows(cuda, dtype, v):
+    """Rows enough for teams of a quarter warp, and the vocabularies at which they stop: odd starts, masks, in place."""
+    x, t = make(2053, v, dtype)
+    x[0::97] = -INF
+    x[1::97, 1:] = -INF
+    x[2::97] = torch.finfo(dtype).min
+    x[3::97, ::2] = -INF
+    t[4::97], t[5::97], t[1::97] = -100, v, 0
+    t[6::97], t[7::97] = 0, v - 1
+    want = check_backward(x, t, 0.7)
+    assert (want[0::97] == 0).all()
+    store = torch.zeros(2053, v + 5, dtype=dtype, device="cuda")
+    check_backward(x, t, 0.7, out=store[:, 1:v + 1])
+    assert (store[:, 0] == 0).all() and (store[:, v + 1:] == 0).all()
+    assert torch.equal(check_backward(x, t, 0.7, out=x), want)
 
 
 def test_gradient_against_differences(cuda):
