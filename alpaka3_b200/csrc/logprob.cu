@@ -898,7 +898,7 @@ namespace a3b
             uint32_t const id = blockIdx.x * (kBlock / L) + threadIdx.x / L, lane = threadIdx.x & (L - 1u);
             if(id >= a.total)
                 return;
-            uint32_t const r = id / a.chunks, base = (id - r * a.chunks) * span;
+            uint32_t const r = id / a.chunks, chunk = id - r * a.chunks, base = chunk * span;
             T const* const row = static_cast<T const*>(a.logits) + a.layout.at(r);
             T* const out = static_cast<T*>(a.grad) + a.gradLayout.at(r);
             // packs on the 16-byte boundaries of the output row, as in the forward pass; the input row may lie differently
@@ -918,8 +918,12 @@ namespace a3b
             {
                 // Infinite or NaN lse, or a row of huge logits (masks of fp32's lowest value and nothing else): element by
                 // element. The product is rounded on its own, as lse is: the largest logit is exactly at 0 then.
-                uint64_t const from = base == 0 ? 0 : head + static_cast<uint64_t>(base) * E;
-                uint64_t const to = base + span >= packs ? a.vocab : head + static_cast<uint64_t>(base + span) * E;
+                // Chunks are counted for a row that starts on a boundary; one with a head may have a pack less, and its last
+                // chunk none at all: that chunk alone takes what is behind the packs, so each element has one writer (in
+                // place a second one would read the first one's gradient).
+                uint64_t const from = base == 0 ? 0 : head + static_cast<uint64_t>(min(packs, base)) * E;
+                uint64_t const to
+                    = chunk + 1 == a.chunks ? a.vocab : head + static_cast<uint64_t>(min(packs, base + span)) * E;
                 for(uint64_t i = from + lane; i < to; i += L)
                 {
                     float const t = __fmul_rn(toFloat(row[i]), a.scale) - lse, p = expf(t);

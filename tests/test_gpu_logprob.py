@@ -519,3 +519,28 @@ def test_refusals(cuda):
                 dict(grad_logits=store[:100].expand(4, 100)), dict(scale=0.0)):
         with pytest.raises(capi.A3BError):
             algo.token_logprobs_backward(**{"grad_logits": g, "logits": x, "targets": t, "lse": lp, "grad_logp": lp, **bad})
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [512, 513, 516, 517, 518, 1024, 1030, 1031, 1032, 1033, 1034, 1035, 1036, 1037, 1038, 1039, 2056])
+def test_gradient_of_lowest_values_in_place(cuda, dtype, v):
+    """Rows of the type's lowest value (for fp32 and bf16 element by element), at every start, where the last chunk has no
+    pack of its own: in place the same bits as apart. Three ordinary rows lie between."""
+    from alpaka3_b200 import algo
+    pitch = v + 16
+    g = torch.Generator(device="cuda").manual_seed(v)
+    buf = (torch.randn(6, pitch, generator=g, device="cuda") * 3).to(dtype)
+    t = torch.randint(0, v, (6,), generator=g, device="cuda")
+    t[2] = v - 1
+    one = torch.ones(6, device="cuda")
+    for start in range(8):
+        store = buf.clone()
+        x = store[:, start:start + v]
+        x[::2] = torch.finfo(dtype).min
+        f = forward(x, t)
+        apart = torch.full((6, pitch), 4.0, dtype=dtype, device="cuda")[:, start:start + v]
+        for out in (apart, x):
+            algo.token_logprobs_backward(out, x, t, f["lse"], entropy=f["entropy"], grad_logp=one, grad_entropy=-one,
+                                         grad_lse=0.5 * one)
+        assert torch.isfinite(apart).all() and torch.equal(x, apart), start
+        assert torch.equal(store[:, :start], buf[:, :start]) and torch.equal(store[:, start + v:], buf[:, start + v:])
