@@ -85,7 +85,8 @@ namespace a3b
         }
 
         // Sums of one share of a row whose largest logit is `high`: s = sum 2^t and u = sum t 2^t over its logits x, with
-        // t = c x + offset, one fused operation. c = scale / ln 2, and offset = -(c high) as it is rounded.
+        // t = c x + offset, one fused operation. c = scale / ln 2, and offset = -(c high) as it is rounded. The largest
+        // logit's own t is what that rounding left: at most 32, as long as |c high| is at most 2^30.
         struct Stats
         {
             float high;
@@ -93,17 +94,20 @@ namespace a3b
             float u;
         };
 
-        // Logits next to one beyond 2^80 differ from it by 2^56 or more, so only those equal to it count: any factor does
-        // that keeps c x in range and takes every other t below -2^16. u is 0 then (and not computed: `u` holds NaN if
-        // there are logits of -infinity, which no clamp separates from a maximum of fp32's lowest value).
-        __device__ __forceinline__ bool isBig(float high)
+        // Beyond that, fp32's steps at `high` are 64 or more in t: all logits but those equal to it together are less than
+        // V 2^-64 of the sum and are left out. Then the factor is a power of two that brings `high` to 2^33 (an exact
+        // product: t = 0 for what equals it, below -500 for all else), and u is 0 (and not computed: `u` holds NaN if there
+        // are logits of -infinity, which no clamp separates from a maximum of fp32's lowest value).
+        __device__ __forceinline__ bool isBig(float high, float c)
         {
-            return !(fabsf(high) <= 0x1p80f);
+            return !(fabsf(high * c) <= 0x1p30f);
         }
 
         __device__ __forceinline__ float factorOf(float high, float c)
         {
-            return isBig(high) && high != -INFINITY ? 0x1p-40f : c;
+            return isBig(high, c) && high != -INFINITY
+                       ? __uint_as_float(((127u + 127u + 33u) << 23) - (__float_as_uint(high) & 0x7f800000u))
+                       : c;
         }
 
         __device__ __forceinline__ float offsetOf(float high, float c)
@@ -117,7 +121,7 @@ namespace a3b
         {
             if(b.high == -INFINITY)
                 return; // nothing in that share
-            bool const big = isBig(high) || isBig(b.high);
+            bool const big = isBig(high, c) || isBig(b.high, c);
             float const d = b.high == high ? 0.0f : big ? -200.0f : fmaxf(offsetOf(high, c) - offsetOf(b.high, c), -200.0f);
             float const f = exp2Approx(d);
             s += f * b.s;
@@ -749,7 +753,7 @@ namespace a3b
 
             // The largest logit's own t is what the rounding of the offset left (not quite 0): s over its 2^t is the sum
             // of e^(z - m), 1 in a row with one logit left.
-            bool const nothing = high == -INFINITY, big = isBig(high);
+            bool const nothing = high == -INFINITY, big = isBig(high, c);
             float const rest = big ? 0.0f : fmaf(high, c, offsetOf(high, c));
             float const lnS = high == INFINITY ? 0.0f : logf(s / exp2Approx(rest));
             auto logpOf = [&](float x) { return nothing ? -INFINITY : fmaf(x - high, a.scale, -lnS); };
@@ -914,7 +918,7 @@ namespace a3b
             float const gl = a.gradLse && !nothing ? a.gradLse[r] : 0.0f;
             float const gh = a.gradEntropy && !nothing ? a.gradEntropy[r] : 0.0f;
             float const h = a.gradEntropy ? a.entropy[r] : 0.0f;
-            if(isBig(lse) && !nothing)
+            if(!(fabsf(lse) <= 0x1p80f) && !nothing)
             {
                 // Infinite or NaN lse, or a row of huge logits (masks of fp32's lowest value and nothing else): element by
                 // element. The product is rounded on its own, as lse is: the largest logit is exactly at 0 then.

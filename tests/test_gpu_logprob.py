@@ -544,3 +544,88 @@ def test_gradient_of_lowest_values_in_place(cuda, dtype, v):
                                          grad_lse=0.5 * one)
         assert torch.isfinite(apart).all() and torch.equal(x, apart), start
         assert torch.equal(store[:, :start], buf[:, :start]) and torch.equal(store[:, start + v:], buf[:, start + v:])
+
+
+# ------------------------------------------------------------------------------------ logits far from zero
+# ln p stays as the formula has it while |z| grows: only the steps of z itself (and of lse) do.
+def far_values(dtype, scale):
+    """+-10^3 .. +-10^38, as far as the type and scale * value hold them."""
+    top = 6e4 if dtype == torch.float16 else 2e38
+    return [s * 10.0**k for k in range(3, 39) for s in (1.0, -1.0) if 10.0**k <= top and 10.0**k * max(scale, 1.0) < 2e38]
+
+
+def far_rows(v, dtype, scale, seed=0):
+    """For each of these values: a row of it alone, all but three logits at it, the first or the second half at it, and a
+    row spread around it; as many targets, some of them on such logits."""
+    g = torch.Generator(device="cuda").manual_seed(seed + v)
+    values = far_values(dtype, scale)
+    base = (torch.randn(5 * len(values), v, generator=g, device="cuda") * 3)
+    for i, w in enumerate(values):
+        rows = base[5 * i:5 * i + 5]
+        keep = torch.randint(0, v, (3,), generator=g, device="cuda")
+        rows[0] = w
+        kept = rows[1, keep].clone()
+        rows[1] = w
+        rows[1, keep] = kept
+        rows[2, :v // 2 + 1] = w
+        rows[3, v // 2:] = w
+        rows[4] += w
+    t = torch.randint(0, v, (len(base),), generator=g, device="cuda")
+    return base.to(dtype), t
+
+
+def check_far(x, t, top, scale, additions):
+    """Exponents are t = c x + offset with offset = -(c high) as rounded to fp32: half a step of it, R <= 2^-24 |c high|, is
+    in every t, and at most 32 (beyond |c high| = 2^30 the offset is exact). So a t of size R + |d| is rounded by u (R + |d|)
+    at most, its power is off by R u more than T(V) counts, s / 2^R by as much; u / s - R takes two sums of terms R times
+    as large, each off by T(V) at most: 2 R T(V) more in the entropy."""
+    v = x.shape[-1]
+    got = forward(x, t, top, scale)
+    q, lse, h = oracle(x, scale, where="cuda")
+    r = (x.double().amax(-1).abs() * scale * 1.4427 * U).clamp(max=32.0)
+    tl = (additions + 20 + 3 * math.log(v + 1) + 4) * U + r * U
+    logp = q.gather(1, t[:, None])[:, 0]
+    close(got["logp"], logp, tl + 4 * U * (logp.abs() + 1))
+    close(got["lse"], lse, tl + 4 * U * (lse.abs() + 1))
+    close(got["entropy"], h, 3 * tl * (1 + math.log(v + 1)) + 2 * r * tl)
+    if top:
+        order = ranks(x, top, where="cuda")
+        assert torch.equal(got["top_index"], order)
+        best = q.gather(1, order)
+        close(got["top_logp"], best, tl[:, None] + 4 * U * (best.abs() + 1))
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.7, 1 / 0.3, 10.0, 1e6])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [5, 300, 2100, 9000, 50257, 140001])
+def test_far_logits(cuda, dtype, v, scale):
+    """All rows in one call, then a few rows a call (slices of a row over a cluster where it is long)."""
+    x, t = far_rows(v, dtype, scale)
+    top = min(v, 5)
+    check_far(x, t, top, scale, v / 64 + 64)
+    step = 9 if v > 20000 else len(x)
+    for lo in range(0, len(x), step):
+        check_far(x[lo:lo + step], t[lo:lo + step], top if lo % 2 else 0, scale, v / 64 + 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,v", [(8200, 65), (8200, 260), (8200, 700), (8192, 5003), (4100, 9001), (2048, 17011)])
+def test_far_logits_in_many_rows(cuda, dtype, rows, v):
+    """The same rows over and over, for the teams that many rows get: a part of a warp, a warp, two and four."""
+    x, t = far_rows(v, dtype, 0.7)
+    again = torch.arange(rows, device="cuda") % len(x)
+    for top in (0, 3):
+        check_far(x[again], t[again], top, 0.7, v / 16 + 64)  # 8 threads a row, two sums each
+
+
+def test_entropy_and_lse_alone_of_far_logits(cuda):
+    """The kernels without entropy, and without a token."""
+    x, t = far_rows(20011, torch.float32, 1.0)
+    full = forward(x, t)
+    for want in (("logp",), ("entropy",), ("lse",), ("logp", "lse")):
+        some = forward(x, t if "logp" in want else None, want=want)
+        for k in want:
+            assert torch.isfinite(some[k]).all()
+            # both within check_far's bounds; a masked token's logp or a row's lse may be of any size
+            size = full[k].abs().double()
+            close(some[k], full[k], 2 * (3 * (20011 / 64 + 120 + 32) * U * (1 + math.log(20012) + 32) + 4 * U * size))
