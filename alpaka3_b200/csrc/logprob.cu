@@ -888,11 +888,19 @@ namespace a3b
         // grad_v = scale (g [v == t] + p_v ((g_lse - g) - g_H (ln p_v + H))). With t = ln p / ln 2 = c x - lse / ln 2, one
         // fused operation, it is 2^t (a + b t), a = scale (g_lse - g - g_H H), b = -scale g_H ln 2. What the roundings of c
         // and lse / ln 2 leave is one number for a row (where p counts, x is near lse / scale): 2^ of it goes into a and b.
+        // It grows with lse, and from some 2^30 would leave fp32's range. A row whose |lse| is above 2^24 (a step of it is 2
+        // or more: rows at a large mask value and nothing else) has its difference formed from lse itself: scale x rounded to
+        // fp32 before lse is taken off, as it was when lse was rounded, so that z <= lse stays true and p <= 1.
         //
         // L threads take a chunk of kBackPacks packs each and need no others: chunks are handed out in the order of
         // memory. Measured on a B200: 4096 x 131072 fp32 643 us, 2048 x 50257 bf16 63 us, HBM-bound. The bound of 40
         // registers (6 blocks of 8 warps an SM) is what took the second one from 148 to 78, the fused exponents the rest.
         constexpr int kBackPacks = 4;
+
+        __device__ __forceinline__ bool isFar(float lse)
+        {
+            return !(fabsf(lse) <= 0x1p24f);
+        }
 
         template<typename T, int L>
         __global__ void __launch_bounds__(kBlock, 6) logprobBackwardKernel(BackwardArgs a)
@@ -902,7 +910,7 @@ namespace a3b
             uint32_t const id = blockIdx.x * (kBlock / L) + threadIdx.x / L, lane = threadIdx.x & (L - 1u);
             if(id >= a.total)
                 return;
-            uint32_t const r = id / a.chunks, chunk = id - r * a.chunks, base = chunk * span;
+            uint32_t const r = id / a.chunks, base = (id - r * a.chunks) * span;
             T const* const row = static_cast<T const*>(a.logits) + a.layout.at(r);
             T* const out = static_cast<T*>(a.grad) + a.gradLayout.at(r);
             // packs on the 16-byte boundaries of the output row, as in the forward pass; the input row may lie differently
@@ -918,21 +926,57 @@ namespace a3b
             float const gl = a.gradLse && !nothing ? a.gradLse[r] : 0.0f;
             float const gh = a.gradEntropy && !nothing ? a.gradEntropy[r] : 0.0f;
             float const h = a.gradEntropy ? a.entropy[r] : 0.0f;
-            if(!(fabsf(lse) <= 0x1p80f) && !nothing)
+            if(isFar(lse) && !nothing)
             {
-                // Infinite or NaN lse, or a row of huge logits (masks of fp32's lowest value and nothing else): element by
-                // element. The product is rounded on its own, as lse is: the largest logit is exactly at 0 then.
-                // Chunks are counted for a row that starts on a boundary; one with a head may have a pack less, and its last
-                // chunk none at all: that chunk alone takes what is behind the packs, so each element has one writer (in
-                // place a second one would read the first one's gradient).
-                uint64_t const from = base == 0 ? 0 : head + static_cast<uint64_t>(min(packs, base)) * E;
-                uint64_t const to
-                    = chunk + 1 == a.chunks ? a.vocab : head + static_cast<uint64_t>(min(packs, base + span)) * E;
-                for(uint64_t i = from + lane; i < to; i += L)
+                // A branch of its own: sharing the other rows' loads and stores cost those 2 to 4%. Whatever has one writer
+                // there has the same one here. With infinite lse the entropy is NaN, but what has no probability has no
+                // gradient: it counts as 0, and the infinite logits' own t is NaN.
+                float const b = -a.scale * gh, a0 = fmaf(b, lse == INFINITY ? 0.0f : h, a.scale * (gl - g)), own = a.scale * g;
+                uint32_t const at = static_cast<uint32_t>(target); // without a token `own` is 0
+                auto one = [&](float x, uint32_t v)
                 {
-                    float const t = __fmul_rn(toFloat(row[i]), a.scale) - lse, p = expf(t);
-                    float const d = p == 0.0f ? 0.0f : p * ((gl - g) - gh * (t + h));
-                    out[i] = fromFloat<T>(a.scale * (counts && static_cast<uint64_t>(target) == i ? g + d : d));
+                    float const t = maxNan(__fmul_rn(x, a.scale) - lse, -200.0f);
+                    float const d = exp2Approx(t * kLog2e) * fmaf(t, b, a0);
+                    return v == at ? d + own : d;
+                };
+                auto gradOf = [&](float2 x, uint32_t v) { return make_float2(one(x.x, v), one(x.y, v + 1)); };
+                constexpr int ahead = E == 4 ? 2 : kBackPacks; // loads in flight; more cost the other rows of fp32 10%
+#pragma unroll 1
+                for(int p0 = 0; p0 < kBackPacks; p0 += ahead)
+                {
+                    unsigned q[ahead][4];
+#pragma unroll
+                    for(int p = 0; p < ahead; ++p)
+                    {
+                        uint32_t const k = base + (p0 + p) * L + lane;
+                        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                        if(k < packs && alike)
+                            v = __ldcs(reinterpret_cast<uint4 const*>(row + head) + k);
+                        q[p][0] = v.x, q[p][1] = v.y, q[p][2] = v.z, q[p][3] = v.w;
+                    }
+#pragma unroll
+                    for(int p = 0; p < ahead; ++p)
+                    {
+                        uint32_t const k = base + (p0 + p) * L + lane, first = head + k * E;
+                        if(k >= packs)
+                            break;
+                        if(!alike)
+                        {
+#pragma unroll
+                            for(int e = 0; e < E; ++e)
+                                PackOf<T>::setRaw(q[p], e, row + first + e);
+                        }
+#pragma unroll
+                        for(int w = 0; w < PackOf<T>::pairs; ++w)
+                            PackOf<T>::setPair(q[p], w, gradOf(PackOf<T>::pair(q[p], w), first + 2 * w));
+                        __stcs(reinterpret_cast<uint4*>(out + head) + k, make_uint4(q[p][0], q[p][1], q[p][2], q[p][3]));
+                    }
+                }
+                // the elements in front of and behind the packs, by the threads of the row's first chunk
+                for(uint32_t j = lane; base == 0 && j < head + tail; j += L)
+                {
+                    uint32_t const v = j < head ? j : a.vocab - tail + j - head;
+                    out[v] = fromFloat<T>(gradOf(make_float2(toFloat(row[v]), 0.0f), v).x);
                 }
                 return;
             }

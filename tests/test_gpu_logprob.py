@@ -629,3 +629,59 @@ def test_entropy_and_lse_alone_of_far_logits(cuda):
             # both within check_far's bounds; a masked token's logp or a row's lse may be of any size
             size = full[k].abs().double()
             close(some[k], full[k], 2 * (3 * (20011 / 64 + 120 + 32) * U * (1 + math.log(20012) + 32) + 4 * U * size))
+
+
+def check_far_backward(x, t, scale, seed=3):
+    """As check_backward, with two things more. Above |lse| = 2^24 the documented product is rounded to fp32 as lse was. Below
+    it the rest that goes into the factors (|rest| <= 2^-22 |lse|, three roundings of 2^-24 each and their ln 2) puts an
+    error of less than 2^-44 |lse| on every p. And a power below 2^-126 is flushed to zero (2^-122 with the rest's 2^4 at
+    most apart from it): what has so small a p is off by its own term at most. Returns p; in place gives the same bits."""
+    from alpaka3_b200 import algo
+    f = forward(x, t, scale=scale)
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    g = [torch.randn(len(x), generator=gen, device="cuda") for _ in range(3)]
+    args = dict(entropy=f["entropy"], grad_logp=g[0], grad_entropy=g[1], grad_lse=g[2], scale=scale)
+    res = torch.full_like(x, 55.0)
+    algo.token_logprobs_backward(res, x, t, f["lse"], **args)
+    lse, ent = f["lse"].double()[:, None], f["entropy"].double()[:, None]
+    counts = ((t >= 0) & (t < x.shape[-1]))[:, None]
+    gp, gh, gl = (k.double()[:, None] for k in g)
+    gp = torch.where(counts, gp, torch.zeros_like(gp))
+    z = x.double() * scale
+    rounded = (x.double() * torch.tensor(scale, dtype=torch.float32).double().item()).float().double()
+    q = torch.where(lse.abs() > 2.0**24, rounded, z) - lse
+    p = q.exp()
+    want = p * ((gl - gp) - gh * (q + ent))
+    want.scatter_add_(1, t.clamp(min=0)[:, None], gp)
+    want *= scale
+    mag = (gl.abs() + gp.abs() + (gh * ent).abs()) + (gh * q).abs()
+    rest = lse.abs() * 2.0**-44 * (lse.abs() <= 2.0**24)
+    step = torch.finfo(x.dtype).eps / 2
+    tol = scale * p * (mag * (2.0**-21 * (1 + q.abs()) + rest) + gh.abs() * rest) + want.abs() * (step + 2 * U)
+    tol = tol + gp.abs() * scale * 2 * U + torch.finfo(x.dtype).tiny * max(step * 2, 2.0**-8)
+    close(res, want, tol + scale * (p * mag).where(p < 2.0**-122, torch.zeros_like(p)))
+    y = x.clone()
+    algo.token_logprobs_backward(y, y, t, f["lse"], **args)
+    assert torch.equal(y, res)
+    return p
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.7, 1 / 0.3, 10.0, 1e6])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [5, 300, 2100, 9001, 50257])
+def test_gradient_of_far_logits(cuda, dtype, v, scale):
+    if dtype == torch.float16 and scale > 100:
+        pytest.skip("the gradients leave fp16's range")
+    x, t = far_rows(v, dtype, scale)
+    t[::7] = -100
+    p = check_far_backward(x, t, scale)
+    # z <= lse stays true of the rounded numbers, so no probability is far above 1 however large lse's own step is
+    assert p.max().item() <= math.exp(2.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [64, 130, 257])
+def test_gradient_of_far_logits_in_many_short_rows(cuda, dtype, v):
+    x, t = far_rows(v, dtype, 0.7)
+    again = torch.arange(2053, device="cuda") % len(x)
+    check_far_backward(x[again], t[again], 0.7)
