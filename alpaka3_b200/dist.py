@@ -146,11 +146,14 @@ def combine_norm(partial, kind="l2"):
 
 def clip_grad_norm(norm, tensors, max_norm, kind="l2"):
     """algo.clip_grad_norm for gradients sharded over the ranks (every element on one rank): the norm over all ranks'
-    tensors, each rank's own scaled by the factor that follows from it."""
+    tensors (norm None: not written), each rank's own scaled by the factor that follows from it. A rank may have none."""
     from . import algo
     if not isinstance(tensors, algo.TensorList):
         tensors = algo.TensorList(tensors)
-    partial = torch.empty(1, dtype=torch.float64, device=norm.device)
+    device = norm.device if norm is not None else tensors.device
+    if device is None:  # nothing here says where: the rank's own device
+        device = torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available() else torch.device("cpu")
+    partial = torch.empty(1, dtype=torch.float64, device=device)
     algo.grad_norm(None, tensors, kind, partial=partial)
     combine_norm(partial, kind)
     return algo.clip_grads(norm, tensors, partial, max_norm, kind)

@@ -219,3 +219,71 @@ def test_combined_norm_two_ranks():
 def test_combined_norm_one_rank():
     from alpaka3_b200 import dist as ad
     assert ad.combine_norm(torch.tensor([4.0], dtype=torch.float64)).item() == 4.0
+
+
+class _CpuList:
+    """Stands for algo.TensorList where there is no GPU."""
+
+    def __init__(self, inputs):
+        self.inputs = list(inputs)
+        self.device = self.inputs[0].device if self.inputs else None
+
+
+def _cpu_grad_norm(norm, tensors, kind="l2", partial=None):
+    x = torch.cat([t.double().flatten() for t in tensors.inputs] + [torch.zeros(1, dtype=torch.float64)])
+    partial.copy_((x.square().sum() if kind == "l2" else x.abs().max()).reshape(1))
+
+
+def _cpu_clip_grads(norm, tensors, partial, max_norm, kind="l2"):
+    value = partial.sqrt() if kind == "l2" else partial
+    for t in tensors.inputs:
+        t.mul_(min(1.0, max_norm / (value.item() + 1e-6)))
+    return None if norm is None else norm.copy_(value)
+
+
+def _clip_worker(rank, port, q):
+    """dist.clip_grad_norm on gloo with the kernels' calls replaced: rank 1 has no shard."""
+    import torch.distributed as td
+
+    from alpaka3_b200 import algo
+    from alpaka3_b200 import dist as ad
+    algo.TensorList, algo.grad_norm, algo.clip_grads = _CpuList, _cpu_grad_norm, _cpu_clip_grads
+    td.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=2)
+    try:
+        got = []
+        for given in (False, True):
+            for kind in ("l2", "max"):
+                shard = [] if rank else [torch.full((8,), 3.0), torch.full((2,), 4.0)]
+                norm = torch.zeros(1) if given else None
+                res = ad.clip_grad_norm(norm, shard, 1.0, kind)
+                got.append((None if res is None else res.item(), [t[0].item() for t in shard]))
+        q.put((rank, got))
+        q.close()
+        q.join_thread()
+    finally:
+        td.destroy_process_group()
+
+
+def test_sharded_clipping_two_ranks():
+    """Every rank takes the same steps: with and without a norm to write, with and without a shard."""
+    import socket
+
+    import torch.multiprocessing as mp
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_clip_worker, args=(r, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    got = dict(q.get(timeout=120) for _ in procs)
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    total = math.sqrt(8 * 9 + 2 * 16)
+    for rank in range(2):
+        for (norm, values), given, size in zip(got[rank], (False, False, True, True), (total, 4.0, total, 4.0)):
+            assert (abs(norm - size) <= 2.0**-23 * size) if given else norm is None
+            want = [] if rank else [3.0 / size, 4.0 / size]
+            assert len(values) == len(want) and all(abs(a - b) <= 1e-5 for a, b in zip(values, want))
