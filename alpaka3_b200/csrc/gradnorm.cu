@@ -136,6 +136,7 @@ namespace a3b
             }
         }
 
+        // the product in fp32, or, where the factor is an fp64 number, in fp64 and rounded to fp32 before T
         template<typename T, typename F>
         __device__ __forceinline__ void scalePack(unsigned* q, F factor)
         {
@@ -148,10 +149,16 @@ namespace a3b
             }
             else
             {
-                float2 const f2 = make_float2(factor, factor);
+                auto scaled = [&](float2 v)
+                {
+                    if constexpr(std::is_same_v<F, double>)
+                        return make_float2(static_cast<float>(v.x * factor), static_cast<float>(v.y * factor));
+                    else
+                        return mul2(v, make_float2(factor, factor));
+                };
 #pragma unroll
                 for(int w = 0; w < PackOf<T>::pairs; ++w)
-                    PackOf<T>::setPair(q, w, mul2(PackOf<T>::pair(q, w), f2));
+                    PackOf<T>::setPair(q, w, scaled(PackOf<T>::pair(q, w)));
             }
         }
 
@@ -384,10 +391,25 @@ namespace a3b
             Chunk<T> x;
             int const lead = leadOf(e.out, sizeof(T));
             x.load(static_cast<T const*>(e.in), e.n, lead, c, lead == leadOf(e.in, sizeof(T)));
-            using S = std::conditional_t<std::is_same_v<T, double>, double, float>;
+            if constexpr(std::is_same_v<T, double>)
+            {
 #pragma unroll
-            for(int p = 0; p < kPacks; ++p)
-                scalePack<T>(x.q[p], static_cast<S>(factor));
+                for(int p = 0; p < kPacks; ++p)
+                    scalePack<T>(x.q[p], factor);
+            }
+            else if(factor >= static_cast<double>(FLT_MIN) || !(factor > 0.0))
+            {
+#pragma unroll
+                for(int p = 0; p < kPacks; ++p)
+                    scalePack<T>(x.q[p], static_cast<float>(factor));
+            }
+            else
+            {
+                // below fp32's normal numbers (norms of 1e38 and more, from elements near FLT_MAX) the factor would lose bits
+#pragma unroll
+                for(int p = 0; p < kPacks; ++p)
+                    scalePack<T>(x.q[p], factor);
+            }
             x.store(static_cast<T*>(e.out), e.n, lead, c);
         }
 

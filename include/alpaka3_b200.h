@@ -330,7 +330,7 @@ A3B_API int a3b_grad_norm(a3b_stream_t stream, a3b_tensor_list const* list, int 
 
 /* out = in * min(1, max_norm / (norm + 1e-6)) for every tensor of the list, with the norm that `partial` (one double on
  * the device, as a3b_grad_norm leaves it or combined over ranks) stands for; the product is formed in fp32 (fp64 for
- * A3B_F64) and rounded once. Tensors in place are not touched where the factor is 1. norm: null, or one element that
+ * A3B_F64, and for a factor below 2^-126) and rounded once. Tensors in place are not touched where the factor is 1. norm: null, or one element that
  * receives the norm. A NaN norm makes every output NaN. The outputs may not overlap one another, and each must be its
  * own input or overlap no input (A3B_ERR_INVALID). max_norm: not negative, not NaN. */
 A3B_API int a3b_clip_grads(a3b_stream_t stream, a3b_tensor_list const* list, int kind, double const* partial,

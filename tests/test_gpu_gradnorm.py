@@ -339,3 +339,18 @@ def test_tail_of_a_training_step(cuda):
     algo.clip_grad_norm(norm, grads, total / 10)
     assert abs(norm.item() - total) <= REL["l2"] * total
     assert abs(exact(grads, "l2") - total / 10) <= 2.0**-8 * total / 10
+
+
+@pytest.mark.parametrize("kind", ["l2", "l1", "max"])
+@pytest.mark.parametrize("dtype", [BF, SF])
+@pytest.mark.parametrize("n", [4099, 300001])
+def test_factors_below_the_normal_numbers(cuda, kind, dtype, n):
+    """Elements near fp32's largest number: max_norm / norm is below 2^-126, and has all its bits. In one cluster and in a
+    block for every chunk."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    for limit in (1.0, 37.0, 1e-3):
+        x = (torch.rand(n, generator=g, device="cuda") * 3e38).to(dtype)
+        small = torch.randn(77, generator=g, device="cuda").to(dtype)
+        outs = [torch.full_like(x, 9.0), torch.full_like(small, 9.0)]
+        check([x, small], limit, kind, outs, norm_dtype=DF)
+        check([x, small], limit, kind, norm_dtype=DF)
