@@ -545,6 +545,14 @@ namespace a3b
             return std::min<uint32_t>(b.chunks, static_cast<uint32_t>(props->smCount) * kBlocksPerSm);
         }
 
+        // whether two stretches of memory share a byte; a null one shares none
+        bool overlap(void const* a, size_t an, void const* b, size_t bn)
+        {
+            auto const x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+            return a && b && (x < y ? y - x < an : x - y < bn);
+        }
+
+        // A block that has the norm writes it while others still read what it comes from: the two lie apart.
         int checkCall(a3b_tensor_list const* list, int kind, double const* partial, int normDtype, void const* norm)
         {
             A3B_REQUIRE(list, "null tensor list");
@@ -553,6 +561,7 @@ namespace a3b
             A3B_REQUIRE(reinterpret_cast<uintptr_t>(norm) % (normDtype == A3B_F64 ? 8u : 4u) == 0u
                             && reinterpret_cast<uintptr_t>(partial) % 8u == 0u,
                         "norm or partial is not aligned to its type");
+            A3B_REQUIRE(!overlap(norm, normDtype == A3B_F64 ? 8u : 4u, partial, 8u), "norm and partial overlap");
             return A3B_OK;
         }
 
@@ -807,7 +816,10 @@ extern "C"
         int const rd = currentDevice(&props);
         if(rd != A3B_OK)
             return rd;
-        A3B_REQUIRE(workspace_bytes >= workspaceOf(list, props), "workspace is too small");
+        size_t const used = workspaceOf(list, props);
+        A3B_REQUIRE(workspace_bytes >= used, "workspace is too small");
+        A3B_REQUIRE(!overlap(workspace, used, norm, norm_dtype == A3B_F64 ? 8u : 4u) && !overlap(workspace, used, partial, 8u),
+                    "norm or partial lies in the workspace");
         auto s = static_cast<cudaStream_t>(stream);
         return withKind(kind, [&](auto k) {
             auto* const partials = static_cast<double*>(workspace);
@@ -864,7 +876,9 @@ extern "C"
         int const rd = currentDevice(&props);
         if(rd != A3B_OK)
             return rd;
-        A3B_REQUIRE(workspace_bytes >= workspaceOf(list, props), "workspace is too small");
+        size_t const used = workspaceOf(list, props);
+        A3B_REQUIRE(workspace_bytes >= used, "workspace is too small");
+        A3B_REQUIRE(!overlap(workspace, used, norm, norm_dtype == A3B_F64 ? 8u : 4u), "norm lies in the workspace");
         auto s = static_cast<cudaStream_t>(stream);
         return withKind(kind, [&](auto k) {
             return launchBoth<k()>(s, list, props, max_norm, static_cast<double*>(workspace), norm_dtype, norm);

@@ -324,7 +324,8 @@ A3B_API size_t a3b_grad_norm_workspace(a3b_tensor_list const* list);
 /* Norm of the whole list, held in fp64 and rounded once to norm (one element of norm_dtype, A3B_F32 or A3B_F64).
  * partial: null, or one double that receives sum x^2, sum |x| or max |x| unrounded, to be combined across ranks (sum,
  * sum, max) before a3b_clip_grads. Either of norm and partial may be null. Squares that leave fp32's range are formed
- * in fp64. The order of the sum depends on the list and the device alone: repeated calls give the same bits. */
+ * in fp64. The order of the sum depends on the list and the device alone: repeated calls give the same bits. Here and
+ * below norm, partial and the workspace lie apart from one another (A3B_ERR_INVALID) and from the tensors. */
 A3B_API int a3b_grad_norm(a3b_stream_t stream, a3b_tensor_list const* list, int kind, void* workspace,
                           size_t workspace_bytes, double* partial, int norm_dtype, void* norm);
 

@@ -354,3 +354,21 @@ def test_factors_below_the_normal_numbers(cuda, kind, dtype, n):
         outs = [torch.full_like(x, 9.0), torch.full_like(small, 9.0)]
         check([x, small], limit, kind, outs, norm_dtype=DF)
         check([x, small], limit, kind, norm_dtype=DF)
+
+
+def test_workspace_apart_from_the_results(cuda):
+    from alpaka3_b200 import algo, capi
+    L, x = capi.lib(), torch.ones(1 << 20, device="cuda")
+    lst = algo.TensorList([x])
+    need = L.a3b_grad_norm_workspace(lst._handle)
+    ws = torch.zeros(need + 64, dtype=torch.uint8, device="cuda")
+    out = torch.zeros(1, dtype=DF, device="cuda")
+    s, p, stream = ws.data_ptr(), out.data_ptr(), algo.stream_handle()
+    for call in (lambda at: L.a3b_grad_norm(stream, lst._handle, 0, s, ws.numel(), p, capi.F32, at),
+                 lambda at: L.a3b_grad_norm(stream, lst._handle, 0, s, ws.numel(), at, capi.F64, p),
+                 lambda at: L.a3b_clip_grad_norm(stream, lst._handle, 0, 1e9, s, ws.numel(), capi.F64, at)):
+        for at in (s, s + need - 8):
+            assert call(at) == capi.ERR_INVALID and "workspace" in capi.last_error()
+        assert call(s + need) == capi.OK  # behind what is used
+    torch.cuda.synchronize()
+    assert ws.view(DF)[need // 8].item() == 1024.0 and (x == 1).all()

@@ -287,3 +287,19 @@ def test_sharded_clipping_two_ranks():
             assert (abs(norm - size) <= 2.0**-23 * size) if given else norm is None
             want = [] if rank else [3.0 / size, 4.0 / size]
             assert len(values) == len(want) and all(abs(a - b) <= 1e-5 for a, b in zip(values, want))
+
+
+def test_norm_and_partial_apart(L):
+    """The norm is written while other blocks still read the partial: one stretch of memory for both is refused."""
+    from alpaka3_b200 import capi
+    F, D = capi.F32, capi.F64
+    rc, h = make(L, [0x40000000], None, [100], [F])
+    assert rc == capi.OK
+    at = lambda d: ctypes.c_void_p(0x10000000 + d)  # noqa: E731
+    for dtype, d, hit in ((D, 0, True), (F, 0, True), (F, 4, True), (D, 8, False), (F, 8, False), (F, -4, False),
+                          (D, -8, False)):
+        for call in (lambda: L.a3b_clip_grads(None, h, 0, P, math.nan, dtype, at(d)),  # refused for its limit if not before
+                     lambda: L.a3b_grad_norm(None, h, 0, None, 0, P, dtype, at(d))):  # ... for the lack of a workspace
+            assert call() == capi.ERR_INVALID
+            assert ("overlap" in capi.last_error()) == hit, (dtype, d, capi.last_error())
+    L.a3b_tensor_list_destroy(h)
