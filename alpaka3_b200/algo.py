@@ -374,18 +374,25 @@ class TensorList:
     """A list of CUDA tensors (float32, float64, float16, bfloat16, mixed as needed, of one device) for grad_norm,
     clip_grads and clip_grad_norm, with the tensors that receive the clipped values: `outputs`, with the dtypes, shapes
     and strides of `inputs`, or the inputs themselves (in place). Each tensor must be dense (its elements fill one
-    stretch of memory, in any order of dimensions).
+    stretch of memory, in any order of dimensions). A None among the inputs (a parameter without a gradient) is left out,
+    and what stands in its place in `outputs` with it.
 
     Making one costs the host about a microsecond per tensor; a program whose gradients stay where they are makes it
     once. It holds the addresses of the tensors as they are now, and keeps those tensors alive."""
 
     def __init__(self, inputs, outputs=None):
         self._handle = None
-        ins = self.inputs = list(inputs)
-        outs = self.outputs = ins if outputs is None else list(outputs)
-        n = len(ins)
-        if len(outs) != n:
+        ins = list(inputs)
+        outs = ins if outputs is None else list(outputs)
+        if len(outs) != len(ins):
             raise ValueError("inputs and outputs must be equally many")
+        if any(t is None for t in ins):
+            given = [k for k, t in enumerate(ins) if t is not None]
+            same = outs is ins
+            ins = [ins[k] for k in given]
+            outs = ins if same else [outs[k] for k in given]
+        self.inputs, self.outputs = ins, outs
+        n = len(ins)
         self.device = ins[0].device if n else None
         index = ins[0].get_device() if n else -1
         codes = [_GRAD_DT.get(t.dtype, -1) for t in ins]

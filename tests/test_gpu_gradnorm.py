@@ -372,3 +372,21 @@ def test_workspace_apart_from_the_results(cuda):
         assert call(s + need) == capi.OK  # behind what is used
     torch.cuda.synchronize()
     assert ws.view(DF)[need // 8].item() == 1024.0 and (x == 1).all()
+
+
+def test_gradients_of_a_model_of_which_some_are_missing(cuda):
+    """A plain sequence of gradients with None among them, in place and to outputs of their own."""
+    from alpaka3_b200 import algo
+    params = [torch.nn.Parameter(torch.randn(k, device="cuda")) for k in (100, 7, 1, 50000)]
+    for p in (params[0], params[3]):
+        p.grad = torch.randn_like(p)
+    grads = [p.grad for p in params]
+    given = [grads[0].clone(), grads[3].clone()]
+    want, norm = exact(given, "l2"), torch.empty(1, device="cuda")
+    outs = [torch.full((k,), 9.0, device="cuda") for k in (100, 7, 1, 50000)]
+    algo.clip_grad_norm(norm, algo.TensorList(grads, outs), want / 2)
+    assert abs(norm.item() - want) <= REL["l2"] * want and (outs[1] == 9).all() and (outs[2] == 9).all()
+    algo.clip_grad_norm(norm, grads, want / 2)
+    assert abs(norm.item() - want) <= REL["l2"] * want and params[1].grad is None
+    for o, g, b in ((outs[0], grads[0], given[0]), (outs[3], grads[3], given[1])):
+        assert torch.equal(o, g) and ((g - b / 2).abs() <= b.abs() * 8 * U).all()

@@ -303,3 +303,14 @@ def test_norm_and_partial_apart(L):
             assert call() == capi.ERR_INVALID
             assert ("overlap" in capi.last_error()) == hit, (dtype, d, capi.last_error())
     L.a3b_tensor_list_destroy(h)
+
+
+def test_parameters_without_a_gradient():
+    """[p.grad for p in parameters] may hold None: such a parameter is left out, with its output."""
+    from alpaka3_b200 import algo
+    assert len(algo.TensorList([None, None])) == 0 and algo.TensorList([None]).device is None
+    assert len(algo.TensorList([None], [torch.zeros(3)])) == 0
+    with pytest.raises(ValueError, match="equally many"):
+        algo.TensorList([None], [])
+    with pytest.raises(ValueError, match="CUDA"):  # what is left is checked as ever
+        algo.TensorList([None, torch.zeros(3)])
