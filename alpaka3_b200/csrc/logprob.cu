@@ -814,9 +814,10 @@ namespace a3b
         // 1000 bf16 with 3 38 / 49; but 100 rows of 500 6.9 / 4.2). More alternatives than half the team's threads are
         // badly bounded by its thread maxima. Other rows of up to 64 packs take tiles of two packs a thread, whose kernel
         // has fewer registers (16 / 18 us for 32768 x 257).
-        // Few long rows are cut into slices over a cluster, as many as the GPU holds at once (a second wave costs more
-        // than a slice gains): 1 / 2 / 4 / 8 slices of 16 rows of 131072 with 20 alternatives 20 / 15 / 11 / 10, of 64
-        // fp32 rows with 5 28 / 19 / 15 / 19.
+        // Few long rows are cut into slices over a cluster, as many as keep three blocks an SM or less (a fourth fits, but more
+        // and shorter slices cost more in joining than they gain): 1 / 2 / 4 / 8 slices of 16 rows of 131072 bf16 with 20
+        // alternatives 20 / 15 / 11 / 10, of 64 fp32 rows with 5 19 / 15 / 12 / 12, of 100 of them 20 / 17 / 14 / 18, of 64 rows
+        // of 50257 bf16 11 / 10 / 8 / 10, of one row of 32000 with 20 8.5 / 7.7 / 7.6 / 8.0 (logits in L2).
         constexpr uint64_t kEnoughWarps = 8192;
 
         template<typename T>
@@ -893,7 +894,7 @@ namespace a3b
         // fp32 before lse is taken off, as it was when lse was rounded, so that z <= lse stays true and p <= 1.
         //
         // L threads take a chunk of kBackPacks packs each and need no others: chunks are handed out in the order of
-        // memory. Measured on a B200: 4096 x 131072 fp32 643 us, 2048 x 50257 bf16 63 us, HBM-bound. The bound of 40
+        // memory. Measured on a B200: 4096 x 131072 fp32 624 us, 2048 x 50257 bf16 63 us, HBM-bound. The bound of 40
         // registers (6 blocks of 8 warps an SM) is what took the second one from 148 to 78, the fused exponents the rest.
         constexpr int kBackPacks = 4;
 
@@ -940,7 +941,7 @@ namespace a3b
                     return v == at ? d + own : d;
                 };
                 auto gradOf = [&](float2 x, uint32_t v) { return make_float2(one(x.x, v), one(x.y, v + 1)); };
-                constexpr int ahead = E == 4 ? 2 : kBackPacks; // loads in flight; more cost the other rows of fp32 10%
+                constexpr int ahead = E == 4 ? 2 : kBackPacks; // loads in flight; 4 cost the other rows of fp32 10%
 #pragma unroll 1
                 for(int p0 = 0; p0 < kBackPacks; p0 += ahead)
                 {

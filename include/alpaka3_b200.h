@@ -274,8 +274,12 @@ A3B_API int a3b_scan(a3b_stream_t stream, int dtype, int inclusive, void const* 
  * A target outside [0, vocab) marks a row without a token: its logp is 0. Logits of -infinity have probability 0 (logp
  * -infinity); a row of nothing else has lse -infinity, entropy 0 and logp -infinity for every token. A NaN in a row
  * makes its lse, logp and entropy NaN. With +infinity in a row its lse is +infinity, its entropy NaN, the logp of a
- * finite logit -infinity and that of +infinity NaN. Repeated calls give the same bits; the order of a row's sums follows
- * from the number of rows, their length and alignment.
+ * finite logit -infinity and that of +infinity NaN. Logits of any finite size are as good as their own steps allow
+ * (masks of -1e9, -1e20 or the lowest value, alone or among others), as long as scale * logit is in fp32's range.
+ * Repeated calls give the same bits; the order of a row's sums follows from the number of rows, their length and
+ * alignment. The outputs may not overlap one another or the inputs.
+ * Time: one pass, but alternatives of a row in rising order enter and leave one after another (2048 rows of 50257 bf16
+ * logits with 20 alternatives: 64 us in no particular order, 3.7 ms if every row rises from its first to its last).
  * At most 2^31 - 1 rows of at most 2^31 - 65 logits (A3B_ERR_TOO_LARGE). */
 A3B_API int a3b_token_logprobs(a3b_stream_t stream, int dtype, void const* logits, uint64_t outer, uint64_t inner,
                                uint64_t vocab, int64_t outer_stride, int64_t inner_stride, double scale, int index_dtype,
@@ -287,9 +291,11 @@ A3B_API int a3b_token_logprobs(a3b_stream_t stream, int dtype, void const* logit
  * lse and entropy: as a3b_token_logprobs wrote them for the same logits, targets and scale. grad_logp, grad_entropy,
  * grad_lse: one fp32 value per row, each may be null (zero); targets may be null if grad_logp is, entropy if
  * grad_entropy is. A row without a token (target outside [0, vocab)) gets nothing from grad_logp; a row with lse
- * -infinity gets zeros. The alternatives have no gradient. grad_logits has the logits' dtype, rounded once, and its
- * own strides; its rows may not overlap. It may be the logits themselves (same address and strides: in place) or must
- * lie wholly before or behind them. */
+ * -infinity gets zeros. Above |lse| = 2^24, where lse's own steps are 2 and more, scale * x is rounded to fp32 before lse
+ * is taken off, as it was when lse was rounded: p stays at most 1. The alternatives have no gradient. grad_logits has the
+ * logits' dtype, rounded once, and its own strides; its rows may not overlap. It may be the logits themselves (same
+ * address and strides: in place) or must lie wholly before or behind them; it may not overlap the arrays of one value per
+ * row. */
 A3B_API int a3b_token_logprobs_backward(a3b_stream_t stream, int dtype, void const* logits, uint64_t outer, uint64_t inner,
                                         uint64_t vocab, int64_t outer_stride, int64_t inner_stride, double scale,
                                         int index_dtype, void const* targets, float const* lse, float const* entropy,
@@ -331,9 +337,9 @@ A3B_API int a3b_grad_norm(a3b_stream_t stream, a3b_tensor_list const* list, int 
 
 /* out = in * min(1, max_norm / (norm + 1e-6)) for every tensor of the list, with the norm that `partial` (one double on
  * the device, as a3b_grad_norm leaves it or combined over ranks) stands for; the product is formed in fp32 (fp64 for
- * A3B_F64, and for a factor below 2^-126) and rounded once. Tensors in place are not touched where the factor is 1. norm: null, or one element that
- * receives the norm. A NaN norm makes every output NaN. The outputs may not overlap one another, and each must be its
- * own input or overlap no input (A3B_ERR_INVALID). max_norm: not negative, not NaN. */
+ * A3B_F64, and for a factor below 2^-126) and rounded once. Tensors in place are not touched where the factor is 1. norm:
+ * null, or one element that receives the norm. A NaN norm makes every output NaN. The outputs may not overlap one
+ * another, and each must be its own input or overlap no input (A3B_ERR_INVALID). max_norm: not negative, not NaN. */
 A3B_API int a3b_clip_grads(a3b_stream_t stream, a3b_tensor_list const* list, int kind, double const* partial,
                            double max_norm, int norm_dtype, void* norm);
 
