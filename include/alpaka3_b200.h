@@ -291,7 +291,8 @@ A3B_API int a3b_token_logprobs(a3b_stream_t stream, int dtype, void const* logit
  * lse and entropy: as a3b_token_logprobs wrote them for the same logits, targets and scale. grad_logp, grad_entropy,
  * grad_lse: one fp32 value per row, each may be null (zero); targets may be null if grad_logp is, entropy if
  * grad_entropy is. A row without a token (target outside [0, vocab)) gets nothing from grad_logp; a row with lse
- * -infinity gets zeros. Above |lse| = 2^24, where lse's own steps are 2 and more, scale * x is rounded to fp32 before lse
+ * -infinity gets zeros; with lse +infinity the finite logits get what grad_logp gives their own token, else 0, and the
+ * infinite ones NaN; with lse NaN all are NaN. Above |lse| = 2^24, where lse's own steps are 2 and more, scale * x is rounded to fp32 before lse
  * is taken off, as it was when lse was rounded: p stays at most 1. The alternatives have no gradient. grad_logits has the
  * logits' dtype, rounded once, and its own strides; its rows may not overlap. It may be the logits themselves (same
  * address and strides: in place) or must lie wholly before or behind them; it may not overlap the arrays of one value per

@@ -685,3 +685,55 @@ def test_gradient_of_far_logits_in_many_short_rows(cuda, dtype, v):
     x, t = far_rows(v, dtype, 0.7)
     again = torch.arange(2053, device="cuda") % len(x)
     check_far_backward(x[again], t[again], 0.7)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [5, 130, 1032, 4099])
+def test_gradient_of_far_logits_to_other_alignments(cuda, dtype, v):
+    """The gradient's rows may start and step differently from the logits': the same bits, the neighbours untouched."""
+    from alpaka3_b200 import algo
+    x, t = far_rows(v, dtype, 1.0)
+    f = forward(x, t)
+    one = torch.ones(len(x), device="cuda")
+    args = dict(entropy=f["entropy"], grad_logp=one, grad_entropy=0.5 * one, grad_lse=-one)
+    want = torch.full_like(x, 55.0)
+    algo.token_logprobs_backward(want, x, t, f["lse"], **args)
+    for a, b, pitch in ((0, 1, v + 3), (3, 0, v + 5), (1, 2, v + 8), (2, 2, v + 4)):
+        src = torch.zeros(len(x), pitch, dtype=dtype, device="cuda")
+        src[:, a:a + v] = x
+        out = torch.full((len(x), v + 11), 9.0, dtype=dtype, device="cuda")
+        algo.token_logprobs_backward(out[:, b:b + v], src[:, a:a + v], t, f["lse"], **args)
+        assert torch.equal(out[:, b:b + v], want), (a, b)
+        assert (out[:, :b] == 9).all() and (out[:, b + v:] == 9).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,v", [(6, 6), (6, 1033), (6, 9000), (2052, 130)])
+def test_gradient_of_infinities_and_nan(cuda, dtype, rows, v):
+    """A NaN makes its row's gradient NaN. Beside +infinity nothing else has a probability: a gradient of 0 but for the
+    token's own term; what is infinite has none that is a number. Without and with the entropy, which is NaN there."""
+    from alpaka3_b200 import algo
+    x, t = make(rows, v, dtype)
+    x[0::6, v // 2] = math.nan
+    x[1::6, v - 1] = INF
+    x[2::6, 0], x[2::6, v // 3] = INF, INF
+    x[3::6, v // 2], x[3::6, 1] = INF, math.nan
+    x[4::6] = -INF
+    t[1::6], t[2::6] = 1, 0
+    f = forward(x, t)
+    one = torch.ones(rows, device="cuda")
+    for more in ({}, dict(entropy=f["entropy"], grad_entropy=one), dict(grad_lse=one)):
+        g = torch.full_like(x, 55.0)
+        algo.token_logprobs_backward(g, x, t, f["lse"], grad_logp=3 * one, scale=1.0, **more)
+        assert torch.isnan(g[0::6]).all() and torch.isnan(g[3::6]).all() and (g[4::6] == 0).all()
+        assert torch.isfinite(g[5::6]).all()
+        for k, holes in ((1, [v - 1]), (2, [0, v // 3])):
+            want = torch.zeros(v, device="cuda")
+            if k == 1:
+                want[1] = 3.0  # the token's own term
+            want[holes] = math.nan
+            for row in g[k::6].float():
+                assert torch.equal(row.nan_to_num(77.0), want.nan_to_num(77.0))
+        same = x.clone()
+        algo.token_logprobs_backward(same, same, t, f["lse"], grad_logp=3 * one, scale=1.0, **more)
+        assert torch.equal(same.nan_to_num(77.0), g.nan_to_num(77.0))
