@@ -275,7 +275,8 @@ A3B_API int a3b_scan(a3b_stream_t stream, int dtype, int inclusive, void const* 
  * -infinity); a row of nothing else has lse -infinity, entropy 0 and logp -infinity for every token. A NaN in a row
  * makes its lse, logp and entropy NaN. With +infinity in a row its lse is +infinity, its entropy NaN, the logp of a
  * finite logit -infinity and that of +infinity NaN. Logits of any finite size are as good as their own steps allow
- * (masks of -1e9, -1e20 or the lowest value, alone or among others), as long as scale * logit is in fp32's range.
+ * (masks of -1e9, -1e20 or the lowest value, alone or among others); where scale * logit is beyond fp32's range it is
+ * infinite: in a row of nothing but such masks lse is -infinity, and the gradient 0.
  * Repeated calls give the same bits; the order of a row's sums follows from the number of rows, their length and
  * alignment. The outputs may not overlap one another or the inputs.
  * Time: one pass, but alternatives of a row in rising order enter and leave one after another (2048 rows of 50257 bf16

@@ -737,3 +737,33 @@ def test_gradient_of_infinities_and_nan(cuda, dtype, rows, v):
         same = x.clone()
         algo.token_logprobs_backward(same, same, t, f["lse"], grad_logp=3 * one, scale=1.0, **more)
         assert torch.equal(same.nan_to_num(77.0), g.nan_to_num(77.0))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [130, 9001])
+def test_lowest_values_at_a_temperature(cuda, dtype, v):
+    """scale * the lowest value is below fp32's range. A row of nothing else: lse -infinity, a gradient of zeros, logp and
+    entropy as for any row of one value. Beside other logits such a mask has no probability, like -infinity."""
+    scale = 1 / 0.3
+    x, t = make(4, v, dtype)
+    x[0] = torch.finfo(dtype).min
+    x[1, ::2], x[2, 3:] = torch.finfo(dtype).min, torch.finfo(dtype).min
+    t[1], t[2] = 1, 4  # a token that is left, and a masked one
+    got = forward(x, t, 3, scale)
+    masked = x.masked_fill(x == torch.finfo(dtype).min, -INF)
+    q, lse, h = oracle(masked, scale)
+    logp = q.gather(1, t[:, None].cpu())[:, 0]
+    logp[0], h[0] = -math.log(v), math.log(v)
+    close(got["logp"], logp, tol_sum(v) + 4 * U * (logp.abs().nan_to_num(posinf=0) + 1))
+    close(got["lse"], lse, tol_sum(v) + 4 * U * (lse.abs().nan_to_num(posinf=0) + 1))
+    close(got["entropy"], h, 3 * tol_sum(v) * (1 + math.log(v + 1)))
+    assert torch.equal(got["top_index"].cpu(), ranks(x, 3))
+    from alpaka3_b200 import algo
+    one = torch.ones(4, device="cuda")
+    grads = []
+    for logits in (x, masked):
+        g = torch.full_like(x, 55.0)
+        algo.token_logprobs_backward(g, logits, t, got["lse"], entropy=got["entropy"], grad_logp=one, grad_entropy=one,
+                                     grad_lse=-one, scale=scale)
+        grads.append(g)
+    assert (grads[0][0] == 0).all() and torch.isfinite(grads[0]).all() and torch.equal(grads[0], grads[1])
