@@ -19,6 +19,10 @@ Reductions of a language model's training and decoding steps, which alpaka3 does
                               log-sum-exp and most likely alternatives, and their gradient
 * :class:`TensorList`, :func:`grad_norm`, :func:`clip_grads`, :func:`clip_grad_norm`  norm and clipping of a list of
                               gradients
+* :func:`rms_norm`, :func:`rms_norm_backward`  root-mean-square norm of rows with the residual's addition, also with an
+                              output in 8 bits, and its gradient
+* :func:`embedding`, :func:`embedding_backward`  rows of a table by tokens, and the table's gradient
+* :func:`verify_drafts`       drafted tokens against the target's probabilities, from given random numbers
 
 Errors raise :class:`alpaka3_b200.capi.A3BError` (the reference throws std::runtime_error on backend errors).
 """
@@ -42,6 +46,7 @@ NORM = {"l2": capi.NORM_L2, "l1": capi.NORM_L1, "max": capi.NORM_MAX}
 _LOGITS_DT = {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
 _GRAD_DT = {**_LOGITS_DT, torch.float64: capi.F64}
 _INDEX_DT = {torch.int64: capi.I64, torch.int32: capi.I32}
+_NORM_OUT_DT = {**_LOGITS_DT, torch.float8_e4m3fn: capi.E4M3, torch.float8_e5m2: capi.E5M2}
 MAP = {"copy": capi.MAP_COPY, "scale": capi.MAP_SCALE, "add": capi.MAP_ADD, "mul": capi.MAP_MUL,
        "axpy": capi.MAP_AXPY, "square": capi.MAP_SQUARE}
 
@@ -502,6 +507,291 @@ def clip_grad_norm(norm, tensors, max_norm, kind="l2", stream=None):
     ws = tensors._scratch(dev, stream)
     _call_on(dev, stream, "a3b_clip_grad_norm", tensors._handle, k, max_norm, ws.data_ptr(), ws.numel(), code, n)
     return norm
+
+
+# ------------------------------------------------------------------------------------------- norm of rows
+def _joint_rows(first, *others):
+    """(outer, inner, n, [outer stride, inner stride of each]) of tensors of one shape, in two levels of rows that fit all
+    of them; each of `others` is (tensor or None, name), `first` too but never None. None has strides 0."""
+    x, name = first
+    shape = x.shape
+    given = [t for t, _ in others if t is not None]
+    if x.dim() > 0 and x.is_contiguous() and all(t.is_contiguous() for t in given):
+        n = shape[-1]
+        return 1, (x.numel() // n if n else 0), n, [(0, n)] * (1 + len(others))
+    for t, label in (first, *others):
+        if t is not None and (t.dim() < 1 or (t.shape[-1] > 1 and t.stride(-1) != 1)):
+            raise ValueError(f"{label}: rows must be contiguous in the last dimension")
+    every = [x, *given]
+    levels = []  # (size, the strides of each)
+    for d in range(x.dim() - 1):
+        size, strides = shape[d], tuple(t.stride(d) for t in every)
+        if size == 1:
+            continue
+        if levels and all(a == size * b for a, b in zip(levels[-1][1], strides)):
+            levels[-1] = (levels[-1][0] * size, strides)
+        else:
+            levels.append((size, strides))
+    if x.numel() == 0:
+        levels = []
+    if len(levels) > 2:
+        raise ValueError(f"{name}: the dimensions before the last do not collapse to two strides")
+    none = (0,) * len(every)
+    (outer, so), (inner, si) = [(1, none)] * (2 - len(levels)) + levels
+    if x.numel() == 0:
+        outer = inner = 0
+    steps = iter(zip(so, si))
+    return outer, inner, shape[-1], [next(steps) if t is not None else (0, 0) for t in (x, *(t for t, _ in others))]
+
+
+def _like(t, name, x, dev, dtype):
+    """t (None passes) has the shape of x, its device and `dtype`."""
+    if t is not None and (t.shape != x.shape or t.dtype != dtype or t.get_device() != dev):
+        raise ValueError(f"{name} must have the shape and device of the rows, and dtype {dtype}")
+
+
+def _data(t):
+    return None if t is None else t.data_ptr()
+
+
+def _row_tensor(x, name):
+    """(dtype code, device index) of a CUDA tensor of rows"""
+    code = _LOGITS_DT.get(x.dtype)
+    if code is None:
+        raise TypeError(f"unsupported {name} dtype {x.dtype}")
+    dev = x.get_device()
+    if dev < 0:
+        raise ValueError(f"{name}: expected a CUDA tensor")
+    if x.dim() < 1:
+        raise ValueError(f"{name}: expected at least one dimension")
+    return code, dev
+
+
+def _weight(weight, x, dev, name="weight"):
+    """dtype code of a weight of x's rows (that of x without one)"""
+    if weight is None:
+        return _LOGITS_DT[x.dtype]
+    if weight.dtype != x.dtype and weight.dtype != torch.float32:
+        raise TypeError(f"{name} must have the dtype of the rows, or float32")
+    if weight.get_device() != dev or weight.numel() != x.shape[-1] or not weight.is_contiguous():
+        raise ValueError(f"{name}: expected {x.shape[-1]} contiguous elements on CUDA device {dev}")
+    return _LOGITS_DT[weight.dtype]
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(entry, dev, *sizes):
+    with torch.cuda.device(dev):
+        size = getattr(capi.lib(), entry)(*sizes)
+    if size == 0:
+        raise capi.A3BError(capi.ERR_CUDA, capi.last_error(), entry)
+    return size
+
+
+def _workspace(entry, dev, stream, *sizes):
+    """Scratch for one call, from torch's allocator in the order of the call's stream."""
+    size = _workspace_bytes(entry, dev, *sizes)
+    if stream is None:
+        return torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", dev))
+    with torch.cuda.stream(stream):
+        return torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", dev))
+
+
+def rms_norm(out, x, weight=None, residual=None, total=None, rstd=None, scales=None, group=None, eps=1e-6, stream=None):
+    """Per row of x (..., n), float32 / float16 / bfloat16: h = x + residual (rounded to x's dtype), written to `total`;
+    1 / sqrt(mean h^2 + eps), written to `rstd` (float32, one per row); out = h * rstd * weight. residual, total, weight and
+    rstd are optional. weight: n elements of x's dtype or float32.
+
+    out has x's dtype, or torch.float8_e4m3fn or float8_e5m2 with `scales` (float32, contiguous, one for each `group` = 32,
+    64 or 128 elements of a row, or one a row with group None): the values are out * scale.
+
+    Rows of all tensors may be strided (heads of a wider product); out may be x or residual, and total may be residual or x
+    (in place). For the gradient keep `total` (x without a residual) and rstd. Infinities, NaN and what may overlap: see
+    a3b_rms_norm. Returns out."""
+    code, dev = _row_tensor(x, "x")
+    target = _NORM_OUT_DT.get(out.dtype)
+    if target is None:
+        raise TypeError(f"unsupported out dtype {out.dtype}")
+    if residual is not None:
+        _like(residual, "residual", x, dev, x.dtype)
+        if total is not None:
+            _like(total, "total", x, dev, x.dtype)
+    elif total is not None:
+        raise ValueError("total needs a residual")
+    if out.shape != x.shape or out.get_device() != dev:
+        raise ValueError("out must have the shape and device of x")
+    wcode = _weight(weight, x, dev)
+    outer, inner, n, ((xo, xi), (ro, ri), (to, ti), (oo, oi)) = _joint_rows((x, "x"), (residual, "residual"),
+                                                                            (total, "total"), (out, "out"))
+    rows = outer * inner
+    size = 0 if group is None else group
+    per_row = -(-n // size) if size else 1
+    _call_on(dev, stream, "a3b_rms_norm", code, outer, inner, n, x.data_ptr(), xo, xi, _data(residual), ro, ri, _data(total),
+             to, ti, target, out.data_ptr(), oo, oi, wcode, _data(weight), eps, _per_row(rstd, "rstd", rows, dev, _F32),
+             _per_row(scales, "scales", rows * per_row, dev, _F32), size)
+    return out
+
+
+def rms_norm_backward(grad_x, grad_out, x, weight, rstd, grad_weight=None, grad_total=None, stream=None):
+    """Gradient of rms_norm's out: given the rows that were normed (`x`: the total, where a residual was added), rstd as
+    rms_norm wrote it, and the gradients of a loss with respect to out and to the total itself (grad_total, None: zero),
+    writes that with respect to the rows to `grad_x` and that with respect to the weight to `grad_weight` (the weight's
+    dtype; None: not computed). With a residual, grad_x is the gradient of both summands. grad_out, grad_total, grad_x have
+    the shape and dtype of x, each any row strides; grad_x may be grad_out, x or grad_total. Returns grad_x."""
+    code, dev = _row_tensor(x, "x")
+    for t, name in ((grad_out, "grad_out"), (grad_x, "grad_x"), (grad_total, "grad_total")):
+        _like(t, name, x, dev, x.dtype)
+    wcode = _weight(weight, x, dev)
+    gcode = wcode
+    if grad_weight is not None:
+        gcode = _weight(grad_weight, x, dev, "grad_weight")
+        if weight is not None and gcode != wcode:
+            raise TypeError("grad_weight must have the dtype of the weight")
+    if rstd is None:
+        raise ValueError("rstd is needed")
+    outer, inner, n, ((xo, xi), (go, gi), (to, ti), (oo, oi)) = _joint_rows((x, "x"), (grad_out, "grad_out"),
+                                                                            (grad_total, "grad_total"), (grad_x, "grad_x"))
+    rows = outer * inner
+    ws = None
+    if grad_weight is not None:
+        ws = _workspace("a3b_rms_norm_backward_workspace", dev, stream, rows, n)
+    _call_on(dev, stream, "a3b_rms_norm_backward", code, outer, inner, n, grad_out.data_ptr(), go, gi, x.data_ptr(), xo, xi,
+             _data(grad_total), to, ti, grad_x.data_ptr(), oo, oi, wcode, _data(weight), _per_row(rstd, "rstd", rows, dev, _F32),
+             gcode, _data(grad_weight), _data(ws), 0 if ws is None else ws.numel())
+    return grad_x
+
+
+# ----------------------------------------------------------------------------------------- rows of a table
+def _table(t, name, dev):
+    """(dtype code, rows, row stride) of a 2-D table of rows on device `dev`"""
+    code, where = _row_tensor(t, name)
+    if where != dev:
+        raise ValueError(f"{name}: expected a tensor on CUDA device {dev}")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: expected two dimensions, rows contiguous")
+    return code, t.shape[0], t.stride(0)
+
+
+def _joined(a, b):
+    if a != b and capi.F32 not in (a, b):
+        raise TypeError("rows and table have one dtype, or one of them is float32")
+
+
+def _token_rows(t, tokens, dev, name):
+    """(dtype code, outer, inner, n, outer stride, inner stride, index code, address) of rows (..., n) for tokens (...)"""
+    code, where = _row_tensor(t, name)
+    if where != dev:
+        raise ValueError(f"{name}: expected a tensor on CUDA device {dev}")
+    if t.shape[:-1] != tokens.shape:
+        raise ValueError(f"{name} must have the tokens' shape, and one dimension behind it")
+    outer, inner, n, ((so, si),) = _joint_rows((t, name))
+    index = _INDEX_DT.get(tokens.dtype, -1)
+    return code, outer, inner, n, so, si, index, _per_row(tokens, "tokens", outer * inner, dev, _INDEX_DT)
+
+
+def embedding(out, weight, tokens, scale=1.0, first=0, stream=None):
+    """out[...] = scale * weight[tokens[...] - first], one row of the table `weight` (rows, n) for each token (int64 or
+    int32, contiguous, any shape; out: that shape and n). A token outside [first, first + rows) gives a row of zeros: padding
+    such as -100, or the tokens of other ranks where the table is cut over ranks. Types: float32 / float16 / bfloat16, both
+    alike or one of them float32. Rows may be strided. Returns out."""
+    dev = weight.get_device()
+    tcode, vocab, stride = _table(weight, "weight", dev)
+    code, outer, inner, n, so, si, index, address = _token_rows(out, tokens, dev, "out")
+    _joined(code, tcode)
+    if weight.shape[1] != n:
+        raise ValueError("out and weight must have rows of the same length")
+    _call_on(dev, stream, "a3b_embedding", tcode, weight.data_ptr(), vocab, stride, first, index, address, outer, inner, n,
+             scale, code, out.data_ptr(), so, si)
+    return out
+
+
+def embedding_backward(grad_weight, grad_out, tokens, scale=1.0, add=None, first=0, stream=None):
+    """Gradient of embedding's out with respect to the table: every row of `grad_weight` (rows, n) is add's row (zero without
+    `add`) plus scale times the sum of grad_out's rows over the places of its token. `add` has the dtype and shape of
+    grad_weight (the gradient from the table's use as a head); it may be grad_weight itself, of which then only rows of
+    tokens that occur are touched. The same bits in every call. Returns grad_weight."""
+    dev = grad_weight.get_device()
+    tcode, vocab, stride = _table(grad_weight, "grad_weight", dev)
+    code, outer, inner, n, so, si, index, address = _token_rows(grad_out, tokens, dev, "grad_out")
+    _joined(code, tcode)
+    if grad_weight.shape[1] != n:
+        raise ValueError("grad_out and grad_weight must have rows of the same length")
+    add_stride = 0
+    if add is not None:
+        acode, _, add_stride = _table(add, "add", dev)
+        if acode != tcode or add.shape != grad_weight.shape:
+            raise ValueError("add must have the dtype and shape of grad_weight")
+    ws = _workspace("a3b_embedding_backward_workspace", dev, stream, outer * inner, n, vocab)
+    _call_on(dev, stream, "a3b_embedding_backward", code, grad_out.data_ptr(), outer, inner, n, so, si, index, address, first,
+             scale, tcode, _data(add), add_stride, grad_weight.data_ptr(), vocab, stride, ws.data_ptr(), ws.numel())
+    return grad_weight
+
+
+# ------------------------------------------------------------------------------------------ drafted tokens
+def _draft_rows(t, name, batch, length, dev, dtype):
+    """(address, batch stride, row stride) of logits (batch, length, vocab)"""
+    if t.dtype != dtype or t.get_device() != dev:
+        raise ValueError(f"{name} must have the dtype and device of the logits")
+    if t.dim() != 3 or t.shape[0] != batch or t.shape[1] != length or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{name}: expected shape ({batch}, {length}, vocab), rows contiguous")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def verify_drafts(tokens, accepted, drafts, logits=None, lse=None, uniform=None, noise=None, draft_logits=None,
+                  draft_lse=None, scale=1.0, draft_scale=None, top_index=None, stream=None):
+    """For every sequence of a batch: how many of its drafted tokens stand against the target's probabilities, to `accepted`
+    (batch), and those tokens, the one drawn behind them, and -1 for the rest, to `tokens` (batch, length + 1).
+
+    drafts (batch, length): the first one outside [0, vocab) ends a sequence's draft. logits (batch, length + 1, vocab),
+    float32 / float16 / bfloat16, and lse (batch, length + 1) as token_logprobs writes it at the same `scale`: position i's
+    row predicts draft i. draft_logits (batch, length, vocab) and draft_lse (batch, length) are those the drafts were drawn
+    from, at draft_scale (None: scale); without them the drafts were certain (looked up). uniform (batch, length): float32 in
+    [0, 1); noise (batch, vocab): float32 exponential variates. Tokens are then distributed as if drawn from the target one
+    by one. length may be 0: one token is drawn from each row.
+
+    top_index (batch, length + 1): the target's most likely token of every row (token_logprobs with one alternative);
+    sequences whose first entry is a token are verified greedily, without random numbers; all of them if logits is None.
+    drafts, tokens, accepted and top_index have one dtype, int64 or int32. See a3b_verify_drafts. Returns tokens."""
+    index = _INDEX_DT.get(drafts.dtype)
+    if index is None:
+        raise TypeError(f"unsupported drafts dtype {drafts.dtype}")
+    dev = drafts.get_device()
+    if dev < 0:
+        raise ValueError("drafts: expected a CUDA tensor")
+    if drafts.dim() != 2:
+        raise ValueError("drafts: expected shape (batch, length)")
+    batch, length = drafts.shape
+    same = (drafts.dtype,)
+    places = batch * (length + 1)
+    code, vocab, at, lb, ls = capi.F32, (1 << 31) - 65, None, 0, 0
+    other, db, ds, noise_at, noise_stride = None, 0, 0, None, 0
+    if logits is not None:
+        code, vocab = _LOGITS_DT.get(logits.dtype), logits.shape[-1]
+        if code is None:
+            raise TypeError(f"unsupported logits dtype {logits.dtype}")
+        if lse is None or noise is None or (uniform is None and length):
+            raise ValueError("logits need lse, uniform and noise")
+        at, lb, ls = _draft_rows(logits, "logits", batch, length + 1, dev, logits.dtype)
+        if draft_logits is not None:
+            if draft_lse is None:
+                raise ValueError("draft_logits need draft_lse")
+            if draft_logits.shape[-1] != vocab:
+                raise ValueError("logits and draft_logits must have the same vocabulary")
+            other, db, ds = _draft_rows(draft_logits, "draft_logits", batch, length, dev, logits.dtype)
+        if (noise.dtype != torch.float32 or noise.get_device() != dev or noise.shape != (batch, vocab)
+                or (vocab > 1 and noise.stride(1) != 1)):
+            raise ValueError(f"noise: expected float32 of shape ({batch}, {vocab}) on CUDA device {dev}, rows contiguous")
+        noise_at, noise_stride = noise.data_ptr(), noise.stride(0)
+    elif top_index is None:
+        raise ValueError("neither logits nor top_index is given")
+    elif draft_logits is not None:
+        raise ValueError("draft_logits need logits")
+    _call_on(dev, stream, "a3b_verify_drafts", code, batch, length, vocab, at, lb, ls,
+             _per_row(lse, "lse", places, dev, _F32), scale, other, db, ds,
+             _per_row(draft_lse, "draft_lse", batch * length, dev, _F32), scale if draft_scale is None else draft_scale, index,
+             _per_row(drafts, "drafts", batch * length, dev, same), _per_row(top_index, "top_index", places, dev, same),
+             _per_row(uniform, "uniform", batch * length, dev, _F32), noise_at, noise_stride,
+             _per_row(tokens, "tokens", places, dev, same), _per_row(accepted, "accepted", batch, dev, same))
+    return tokens
 
 
 # ------------------------------------------------------------------------------------------------------- nBody

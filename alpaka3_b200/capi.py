@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get("A3B_LIBRARY") or os.path.join(_HERE, "lib", "libalpak
 # status codes
 OK, ERR_INVALID, ERR_CUDA, ERR_UNSUPPORTED, ERR_TIMEOUT, ERR_NOMEM, ERR_TOO_LARGE = range(7)
 # dtypes
-I32, U32, I64, U64, F32, F64, F16, BF16 = range(8)
+I32, U32, I64, U64, F32, F64, F16, BF16, E4M3, E5M2 = range(10)
 # norms over a tensor list
 NORM_L2, NORM_L1, NORM_MAX = range(3)
 # reduce / transform functors
@@ -79,6 +79,17 @@ SIGNATURES = {
     "a3b_grad_norm": [_P, _P, _I, _P, ctypes.c_size_t, _P, _I, _P],
     "a3b_clip_grads": [_P, _P, _I, _P, _D, _I, _P],
     "a3b_clip_grad_norm": [_P, _P, _I, _D, _P, ctypes.c_size_t, _I, _P],
+    "a3b_rms_norm": [_P, _I, _U64, _U64, _U64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _I64, _I64, _I, _P,
+                     _D, _P, _P, _U32],
+    "a3b_rms_norm_backward_workspace": [_U64, _U64],
+    "a3b_rms_norm_backward": [_P, _I, _U64, _U64, _U64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I,
+                              _P, _P, _I, _P, _P, ctypes.c_size_t],
+    "a3b_embedding": [_P, _I, _P, _U64, _I64, _I64, _I, _P, _U64, _U64, _U64, _D, _I, _P, _I64, _I64],
+    "a3b_embedding_backward_workspace": [_U64, _U64, _U64],
+    "a3b_embedding_backward": [_P, _I, _P, _U64, _U64, _U64, _I64, _I64, _I, _P, _I64, _D, _I, _P, _I64, _P, _U64, _I64, _P,
+                               ctypes.c_size_t],
+    "a3b_verify_drafts": [_P, _I, _U64, _U64, _U64, _P, _I64, _I64, _P, _D, _P, _I64, _I64, _P, _D, _I, _P, _P, _P, _P, _I64,
+                          _P, _P],
     "a3b_nbody_update_velocities": [_P, _P, _P, _P, _P, _U64, _U64, _U64, _P, _P, _P, _F, _F],
     "a3b_nbody_step": [_P, _P, _P, _P, _P, _U64, _U64, _U64, _P, _P, _P, _F, _F],
     "a3b_haccmk_step10": [_P, _P, _P, _P, _P, _I, _I, _F, _F, _F, _P, _P, _P],
@@ -97,7 +108,8 @@ SIGNATURES = {
     "a3b_debug_early_start_probe": [_I, _P, _P, _P, _U64, _P, _P],
 }
 _RESTYPES = {"a3b_last_error": ctypes.c_char_p, "a3b_scan_buffer_size": ctypes.c_size_t,
-             "a3b_grad_norm_workspace": ctypes.c_size_t, "a3b_ipc_handle_size": ctypes.c_size_t,
+             "a3b_grad_norm_workspace": ctypes.c_size_t, "a3b_rms_norm_backward_workspace": ctypes.c_size_t,
+             "a3b_embedding_backward_workspace": ctypes.c_size_t, "a3b_ipc_handle_size": ctypes.c_size_t,
              "a3b_halo_bytes": ctypes.c_size_t}
 
 

@@ -1,0 +1,1063 @@
+// Root-mean-square norm of rows, with the residual's addition in front and an output in 8 bits behind it, and its gradient.
+//
+//   h = x + residual,  r = (mean h^2 + eps)^(-1/2),  y = h r w,  q = y / s with s = max|y| / (largest 8-bit value)
+//   dy = g w,  c = mean(dy h r),  dh = r (dy - h r c) + dtotal,  dw = sum over rows of g h r
+//
+// Both are bound by memory: about 5 and 9 operations an element against 4 to 16 bytes. So every row is read once and stays
+// in registers between its sum and its output; a row is one team's (part of a warp, a warp or a block, by its length), and
+// teams are many, so that while one waits in its reduction others load.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "layout.cuh"
+#include "rows.cuh"
+
+namespace a3b
+{
+    namespace
+    {
+        // E elements of T (one 16-byte pack, or a single element where rows do not allow packs) as raw words.
+        template<typename T, int E>
+        struct Access
+        {
+            static constexpr int words = E == 1 ? 1 : 4;
+
+            static __device__ __forceinline__ void load(unsigned* w, T const* p)
+            {
+                if constexpr(E == 1)
+                {
+                    if constexpr(sizeof(T) == 4)
+                        w[0] = *reinterpret_cast<unsigned const*>(p);
+                    else
+                        w[0] = *reinterpret_cast<unsigned short const*>(p);
+                }
+                else
+                {
+                    uint4 const v = *reinterpret_cast<uint4 const*>(p);
+                    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                }
+            }
+            static __device__ __forceinline__ void store(T* p, unsigned const* w)
+            {
+                if constexpr(E == 1)
+                {
+                    if constexpr(sizeof(T) == 4)
+                        *reinterpret_cast<unsigned*>(p) = w[0];
+                    else
+                        *reinterpret_cast<unsigned short*>(p) = static_cast<unsigned short>(w[0]);
+                }
+                else
+                    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            static __device__ __forceinline__ void unpack(float* v, unsigned const* w)
+            {
+                if constexpr(E == 1)
+                    v[0] = PackOf<T>::pair(w, 0).x;
+                else
+#pragma unroll
+                    for(int k = 0; k < E / 2; ++k)
+                    {
+                        float2 const f = PackOf<T>::pair(w, k);
+                        v[2 * k] = f.x, v[2 * k + 1] = f.y;
+                    }
+            }
+            // rounded to the nearest value of T
+            static __device__ __forceinline__ void pack(unsigned* w, float const* v)
+            {
+                if constexpr(E == 1)
+                {
+                    unsigned two[2];
+                    PackOf<T>::setPair(two, 0, make_float2(v[0], 0.f));
+                    w[0] = two[0];
+                }
+                else
+#pragma unroll
+                    for(int k = 0; k < E / 2; ++k)
+                        PackOf<T>::setPair(w, k, make_float2(v[2 * k], v[2 * k + 1]));
+            }
+        };
+        template<>
+        __device__ __forceinline__ void Access<float, 1>::unpack(float* v, unsigned const* w)
+        {
+            v[0] = __uint_as_float(w[0]);
+        }
+        template<>
+        __device__ __forceinline__ void Access<float, 1>::pack(unsigned* w, float const* v)
+        {
+            w[0] = __float_as_uint(v[0]);
+        }
+
+        // E weights, of T or fp32, in the 16-byte words they come in
+        template<typename WT, int E>
+        struct Weights
+        {
+            static constexpr int words = E == 1 ? 1 : E * static_cast<int>(sizeof(WT)) / 4;
+
+            static __device__ __forceinline__ void load(unsigned* w, WT const* p)
+            {
+                if constexpr(E == 1)
+                    Access<WT, 1>::load(w, p);
+                else
+#pragma unroll
+                    for(int k = 0; k < words / 4; ++k)
+                    {
+                        uint4 const v = __ldg(reinterpret_cast<uint4 const*>(p) + k);
+                        w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
+                    }
+            }
+            static __device__ __forceinline__ void unpack(float* v, unsigned const* w)
+            {
+                if constexpr(E == 1)
+                    Access<WT, 1>::unpack(v, w);
+                else if constexpr(std::is_same_v<WT, float>)
+#pragma unroll
+                    for(int k = 0; k < E; ++k)
+                        v[k] = __uint_as_float(w[k]);
+                else
+                    Access<WT, E>::unpack(v, w);
+            }
+        };
+
+        // ------------------------------------------------------------------------------------- sums over a team
+        // Butterflies: every lane ends with the same bits.
+        template<int L, typename V>
+        __device__ __forceinline__ V lanesSum(V v)
+        {
+#pragma unroll
+            for(int d = L / 2; d > 0; d /= 2)
+                v += __shfl_xor_sync(kFullMask, v, d);
+            return v;
+        }
+
+        __device__ __forceinline__ float lanesMax(float v, int lanes)
+        {
+            for(int d = lanes / 2; d > 0; d /= 2)
+                v = maxNan(v, __shfl_xor_sync(kFullMask, v, d));
+            return v;
+        }
+
+        // Sum over the team: L lanes, or the block (L = 0) by way of `room` (one value a warp), which the next sum may
+        // not use before another barrier.
+        template<int L, typename V>
+        __device__ __forceinline__ V teamSum(V v, V* room)
+        {
+            if constexpr(L > 0)
+                return lanesSum<L>(v);
+            else
+            {
+                v = lanesSum<32>(v);
+                unsigned const warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+                if(lane == 0)
+                    room[warp] = v;
+                __syncthreads();
+                return lanesSum<32>(lane < warps ? room[lane] : V(0));
+            }
+        }
+
+        template<int L>
+        __device__ __forceinline__ float teamMax(float v, float* room)
+        {
+            if constexpr(L > 0)
+                return lanesMax(v, L);
+            else
+            {
+                v = lanesMax(v, 32);
+                unsigned const warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+                if(lane == 0)
+                    room[warp] = v;
+                __syncthreads();
+                return lanesMax(lane < warps ? room[lane] : 0.f, 32);
+            }
+        }
+
+        // ---------------------------------------------------------------------------------------------- forward
+        struct NormArgs
+        {
+            void const* x;
+            void const* residual; // may be null
+            void* total; // may be null
+            void* out;
+            RowStep xs, rs, ts, os;
+            uint32_t rows, inner, n;
+            bool one;
+            void const* weight; // may be null
+            float* rstd; // may be null
+            float* scales; // 8-bit outputs
+            uint32_t group, groups; // elements that share a scale (0: the row), and groups a row
+            bool e5m2;
+            double eps;
+        };
+
+        // fp32 squares are exact enough unless their sum leaves fp32's range: above it, or below it with nothing from eps.
+        __device__ __forceinline__ bool sumLost(float sum, double eps)
+        {
+            return !(sum < INFINITY) || (sum < 0x1p-100f && eps < 0x1p-60);
+        }
+
+        __device__ __forceinline__ float rootOf(float sum, uint32_t n, double eps)
+        {
+            return 1.f / sqrtf(sum / static_cast<float>(n) + static_cast<float>(eps));
+        }
+        __device__ __forceinline__ float rootOf(double sum, uint32_t n, double eps)
+        {
+            return static_cast<float>(1. / sqrt(sum / n + eps));
+        }
+
+        // The scale of a group whose largest magnitude is `high`, and what its values are multiplied with. A scale below
+        // fp32's normal numbers has no reciprocal there: its values are divided (`divide`).
+        struct Scale
+        {
+            float scale, inverse;
+            bool divide;
+
+            __device__ __forceinline__ Scale(float high, bool e5m2)
+            {
+                scale = high / (e5m2 ? 57344.f : 448.f);
+                divide = scale > 0.f && scale < 0x1p-126f;
+                inverse = scale == 0.f || divide ? 0.f : 1.f / scale;
+            }
+            __device__ __forceinline__ float operator()(float y) const
+            {
+                return divide ? __fdiv_rn(y, scale) : y * inverse;
+            }
+        };
+
+        // two values rounded to 8 bits, beyond the largest to the largest
+        __device__ __forceinline__ unsigned eight(float a, float b, bool e5m2)
+        {
+            return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, e5m2 ? __NV_E5M2 : __NV_E4M3);
+        }
+
+        // One row a team of L lanes (0: a block), P accesses of E elements a lane; the whole row is in registers.
+        template<typename T, typename WT, int E, int P, int L, bool F8>
+        __global__ void __launch_bounds__(L == 0 ? 1024 : 128) rmsNormKernel(NormArgs a)
+        {
+            using A = Access<T, E>;
+            using W = Weights<WT, E>;
+            __shared__ float roomF[32], roomM[32];
+            __shared__ double roomD[32];
+            uint32_t const lanes = L == 0 ? blockDim.x : L, t = L == 0 ? threadIdx.x : threadIdx.x % (L == 0 ? 1 : L);
+            uint32_t const team = L == 0 ? blockIdx.x : blockIdx.x * (128u / (L == 0 ? 1 : L)) + threadIdx.x / (L == 0 ? 1 : L);
+            bool const live = team < a.rows;
+            uint32_t const row = live ? team : a.rows - 1u, packs = a.n / E;
+            T const* x = static_cast<T const*>(a.x) + a.xs.at(row, a.inner, a.one);
+            WT const* weight = static_cast<WT const*>(a.weight);
+
+            unsigned raw[P][A::words], add[P][A::words];
+#pragma unroll
+            for(int p = 0; p < P; ++p)
+                if(uint32_t const k = p * lanes + t; k < packs)
+                    A::load(raw[p], x + static_cast<size_t>(k) * E);
+            if(a.residual)
+            {
+                T const* r = static_cast<T const*>(a.residual) + a.rs.at(row, a.inner, a.one);
+#pragma unroll
+                for(int p = 0; p < P; ++p)
+                    if(uint32_t const k = p * lanes + t; k < packs)
+                        A::load(add[p], r + static_cast<size_t>(k) * E);
+            }
+            // with the row's loads under way; more than two packs' weights would cost blocks an SM
+            constexpr bool early = P * W::words <= 16;
+            unsigned wraw[early ? P : 1][W::words];
+            if(early && weight)
+#pragma unroll
+                for(int p = 0; p < P; ++p)
+                    if(uint32_t const k = p * lanes + t; k < packs)
+                        W::load(wraw[early ? p : 0], weight + static_cast<size_t>(k) * E);
+
+            float h[P][E];
+            float sum = 0.f;
+#pragma unroll
+            for(int p = 0; p < P; ++p)
+            {
+                uint32_t const k = p * lanes + t;
+                if(k < packs)
+                    A::unpack(h[p], raw[p]);
+                else
+#pragma unroll
+                    for(int e = 0; e < E; ++e)
+                        h[p][e] = 0.f;
+                if(a.residual && k < packs)
+                {
+                    float more[E];
+                    A::unpack(more, add[p]);
+#pragma unroll
+                    for(int e = 0; e < E; ++e)
+                        h[p][e] += more[e];
+                    // The sum is rounded to the rows' type, stored or not: the norm is that of the row which the next
+                    // layer and the gradient read.
+                    A::pack(raw[p], h[p]);
+                    A::unpack(h[p], raw[p]);
+                    if(a.total && live)
+                        A::store(static_cast<T*>(a.total) + a.ts.at(row, a.inner, a.one) + static_cast<size_t>(k) * E, raw[p]);
+                }
+#pragma unroll
+                for(int e = 0; e < E; ++e)
+                    sum = fmaf(h[p][e], h[p][e], sum);
+            }
+            sum = teamSum<L>(sum, roomF);
+            float r;
+            if(L == 0 ? sumLost(sum, a.eps) : __any_sync(kFullMask, sumLost(sum, a.eps)))
+            {
+                double wide = 0.;
+#pragma unroll
+                for(int p = 0; p < P; ++p)
+#pragma unroll
+                    for(int e = 0; e < E; ++e)
+                        wide = fma(static_cast<double>(h[p][e]), static_cast<double>(h[p][e]), wide);
+                wide = teamSum<L>(wide, roomD);
+                r = sumLost(sum, a.eps) ? rootOf(wide, a.n, a.eps) : rootOf(sum, a.n, a.eps);
+            }
+            else
+                r = rootOf(sum, a.n, a.eps);
+            if(a.rstd && t == 0 && live)
+                a.rstd[row] = r;
+
+            T* out = static_cast<T*>(a.out) + (F8 ? 0 : a.os.at(row, a.inner, a.one));
+            float high = 0.f;
+#pragma unroll
+            for(int p = 0; p < P; ++p)
+            {
+                uint32_t const k = p * lanes + t;
+                if(weight && k < packs)
+                {
+                    float w[E];
+                    if constexpr(early)
+                        W::unpack(w, wraw[p]);
+                    else
+                    {
+                        unsigned words[W::words];
+                        W::load(words, weight + static_cast<size_t>(k) * E);
+                        W::unpack(w, words);
+                    }
+#pragma unroll
+                    for(int e = 0; e < E; ++e)
+                        h[p][e] = h[p][e] * r * w[e];
+                }
+                else
+#pragma unroll
+                    for(int e = 0; e < E; ++e)
+                        h[p][e] = k < packs ? h[p][e] * r : 0.f;
+                if constexpr(!F8)
+                {
+                    if(k < packs && live)
+                    {
+                        A::pack(raw[p], h[p]);
+                        A::store(out + static_cast<size_t>(k) * E, raw[p]);
+                    }
+                }
+                else
+#pragma unroll
+                    for(int e = 0; e < E; ++e)
+                        high = maxNan(high, fabsf(h[p][e]));
+            }
+            if constexpr(F8)
+            {
+                static_assert(E > 1 && (L == 0 || L == 32), "groups lie on neighbouring lanes");
+                auto* out8 = static_cast<unsigned char*>(a.out) + a.os.at(row, a.inner, a.one);
+                float* scales = a.scales + static_cast<size_t>(row) * a.groups;
+                if(a.group == 0)
+                    high = teamMax<L>(high, roomM);
+                int const near = static_cast<int>(a.group) / E; // lanes of one group
+#pragma unroll
+                for(int p = 0; p < P; ++p)
+                {
+                    uint32_t const k = p * lanes + t;
+                    if(a.group != 0)
+                    {
+                        high = 0.f;
+#pragma unroll
+                        for(int e = 0; e < E; ++e)
+                            high = maxNan(high, fabsf(h[p][e]));
+                        high = lanesMax(high, near);
+                    }
+                    Scale const s(high, a.e5m2);
+                    if(k < packs && live)
+                    {
+                        if(a.group != 0 ? k % near == 0 : k == 0)
+                            scales[a.group != 0 ? k / near : 0] = s.scale;
+                        unsigned w[E / 4];
+#pragma unroll
+                        for(int e = 0; e < E; e += 4)
+                            w[e / 4] = eight(s(h[p][e]), s(h[p][e + 1]), a.e5m2)
+                                       | (eight(s(h[p][e + 2]), s(h[p][e + 3]), a.e5m2) << 16);
+                        if constexpr(E == 8)
+                            *reinterpret_cast<uint2*>(out8 + static_cast<size_t>(k) * E) = make_uint2(w[0], w[1]);
+                        else
+                            *reinterpret_cast<unsigned*>(out8 + static_cast<size_t>(k) * E) = w[0];
+                    }
+                }
+            }
+        }
+
+        // Rows that no team holds (longer than 32768 16-bit or 16384 32-bit elements), and 8-bit outputs of rows without
+        // 16-byte packs: one block a row, which goes over it two to four times, element by element; the later passes
+        // find it in L2.
+        constexpr int kLongThreads = 512;
+
+        template<typename T, typename WT>
+        __global__ void __launch_bounds__(kLongThreads) rmsNormLongKernel(NormArgs a, int kind) // kind: 0 T, 1 8 bits
+        {
+            __shared__ float roomF[32], roomM[32];
+            __shared__ double roomD[32];
+            uint32_t const row = blockIdx.x, t = threadIdx.x;
+            T const* x = static_cast<T const*>(a.x) + a.xs.at(row, a.inner, a.one);
+            T const* add = a.residual ? static_cast<T const*>(a.residual) + a.rs.at(row, a.inner, a.one) : nullptr;
+            T* total = a.total ? static_cast<T*>(a.total) + a.ts.at(row, a.inner, a.one) : nullptr;
+            WT const* weight = static_cast<WT const*>(a.weight);
+            // a sum that was stored is read back: x and residual may have given it their place
+            auto value = [&](uint32_t k)
+            {
+                if(total && add)
+                    return toFloat(total[k]);
+                float const v = toFloat(x[k]);
+                return add ? toFloat(fromFloat<T>(v + toFloat(add[k]))) : v;
+            };
+            float sum = 0.f;
+#pragma unroll 4
+            for(uint32_t k = t; k < a.n; k += kLongThreads)
+            {
+                float v = toFloat(x[k]);
+                if(add)
+                {
+                    T const s = fromFloat<T>(v + toFloat(add[k]));
+                    if(total)
+                        total[k] = s;
+                    v = toFloat(s);
+                }
+                sum = fmaf(v, v, sum);
+            }
+            sum = teamSum<0>(sum, roomF); // also orders the stores of `total` before the reads below
+            float r;
+            if(sumLost(sum, a.eps))
+            {
+                double wide = 0.;
+                for(uint32_t k = t; k < a.n; k += kLongThreads)
+                {
+                    double const v = value(k);
+                    wide = fma(v, v, wide);
+                }
+                r = rootOf(teamSum<0>(wide, roomD), a.n, a.eps);
+            }
+            else
+                r = rootOf(sum, a.n, a.eps);
+            if(a.rstd && t == 0)
+                a.rstd[row] = r;
+            auto y = [&](uint32_t k)
+            {
+                float const v = value(k) * r;
+                return weight ? v * toFloat(weight[k]) : v;
+            };
+            if(kind == 0)
+            {
+                T* out = static_cast<T*>(a.out) + a.os.at(row, a.inner, a.one);
+#pragma unroll 4
+                for(uint32_t k = t; k < a.n; k += kLongThreads)
+                    out[k] = fromFloat<T>(y(k));
+                return;
+            }
+            auto* out = static_cast<unsigned char*>(a.out) + a.os.at(row, a.inner, a.one);
+            float* scales = a.scales + static_cast<size_t>(row) * a.groups;
+            if(a.group == 0)
+            {
+                float high = 0.f;
+#pragma unroll 4
+                for(uint32_t k = t; k < a.n; k += kLongThreads)
+                    high = maxNan(high, fabsf(y(k)));
+                Scale const s(teamMax<0>(high, roomM), a.e5m2);
+                if(t == 0)
+                    scales[0] = s.scale;
+#pragma unroll 4
+                for(uint32_t k = t; k < a.n; k += kLongThreads)
+                    out[k] = static_cast<unsigned char>(eight(s(y(k)), 0.f, a.e5m2));
+                return;
+            }
+            // a warp takes a group of 32, 64 or 128 elements
+            uint32_t const warp = t / 32, lane = t % 32;
+            for(uint32_t g = warp; g < a.groups; g += kLongThreads / 32)
+            {
+                float v[4], high = 0.f;
+#pragma unroll
+                for(uint32_t e = 0; e < 4; ++e)
+                {
+                    uint32_t const in = e * 32 + lane, k = g * a.group + in;
+                    v[e] = in < a.group && k < a.n ? y(k) : 0.f;
+                    high = maxNan(high, fabsf(v[e]));
+                }
+                Scale const s(lanesMax(high, 32), a.e5m2);
+                if(lane == 0)
+                    scales[g] = s.scale;
+#pragma unroll
+                for(uint32_t e = 0; e < 4; ++e)
+                    if(uint32_t const in = e * 32 + lane, k = g * a.group + in; in < a.group && k < a.n)
+                        out[k] = static_cast<unsigned char>(eight(s(v[e]), 0.f, a.e5m2));
+            }
+        }
+
+        uint32_t roundUp(uint32_t v, uint32_t to)
+        {
+            return (v + to - 1) / to * to;
+        }
+
+        template<typename T, typename WT, bool F8>
+        int launchNorm(cudaStream_t stream, DeviceProps const* props, NormArgs const& a, bool packed)
+        {
+            constexpr int E = PackOf<T>::E;
+            auto teams = [&](uint32_t lanes) { return (a.rows + 128 / lanes - 1) / (128 / lanes); };
+            if(packed)
+            {
+                uint32_t const packs = a.n / E;
+                bool const many = a.rows >= 4u * static_cast<uint32_t>(props->smCount);
+                if(!F8 && packs <= 8 && many)
+                    rmsNormKernel<T, WT, E, 1, F8 ? 32 : 8, F8><<<teams(8), 128, 0, stream>>>(a);
+                else if(!F8 && packs <= 16 && many)
+                    rmsNormKernel<T, WT, E, 1, F8 ? 32 : 16, F8><<<teams(16), 128, 0, stream>>>(a);
+                else if(packs <= 32)
+                    rmsNormKernel<T, WT, E, 1, 32, F8><<<teams(32), 128, 0, stream>>>(a);
+                else if(packs <= 64 && many)
+                    rmsNormKernel<T, WT, E, 2, 32, F8><<<teams(32), 128, 0, stream>>>(a);
+                else if(packs <= 128 && many)
+                    rmsNormKernel<T, WT, E, 4, 32, F8><<<teams(32), 128, 0, stream>>>(a);
+                else if(packs <= 1024 && !many)
+                    rmsNormKernel<T, WT, E, 1, 0, F8><<<a.rows, roundUp(packs, 32), 0, stream>>>(a);
+                else if(packs <= 2048)
+                    rmsNormKernel<T, WT, E, 2, 0, F8><<<a.rows, roundUp((packs + 1) / 2, 32), 0, stream>>>(a);
+                else if(packs <= 4096)
+                    rmsNormKernel<T, WT, E, 4, 0, F8><<<a.rows, roundUp((packs + 3) / 4, 32), 0, stream>>>(a);
+                else
+                    rmsNormLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a, F8);
+            }
+            else if constexpr(!F8)
+            {
+                if(a.n <= 2048)
+                    rmsNormKernel<T, WT, 1, 4, 0, false><<<a.rows, roundUp((a.n + 3) / 4, 32), 0, stream>>>(a);
+                else if(a.n <= 16384)
+                    rmsNormKernel<T, WT, 1, 16, 0, false><<<a.rows, roundUp((a.n + 15) / 16, 32), 0, stream>>>(a);
+                else
+                    rmsNormLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a, 0);
+            }
+            else
+                rmsNormLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a, 1);
+            A3B_CHECK_LAUNCH("rmsNormKernel");
+            return A3B_OK;
+        }
+
+        // --------------------------------------------------------------------------------------------- backward
+        struct NormBackArgs
+        {
+            void const* g;
+            void const* x;
+            void const* gtotal; // may be null
+            void* gx;
+            RowStep gs, xs, ts, os;
+            uint32_t rows, inner, n;
+            bool one;
+            void const* weight; // may be null
+            float const* rstd;
+            float* partial; // one row of n sums a block; null: no gradient of the weight
+        };
+
+        // Teams go from row to row, a lane always at the same columns, so that the weight's gradient gathers in registers;
+        // a block adds up its teams' and writes one row of partial sums. The next row's loads run under this row's sum.
+        template<typename T, typename WT, int E, int P, int L>
+        __global__ void __launch_bounds__(L == 0 ? 512 : 256) rmsNormBackwardKernel(NormBackArgs a)
+        {
+            using A = Access<T, E>;
+            using W = Weights<WT, E>;
+            constexpr bool ahead = P * A::words <= 8;
+            __shared__ float roomF[2][32];
+            extern __shared__ float sums[];
+            uint32_t const lanes = L == 0 ? blockDim.x : L, t = L == 0 ? threadIdx.x : threadIdx.x % (L == 0 ? 1 : L);
+            uint32_t const perBlock = L == 0 ? 1u : 256u / (L == 0 ? 1 : L), mine = L == 0 ? 0u : threadIdx.x / (L == 0 ? 1 : L);
+            uint32_t const packs = a.n / E, step = gridDim.x * perBlock;
+            WT const* weight = static_cast<WT const*>(a.weight);
+            unsigned wraw[ahead ? P : 1][W::words]; // held only where that leaves room; else read from L1 row by row
+            float dw[P][E];
+#pragma unroll
+            for(int p = 0; p < P; ++p)
+            {
+                if(uint32_t const k = p * lanes + t; ahead && weight && k < packs)
+                    W::load(wraw[ahead ? p : 0], weight + static_cast<size_t>(k) * E);
+#pragma unroll
+                for(int e = 0; e < E; ++e)
+                    dw[p][e] = 0.f;
+            }
+            unsigned graw[P][A::words], xraw[P][A::words];
+            float r = 0.f;
+            auto load = [&](uint32_t row)
+            {
+                T const* g = static_cast<T const*>(a.g) + a.gs.at(row, a.inner, a.one);
+                T const* x = static_cast<T const*>(a.x) + a.xs.at(row, a.inner, a.one);
+#pragma unroll
+                for(int p = 0; p < P; ++p)
+                    if(uint32_t const k = p * lanes + t; k < packs)
+                    {
+                        A::load(graw[p], g + static_cast<size_t>(k) * E);
+                        A::load(xraw[p], x + static_cast<size_t>(k) * E);
+                    }
+                r = a.rstd[row];
+            };
+            // of access p: k = x r, g, and d = g w
+            auto terms = [&](int p, float* hat, float* g, float* d)
+            {
+                A::unpack(hat, xraw[p]);
+                A::unpack(g, graw[p]);
+                float w[E];
+                if(weight)
+                {
+                    if constexpr(ahead)
+                        W::unpack(w, wraw[p]);
+                    else
+                    {
+                        unsigned words[W::words];
+                        W::load(words, weight + static_cast<size_t>(p * lanes + t) * E);
+                        W::unpack(w, words);
+                    }
+                }
+#pragma unroll
+                for(int e = 0; e < E; ++e)
+                {
+                    hat[e] *= r;
+                    d[e] = weight ? g[e] * w[e] : g[e];
+                }
+            };
+            // all teams of a block make the same number of steps: they share the warps' shuffles
+            uint32_t row = blockIdx.x * perBlock + mine;
+            if(ahead)
+                load(row < a.rows ? row : a.rows - 1u);
+            int flip = 0;
+            for(uint32_t first = blockIdx.x * perBlock; first < a.rows; first += step, row += step)
+            {
+                bool const live = row < a.rows;
+                uint32_t const here = live ? row : a.rows - 1u;
+                if(!ahead)
+                    load(here);
+                float hat[ahead ? P : 1][E], d[ahead ? P : 1][E];
+                float const rhere = r;
+                float c = 0.f;
+#pragma unroll
+                for(int p = 0; p < P; ++p)
+                    if(uint32_t const k = p * lanes + t; k < packs)
+                    {
+                        int const at = ahead ? p : 0;
+                        float g[E];
+                        terms(p, hat[at], g, d[at]);
+#pragma unroll
+                        for(int e = 0; e < E; ++e)
+                        {
+                            if(live)
+                                dw[p][e] = fmaf(g[e], hat[at][e], dw[p][e]);
+                            c = fmaf(d[at][e], hat[at][e], c);
+                        }
+                    }
+                unsigned traw[ahead ? P : 1][A::words];
+                T const* gt = a.gtotal ? static_cast<T const*>(a.gtotal) + a.ts.at(here, a.inner, a.one) : nullptr;
+                if(ahead && gt)
+#pragma unroll
+                    for(int p = 0; p < P; ++p)
+                        if(uint32_t const k = p * lanes + t; k < packs)
+                            A::load(traw[ahead ? p : 0], gt + static_cast<size_t>(k) * E);
+                if(ahead)
+                    load(row + step < a.rows ? row + step : a.rows - 1u);
+                c = teamSum<L>(c, roomF[flip]) / static_cast<float>(a.n);
+                flip ^= 1;
+                T* gx = static_cast<T*>(a.gx) + a.os.at(here, a.inner, a.one);
+#pragma unroll
+                for(int p = 0; p < P; ++p)
+                    if(uint32_t const k = p * lanes + t; k < packs && live)
+                    {
+                        int const at = ahead ? p : 0;
+                        if constexpr(!ahead)
+                        {
+                            float g[E];
+                            terms(p, hat[at], g, d[at]);
+                            if(gt)
+                                A::load(traw[at], gt + static_cast<size_t>(k) * E);
+                        }
+#pragma unroll
+                        for(int e = 0; e < E; ++e)
+                            d[at][e] = rhere * fmaf(-hat[at][e], c, d[at][e]);
+                        unsigned raw[A::words];
+                        if(gt)
+                        {
+                            float more[E];
+                            A::unpack(more, traw[at]);
+#pragma unroll
+                            for(int e = 0; e < E; ++e)
+                                d[at][e] += more[e];
+                        }
+                        A::pack(raw, d[at]);
+                        A::store(gx + static_cast<size_t>(k) * E, raw);
+                    }
+            }
+            if(!a.partial)
+                return;
+            float* partial = a.partial + static_cast<size_t>(blockIdx.x) * a.n;
+            if constexpr(L == 0)
+            {
+#pragma unroll
+                for(int p = 0; p < P; ++p)
+                    if(uint32_t const k = p * lanes + t; k < packs)
+#pragma unroll
+                        for(int e = 0; e < E; ++e)
+                            partial[static_cast<size_t>(k) * E + e] = dw[p][e];
+            }
+            else
+            {
+                for(uint32_t turn = 0; turn < perBlock; ++turn) // in the teams' order: the same bits every time
+                {
+                    if(turn == mine)
+#pragma unroll
+                        for(int p = 0; p < P; ++p)
+                            if(uint32_t const k = p * lanes + t; k < packs)
+#pragma unroll
+                                for(int e = 0; e < E; ++e)
+                                    sums[k * E + e] = turn == 0 ? dw[p][e] : sums[k * E + e] + dw[p][e];
+                    __syncthreads();
+                }
+                for(uint32_t k = threadIdx.x; k < a.n; k += 256u)
+                    partial[k] = sums[k];
+            }
+        }
+
+        // Rows that no team holds: two passes over the row for its gradient ...
+        template<typename T, typename WT>
+        __global__ void __launch_bounds__(kLongThreads) rmsNormBackwardLongKernel(NormBackArgs a)
+        {
+            __shared__ float roomF[32];
+            uint32_t const row = blockIdx.x, t = threadIdx.x;
+            T const* g = static_cast<T const*>(a.g) + a.gs.at(row, a.inner, a.one);
+            T const* x = static_cast<T const*>(a.x) + a.xs.at(row, a.inner, a.one);
+            T const* gt = a.gtotal ? static_cast<T const*>(a.gtotal) + a.ts.at(row, a.inner, a.one) : nullptr;
+            T* gx = static_cast<T*>(a.gx) + a.os.at(row, a.inner, a.one);
+            WT const* weight = static_cast<WT const*>(a.weight);
+            float const r = a.rstd[row];
+            float c = 0.f;
+#pragma unroll 4
+            for(uint32_t k = t; k < a.n; k += kLongThreads)
+                c = fmaf(toFloat(g[k]) * (weight ? toFloat(weight[k]) : 1.f), toFloat(x[k]) * r, c);
+            c = teamSum<0>(c, roomF) / static_cast<float>(a.n);
+#pragma unroll 4
+            for(uint32_t k = t; k < a.n; k += kLongThreads)
+            {
+                float const d = r * fmaf(-toFloat(x[k]) * r, c, toFloat(g[k]) * (weight ? toFloat(weight[k]) : 1.f));
+                gx[k] = fromFloat<T>(gt ? d + toFloat(gt[k]) : d);
+            }
+        }
+
+        // ... and, in front of it (gx may be g or x), the weight's: a block sums 32 columns over a share of the rows.
+        template<typename T>
+        __global__ void __launch_bounds__(256) rmsNormWeightKernel(NormBackArgs a)
+        {
+            __shared__ float part[8][32];
+            uint32_t const lane = threadIdx.x % 32, warp = threadIdx.x / 32, k = blockIdx.x * 32 + lane;
+            float s = 0.f;
+            if(k < a.n)
+#pragma unroll 4
+                for(uint32_t row = blockIdx.y * 8 + warp; row < a.rows; row += gridDim.y * 8)
+                {
+                    float const g = toFloat(static_cast<T const*>(a.g)[a.gs.at(row, a.inner, a.one) + k]);
+                    float const x = toFloat(static_cast<T const*>(a.x)[a.xs.at(row, a.inner, a.one) + k]);
+                    s = fmaf(g, x * a.rstd[row], s);
+                }
+            part[warp][lane] = s;
+            __syncthreads();
+            if(warp == 0 && k < a.n)
+            {
+#pragma unroll
+                for(int w = 1; w < 8; ++w)
+                    s += part[w][lane];
+                a.partial[static_cast<size_t>(blockIdx.y) * a.n + k] = s;
+            }
+        }
+
+        // dw = the sum of the partial rows, in their order within and over the warps: a block has 32 columns, its warps
+        // every 32nd row.
+        template<typename WT>
+        __global__ void __launch_bounds__(1024) rmsNormFoldKernel(float const* partial, uint32_t count, uint32_t n, WT* out)
+        {
+            __shared__ float part[32][33];
+            uint32_t const lane = threadIdx.x % 32, warp = threadIdx.x / 32, k = blockIdx.x * 32 + lane;
+            float s = 0.f;
+            if(k < n)
+#pragma unroll 4
+                for(uint32_t row = warp; row < count; row += 32)
+                    s += partial[static_cast<size_t>(row) * n + k];
+            part[warp][lane] = s;
+            __syncthreads();
+            s = lanesSum<32>(part[lane][warp]); // now the warp has one column
+            if(lane == 0 && blockIdx.x * 32 + warp < n)
+                out[blockIdx.x * 32 + warp] = fromFloat<WT>(s);
+        }
+
+        // Rows of partial sums at most: as many blocks as the SMs hold of the kernel above (by its launch bounds), fewer
+        // where there are fewer rows.
+        uint32_t partialRows(DeviceProps const* props, uint64_t rows)
+        {
+            return static_cast<uint32_t>(std::min<uint64_t>(rows, 4ull * static_cast<unsigned>(props->smCount)));
+        }
+
+        template<typename T, typename WT>
+        int launchNormBackward(cudaStream_t stream, DeviceProps const* props, NormBackArgs const& a, bool packed, WT* gw)
+        {
+            constexpr int E = PackOf<T>::E;
+            uint32_t const limit = partialRows(props, a.rows);
+            uint32_t blocks = limit;
+            auto teams = [&](uint32_t lanes) { return blocks = std::min(limit, (a.rows + 256 / lanes - 1) / (256 / lanes)); };
+            size_t const room = a.partial ? a.n * sizeof(float) : 0;
+            uint32_t const packs = packed ? a.n / E : a.n;
+            auto longRows = [&]
+            {
+                if(a.partial)
+                {
+                    blocks = std::min<uint32_t>(limit, 64);
+                    rmsNormWeightKernel<T><<<dim3((a.n + 31) / 32, blocks), 256, 0, stream>>>(a);
+                }
+                rmsNormBackwardLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a);
+            };
+            if(packed && packs <= 16)
+                rmsNormBackwardKernel<T, WT, E, 1, 16><<<teams(16), 256, room, stream>>>(a);
+            else if(packed && packs <= 32)
+                rmsNormBackwardKernel<T, WT, E, 1, 32><<<teams(32), 256, room, stream>>>(a);
+            else if(packed && packs <= 64)
+                rmsNormBackwardKernel<T, WT, E, 2, 32><<<teams(32), 256, room, stream>>>(a);
+            else if(packed && packs <= 1024)
+                rmsNormBackwardKernel<T, WT, E, 2, 0><<<blocks, roundUp((packs + 1) / 2, 32), 0, stream>>>(a);
+            else if(packed && packs <= 2048)
+                rmsNormBackwardKernel<T, WT, E, 4, 0><<<blocks, roundUp((packs + 3) / 4, 32), 0, stream>>>(a);
+            else if(!packed && packs <= 2048)
+                rmsNormBackwardKernel<T, WT, 1, 4, 0><<<blocks, roundUp((packs + 3) / 4, 32), 0, stream>>>(a);
+            else if(!packed && packs <= 8192)
+                rmsNormBackwardKernel<T, WT, 1, 16, 0><<<blocks, roundUp((packs + 15) / 16, 32), 0, stream>>>(a);
+            else
+                longRows();
+            A3B_CHECK_LAUNCH("rmsNormBackwardKernel");
+            if(a.partial)
+            {
+                rmsNormFoldKernel<WT><<<(a.n + 31) / 32, 1024, 0, stream>>>(a.partial, blocks, a.n, gw);
+                A3B_CHECK_LAUNCH("rmsNormFoldKernel");
+            }
+            return A3B_OK;
+        }
+
+        // ------------------------------------------------------------------------------------------ arguments
+        int checkShape(int dtype, uint64_t outer, uint64_t inner, uint64_t n, double eps)
+        {
+            A3B_REQUIRE(rowTypeSize(dtype) != 0, "rows must be f32, f16 or bf16");
+            A3B_REQUIRE(n > 0, "a row needs at least one element");
+            A3B_REQUIRE(eps >= 0 && eps <= 0x1p100, "eps must lie between 0 and 2^100");
+            A3B_REQUIRE(outer == 0 || inner <= UINT64_MAX / outer, "rows overflow");
+            if(n > static_cast<uint64_t>(INT_MAX) - 64 || outer * inner > static_cast<uint64_t>(INT_MAX))
+            {
+                setError("at most 2^31 - 1 rows of 2^31 - 65 elements");
+                return A3B_ERR_TOO_LARGE;
+            }
+            return A3B_OK;
+        }
+    } // namespace
+} // namespace a3b
+
+using namespace a3b;
+
+extern "C"
+{
+    int a3b_rms_norm(
+        a3b_stream_t stream,
+        int dtype,
+        uint64_t outer,
+        uint64_t inner,
+        uint64_t n,
+        void const* x,
+        int64_t x_outer_stride,
+        int64_t x_inner_stride,
+        void const* residual,
+        int64_t residual_outer_stride,
+        int64_t residual_inner_stride,
+        void* total,
+        int64_t total_outer_stride,
+        int64_t total_inner_stride,
+        int out_dtype,
+        void* out,
+        int64_t out_outer_stride,
+        int64_t out_inner_stride,
+        int weight_dtype,
+        void const* weight,
+        double eps,
+        float* rstd,
+        float* scales,
+        uint32_t group)
+    {
+        int const rc = checkShape(dtype, outer, inner, n, eps);
+        if(rc != A3B_OK)
+            return rc;
+        bool const eightBits = out_dtype == A3B_E4M3 || out_dtype == A3B_E5M2;
+        A3B_REQUIRE(out_dtype == dtype || eightBits, "the output has the rows' type, e4m3 or e5m2");
+        A3B_REQUIRE(!weight || weight_dtype == dtype || weight_dtype == A3B_F32, "the weight has the rows' type or f32");
+        A3B_REQUIRE(group == 0 || (eightBits && (group == 32 || group == 64 || group == 128)),
+                    "groups of 8-bit outputs have 32, 64 or 128 elements");
+        if(outer * inner == 0)
+            return A3B_OK;
+        A3B_REQUIRE(x && out, "null rows or output");
+        A3B_REQUIRE(!total || residual, "a sum needs a residual");
+        A3B_REQUIRE(eightBits == (scales != nullptr), "scales belong to 8-bit outputs");
+        int const es = rowTypeSize(dtype), os = eightBits ? 1 : es, ws = weight_dtype == A3B_F32 ? 4 : 2;
+        A3B_REQUIRE(alignedTo(es, {x, residual, total}) && alignedTo(os, {out}) && alignedTo(ws, {weight})
+                        && alignedTo(4, {rstd, scales}),
+                    "an array is not aligned to its type");
+        uint64_t const rows = outer * inner, groups = group ? (n + group - 1) / group : 1;
+        Stretch const sx = Stretch::rows(x, outer, inner, x_outer_stride, x_inner_stride, n, es);
+        Stretch const sr = Stretch::rows(residual, outer, inner, residual_outer_stride, residual_inner_stride, n, es);
+        Stretch const st = Stretch::rows(total, outer, inner, total_outer_stride, total_inner_stride, n, es);
+        Stretch const so = Stretch::rows(out, outer, inner, out_outer_stride, out_inner_stride, n, os);
+        Stretch const sw = Stretch::dense(weight, static_cast<Wide>(n) * ws);
+        Stretch const s1 = Stretch::dense(rstd, static_cast<Wide>(rows) * 4);
+        Stretch const s8 = Stretch::dense(scales, static_cast<Wide>(rows) * groups * 4);
+        A3B_REQUIRE(so.separate() && (!total || st.separate()), "rows of an output overlap");
+        for(Stretch const* w : {&so, &st})
+            for(Stretch const* r : {&sx, &sr})
+                A3B_REQUIRE(w->empty() || w->sameAs(*r) || w->apart(*r),
+                            "an output overlaps its inputs (only the same rows in place are allowed)");
+        A3B_REQUIRE(so.apart(st), "the outputs overlap");
+        for(Stretch const* w : {&so, &st, &s1, &s8})
+            A3B_REQUIRE(w->apart(sw), "an output overlaps the weight");
+        for(Stretch const* w : {&sx, &sr, &st, &so})
+            A3B_REQUIRE(w->apart(s1) && w->apart(s8), "rows overlap rstd or the scales");
+        A3B_REQUIRE(s1.apart(s8), "the outputs overlap");
+        DeviceProps const* props = nullptr;
+        int const rd = currentDevice(&props);
+        if(rd != A3B_OK)
+            return rd;
+        int const E = 16 / es;
+        auto fits = [&](void const* p, int64_t a, int64_t b, int size, int to)
+        { return !p || rowsAligned(p, outer, inner, a, b, size, to); };
+        bool const packed = n % E == 0 && fits(x, x_outer_stride, x_inner_stride, es, 16)
+                            && fits(residual, residual_outer_stride, residual_inner_stride, es, 16)
+                            && fits(total, total_outer_stride, total_inner_stride, es, 16)
+                            && fits(out, out_outer_stride, out_inner_stride, os, eightBits ? E : 16) && alignedTo(16, {weight});
+        bool const one = outer == 1;
+        NormArgs a{x, residual, total, out, {x_outer_stride, x_inner_stride}, {residual_outer_stride, residual_inner_stride},
+                   {total_outer_stride, total_inner_stride}, {out_outer_stride, out_inner_stride},
+                   static_cast<uint32_t>(rows), static_cast<uint32_t>(inner), static_cast<uint32_t>(n), one, weight, rstd,
+                   scales, group, static_cast<uint32_t>(groups), out_dtype == A3B_E5M2, eps};
+        auto s = static_cast<cudaStream_t>(stream);
+        bool const wide = weight && weight_dtype == A3B_F32;
+        if(dtype == A3B_F32)
+            return eightBits ? launchNorm<float, float, true>(s, props, a, packed)
+                             : launchNorm<float, float, false>(s, props, a, packed);
+        if(dtype == A3B_F16)
+        {
+            if(wide)
+                return eightBits ? launchNorm<__half, float, true>(s, props, a, packed)
+                                 : launchNorm<__half, float, false>(s, props, a, packed);
+            return eightBits ? launchNorm<__half, __half, true>(s, props, a, packed)
+                             : launchNorm<__half, __half, false>(s, props, a, packed);
+        }
+        if(wide)
+            return eightBits ? launchNorm<__nv_bfloat16, float, true>(s, props, a, packed)
+                             : launchNorm<__nv_bfloat16, float, false>(s, props, a, packed);
+        return eightBits ? launchNorm<__nv_bfloat16, __nv_bfloat16, true>(s, props, a, packed)
+                         : launchNorm<__nv_bfloat16, __nv_bfloat16, false>(s, props, a, packed);
+    }
+
+    size_t a3b_rms_norm_backward_workspace(uint64_t rows, uint64_t n)
+    {
+        DeviceProps const* props = nullptr;
+        if(currentDevice(&props) != A3B_OK)
+            return 0;
+        if(rows == 0 || n == 0 || n > static_cast<uint64_t>(INT_MAX) || rows > static_cast<uint64_t>(INT_MAX))
+            return 16;
+        return std::max<size_t>(16, static_cast<size_t>(partialRows(props, rows)) * n * sizeof(float));
+    }
+
+    int a3b_rms_norm_backward(
+        a3b_stream_t stream,
+        int dtype,
+        uint64_t outer,
+        uint64_t inner,
+        uint64_t n,
+        void const* grad_out,
+        int64_t grad_out_outer_stride,
+        int64_t grad_out_inner_stride,
+        void const* x,
+        int64_t x_outer_stride,
+        int64_t x_inner_stride,
+        void const* grad_total,
+        int64_t grad_total_outer_stride,
+        int64_t grad_total_inner_stride,
+        void* grad_x,
+        int64_t grad_x_outer_stride,
+        int64_t grad_x_inner_stride,
+        int weight_dtype,
+        void const* weight,
+        float const* rstd,
+        int grad_weight_dtype,
+        void* grad_weight,
+        void* workspace,
+        size_t workspace_bytes)
+    {
+        int const rc = checkShape(dtype, outer, inner, n, 0.);
+        if(rc != A3B_OK)
+            return rc;
+        A3B_REQUIRE(!weight || weight_dtype == dtype || weight_dtype == A3B_F32, "the weight has the rows' type or f32");
+        A3B_REQUIRE(!grad_weight || grad_weight_dtype == dtype || grad_weight_dtype == A3B_F32,
+                    "the weight's gradient has the rows' type or f32");
+        A3B_REQUIRE(!grad_weight || !weight || grad_weight_dtype == weight_dtype, "the weight's gradient has the weight's type");
+        auto s = static_cast<cudaStream_t>(stream);
+        int const es = rowTypeSize(dtype), ws = (weight ? weight_dtype : grad_weight_dtype) == A3B_F32 ? 4 : 2;
+        A3B_REQUIRE(alignedTo(ws, {weight, grad_weight}), "an array is not aligned to its type");
+        if(outer * inner == 0)
+        {
+            if(grad_weight) // the sum over no rows
+                A3B_CUDA(cudaMemsetAsync(grad_weight, 0, n * static_cast<size_t>(ws), s));
+            return A3B_OK;
+        }
+        A3B_REQUIRE(grad_out && x && grad_x && rstd, "null rows, rstd or output");
+        A3B_REQUIRE(alignedTo(es, {grad_out, x, grad_total, grad_x}) && alignedTo(4, {rstd}), "an array is not aligned to its type");
+        uint64_t const rows = outer * inner;
+        Stretch const sg = Stretch::rows(grad_out, outer, inner, grad_out_outer_stride, grad_out_inner_stride, n, es);
+        Stretch const sx = Stretch::rows(x, outer, inner, x_outer_stride, x_inner_stride, n, es);
+        Stretch const st = Stretch::rows(grad_total, outer, inner, grad_total_outer_stride, grad_total_inner_stride, n, es);
+        Stretch const so = Stretch::rows(grad_x, outer, inner, grad_x_outer_stride, grad_x_inner_stride, n, es);
+        Stretch const sw = Stretch::dense(weight, static_cast<Wide>(n) * ws);
+        Stretch const sd = Stretch::dense(grad_weight, static_cast<Wide>(n) * ws);
+        Stretch const s1 = Stretch::dense(rstd, static_cast<Wide>(rows) * 4);
+        Stretch const s2 = Stretch::dense(grad_weight ? workspace : nullptr, static_cast<Wide>(workspace_bytes));
+        A3B_REQUIRE(so.separate(), "rows of grad_x overlap");
+        for(Stretch const* r : {&sg, &sx, &st})
+        {
+            A3B_REQUIRE(r->empty() || so.sameAs(*r) || so.apart(*r),
+                        "grad_x overlaps its inputs (only the same rows in place are allowed)");
+            A3B_REQUIRE(r->apart(sd) && r->apart(s2), "the weight's gradient or the workspace overlaps the rows");
+        }
+        A3B_REQUIRE(so.apart(sd) && so.apart(s2) && so.apart(sw) && so.apart(s1) && sd.apart(sw) && sd.apart(s1) && sd.apart(s2)
+                        && s2.apart(sw) && s2.apart(s1),
+                    "outputs and workspace must lie apart from one another, the weight and rstd");
+        DeviceProps const* props = nullptr;
+        int const rd = currentDevice(&props);
+        if(rd != A3B_OK)
+            return rd;
+        A3B_REQUIRE(!grad_weight || (workspace && alignedTo(16, {workspace})
+                                     && workspace_bytes >= a3b_rms_norm_backward_workspace(rows, n)),
+                    "the workspace is missing, too small or not aligned to 16 bytes");
+        int const E = 16 / es;
+        auto fits = [&](void const* p, int64_t a, int64_t b) { return !p || rowsAligned(p, outer, inner, a, b, es, 16); };
+        bool const packed = n % E == 0 && fits(grad_out, grad_out_outer_stride, grad_out_inner_stride)
+                            && fits(x, x_outer_stride, x_inner_stride)
+                            && fits(grad_total, grad_total_outer_stride, grad_total_inner_stride)
+                            && fits(grad_x, grad_x_outer_stride, grad_x_inner_stride) && alignedTo(16, {weight});
+        NormBackArgs a{grad_out, x, grad_total, grad_x, {grad_out_outer_stride, grad_out_inner_stride},
+                       {x_outer_stride, x_inner_stride}, {grad_total_outer_stride, grad_total_inner_stride},
+                       {grad_x_outer_stride, grad_x_inner_stride}, static_cast<uint32_t>(rows), static_cast<uint32_t>(inner),
+                       static_cast<uint32_t>(n), outer == 1, weight, rstd,
+                       grad_weight ? static_cast<float*>(workspace) : nullptr};
+        bool const wide = ws == 4;
+        if(dtype == A3B_F32)
+            return launchNormBackward<float, float>(s, props, a, packed, static_cast<float*>(grad_weight));
+        if(dtype == A3B_F16)
+            return wide ? launchNormBackward<__half, float>(s, props, a, packed, static_cast<float*>(grad_weight))
+                        : launchNormBackward<__half, __half>(s, props, a, packed, static_cast<__half*>(grad_weight));
+        return wide ? launchNormBackward<__nv_bfloat16, float>(s, props, a, packed, static_cast<float*>(grad_weight))
+                    : launchNormBackward<__nv_bfloat16, __nv_bfloat16>(s, props, a, packed, static_cast<__nv_bfloat16*>(grad_weight));
+    }
+}

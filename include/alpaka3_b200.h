@@ -47,8 +47,10 @@ enum a3b_dtype
     A3B_U64 = 3,
     A3B_F32 = 4,
     A3B_F64 = 5,
-    A3B_F16 = 6, /* IEEE half and bfloat16: only for the entry points over logits and gradients that name them */
-    A3B_BF16 = 7
+    A3B_F16 = 6, /* IEEE half and bfloat16: only for the entry points over logits, rows and gradients that name them */
+    A3B_BF16 = 7,
+    A3B_E4M3 = 8, /* 8-bit floating point (largest values 448 and 57344): only outputs of a3b_rms_norm */
+    A3B_E5M2 = 9
 };
 
 /* binary reduce functors: std::plus, ScalarFunc{min}, ScalarFunc{max} (test/unit/algorithm/reduce.cpp:22-56) */
@@ -348,6 +350,120 @@ A3B_API int a3b_clip_grads(a3b_stream_t stream, a3b_tensor_list const* list, int
 /* a3b_grad_norm and a3b_clip_grads in one call. */
 A3B_API int a3b_clip_grad_norm(a3b_stream_t stream, a3b_tensor_list const* list, int kind, double max_norm,
                                void* workspace, size_t workspace_bytes, int norm_dtype, void* norm);
+
+/* --------------------------------------------------------------------------------- root-mean-square norm (rows) */
+
+/* Over every row of n elements: h = x + residual (rounded to dtype), r = 1 / sqrt(mean h^2 + eps), out = h * r * weight.
+ * No counterpart in alpaka3: transformReduce with one result a row, and a transform with that result.
+ *
+ * Rows of dtype A3B_F32, A3B_F16 or A3B_BF16: row o * inner + i (o < outer, i < inner) of each array starts at element
+ * o * outer_stride + i * inner_stride and is contiguous. residual: null or rows that are added; total: null or rows that
+ * receive h (needs a residual). Rounded or not stored, it is the rounded h that is normed, so that a gradient which reads
+ * `total` is that of what was computed. weight: n elements of dtype or A3B_F32, null: ones. rstd: null or one fp32 value a
+ * row that receives r, for the gradient. The sum of squares is held in fp32, or in fp64 where that leaves fp32's range
+ * (elements beyond 1e19, or below 1e-15 with an eps below 2^-60); every stored value is rounded once.
+ *
+ * out has dtype, or A3B_E4M3 or A3B_E5M2 with scales: groups of `group` elements of a row (32, 64 or 128, the last of a row
+ * may be shorter; 0: the whole row) share the scale s = max |y| / L, L = 448 or 57344, y = h * r * weight in fp32, and
+ * out = y * (1 / s) rounded to the nearest 8-bit value, at most L. scales: fp32, dense, ceil(n / group) (or 1) a row. A
+ * group of zeros has scale 0.
+ *
+ * NaN in a row makes its out and rstd NaN; an infinity makes rstd 0, itself NaN and the others 0. A row of zeros with eps 0
+ * has rstd infinity and NaN as output. A group with a NaN has scale NaN and NaN throughout.
+ * An output may be an input of the same type in place (same address and strides: total = residual, out = x, ...); otherwise
+ * outputs must lie apart from the inputs and from one another: wholly before or behind, or beside them in rows whose steps
+ * are all multiples of one length that holds both (parts of one wider row). Rows of an output may not overlap. The order of
+ * a row's sums follows from its length, alignment and the number of rows. At most 2^31 - 1 rows of 2^31 - 65 elements
+ * (A3B_ERR_TOO_LARGE). One launch. */
+A3B_API int a3b_rms_norm(a3b_stream_t stream, int dtype, uint64_t outer, uint64_t inner, uint64_t n, void const* x,
+                         int64_t x_outer_stride, int64_t x_inner_stride, void const* residual,
+                         int64_t residual_outer_stride, int64_t residual_inner_stride, void* total,
+                         int64_t total_outer_stride, int64_t total_inner_stride, int out_dtype, void* out,
+                         int64_t out_outer_stride, int64_t out_inner_stride, int weight_dtype, void const* weight, double eps,
+                         float* rstd, float* scales, uint32_t group);
+
+/* Bytes of device scratch that a3b_rms_norm_backward needs for grad_weight on the current device (any contents; nothing is
+ * kept in it between calls). Calls that overlap on the GPU need one each. 0 on failure. */
+A3B_API size_t a3b_rms_norm_backward_workspace(uint64_t rows, uint64_t n);
+
+/* Gradient of a3b_rms_norm's out (as if not rounded to 8 bits): with d = grad_out * weight and k = x * rstd,
+ *   grad_x = rstd * (d - k * mean(d * k)) + grad_total,   grad_weight = sum over rows of grad_out * k.
+ * x: the rows that were normed (`total`, where there was a residual; grad_x is then the gradient of x and of residual
+ * alike), rstd: as a3b_rms_norm wrote it; grad_total: null or the gradient that reaches `total` itself. grad_out, x,
+ * grad_total and grad_x have dtype and each its strides. grad_weight: null or n elements of the weight's type (dtype or
+ * A3B_F32 without a weight); it needs a workspace of a3b_rms_norm_backward_workspace bytes, 16-byte aligned. All sums are
+ * held in fp32 (a row's positions and the rows in a fixed order: repeated calls give the same bits) and rounded once.
+ * grad_x may be grad_out, x or grad_total in place. No rows: grad_weight is set to zero. */
+A3B_API int a3b_rms_norm_backward(a3b_stream_t stream, int dtype, uint64_t outer, uint64_t inner, uint64_t n,
+                                  void const* grad_out, int64_t grad_out_outer_stride, int64_t grad_out_inner_stride,
+                                  void const* x, int64_t x_outer_stride, int64_t x_inner_stride, void const* grad_total,
+                                  int64_t grad_total_outer_stride, int64_t grad_total_inner_stride, void* grad_x,
+                                  int64_t grad_x_outer_stride, int64_t grad_x_inner_stride, int weight_dtype,
+                                  void const* weight, float const* rstd, int grad_weight_dtype, void* grad_weight,
+                                  void* workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------------- rows of a table, by tokens */
+
+/* out_i = scale * row t_i of the table, for count = outer * inner tokens t (A3B_I32 or A3B_I64, dense): a transform whose
+ * input is picked by an index. The table holds the rows of the tokens [first, first + vocab), n elements each, row_stride
+ * apart; a token outside it gives a row of zeros (as a table cut over ranks wants, and as -100 for padding). Row
+ * o * inner + i of out starts at element o * outer_stride + i * inner_stride. Types: A3B_F32, A3B_F16 or A3B_BF16, both
+ * alike, or one of them A3B_F32; the product is formed in fp32 and rounded once. scale: any finite fp32 value. The output's
+ * rows may not overlap one another, the table or the tokens (beside them in rows of steps that are all multiples of one
+ * length is apart). At most 2^31 - 65 tokens, rows of the table and elements a row (A3B_ERR_TOO_LARGE; rows of more than
+ * eight million elements too). One launch. */
+A3B_API int a3b_embedding(a3b_stream_t stream, int table_dtype, void const* table, uint64_t vocab, int64_t table_stride,
+                          int64_t first, int index_dtype, void const* tokens, uint64_t outer, uint64_t inner, uint64_t n,
+                          double scale, int out_dtype, void* out, int64_t out_outer_stride, int64_t out_inner_stride);
+
+/* Bytes of device scratch that a3b_embedding_backward needs for `count` tokens on the current device (any contents; nothing
+ * is kept in it between calls). Calls that overlap on the GPU need one each. 0 on failure. */
+A3B_API size_t a3b_embedding_backward_workspace(uint64_t count, uint64_t n, uint64_t vocab);
+
+/* Gradient of a3b_embedding with respect to the table: row v of grad_table = add_v + scale * the sum of grad_out_i over the
+ * positions i whose token is first + v, zero (add_v) for tokens that do not occur. add: null, or rows of grad_table's type
+ * that are added (the gradient from the table's other use as a head); add may be grad_table itself, of which then only the
+ * rows of tokens that occur are touched. Types as in a3b_embedding: grad_out is of its out_dtype, the table of its
+ * table_dtype. Sums are held in fp32 and rounded once; their order follows from count, n and vocab (and the device) alone:
+ * repeated calls give the same bits. grad_out's rows may have any strides; grad_table's may not overlap. workspace: 16-byte
+ * aligned, of a3b_embedding_backward_workspace bytes. grad_table and workspace lie apart from all inputs. */
+A3B_API int a3b_embedding_backward(a3b_stream_t stream, int grad_dtype, void const* grad_out, uint64_t outer, uint64_t inner,
+                                   uint64_t n, int64_t grad_outer_stride, int64_t grad_inner_stride, int index_dtype,
+                                   void const* tokens, int64_t first, double scale, int table_dtype, void const* add,
+                                   int64_t add_stride, void* grad_table, uint64_t vocab, int64_t table_stride,
+                                   void* workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------------- verification of drafted tokens */
+
+/* For every sequence b of a batch, `length` drafted tokens t (A3B_I32 or A3B_I64; the first one outside [0, vocab) ends the
+ * sequence's draft) against the target's logits (length + 1 rows a sequence: position i's row predicts draft i) and the
+ * draft's own (length rows; null: the drafts were certain, q is 1 at t and 0 elsewhere):
+ *   p_v = e^(scale * z_v - lse),  q_v = e^(draft_scale * z'_v - draft_lse), lse and draft_lse as a3b_token_logprobs writes
+ * them. Draft i stands while uniform_i * q(t_i) < p(t_i). At the first that does not, one token is drawn from the rates
+ * (p_v - q_v)+, behind the last one that stands from the rates p_v (also where no rate is left otherwise): the token with
+ * the largest rate_v / noise_v, a tie to the lowest. With uniform in [0, 1) and noise independent exponential variates the
+ * tokens are distributed as if drawn from the target one by one. Comparisons and quotients are those of the formula in 64
+ * bits.
+ *
+ * tokens (length + 1 a sequence): the drafts that stand, the drawn token, -1 behind it; accepted: how many stand. A row with
+ * nothing left (lse -infinity), a NaN or +infinity draws -1. A NaN in the draft's row refuses its draft and takes nothing
+ * away. noise is positive; what is not takes no part or, at 0, wins where its rate is positive.
+ *
+ * Greedy sequences: top_index (null: none; length + 1 a sequence) holds the target's most likely token for every row, as
+ * a3b_token_logprobs gives with one alternative. A sequence whose first entry is a token is verified greedily: draft i stands
+ * while it equals top_index i, and the next entry follows. logits may be null if all sequences are greedy; then lse, uniform
+ * and noise may be, too.
+ *
+ * logits: row (b, i) starts at element b * batch_stride + i * stride, likewise draft_logits; noise: row b at b *
+ * noise_stride; rows are contiguous, everything else is dense. index_dtype is that of drafts, top_index, tokens and
+ * accepted. scale, draft_scale: between 2^-20 and 2^20. The outputs lie apart from one another and from the inputs. One
+ * launch. At most 2^31 - 1 rows of 2^31 - 65 logits (A3B_ERR_TOO_LARGE). */
+A3B_API int a3b_verify_drafts(a3b_stream_t stream, int dtype, uint64_t batch, uint64_t length, uint64_t vocab,
+                              void const* logits, int64_t logits_batch_stride, int64_t logits_stride, float const* lse,
+                              double scale, void const* draft_logits, int64_t draft_batch_stride, int64_t draft_stride,
+                              float const* draft_lse, double draft_scale, int index_dtype, void const* drafts,
+                              void const* top_index, float const* uniform, float const* noise, int64_t noise_stride,
+                              void* tokens, void* accepted);
 
 /* ----------------------------------------------------------------------------------------------------- nBody */
 
