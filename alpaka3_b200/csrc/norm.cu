@@ -21,8 +21,30 @@ namespace a3b
         template<typename T, int E>
         struct Access
         {
-            static constexpr int words = E == 1 ? 1 : 4;
+            static constexpr int words = E == 1 ? 1 : 4, pairs = E == 1 ? 1 : E / 2;
 
+            // a single element is a pair with 0
+            static __device__ __forceinline__ float2 pair(unsigned const* w, int k)
+            {
+                if constexpr(E > 1)
+                    return PackOf<T>::pair(w, k);
+                else if constexpr(sizeof(T) == 4)
+                    return make_float2(__uint_as_float(w[0]), 0.f);
+                else
+                    return make_float2(PackOf<T>::pair(w, 0).x, 0.f);
+            }
+            // rounded to the nearest values of T
+            static __device__ __forceinline__ void setPair(unsigned* w, int k, float2 v)
+            {
+                if constexpr(E > 1)
+                    PackOf<T>::setPair(w, k, v);
+                else
+                {
+                    unsigned two[2];
+                    PackOf<T>::setPair(two, 0, v);
+                    w[0] = two[0];
+                }
+            }
             static __device__ __forceinline__ void load(unsigned* w, T const* p)
             {
                 if constexpr(E == 1)
@@ -106,6 +128,15 @@ namespace a3b
                         w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
                     }
             }
+            static __device__ __forceinline__ float2 pair(unsigned const* w, int k)
+            {
+                if constexpr(E == 1)
+                    return Access<WT, 1>::pair(w, 0);
+                else if constexpr(std::is_same_v<WT, float>)
+                    return make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+                else
+                    return PackOf<WT>::pair(w, k);
+            }
             static __device__ __forceinline__ void unpack(float* v, unsigned const* w)
             {
                 if constexpr(E == 1)
@@ -187,51 +218,126 @@ namespace a3b
             uint32_t group, groups; // elements that share a scale (0: the row), and groups a row
             bool e5m2;
             double eps;
+            float eps32, inverse; // inverse: 1 / n
+            bool tiny; // eps gives nothing to sums below fp32's range
         };
 
         // fp32 squares are exact enough unless their sum leaves fp32's range: above it, or below it with nothing from eps.
-        __device__ __forceinline__ bool sumLost(float sum, double eps)
+        __device__ __forceinline__ bool sumLost(float sum, bool tiny)
         {
-            return !(sum < INFINITY) || (sum < 0x1p-100f && eps < 0x1p-60);
+            return !(sum < INFINITY) || (tiny && sum < 0x1p-100f);
         }
 
-        __device__ __forceinline__ float rootOf(float sum, uint32_t n, double eps)
+        // rsqrtf is off by two units at most: with the product's and the sum's roundings 2^-21, where a row's own sum may lose
+        // more; the division and square root it replaces cost short rows a fifth of their time
+        __device__ __forceinline__ float rootOf(float sum, float inverse, float eps)
         {
-            return 1.f / sqrtf(sum / static_cast<float>(n) + static_cast<float>(eps));
+            return rsqrtf(fmaf(sum, inverse, eps));
         }
         __device__ __forceinline__ float rootOf(double sum, uint32_t n, double eps)
         {
             return static_cast<float>(1. / sqrt(sum / n + eps));
         }
 
-        // The scale of a group whose largest magnitude is `high`, and what its values are multiplied with. A scale below
-        // fp32's normal numbers has no reciprocal there: its values are divided (`divide`).
-        struct Scale
+        __device__ __noinline__ float2 quotient(float2 v, float by)
         {
-            float scale, inverse;
-            bool divide;
+            return make_float2(__fdiv_rn(v.x, by), __fdiv_rn(v.y, by));
+        }
 
-            __device__ __forceinline__ Scale(float high, bool e5m2)
+        // The scale of a group whose largest magnitude is `high`: a product with the rounded 1 / largest, two roundings in
+        // all, and its reciprocal to one unit; both far below 8 bits' own step. A scale below fp32's normal numbers has no
+        // reciprocal there: its values are divided.
+        template<int N>
+        __device__ __forceinline__ float scaled(float high, bool e5m2, float2 (&y)[N])
+        {
+            float const scale = high * (e5m2 ? 1.f / 57344.f : 1.f / 448.f);
+            if(scale > 0.f && scale < 0x1p-126f)
             {
-                scale = high / (e5m2 ? 57344.f : 448.f);
-                divide = scale > 0.f && scale < 0x1p-126f;
-                inverse = scale == 0.f || divide ? 0.f : 1.f / scale;
+#pragma unroll
+                for(int k = 0; k < N; ++k)
+                    y[k] = quotient(y[k], scale);
             }
-            __device__ __forceinline__ float operator()(float y) const
+            else
             {
-                return divide ? __fdiv_rn(y, scale) : y * inverse;
+                float inverse;
+                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
+                inverse = scale == 0.f ? 0.f : inverse;
+#pragma unroll
+                for(int k = 0; k < N; ++k)
+                    y[k] = mul2(y[k], make_float2(inverse, inverse));
             }
-        };
+            return scale;
+        }
 
         // two values rounded to 8 bits, beyond the largest to the largest
-        __device__ __forceinline__ unsigned eight(float a, float b, bool e5m2)
+        __device__ __forceinline__ unsigned eight(float2 v, bool e5m2)
         {
-            return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, e5m2 ? __NV_E5M2 : __NV_E4M3);
+            return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, e5m2 ? __NV_E5M2 : __NV_E4M3);
+        }
+
+        // A row stays in registers as the words it is stored in (half the registers of its fp32 values, so twice the blocks an
+        // SM; unpacking it again costs less than the spills of holding it did) and is computed on in pairs.
+
+        // Adds the residual's words to a lane's, stores the sum, and returns the lane's sum of squares.
+        template<typename T, int E, int P>
+        __device__ __forceinline__ float addRow(NormArgs const& a, uint32_t row, bool live, uint32_t lanes, uint32_t t,
+                                                unsigned (&raw)[P][Access<T, E>::words],
+                                                unsigned const (&add)[P][Access<T, E>::words])
+        {
+            using A = Access<T, E>;
+            uint32_t const packs = a.n / E;
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for(int p = 0; p < P; ++p)
+                if(uint32_t const k = p * lanes + t; k < packs)
+                {
+                    if(a.residual)
+                    {
+                        // The sum is rounded to the rows' type, stored or not: the norm is that of the row which the next
+                        // layer and the gradient read.
+#pragma unroll
+                        for(int e = 0; e < A::pairs; ++e)
+                            A::setPair(raw[p], e, add2(A::pair(raw[p], e), A::pair(add[p], e)));
+                        if(a.total && live)
+                            A::store(static_cast<T*>(a.total) + a.ts.at(row, a.inner, a.one) + static_cast<size_t>(k) * E, raw[p]);
+                    }
+#pragma unroll
+                    for(int e = 0; e < A::pairs; ++e)
+                    {
+                        float2 const h = A::pair(raw[p], e);
+                        sum = fma2(h, h, sum);
+                    }
+                }
+            return sum.x + sum.y;
+        }
+
+        // 1 / sqrt(mean h^2 + eps) from the team's sum of squares, or in fp64 from h itself where that is lost
+        template<typename T, int E, int P, int L>
+        __device__ __forceinline__ float rootRow(NormArgs const& a, uint32_t lanes, uint32_t t, float sum,
+                                                 unsigned const (&raw)[P][Access<T, E>::words], double* roomD)
+        {
+            using A = Access<T, E>;
+            bool const lost = sumLost(sum, a.tiny);
+            if(!(L == 0 ? lost : __any_sync(kFullMask, lost)))
+                return rootOf(sum, a.inverse, a.eps32);
+            double wide = 0.;
+#pragma unroll
+            for(int p = 0; p < P; ++p)
+                if(p * lanes + t < a.n / E)
+#pragma unroll
+                    for(int e = 0; e < A::pairs; ++e)
+                    {
+                        float2 const h = A::pair(raw[p], e);
+                        wide = fma(static_cast<double>(h.x), static_cast<double>(h.x), wide);
+                        wide = fma(static_cast<double>(h.y), static_cast<double>(h.y), wide);
+                    }
+            wide = teamSum<L>(wide, roomD);
+            return lost ? rootOf(wide, a.n, a.eps) : rootOf(sum, a.inverse, a.eps32);
         }
 
         // One row a team of L lanes (0: a block), P accesses of E elements a lane; the whole row is in registers.
         template<typename T, typename WT, int E, int P, int L, bool F8>
-        __global__ void __launch_bounds__(L == 0 ? 1024 : 128) rmsNormKernel(NormArgs a)
+        __global__ void __launch_bounds__(L > 0 ? 128 : P == 2 ? 512 : 1024, L > 0 || P != 2 ? 1 : 3) rmsNormKernel(NormArgs a)
         {
             using A = Access<T, E>;
             using W = Weights<WT, E>;
@@ -258,7 +364,7 @@ namespace a3b
                         A::load(add[p], r + static_cast<size_t>(k) * E);
             }
             // with the row's loads under way; more than two packs' weights would cost blocks an SM
-            constexpr bool early = P * W::words <= 16;
+            constexpr bool early = P * W::words <= 8;
             unsigned wraw[early ? P : 1][W::words];
             if(early && weight)
 #pragma unroll
@@ -266,127 +372,153 @@ namespace a3b
                     if(uint32_t const k = p * lanes + t; k < packs)
                         W::load(wraw[early ? p : 0], weight + static_cast<size_t>(k) * E);
 
-            float h[P][E];
-            float sum = 0.f;
-#pragma unroll
-            for(int p = 0; p < P; ++p)
-            {
-                uint32_t const k = p * lanes + t;
-                if(k < packs)
-                    A::unpack(h[p], raw[p]);
-                else
-#pragma unroll
-                    for(int e = 0; e < E; ++e)
-                        h[p][e] = 0.f;
-                if(a.residual && k < packs)
-                {
-                    float more[E];
-                    A::unpack(more, add[p]);
-#pragma unroll
-                    for(int e = 0; e < E; ++e)
-                        h[p][e] += more[e];
-                    // The sum is rounded to the rows' type, stored or not: the norm is that of the row which the next
-                    // layer and the gradient read.
-                    A::pack(raw[p], h[p]);
-                    A::unpack(h[p], raw[p]);
-                    if(a.total && live)
-                        A::store(static_cast<T*>(a.total) + a.ts.at(row, a.inner, a.one) + static_cast<size_t>(k) * E, raw[p]);
-                }
-#pragma unroll
-                for(int e = 0; e < E; ++e)
-                    sum = fmaf(h[p][e], h[p][e], sum);
-            }
-            sum = teamSum<L>(sum, roomF);
-            float r;
-            if(L == 0 ? sumLost(sum, a.eps) : __any_sync(kFullMask, sumLost(sum, a.eps)))
-            {
-                double wide = 0.;
-#pragma unroll
-                for(int p = 0; p < P; ++p)
-#pragma unroll
-                    for(int e = 0; e < E; ++e)
-                        wide = fma(static_cast<double>(h[p][e]), static_cast<double>(h[p][e]), wide);
-                wide = teamSum<L>(wide, roomD);
-                r = sumLost(sum, a.eps) ? rootOf(wide, a.n, a.eps) : rootOf(sum, a.n, a.eps);
-            }
-            else
-                r = rootOf(sum, a.n, a.eps);
+            float const sum = teamSum<L>(addRow<T, E, P>(a, row, live, lanes, t, raw, add), roomF);
+            float const r = rootRow<T, E, P, L>(a, lanes, t, sum, raw, roomD);
             if(a.rstd && t == 0 && live)
                 a.rstd[row] = r;
 
-            T* out = static_cast<T*>(a.out) + (F8 ? 0 : a.os.at(row, a.inner, a.one));
-            float high = 0.f;
-#pragma unroll
-            for(int p = 0; p < P; ++p)
+            // y of access p, in pairs
+            auto scaledRow = [&](int p, float2 (&y)[A::pairs])
             {
                 uint32_t const k = p * lanes + t;
-                if(weight && k < packs)
+                if constexpr(!early)
+                    if(weight)
+                        W::load(wraw[0], weight + static_cast<size_t>(k) * E);
+#pragma unroll
+                for(int e = 0; e < A::pairs; ++e)
                 {
-                    float w[E];
-                    if constexpr(early)
-                        W::unpack(w, wraw[p]);
-                    else
-                    {
-                        unsigned words[W::words];
-                        W::load(words, weight + static_cast<size_t>(k) * E);
-                        W::unpack(w, words);
-                    }
-#pragma unroll
-                    for(int e = 0; e < E; ++e)
-                        h[p][e] = h[p][e] * r * w[e];
+                    y[e] = mul2(A::pair(raw[p], e), make_float2(r, r));
+                    if(weight)
+                        y[e] = mul2(y[e], W::pair(wraw[early ? p : 0], e));
                 }
-                else
+            };
+            auto largest = [&](float2 const (&y)[A::pairs])
+            {
+                float high = 0.f;
 #pragma unroll
-                    for(int e = 0; e < E; ++e)
-                        h[p][e] = k < packs ? h[p][e] * r : 0.f;
-                if constexpr(!F8)
-                {
-                    if(k < packs && live)
+                for(int e = 0; e < A::pairs; ++e)
+                    high = maxNan(high, maxNan(fabsf(y[e].x), fabsf(y[e].y)));
+                return high;
+            };
+            if constexpr(!F8)
+            {
+                T* out = static_cast<T*>(a.out) + a.os.at(row, a.inner, a.one);
+#pragma unroll
+                for(int p = 0; p < P; ++p)
+                    if(uint32_t const k = p * lanes + t; k < packs && live)
                     {
-                        A::pack(raw[p], h[p]);
-                        A::store(out + static_cast<size_t>(k) * E, raw[p]);
-                    }
-                }
-                else
+                        float2 y[A::pairs];
+                        scaledRow(p, y);
+                        unsigned words[A::words];
 #pragma unroll
-                    for(int e = 0; e < E; ++e)
-                        high = maxNan(high, fabsf(h[p][e]));
+                        for(int e = 0; e < A::pairs; ++e)
+                            A::setPair(words, e, y[e]);
+                        A::store(out + static_cast<size_t>(k) * E, words);
+                    }
             }
-            if constexpr(F8)
+            else
             {
                 static_assert(E > 1 && (L == 0 || L == 32), "groups lie on neighbouring lanes");
-                auto* out8 = static_cast<unsigned char*>(a.out) + a.os.at(row, a.inner, a.one);
+                auto* out = static_cast<unsigned char*>(a.out) + a.os.at(row, a.inner, a.one);
                 float* scales = a.scales + static_cast<size_t>(row) * a.groups;
-                if(a.group == 0)
-                    high = teamMax<L>(high, roomM);
                 int const near = static_cast<int>(a.group) / E; // lanes of one group
+                float high = 0.f;
+                if(a.group == 0)
+                {
+#pragma unroll
+                    for(int p = 0; p < P; ++p)
+                        if(p * lanes + t < packs)
+                        {
+                            float2 y[A::pairs];
+                            scaledRow(p, y);
+                            high = maxNan(high, largest(y));
+                        }
+                    high = teamMax<L>(high, roomM);
+                }
 #pragma unroll
                 for(int p = 0; p < P; ++p)
                 {
                     uint32_t const k = p * lanes + t;
-                    if(a.group != 0)
-                    {
-                        high = 0.f;
+                    float2 y[A::pairs];
 #pragma unroll
-                        for(int e = 0; e < E; ++e)
-                            high = maxNan(high, fabsf(h[p][e]));
-                        high = lanesMax(high, near);
-                    }
-                    Scale const s(high, a.e5m2);
+                    for(int e = 0; e < A::pairs; ++e)
+                        y[e] = make_float2(0.f, 0.f);
+                    if(k < packs)
+                        scaledRow(p, y);
+                    if(a.group != 0)
+                        high = lanesMax(largest(y), near);
+                    float const scale = scaled<A::pairs>(high, a.e5m2, y);
                     if(k < packs && live)
                     {
                         if(a.group != 0 ? k % near == 0 : k == 0)
-                            scales[a.group != 0 ? k / near : 0] = s.scale;
+                            scales[a.group != 0 ? k / near : 0] = scale;
                         unsigned w[E / 4];
 #pragma unroll
-                        for(int e = 0; e < E; e += 4)
-                            w[e / 4] = eight(s(h[p][e]), s(h[p][e + 1]), a.e5m2)
-                                       | (eight(s(h[p][e + 2]), s(h[p][e + 3]), a.e5m2) << 16);
+                        for(int e = 0; e < E / 4; ++e)
+                            w[e] = eight(y[2 * e], a.e5m2) | (eight(y[2 * e + 1], a.e5m2) << 16);
                         if constexpr(E == 8)
-                            *reinterpret_cast<uint2*>(out8 + static_cast<size_t>(k) * E) = make_uint2(w[0], w[1]);
+                            *reinterpret_cast<uint2*>(out + static_cast<size_t>(k) * E) = make_uint2(w[0], w[1]);
                         else
-                            *reinterpret_cast<unsigned*>(out8 + static_cast<size_t>(k) * E) = w[0];
+                            *reinterpret_cast<unsigned*>(out + static_cast<size_t>(k) * E) = w[0];
                     }
+                }
+            }
+        }
+
+        // Short rows in great number: a team of L lanes has R of them at once, one access a lane each, so that R rows' loads
+        // are under way (with one, a block waits for 2 KB).
+        template<typename T, typename WT, int E, int L, int R>
+        __global__ void __launch_bounds__(128) rmsNormShortKernel(NormArgs a)
+        {
+            using A = Access<T, E>;
+            using W = Weights<WT, E>;
+            constexpr uint32_t teams = 128 / L;
+            uint32_t const t = threadIdx.x % L, first = blockIdx.x * (teams * R) + threadIdx.x / L;
+            bool const in = t < a.n / E;
+            WT const* weight = static_cast<WT const*>(a.weight);
+            unsigned raw[R][1][A::words], add[R][1][A::words], wraw[W::words];
+#pragma unroll
+            for(int q = 0; q < R; ++q)
+            {
+                uint32_t const row = min(first + q * teams, a.rows - 1u);
+                if(in)
+                    A::load(raw[q][0], static_cast<T const*>(a.x) + a.xs.at(row, a.inner, a.one) + t * E);
+                if(in && a.residual)
+                    A::load(add[q][0], static_cast<T const*>(a.residual) + a.rs.at(row, a.inner, a.one) + t * E);
+            }
+            if(in && weight)
+                W::load(wraw, weight + t * E);
+            float sum[R];
+#pragma unroll
+            for(int q = 0; q < R; ++q)
+            {
+                uint32_t const row = first + q * teams;
+                sum[q] = addRow<T, E, 1>(a, min(row, a.rows - 1u), row < a.rows, L, t, raw[q], add[q]);
+            }
+#pragma unroll
+            for(int q = 0; q < R; ++q)
+                sum[q] = lanesSum<L>(sum[q]);
+#pragma unroll
+            for(int q = 0; q < R; ++q)
+            {
+                uint32_t const row = first + q * teams;
+                float const r = rootRow<T, E, 1, L>(a, L, t, sum[q], raw[q], nullptr);
+                if(row >= a.rows)
+                    continue;
+                if(a.rstd && t == 0)
+                    a.rstd[row] = r;
+                if(in)
+                {
+                    unsigned words[A::words];
+#pragma unroll
+                    for(int e = 0; e < A::pairs; ++e)
+                    {
+                        float2 y = mul2(A::pair(raw[q][0], e), make_float2(r, r));
+                        if(weight)
+                            y = mul2(y, W::pair(wraw, e));
+                        A::setPair(words, e, y);
+                    }
+                    A::store(static_cast<T*>(a.out) + a.os.at(row, a.inner, a.one) + t * E, words);
                 }
             }
         }
@@ -430,7 +562,7 @@ namespace a3b
             }
             sum = teamSum<0>(sum, roomF); // also orders the stores of `total` before the reads below
             float r;
-            if(sumLost(sum, a.eps))
+            if(sumLost(sum, a.tiny))
             {
                 double wide = 0.;
                 for(uint32_t k = t; k < a.n; k += kLongThreads)
@@ -441,7 +573,7 @@ namespace a3b
                 r = rootOf(teamSum<0>(wide, roomD), a.n, a.eps);
             }
             else
-                r = rootOf(sum, a.n, a.eps);
+                r = rootOf(sum, a.inverse, a.eps32);
             if(a.rstd && t == 0)
                 a.rstd[row] = r;
             auto y = [&](uint32_t k)
@@ -465,33 +597,38 @@ namespace a3b
 #pragma unroll 4
                 for(uint32_t k = t; k < a.n; k += kLongThreads)
                     high = maxNan(high, fabsf(y(k)));
-                Scale const s(teamMax<0>(high, roomM), a.e5m2);
-                if(t == 0)
-                    scales[0] = s.scale;
+                high = teamMax<0>(high, roomM);
 #pragma unroll 4
                 for(uint32_t k = t; k < a.n; k += kLongThreads)
-                    out[k] = static_cast<unsigned char>(eight(s(y(k)), 0.f, a.e5m2));
+                {
+                    float2 v[1] = {make_float2(y(k), 0.f)};
+                    float const scale = scaled(high, a.e5m2, v);
+                    if(k == 0)
+                        scales[0] = scale;
+                    out[k] = static_cast<unsigned char>(eight(v[0], a.e5m2));
+                }
                 return;
             }
             // a warp takes a group of 32, 64 or 128 elements
             uint32_t const warp = t / 32, lane = t % 32;
             for(uint32_t g = warp; g < a.groups; g += kLongThreads / 32)
             {
-                float v[4], high = 0.f;
+                float2 v[4];
+                float high = 0.f;
 #pragma unroll
                 for(uint32_t e = 0; e < 4; ++e)
                 {
                     uint32_t const in = e * 32 + lane, k = g * a.group + in;
-                    v[e] = in < a.group && k < a.n ? y(k) : 0.f;
-                    high = maxNan(high, fabsf(v[e]));
+                    v[e] = make_float2(in < a.group && k < a.n ? y(k) : 0.f, 0.f);
+                    high = maxNan(high, fabsf(v[e].x));
                 }
-                Scale const s(lanesMax(high, 32), a.e5m2);
+                float const scale = scaled(lanesMax(high, 32), a.e5m2, v);
                 if(lane == 0)
-                    scales[g] = s.scale;
+                    scales[g] = scale;
 #pragma unroll
                 for(uint32_t e = 0; e < 4; ++e)
                     if(uint32_t const in = e * 32 + lane, k = g * a.group + in; in < a.group && k < a.n)
-                        out[k] = static_cast<unsigned char>(eight(s(v[e]), 0.f, a.e5m2));
+                        out[k] = static_cast<unsigned char>(eight(v[e], a.e5m2));
             }
         }
 
@@ -509,7 +646,19 @@ namespace a3b
             {
                 uint32_t const packs = a.n / E;
                 bool const many = a.rows >= 4u * static_cast<uint32_t>(props->smCount);
-                if(!F8 && packs <= 8 && many)
+                // Two rows a team where that leaves eight blocks an SM (65536 x 128 bf16 8.2 us, 9.2 with one, 8.8 with four; but
+                // 4096 x 128 2.5, 2.1 with one).
+                uint32_t const part = packs <= 8 ? 8 : packs <= 16 ? 16 : 32, pairBlocks = (a.rows + 256 / part - 1) / (256 / part);
+                if(!F8 && packs <= 32 && pairBlocks >= 8u * static_cast<uint32_t>(props->smCount))
+                {
+                    if(part == 8)
+                        rmsNormShortKernel<T, WT, E, 8, 2><<<pairBlocks, 128, 0, stream>>>(a);
+                    else if(part == 16)
+                        rmsNormShortKernel<T, WT, E, 16, 2><<<pairBlocks, 128, 0, stream>>>(a);
+                    else
+                        rmsNormShortKernel<T, WT, E, 32, 2><<<pairBlocks, 128, 0, stream>>>(a);
+                }
+                else if(!F8 && packs <= 8 && many)
                     rmsNormKernel<T, WT, E, 1, F8 ? 32 : 8, F8><<<teams(8), 128, 0, stream>>>(a);
                 else if(!F8 && packs <= 16 && many)
                     rmsNormKernel<T, WT, E, 1, F8 ? 32 : 16, F8><<<teams(16), 128, 0, stream>>>(a);
@@ -521,7 +670,7 @@ namespace a3b
                     rmsNormKernel<T, WT, E, 4, 32, F8><<<teams(32), 128, 0, stream>>>(a);
                 else if(packs <= 1024 && !many)
                     rmsNormKernel<T, WT, E, 1, 0, F8><<<a.rows, roundUp(packs, 32), 0, stream>>>(a);
-                else if(packs <= 2048)
+                else if(packs <= 1024)
                     rmsNormKernel<T, WT, E, 2, 0, F8><<<a.rows, roundUp((packs + 1) / 2, 32), 0, stream>>>(a);
                 else if(packs <= 4096)
                     rmsNormKernel<T, WT, E, 4, 0, F8><<<a.rows, roundUp((packs + 3) / 4, 32), 0, stream>>>(a);
@@ -939,7 +1088,8 @@ extern "C"
         NormArgs a{x, residual, total, out, {x_outer_stride, x_inner_stride}, {residual_outer_stride, residual_inner_stride},
                    {total_outer_stride, total_inner_stride}, {out_outer_stride, out_inner_stride},
                    static_cast<uint32_t>(rows), static_cast<uint32_t>(inner), static_cast<uint32_t>(n), one, weight, rstd,
-                   scales, group, static_cast<uint32_t>(groups), out_dtype == A3B_E5M2, eps};
+                   scales, group, static_cast<uint32_t>(groups), out_dtype == A3B_E5M2, eps, static_cast<float>(eps),
+                   1.f / static_cast<float>(n), eps < 0x1p-60};
         auto s = static_cast<cudaStream_t>(stream);
         bool const wide = weight && weight_dtype == A3B_F32;
         if(dtype == A3B_F32)

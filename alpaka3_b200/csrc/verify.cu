@@ -4,11 +4,14 @@
 //   draft i stands while u_i q(t_i) < p(t_i);  at the first that does not, the token is drawn from (p - q)+, and behind
 //   drafts that all stand from p: the first of exponential clocks with these rates, argmax of rate_v / noise_v.
 //
-// Every token that comes out is what the formula gives in 64 bits for these inputs, at the cost of 32: the tests take a few
-// exponentials and are done in fp64; of the draw, a pass in fp32 gives every quotient an interval that holds its true value,
-// and only the tokens whose interval reaches the best lower end (mostly one) are computed again in fp64. The pass reads one
-// row of the target, one of the noise and, after a refusal, one of the draft, and is bound by memory where sequences are
-// many, by latency where they are few: a cluster of blocks shares one sequence.
+// Every token that comes out is what the formula gives in 64 bits for these inputs, at the cost of 32: in fp32 every
+// probability and quotient has an interval that holds its true value, and only what intervals cannot tell apart (drafts next
+// to the border, quotients next to the largest) is computed again in fp64; mostly that is nothing.
+//
+// As (p - q)+ <= p, a token can only win if p_v / noise_v reaches the best lower end known so far. So the draw reads one row
+// of the target and one of the noise, tests p_v against a product, without a division, and reads of the draft's row only what
+// stands where that test passes (a few dozen tokens). It is bound by memory where sequences are many, by latency where they
+// are few: a cluster of blocks shares one sequence.
 #include <algorithm>
 
 #include "layout.cuh"
@@ -100,7 +103,7 @@ namespace a3b
             }
         };
 
-        __device__ __forceinline__ double exactly(double scale, float z, float lse)
+        __device__ __noinline__ double exactly(double scale, float z, float lse)
         {
             return exp(scale * static_cast<double>(z) - static_cast<double>(lse));
         }
@@ -133,7 +136,23 @@ namespace a3b
             return b;
         }
 
-        // How many drafts stand; every thread of the block gets the same answer. Also reads the drafts' ends.
+        // Whether a draft stands, u q < p: by intervals in fp32 where they lie apart, else in 64 bits.
+        __device__ __forceinline__ bool stands(VerifyArgs const& a, float z, float lse, bool other, float y, float draftLse, float u)
+        {
+            Rough const p(a.scale, lse), q(a.draftScale, draftLse);
+            float const have = p(z), need = u * (other ? q(y) : 1.f);
+            float const wide = fmaf(other ? fmaxf(p.off, q.off) : p.off, have + need, 0x1p-125f);
+            if(!p.far() && !(other && q.far()))
+            {
+                if(need + wide < have)
+                    return true;
+                if(need > have + wide)
+                    return false;
+            }
+            return static_cast<double>(u) * (other ? exactly(a.draftScale, y, draftLse) : 1.) < exactly(a.scale, z, lse);
+        }
+
+        // How many drafts stand; every thread of the block gets the same answer.
         template<typename T>
         __device__ __forceinline__ uint32_t accepted(VerifyArgs const& a, uint32_t b, bool* refused)
         {
@@ -145,25 +164,26 @@ namespace a3b
                 uint32_t const i = first + lane;
                 int64_t const t = i < a.length ? a.index(a.drafts, at + i) : -1;
                 bool const known = a.known(t);
-                bool stands = false;
+                bool yes = false;
                 if(known)
                 {
                     T const* row = static_cast<T const*>(a.logits) + static_cast<int64_t>(b) * a.ls.outer
                                    + static_cast<int64_t>(i) * a.ls.step;
-                    double const p = exactly(a.scale, toFloat(row[t]), a.lse[at + b + i]);
-                    double q = 1.;
+                    float const z = toFloat(row[t]), lse = a.lse[at + b + i], u = a.uniform[at + i];
+                    float y = 0.f, draftLse = 0.f;
                     if(a.draft)
                     {
                         T const* other = static_cast<T const*>(a.draft) + static_cast<int64_t>(b) * a.ds.outer
                                          + static_cast<int64_t>(i) * a.ds.step;
-                        q = exactly(a.draftScale, toFloat(other[t]), a.draftLse[at + i]);
+                        y = toFloat(other[t]);
+                        draftLse = a.draftLse[at + i];
                     }
-                    stands = static_cast<double>(a.uniform[at + i]) * q < p;
+                    yes = stands(a, z, lse, a.draft != nullptr, y, draftLse, u);
                 }
-                unsigned const yes = __ballot_sync(kFullMask, stands), some = __ballot_sync(kFullMask, known);
-                if(yes != kFullMask)
+                unsigned const all = __ballot_sync(kFullMask, yes), some = __ballot_sync(kFullMask, known);
+                if(all != kFullMask)
                 {
-                    uint32_t const n = __ffs(~yes) - 1;
+                    uint32_t const n = __ffs(~all) - 1;
                     *refused = (some >> n) & 1u;
                     return first + n;
                 }
@@ -172,48 +192,26 @@ namespace a3b
             return a.length;
         }
 
-        // E neighbouring elements of the three rows
+        // E neighbouring logits, or single ones
         template<typename T, int E>
-        struct Terms
+        struct Lot
         {
             static constexpr int words = E == 1 ? 1 : 4;
-            unsigned z[words], y[words];
-            float noise[E];
+            unsigned w[words];
 
-            __device__ __forceinline__ void load(T const* row, T const* other, float const* clock, uint32_t k)
+            __device__ __forceinline__ void load(T const* row, uint32_t k)
             {
-                if constexpr(E == 1)
+                if constexpr(E > 1)
                 {
-                    z[0] = raw(row + k);
-                    if(other)
-                        y[0] = raw(other + k);
-                    noise[0] = clock[k];
+                    uint4 const v = *reinterpret_cast<uint4 const*>(row + static_cast<size_t>(k) * E);
+                    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
                 }
+                else if constexpr(sizeof(T) == 4)
+                    w[0] = *reinterpret_cast<unsigned const*>(row + k);
                 else
-                {
-                    uint4 v = *reinterpret_cast<uint4 const*>(row + static_cast<size_t>(k) * E);
-                    z[0] = v.x, z[1] = v.y, z[2] = v.z, z[3] = v.w;
-                    if(other)
-                    {
-                        v = *reinterpret_cast<uint4 const*>(other + static_cast<size_t>(k) * E);
-                        y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
-                    }
-#pragma unroll
-                    for(int e = 0; e < E; e += 4)
-                    {
-                        float4 const f = *reinterpret_cast<float4 const*>(clock + static_cast<size_t>(k) * E + e);
-                        noise[e] = f.x, noise[e + 1] = f.y, noise[e + 2] = f.z, noise[e + 3] = f.w;
-                    }
-                }
+                    w[0] = *reinterpret_cast<unsigned short const*>(row + k);
             }
-            static __device__ __forceinline__ unsigned raw(T const* p)
-            {
-                if constexpr(sizeof(T) == 4)
-                    return *reinterpret_cast<unsigned const*>(p);
-                else
-                    return *reinterpret_cast<unsigned short const*>(p);
-            }
-            static __device__ __forceinline__ void unpack(float* v, unsigned const* w)
+            __device__ __forceinline__ void unpack(float* v) const
             {
                 if constexpr(E == 1 && std::is_same_v<T, float>)
                     v[0] = __uint_as_float(w[0]);
@@ -229,51 +227,107 @@ namespace a3b
             }
         };
 
-        template<typename T, int E>
-        __device__ __forceinline__ void roughly(Terms<T, E> const& t, bool other, uint32_t certain, uint32_t first, Rough const& p,
-                                                Rough const& q, Ends* ends)
+        template<int E>
+        __device__ __forceinline__ void loadNoise(float* noise, float const* clock, uint32_t k)
         {
-            float z[E], y[E];
-            Terms<T, E>::unpack(z, t.z);
-            if(other)
-                Terms<T, E>::unpack(y, t.y);
-            float const off = other ? fmaxf(p.off, q.off) : p.off;
+            if constexpr(E == 1)
+                noise[0] = clock[k];
+            else
 #pragma unroll
-            for(int e = 0; e < E; ++e)
-                p.widen(z[e], other ? q(y[e]) : first + e == certain ? 1.f : 0.f, t.noise[e], off, ends);
+                for(int e = 0; e < E; e += 4)
+                {
+                    float4 const f = *reinterpret_cast<float4 const*>(clock + static_cast<size_t>(k) * E + e);
+                    noise[e] = f.x, noise[e + 1] = f.y, noise[e + 2] = f.z, noise[e + 3] = f.w;
+                }
         }
 
-        // Token i in 64 bits, if its interval reaches `bar` (or intervals say nothing: `far`).
-        template<typename T>
-        __device__ __noinline__ void again(VerifyArgs const& a, T const* row, T const* other, float const* clock, uint32_t certain,
-                                           float lse, float draftLse, float bar, bool far, uint32_t i, Best* best)
+        constexpr uint32_t kList = 1024;
+
+        // This thread's lots first, first + kThreads, ...: tokens with p / noise >= least go to the list. U lots are loaded
+        // together, without conditions between the loads: 64 x 131072 bf16 takes 17.5 us with two packs together, 18.8 with
+        // one, 18.4 with three; 256 x 50257 fp32 (single tokens) 31.6 with eight, 35.9 with four, 39 with twelve (spills);
+        // stages in shared memory filled by bulk copies took 26 and 39 (a barrier a stage).
+        template<typename T, int E, int U>
+        __device__ __forceinline__ void scan(T const* row, float const* clock, uint32_t first, uint32_t end, Rough const& p, float least,
+                                             uint32_t* list, unsigned* listed)
         {
-            float const z = toFloat(row[i]), y = other ? toFloat(other[i]) : 0.f, noise = clock[i];
-            if(!far)
+            float const more = 1.f + p.off;
+            auto test = [&](Lot<T, E> const& t, float const* noise, uint32_t k)
             {
-                Rough const p(a.scale, lse), q(a.draftScale, draftLse);
-                Ends ends{-INFINITY, -INFINITY};
-                p.widen(z, other ? q(y) : i == certain ? 1.f : 0.f, noise, other ? fmaxf(p.off, q.off) : p.off, &ends);
-                if(!(ends.high >= bar))
-                    return;
+                float z[E];
+                t.unpack(z);
+                unsigned pass = 0;
+#pragma unroll
+                for(int e = 0; e < E; ++e)
+                    pass |= fmaf(p(z[e]), more, 0x1p-125f) >= least * noise[e] ? 1u << e : 0u; // not where either is NaN
+                while(pass)
+                {
+                    unsigned const e = __ffs(pass) - 1, at = atomicAdd(listed, 1u);
+                    pass &= pass - 1;
+                    if(at < kList)
+                        list[at] = k * E + e;
+                }
+            };
+            uint32_t k = first;
+            if constexpr(U > 1)
+            {
+#pragma unroll 1
+                for(; k + (U - 1) * kThreads < end; k += U * kThreads)
+                {
+                    Lot<T, E> t[U];
+                    float noise[U][E];
+#pragma unroll
+                    for(int u = 0; u < U; ++u)
+                    {
+                        t[u].load(row, k + u * kThreads);
+                        loadNoise<E>(noise[u], clock, k + u * kThreads);
+                    }
+#pragma unroll
+                    for(int u = 0; u < U; ++u)
+                        test(t[u], noise[u], k + u * kThreads);
+                }
             }
-            double rate = exactly(a.scale, z, lse);
+#pragma unroll 1
+            for(; k < end; k += kThreads)
+            {
+                Lot<T, E> t;
+                float noise[E];
+                t.load(row, k);
+                loadNoise<E>(noise, clock, k);
+                test(t, noise, k);
+            }
+        }
+
+        // token i in 64 bits
+        template<typename T>
+        __device__ __forceinline__ void again(VerifyArgs const& a, T const* row, T const* other, float const* clock, uint32_t certain,
+                                              float lse, float draftLse, uint32_t i, Best* best)
+        {
+            double rate = exactly(a.scale, toFloat(row[i]), lse);
             if(other)
-                rate -= exactly(a.draftScale, y, draftLse);
+                rate -= exactly(a.draftScale, toFloat(other[i]), draftLse);
             else if(i == certain)
                 rate -= 1.;
             if(rate > 0.)
-                best->take(rate / static_cast<double>(noise), i);
+                best->take(rate / static_cast<double>(clock[i]), i);
         }
 
-        template<typename T>
-        __global__ void __launch_bounds__(kThreads) verifyKernel(VerifyArgs a)
+        constexpr uint32_t kReach = 64;
+
+        // Packed: every row of logits, draft and noise begins at 16 bytes.
+        template<typename T, bool Packed>
+        __global__ void __launch_bounds__(kThreads, 4) verifyKernel(VerifyArgs a)
         {
             constexpr int E = PackOf<T>::E, kWarps = kThreads / 32;
             __shared__ float lows[kWarps];
             __shared__ float blockLow;
             __shared__ Best bests[kWarps];
             __shared__ Best blockBest;
+            __shared__ uint32_t list[kList];
+            __shared__ unsigned listed;
+            __shared__ bool blockFull;
+            __shared__ uint32_t found[kReach]; // of the cluster's first block: tokens whose interval reaches the best lower end
+            __shared__ unsigned founds;
             unsigned const rank = clusterRank(), blocks = clusterBlocks();
             uint32_t const b = blockIdx.x / blocks, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
             size_t const at = static_cast<size_t>(b) * a.length, to = at + b;
@@ -306,13 +360,31 @@ namespace a3b
                 return;
             }
 
+            // The block's share of the vocabulary: lots [low, high) of E tokens, and behind the last lot single ones.
+            uint32_t const lots = Packed ? a.vocab / E : 0, per = (lots + blocks - 1) / blocks;
+            uint32_t const low = min(rank * per, lots), high = min(low + per, lots);
+            uint32_t const ones = a.vocab - lots * E, onesPer = (ones + blocks - 1) / blocks;
+            uint32_t const oneLow = lots * E + min(rank * onesPer, ones), oneHigh = min(oneLow + onesPer, a.vocab);
+            float const* clock = a.noise + static_cast<int64_t>(b) * a.noiseStride;
+            if(tid == 0)
+            {
+                founds = 0;
+                // the noise needs no decision: it comes into L2 while the drafts are tested
+                auto at16 = [&](size_t i) { return reinterpret_cast<uintptr_t>(clock + i); };
+                uintptr_t const from = (at16(Packed ? low * static_cast<size_t>(E) : oneLow) + 15) & ~uintptr_t(15);
+                uintptr_t const end = at16(Packed ? high * static_cast<size_t>(E) : oneHigh) & ~uintptr_t(15);
+                if(end > from)
+                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from),
+                                 "r"(static_cast<unsigned>(min(end - from, uintptr_t(1) << 20))));
+            }
+
             bool refused = false;
             uint32_t const n = accepted<T>(a, b, &refused);
             T const* row = static_cast<T const*>(a.logits) + static_cast<int64_t>(b) * a.ls.outer + static_cast<int64_t>(n) * a.ls.step;
             float const lse = a.lse[to + n];
-            float const* clock = a.noise + static_cast<int64_t>(b) * a.noiseStride;
             Rough const p(a.scale, lse);
-            Best result{0., UINT32_MAX};
+            uint32_t drawn = UINT32_MAX;
+            bool certainly = false;
             // once with what the draft took away; if that leaves nothing, once more without
             for(int turn = refused ? 0 : 1; turn < 2; ++turn)
             {
@@ -331,100 +403,190 @@ namespace a3b
                         certain = static_cast<uint32_t>(a.index(a.drafts, at + n));
                 }
                 Rough const q(a.draftScale, draftLse);
-                bool const packed = ((reinterpret_cast<uintptr_t>(row) | reinterpret_cast<uintptr_t>(other)
-                                      | reinterpret_cast<uintptr_t>(clock)) & 15u) == 0u;
-                uint32_t const packs = packed ? a.vocab / E : 0, step = blocks * kThreads, mine = rank * kThreads + tid;
                 bool const far = p.far() || q.far(); // then every token is computed in 64 bits
-                Ends ends{-INFINITY, far ? INFINITY : -INFINITY};
+                float const off = other ? fmaxf(p.off, q.off) : p.off;
+                auto interval = [&](uint32_t i)
+                {
+                    Ends one{-INFINITY, -INFINITY};
+                    p.widen(toFloat(row[i]), other ? q(toFloat(other[i])) : i == certain ? 1.f : 0.f, clock[i], off, &one);
+                    return one;
+                };
+                auto blockMax = [&](float v)
+                {
+#pragma unroll
+                    for(int d = 16; d > 0; d /= 2)
+                        v = fmaxf(v, __shfl_xor_sync(kFullMask, v, d));
+                    if(lane == 0)
+                        lows[warp] = v;
+                    __syncthreads();
+#pragma unroll
+                    for(int w = 0; w < kWarps; ++w)
+                        v = fmaxf(v, lows[w]);
+                    __syncthreads(); // `lows` may be written again
+                    return v;
+                };
+                float least = 0.f, upper[kList / kThreads];
+                bool full = far;
                 if(!far)
                 {
-#pragma unroll 2
-                    for(uint32_t k = mine; k < packs; k += step)
+                    // a first bound from the first lot of each thread, or its first four tokens
+                    Ends ends{-INFINITY, -INFINITY};
+                    if(Packed && low + tid < high)
                     {
-                        Terms<T, E> t;
-                        t.load(row, other, clock, k);
-                        roughly<T, E>(t, other, certain, k * E, p, q, &ends);
+                        Lot<T, E> t, s;
+                        float z[E], y[E], noise[E];
+                        t.load(row, low + tid);
+                        if(other)
+                            s.load(other, low + tid);
+                        loadNoise<E>(noise, clock, low + tid);
+                        t.unpack(z);
+                        if(other)
+                            s.unpack(y);
+#pragma unroll
+                        for(int e = 0; e < E; ++e)
+                            p.widen(z[e], other ? q(y[e]) : (low + tid) * E + e == certain ? 1.f : 0.f, noise[e], off, &ends);
                     }
-#pragma unroll 4
-                    for(uint32_t k = packs * E + mine; k < a.vocab; k += step)
+                    else if(!Packed)
+#pragma unroll
+                        for(int u = 0; u < 4; ++u)
+                            if(uint32_t const i = oneLow + u * kThreads + tid; i < oneHigh)
+                                ends.low = fmaxf(ends.low, interval(i).low);
+                    // Then what can reach the bound; more than the list holds give a better bound and another try.
+                    full = true;
+                    for(int round = 0; full && round < 4; ++round)
                     {
-                        Terms<T, 1> t;
-                        t.load(row, other, clock, k);
-                        roughly<T, 1>(t, other, certain, k, p, q, &ends);
+                        if(tid == 0)
+                            listed = 0;
+                        float const better = blockMax(ends.low);
+                        if(round > 0 && !(better > least))
+                            break;
+                        least = fmaxf(least, better);
+                        if constexpr(Packed)
+                            scan<T, E, 2>(row, clock, low + tid, high, p, least, list, &listed);
+                        scan<T, 1, 8>(row, clock, oneLow + tid, oneHigh, p, least, list, &listed);
+                        __syncthreads();
+                        full = listed > kList;
+#pragma unroll
+                        for(int u = 0; u < static_cast<int>(kList) / kThreads; ++u)
+                        {
+                            uint32_t const k = u * kThreads + tid;
+                            Ends one{-INFINITY, -INFINITY};
+                            if(k < min(listed, kList))
+                                one = interval(list[k]);
+                            upper[u] = one.high;
+                            ends.low = fmaxf(ends.low, one.low);
+                        }
+                        __syncthreads(); // `listed` has been read
                     }
+                    least = fmaxf(least, blockMax(ends.low));
                 }
+                if(tid == 0)
+                {
+                    blockLow = least;
+                    blockFull = full;
+                }
+                clusterArrive();
+                clusterWait();
                 // the best lower end of the sequence
-                float low = ends.low;
-#pragma unroll
-                for(int d = 16; d > 0; d /= 2)
-                    low = fmaxf(low, __shfl_xor_sync(kFullMask, low, d));
-                if(lane == 0)
-                    lows[warp] = low;
-                __syncthreads();
-                if(tid == 0)
-                {
-#pragma unroll
-                    for(int w = 1; w < kWarps; ++w)
-                        low = fmaxf(low, lows[w]);
-                    blockLow = low;
-                }
-                clusterArrive();
-                clusterWait();
-                float bar = -INFINITY;
+                float bar = 0.f;
+                bool useless = false;
                 for(unsigned r = 0; r < blocks; ++r)
+                {
                     bar = fmaxf(bar, *inBlock(&blockLow, r));
-                // the few tokens that reach it, in 64 bits
-                Best best{0., UINT32_MAX};
-                if(ends.high >= bar)
-                {
-                    for(uint32_t k = mine; k < packs; k += step)
-                        for(uint32_t e = 0; e < E; ++e)
-                            again<T>(a, row, other, clock, certain, lse, draftLse, bar, far, k * E + e, &best);
-                    for(uint32_t k = packs * E + mine; k < a.vocab; k += step)
-                        again<T>(a, row, other, clock, certain, lse, draftLse, bar, far, k, &best);
+                    useless |= *inBlock(&blockFull, r);
                 }
-                best = warpBest(best);
-                if(lane == 0)
-                    bests[warp] = best;
-                __syncthreads();
-                if(tid == 0)
+                if(bar > 0.f && bar < INFINITY && !useless)
                 {
+                    // The token with this lower end has a positive rate. If no other one reaches it, it is the token, and
+                    // nothing is computed again.
 #pragma unroll
-                    for(int w = 1; w < kWarps; ++w)
-                        best.take(bests[w].score, bests[w].index);
-                    blockBest = best;
+                    for(int u = 0; u < static_cast<int>(kList) / kThreads; ++u)
+                        if(upper[u] >= bar)
+                        {
+                            unsigned const k = atomicAdd(inBlock(&founds, 0), 1u);
+                            if(k < kReach)
+                                *inBlock(found + k, 0) = list[u * kThreads + tid];
+                        }
+                    __syncwarp();
+                    clusterArrive();
+                    clusterWait();
+                    unsigned const all = *inBlock(&founds, 0);
+                    certainly = all <= kReach;
+                    if(certainly)
+                    {
+                        clusterArrive(); // the first block may leave when all have read its count
+                        if(rank != 0)
+                        {
+                            clusterWait();
+                            return;
+                        }
+                        if(all == 1)
+                            drawn = found[0];
+                        else if(warp == 0)
+                        {
+                            Best best{0., UINT32_MAX};
+                            for(uint32_t k = lane; k < all; k += 32)
+                                again<T>(a, row, other, clock, certain, lse, draftLse, found[k], &best);
+                            drawn = warpBest(best).index;
+                        }
+                    }
                 }
-                clusterArrive();
-                clusterWait();
-                for(unsigned r = 0; r < blocks; ++r)
+                if(!certainly)
                 {
-                    Best const* far = inBlock(&blockBest, r);
-                    result.take(far->score, far->index);
+                    // Intervals say nothing (rows with nothing left, far logits, many equal quotients, noise at 0): all tokens in
+                    // 64 bits.
+                    Best best{0., UINT32_MAX};
+                    for(uint32_t i = low * E + tid; i < high * E; i += kThreads)
+                        again<T>(a, row, other, clock, certain, lse, draftLse, i, &best);
+                    for(uint32_t i = oneLow + tid; i < oneHigh; i += kThreads)
+                        again<T>(a, row, other, clock, certain, lse, draftLse, i, &best);
+                    best = warpBest(best);
+                    if(lane == 0)
+                        bests[warp] = best;
+                    __syncthreads();
+                    if(tid == 0)
+                    {
+#pragma unroll
+                        for(int w = 1; w < kWarps; ++w)
+                            best.take(bests[w].score, bests[w].index);
+                        blockBest = best;
+                    }
+                    clusterArrive();
+                    clusterWait();
+                    Best result{0., UINT32_MAX};
+                    for(unsigned r = 0; r < blocks; ++r)
+                    {
+                        Best const* there = inBlock(&blockBest, r);
+                        result.take(there->score, there->index);
+                    }
+                    drawn = result.index;
                 }
-                if(result.index != UINT32_MAX)
-                    break; // the same in every thread of the cluster
+                if(certainly || drawn != UINT32_MAX)
+                    break; // the same in every thread of the cluster that is still here
             }
             if(rank == 0 && warp == 0)
             {
                 for(uint32_t i = lane; i <= a.length; i += 32)
                     a.put(a.tokens, to + i,
-                          i > n ? -1 : i < n ? a.index(a.drafts, at + i) : result.index == UINT32_MAX ? -1 : static_cast<int64_t>(result.index));
+                          i > n ? -1 : i < n ? a.index(a.drafts, at + i) : drawn == UINT32_MAX ? -1 : static_cast<int64_t>(drawn));
                 if(lane == 0)
                     a.put(a.accepted, b, n);
             }
             // no block leaves while another may still read its shared memory
-            clusterArrive();
+            __syncwarp();
+            if(!certainly)
+                clusterArrive();
             clusterWait();
         }
 
         template<typename T>
-        int launchVerify(cudaStream_t stream, DeviceProps const* props, VerifyArgs const& a)
+        int launchVerify(cudaStream_t stream, DeviceProps const* props, VerifyArgs const& a, bool packed)
         {
             // A cluster of up to eight blocks a sequence: as many as leave each thread about two packs, and fewer when the
-            // sequences alone fill the GPU.
+            // sequences alone fill the GPU (four blocks an SM).
             constexpr uint32_t E = PackOf<T>::E;
             uint32_t blocks = 1;
-            uint64_t const room = 8ull * static_cast<unsigned>(props->smCount);
+            uint64_t const room = 4ull * static_cast<unsigned>(props->smCount);
             if(a.logits)
                 while(blocks < 8 && a.vocab > blocks * kThreads * E && static_cast<uint64_t>(a.batch) * blocks * 2 <= room)
                     blocks *= 2;
@@ -440,7 +602,7 @@ namespace a3b
             attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
             config.attrs = &attribute;
             config.numAttrs = 1;
-            A3B_CUDA(cudaLaunchKernelEx(&config, verifyKernel<T>, a));
+            A3B_CUDA(cudaLaunchKernelEx(&config, packed ? verifyKernel<T, true> : verifyKernel<T, false>, a));
             return A3B_OK;
         }
     } // namespace
@@ -518,11 +680,14 @@ extern "C"
                      {draft_batch_stride, draft_stride}, draft_lse, drafts, top_index, uniform, noise, noise_stride, tokens, accepted,
                      static_cast<uint32_t>(batch), static_cast<uint32_t>(length), static_cast<uint32_t>(vocab),
                      index_dtype == A3B_I64, scale, draft_scale};
+        bool const packed = rowsAligned(logits, batch, length + 1, logits_batch_stride, logits_stride, es, 16)
+                            && (!a.draft || rowsAligned(draft_logits, batch, length, draft_batch_stride, draft_stride, es, 16))
+                            && rowsAligned(noise, 1, batch, 0, noise_stride, 4, 16);
         auto s = static_cast<cudaStream_t>(stream);
         if(dtype == A3B_F32)
-            return launchVerify<float>(s, props, a);
+            return launchVerify<float>(s, props, a, packed);
         if(dtype == A3B_F16)
-            return launchVerify<__half>(s, props, a);
-        return launchVerify<__nv_bfloat16>(s, props, a);
+            return launchVerify<__half>(s, props, a, packed);
+        return launchVerify<__nv_bfloat16>(s, props, a, packed);
     }
 }
