@@ -510,48 +510,39 @@ def clip_grad_norm(norm, tensors, max_norm, kind="l2", stream=None):
 
 
 # ------------------------------------------------------------------------------------------- norm of rows
-def _joint_rows(first, *others):
-    """(outer, inner, n, [outer stride, inner stride of each]) of tensors of one shape, in two levels of rows that fit all
-    of them; each of `others` is (tensor or None, name), `first` too but never None. None has strides 0."""
-    x, name = first
+def _joint_rows(*tensors):
+    """(outer, inner, n, [(outer stride, inner stride) of each]) of tensors of one shape, in two levels of rows that fit all
+    of them; each is (tensor or None, name), the first never None. None has strides 0."""
+    x, name = tensors[0]
     shape = x.shape
-    given = [t for t, _ in others if t is not None]
-    if x.dim() > 0 and x.is_contiguous() and all(t.is_contiguous() for t in given):
-        n = shape[-1]
-        return 1, (x.numel() // n if n else 0), n, [(0, n)] * (1 + len(others))
-    for t, label in (first, *others):
+    for t, label in tensors:
         if t is not None and (t.dim() < 1 or (t.shape[-1] > 1 and t.stride(-1) != 1)):
             raise ValueError(f"{label}: rows must be contiguous in the last dimension")
-    every = [x, *given]
+    if x.numel() == 0:
+        return 0, 0, shape[-1], [(0, 0)] * len(tensors)
+    if len(shape) == 2:
+        return 1, shape[0], shape[1], [(0, 0) if t is None else (0, t.stride(0)) for t, _ in tensors]
+    given = [t for t, _ in tensors if t is not None]
     levels = []  # (size, the strides of each)
     for d in range(x.dim() - 1):
-        size, strides = shape[d], tuple(t.stride(d) for t in every)
+        size, strides = shape[d], tuple(t.stride(d) for t in given)
         if size == 1:
             continue
         if levels and all(a == size * b for a, b in zip(levels[-1][1], strides)):
             levels[-1] = (levels[-1][0] * size, strides)
         else:
             levels.append((size, strides))
-    if x.numel() == 0:
-        levels = []
     if len(levels) > 2:
         raise ValueError(f"{name}: the dimensions before the last do not collapse to two strides")
-    none = (0,) * len(every)
+    none = (0,) * len(given)
     (outer, so), (inner, si) = [(1, none)] * (2 - len(levels)) + levels
-    if x.numel() == 0:
-        outer = inner = 0
     steps = iter(zip(so, si))
-    return outer, inner, shape[-1], [next(steps) if t is not None else (0, 0) for t in (x, *(t for t, _ in others))]
+    return outer, inner, shape[-1], [(0, 0) if t is None else next(steps) for t, _ in tensors]
 
 
-def _like(t, name, x, dev, dtype):
-    """t (None passes) has the shape of x, its device and `dtype`."""
-    if t is not None and (t.shape != x.shape or t.dtype != dtype or t.get_device() != dev):
+def _like(t, name, shape, dev, dtype):
+    if t.shape != shape or t.dtype != dtype or t.get_device() != dev:
         raise ValueError(f"{name} must have the shape and device of the rows, and dtype {dtype}")
-
-
-def _data(t):
-    return None if t is None else t.data_ptr()
 
 
 def _row_tensor(x, name):
@@ -567,14 +558,12 @@ def _row_tensor(x, name):
     return code, dev
 
 
-def _weight(weight, x, dev, name="weight"):
-    """dtype code of a weight of x's rows (that of x without one)"""
-    if weight is None:
-        return _LOGITS_DT[x.dtype]
-    if weight.dtype != x.dtype and weight.dtype != torch.float32:
+def _weight(weight, dtype, n, dev, name="weight"):
+    """dtype code of a weight of rows of n elements of `dtype`"""
+    if weight.dtype != dtype and weight.dtype != torch.float32:
         raise TypeError(f"{name} must have the dtype of the rows, or float32")
-    if weight.get_device() != dev or weight.numel() != x.shape[-1] or not weight.is_contiguous():
-        raise ValueError(f"{name}: expected {x.shape[-1]} contiguous elements on CUDA device {dev}")
+    if weight.get_device() != dev or weight.numel() != n or not weight.is_contiguous():
+        raise ValueError(f"{name}: expected {n} contiguous elements on CUDA device {dev}")
     return _LOGITS_DT[weight.dtype]
 
 
@@ -587,13 +576,13 @@ def _workspace_bytes(entry, dev, *sizes):
     return size
 
 
-def _workspace(entry, dev, stream, *sizes):
-    """Scratch for one call, from torch's allocator in the order of the call's stream."""
-    size = _workspace_bytes(entry, dev, *sizes)
+def _workspace(entry, device, stream, *sizes):
+    """(scratch for one call, from torch's allocator in the order of the call's stream; its size in bytes)"""
+    size = _workspace_bytes(entry, device.index, *sizes)
     if stream is None:
-        return torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", dev))
+        return torch.empty(size, dtype=torch.uint8, device=device), size
     with torch.cuda.stream(stream):
-        return torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", dev))
+        return torch.empty(size, dtype=torch.uint8, device=device), size
 
 
 def rms_norm(out, x, weight=None, residual=None, total=None, rstd=None, scales=None, group=None, eps=1e-6, stream=None):
@@ -611,23 +600,41 @@ def rms_norm(out, x, weight=None, residual=None, total=None, rstd=None, scales=N
     target = _NORM_OUT_DT.get(out.dtype)
     if target is None:
         raise TypeError(f"unsupported out dtype {out.dtype}")
-    if residual is not None:
-        _like(residual, "residual", x, dev, x.dtype)
-        if total is not None:
-            _like(total, "total", x, dev, x.dtype)
-    elif total is not None:
-        raise ValueError("total needs a residual")
-    if out.shape != x.shape or out.get_device() != dev:
+    shape, dtype = x.shape, x.dtype
+    n = shape[-1]
+    if out.shape != shape or out.get_device() != dev:
         raise ValueError("out must have the shape and device of x")
-    wcode = _weight(weight, x, dev)
-    outer, inner, n, ((xo, xi), (ro, ri), (to, ti), (oo, oi)) = _joint_rows((x, "x"), (residual, "residual"),
-                                                                            (total, "total"), (out, "out"))
-    rows = outer * inner
-    size = 0 if group is None else group
-    per_row = -(-n // size) if size else 1
-    _call_on(dev, stream, "a3b_rms_norm", code, outer, inner, n, x.data_ptr(), xo, xi, _data(residual), ro, ri, _data(total),
-             to, ti, target, out.data_ptr(), oo, oi, wcode, _data(weight), eps, _per_row(rstd, "rstd", rows, dev, _F32),
-             _per_row(scales, "scales", rows * per_row, dev, _F32), size)
+    flat = x.is_contiguous() and out.is_contiguous()
+    res = tot = 0
+    if residual is not None:
+        _like(residual, "residual", shape, dev, dtype)
+        res = residual.data_ptr()
+        flat = flat and residual.is_contiguous()
+    if total is not None:
+        if residual is None:
+            raise ValueError("total needs a residual")
+        _like(total, "total", shape, dev, dtype)
+        tot = total.data_ptr()
+        flat = flat and total.is_contiguous()
+    wcode, wat = code, 0
+    if weight is not None:
+        wcode, wat = _weight(weight, dtype, n, dev), weight.data_ptr()
+    if flat:
+        outer, inner = 1, x.numel() // n if n else 0
+        xo = ro = to = oo = 0
+        xi = ri = ti = oi = n
+    else:
+        outer, inner, _, ((xo, xi), (ro, ri), (to, ti), (oo, oi)) = _joint_rows((x, "x"), (residual, "residual"),
+                                                                                (total, "total"), (out, "out"))
+    size = group or 0
+    rat = sat = 0
+    if rstd is not None:
+        rat = _per_row(rstd, "rstd", outer * inner, dev, _F32)
+    if scales is not None:
+        sat = _per_row(scales, "scales", outer * inner * (-(-n // size) if size else 1), dev, _F32)
+    _call_on(dev, stream, "a3b_rms_norm",
+             capi.RMS_NORM_ARGS.pack(outer, inner, n, x.data_ptr(), xo, xi, res, ro, ri, tot, to, ti, out.data_ptr(), oo, oi,
+                                     wat, rat, sat, eps, code, target, wcode, size))
     return out
 
 
@@ -638,54 +645,74 @@ def rms_norm_backward(grad_x, grad_out, x, weight, rstd, grad_weight=None, grad_
     dtype; None: not computed). With a residual, grad_x is the gradient of both summands. grad_out, grad_total, grad_x have
     the shape and dtype of x, each any row strides; grad_x may be grad_out, x or grad_total. Returns grad_x."""
     code, dev = _row_tensor(x, "x")
-    for t, name in ((grad_out, "grad_out"), (grad_x, "grad_x"), (grad_total, "grad_total")):
-        _like(t, name, x, dev, x.dtype)
-    wcode = _weight(weight, x, dev)
-    gcode = wcode
-    if grad_weight is not None:
-        gcode = _weight(grad_weight, x, dev, "grad_weight")
-        if weight is not None and gcode != wcode:
-            raise TypeError("grad_weight must have the dtype of the weight")
+    shape, dtype = x.shape, x.dtype
+    n = shape[-1]
+    _like(grad_out, "grad_out", shape, dev, dtype)
+    _like(grad_x, "grad_x", shape, dev, dtype)
+    flat = x.is_contiguous() and grad_out.is_contiguous() and grad_x.is_contiguous()
+    tot = 0
+    if grad_total is not None:
+        _like(grad_total, "grad_total", shape, dev, dtype)
+        tot = grad_total.data_ptr()
+        flat = flat and grad_total.is_contiguous()
+    wcode, wat = code, 0
+    if weight is not None:
+        wcode, wat = _weight(weight, dtype, n, dev), weight.data_ptr()
     if rstd is None:
         raise ValueError("rstd is needed")
-    outer, inner, n, ((xo, xi), (go, gi), (to, ti), (oo, oi)) = _joint_rows((x, "x"), (grad_out, "grad_out"),
-                                                                            (grad_total, "grad_total"), (grad_x, "grad_x"))
+    if flat:
+        outer, inner = 1, x.numel() // n if n else 0
+        xo = go = to = oo = 0
+        xi = gi = ti = oi = n
+    else:
+        outer, inner, _, ((xo, xi), (go, gi), (to, ti), (oo, oi)) = _joint_rows((x, "x"), (grad_out, "grad_out"),
+                                                                                (grad_total, "grad_total"), (grad_x, "grad_x"))
     rows = outer * inner
-    ws = None
+    gcode, gat, at, size = wcode, 0, 0, 0
     if grad_weight is not None:
-        ws = _workspace("a3b_rms_norm_backward_workspace", dev, stream, rows, n)
-    _call_on(dev, stream, "a3b_rms_norm_backward", code, outer, inner, n, grad_out.data_ptr(), go, gi, x.data_ptr(), xo, xi,
-             _data(grad_total), to, ti, grad_x.data_ptr(), oo, oi, wcode, _data(weight), _per_row(rstd, "rstd", rows, dev, _F32),
-             gcode, _data(grad_weight), _data(ws), 0 if ws is None else ws.numel())
+        gcode, gat = _weight(grad_weight, dtype, n, dev, "grad_weight"), grad_weight.data_ptr()
+        if weight is not None and gcode != wcode:
+            raise TypeError("grad_weight must have the dtype of the weight")
+        ws, size = _workspace("a3b_rms_norm_backward_workspace", x.device, stream, rows, n)
+        at = ws.data_ptr()
+    _call_on(dev, stream, "a3b_rms_norm_backward",
+             capi.RMS_NORM_BACKWARD_ARGS.pack(outer, inner, n, grad_out.data_ptr(), go, gi, x.data_ptr(), xo, xi, tot, to, ti,
+                                              grad_x.data_ptr(), oo, oi, wat, _per_row(rstd, "rstd", rows, dev, _F32), gat, at,
+                                              size, code, wcode, gcode, 0))
     return grad_x
 
 
 # ----------------------------------------------------------------------------------------- rows of a table
 def _table(t, name, dev):
-    """(dtype code, rows, row stride) of a 2-D table of rows on device `dev`"""
+    """(dtype code, row stride) of a 2-D table of rows on device `dev`"""
     code, where = _row_tensor(t, name)
     if where != dev:
         raise ValueError(f"{name}: expected a tensor on CUDA device {dev}")
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"{name}: expected two dimensions, rows contiguous")
-    return code, t.shape[0], t.stride(0)
+    return code, t.stride(0)
 
 
-def _joined(a, b):
-    if a != b and capi.F32 not in (a, b):
-        raise TypeError("rows and table have one dtype, or one of them is float32")
-
-
-def _token_rows(t, tokens, dev, name):
-    """(dtype code, outer, inner, n, outer stride, inner stride, index code, address) of rows (..., n) for tokens (...)"""
+def _token_rows(t, tokens, dev, table, tcode, name):
+    """(dtype code, outer, inner, n, outer stride, inner stride, index code, address of the tokens) of rows (..., n) that
+    belong to tokens (...) and to rows of `table`"""
     code, where = _row_tensor(t, name)
     if where != dev:
         raise ValueError(f"{name}: expected a tensor on CUDA device {dev}")
-    if t.shape[:-1] != tokens.shape:
+    shape = t.shape
+    n = shape[-1]
+    if shape[:-1] != tokens.shape:
         raise ValueError(f"{name} must have the tokens' shape, and one dimension behind it")
-    outer, inner, n, ((so, si),) = _joint_rows((t, name))
-    index = _INDEX_DT.get(tokens.dtype, -1)
-    return code, outer, inner, n, so, si, index, _per_row(tokens, "tokens", outer * inner, dev, _INDEX_DT)
+    if table.shape[1] != n:
+        raise ValueError(f"{name} and the table must have rows of the same length")
+    if code != tcode and capi.F32 not in (code, tcode):
+        raise TypeError("rows and table have one dtype, or one of them is float32")
+    if t.is_contiguous():
+        outer, inner, so, si = 1, tokens.numel(), 0, n
+    else:
+        outer, inner, _, ((so, si),) = _joint_rows((t, name))
+    return (code, outer, inner, n, so, si, _INDEX_DT.get(tokens.dtype, -1),
+            _per_row(tokens, "tokens", outer * inner, dev, _INDEX_DT))
 
 
 def embedding(out, weight, tokens, scale=1.0, first=0, stream=None):
@@ -694,13 +721,11 @@ def embedding(out, weight, tokens, scale=1.0, first=0, stream=None):
     such as -100, or the tokens of other ranks where the table is cut over ranks. Types: float32 / float16 / bfloat16, both
     alike or one of them float32. Rows may be strided. Returns out."""
     dev = weight.get_device()
-    tcode, vocab, stride = _table(weight, "weight", dev)
-    code, outer, inner, n, so, si, index, address = _token_rows(out, tokens, dev, "out")
-    _joined(code, tcode)
-    if weight.shape[1] != n:
-        raise ValueError("out and weight must have rows of the same length")
-    _call_on(dev, stream, "a3b_embedding", tcode, weight.data_ptr(), vocab, stride, first, index, address, outer, inner, n,
-             scale, code, out.data_ptr(), so, si)
+    tcode, stride = _table(weight, "weight", dev)
+    code, outer, inner, n, so, si, index, at = _token_rows(out, tokens, dev, weight, tcode, "out")
+    _call_on(dev, stream, "a3b_embedding",
+             capi.EMBEDDING_ARGS.pack(outer, inner, n, weight.shape[0], first, weight.data_ptr(), stride, at, out.data_ptr(),
+                                      so, si, scale, tcode, index, code, 0))
     return out
 
 
@@ -710,30 +735,32 @@ def embedding_backward(grad_weight, grad_out, tokens, scale=1.0, add=None, first
     grad_weight (the gradient from the table's use as a head); it may be grad_weight itself, of which then only rows of
     tokens that occur are touched. The same bits in every call. Returns grad_weight."""
     dev = grad_weight.get_device()
-    tcode, vocab, stride = _table(grad_weight, "grad_weight", dev)
-    code, outer, inner, n, so, si, index, address = _token_rows(grad_out, tokens, dev, "grad_out")
-    _joined(code, tcode)
-    if grad_weight.shape[1] != n:
-        raise ValueError("grad_out and grad_weight must have rows of the same length")
-    add_stride = 0
+    tcode, stride = _table(grad_weight, "grad_weight", dev)
+    code, outer, inner, n, so, si, index, at = _token_rows(grad_out, tokens, dev, grad_weight, tcode, "grad_out")
+    more = more_stride = 0
     if add is not None:
-        acode, _, add_stride = _table(add, "add", dev)
+        acode, more_stride = _table(add, "add", dev)
         if acode != tcode or add.shape != grad_weight.shape:
             raise ValueError("add must have the dtype and shape of grad_weight")
-    ws = _workspace("a3b_embedding_backward_workspace", dev, stream, outer * inner, n, vocab)
-    _call_on(dev, stream, "a3b_embedding_backward", code, grad_out.data_ptr(), outer, inner, n, so, si, index, address, first,
-             scale, tcode, _data(add), add_stride, grad_weight.data_ptr(), vocab, stride, ws.data_ptr(), ws.numel())
+        more = add.data_ptr()
+    vocab = grad_weight.shape[0]
+    ws, size = _workspace("a3b_embedding_backward_workspace", grad_weight.device, stream, outer * inner, n, vocab)
+    _call_on(dev, stream, "a3b_embedding_backward",
+             capi.EMBEDDING_BACKWARD_ARGS.pack(outer, inner, n, vocab, first, grad_out.data_ptr(), so, si, at, more, more_stride,
+                                               grad_weight.data_ptr(), stride, ws.data_ptr(), size, scale, code, index, tcode, 0))
     return grad_weight
 
 
 # ------------------------------------------------------------------------------------------ drafted tokens
 def _draft_rows(t, name, batch, length, dev, dtype):
     """(address, batch stride, row stride) of logits (batch, length, vocab)"""
+    shape = t.shape
     if t.dtype != dtype or t.get_device() != dev:
-        raise ValueError(f"{name} must have the dtype and device of the logits")
-    if t.dim() != 3 or t.shape[0] != batch or t.shape[1] != length or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise ValueError(f"{name} must have the dtype of the logits and lie on CUDA device {dev}")
+    if len(shape) != 3 or shape[0] != batch or shape[1] != length or (shape[2] > 1 and t.stride(2) != 1):
         raise ValueError(f"{name}: expected shape ({batch}, {length}, vocab), rows contiguous")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    so, si, _ = t.stride()
+    return t.data_ptr(), so, si
 
 
 def verify_drafts(tokens, accepted, drafts, logits=None, lse=None, uniform=None, noise=None, draft_logits=None,
@@ -757,20 +784,22 @@ def verify_drafts(tokens, accepted, drafts, logits=None, lse=None, uniform=None,
     dev = drafts.get_device()
     if dev < 0:
         raise ValueError("drafts: expected a CUDA tensor")
-    if drafts.dim() != 2:
+    shape = drafts.shape
+    if len(shape) != 2:
         raise ValueError("drafts: expected shape (batch, length)")
-    batch, length = drafts.shape
+    batch, length = shape
     same = (drafts.dtype,)
     places = batch * (length + 1)
-    code, vocab, at, lb, ls = capi.F32, (1 << 31) - 65, None, 0, 0
-    other, db, ds, noise_at, noise_stride = None, 0, 0, None, 0
+    code, vocab, at, lb, ls = capi.F32, (1 << 31) - 65, 0, 0, 0
+    other, db, ds, noise_at, noise_stride = 0, 0, 0, 0, 0
     if logits is not None:
-        code, vocab = _LOGITS_DT.get(logits.dtype), logits.shape[-1]
+        code = _LOGITS_DT.get(logits.dtype)
         if code is None:
             raise TypeError(f"unsupported logits dtype {logits.dtype}")
         if lse is None or noise is None or (uniform is None and length):
             raise ValueError("logits need lse, uniform and noise")
         at, lb, ls = _draft_rows(logits, "logits", batch, length + 1, dev, logits.dtype)
+        vocab = logits.shape[2]
         if draft_logits is not None:
             if draft_lse is None:
                 raise ValueError("draft_logits need draft_lse")
@@ -785,12 +814,16 @@ def verify_drafts(tokens, accepted, drafts, logits=None, lse=None, uniform=None,
         raise ValueError("neither logits nor top_index is given")
     elif draft_logits is not None:
         raise ValueError("draft_logits need logits")
-    _call_on(dev, stream, "a3b_verify_drafts", code, batch, length, vocab, at, lb, ls,
-             _per_row(lse, "lse", places, dev, _F32), scale, other, db, ds,
-             _per_row(draft_lse, "draft_lse", batch * length, dev, _F32), scale if draft_scale is None else draft_scale, index,
-             _per_row(drafts, "drafts", batch * length, dev, same), _per_row(top_index, "top_index", places, dev, same),
-             _per_row(uniform, "uniform", batch * length, dev, _F32), noise_at, noise_stride,
-             _per_row(tokens, "tokens", places, dev, same), _per_row(accepted, "accepted", batch, dev, same))
+    _call_on(dev, stream, "a3b_verify_drafts",
+             capi.VERIFY_DRAFTS_ARGS.pack(batch, length, vocab, at, lb, ls, other, db, ds,
+                                          _per_row(lse, "lse", places, dev, _F32) or 0,
+                                          _per_row(draft_lse, "draft_lse", batch * length, dev, _F32) or 0, scale,
+                                          scale if draft_scale is None else draft_scale,
+                                          _per_row(drafts, "drafts", batch * length, dev, same),
+                                          _per_row(top_index, "top_index", places, dev, same) or 0,
+                                          _per_row(uniform, "uniform", batch * length, dev, _F32) or 0, noise_at, noise_stride,
+                                          _per_row(tokens, "tokens", places, dev, same),
+                                          _per_row(accepted, "accepted", batch, dev, same), code, index))
     return tokens
 
 

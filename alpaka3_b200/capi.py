@@ -7,6 +7,7 @@ missing, :func:`lib` raises :class:`LibraryNotBuilt` (run ``python -m alpaka3_b2
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # A3B_LIBRARY selects another build of the same library (e.g. a tuning variant); default: the in-tree build
@@ -79,17 +80,13 @@ SIGNATURES = {
     "a3b_grad_norm": [_P, _P, _I, _P, ctypes.c_size_t, _P, _I, _P],
     "a3b_clip_grads": [_P, _P, _I, _P, _D, _I, _P],
     "a3b_clip_grad_norm": [_P, _P, _I, _D, _P, ctypes.c_size_t, _I, _P],
-    "a3b_rms_norm": [_P, _I, _U64, _U64, _U64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _I64, _I64, _I, _P,
-                     _D, _P, _P, _U32],
+    "a3b_rms_norm": [_P, _P],
     "a3b_rms_norm_backward_workspace": [_U64, _U64],
-    "a3b_rms_norm_backward": [_P, _I, _U64, _U64, _U64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I,
-                              _P, _P, _I, _P, _P, ctypes.c_size_t],
-    "a3b_embedding": [_P, _I, _P, _U64, _I64, _I64, _I, _P, _U64, _U64, _U64, _D, _I, _P, _I64, _I64],
+    "a3b_rms_norm_backward": [_P, _P],
+    "a3b_embedding": [_P, _P],
     "a3b_embedding_backward_workspace": [_U64, _U64, _U64],
-    "a3b_embedding_backward": [_P, _I, _P, _U64, _U64, _U64, _I64, _I64, _I, _P, _I64, _D, _I, _P, _I64, _P, _U64, _I64, _P,
-                               ctypes.c_size_t],
-    "a3b_verify_drafts": [_P, _I, _U64, _U64, _U64, _P, _I64, _I64, _P, _D, _P, _I64, _I64, _P, _D, _I, _P, _P, _P, _P, _I64,
-                          _P, _P],
+    "a3b_embedding_backward": [_P, _P],
+    "a3b_verify_drafts": [_P, _P],
     "a3b_nbody_update_velocities": [_P, _P, _P, _P, _P, _U64, _U64, _U64, _P, _P, _P, _F, _F],
     "a3b_nbody_step": [_P, _P, _P, _P, _P, _U64, _U64, _U64, _P, _P, _P, _F, _F],
     "a3b_haccmk_step10": [_P, _P, _P, _P, _P, _I, _I, _F, _F, _F, _P, _P, _P],
@@ -111,6 +108,15 @@ _RESTYPES = {"a3b_last_error": ctypes.c_char_p, "a3b_scan_buffer_size": ctypes.c
              "a3b_grad_norm_workspace": ctypes.c_size_t, "a3b_rms_norm_backward_workspace": ctypes.c_size_t,
              "a3b_embedding_backward_workspace": ctypes.c_size_t, "a3b_ipc_handle_size": ctypes.c_size_t,
              "a3b_halo_bytes": ctypes.c_size_t}
+
+
+# Arguments that travel in a structure, packed by field (an address of 0 is null): a call converts one pointer instead of two
+# dozen values.
+RMS_NORM_ARGS = struct.Struct("@3Q Pqq Pqq Pqq Pqq 3P d 3i I")
+RMS_NORM_BACKWARD_ARGS = struct.Struct("@3Q Pqq Pqq Pqq Pqq 4P Q 4i")
+EMBEDDING_ARGS = struct.Struct("@4Q q Pq P Pqq d 4i")
+EMBEDDING_BACKWARD_ARGS = struct.Struct("@4Q q Pqq P Pq Pq PQ d 4i")
+VERIFY_DRAFTS_ARGS = struct.Struct("@3Q Pqq Pqq 2P 2d 4P q 2P 2i")
 
 
 class LibraryNotBuilt(RuntimeError):

@@ -706,35 +706,26 @@ using namespace a3b;
 
 extern "C"
 {
-    int a3b_embedding(
-        a3b_stream_t stream,
-        int table_dtype,
-        void const* table,
-        uint64_t vocab,
-        int64_t table_stride,
-        int64_t first,
-        int index_dtype,
-        void const* tokens,
-        uint64_t outer,
-        uint64_t inner,
-        uint64_t n,
-        double scale,
-        int out_dtype,
-        void* out,
-        int64_t out_outer_stride,
-        int64_t out_inner_stride)
+    int a3b_embedding(a3b_stream_t stream, a3b_embedding_args const* args)
     {
+        A3B_REQUIRE(args, "null arguments");
+        uint64_t const outer = args->outer, inner = args->inner, n = args->n, vocab = args->vocab;
+        int64_t const first = args->first, table_stride = args->table_stride;
+        void const *table = args->table, *tokens = args->tokens;
+        a3b_rows const& out = args->out;
+        double const scale = args->scale;
+        int const table_dtype = args->table_dtype, index_dtype = args->index_dtype, out_dtype = args->out_dtype;
         int const rc = checkTypes(out_dtype, table_dtype, index_dtype, vocab, outer, inner, n, scale);
         if(rc != A3B_OK)
             return rc;
         uint64_t const count = outer * inner;
         if(count == 0)
             return A3B_OK;
-        A3B_REQUIRE(tokens && out && (table || vocab == 0), "null tokens, table or output");
+        A3B_REQUIRE(tokens && out.data && (table || vocab == 0), "null tokens, table or output");
         int const ts = rowTypeSize(table_dtype), os = rowTypeSize(out_dtype), is = index_dtype == A3B_I64 ? 8 : 4;
-        A3B_REQUIRE(alignedTo(ts, {table}) && alignedTo(os, {out}) && alignedTo(is, {tokens}), "an array is not aligned to its type");
+        A3B_REQUIRE(alignedTo(ts, {table}) && alignedTo(os, {out.data}) && alignedTo(is, {tokens}), "an array is not aligned to its type");
         Stretch const st = Stretch::rows(vocab ? table : nullptr, 1, vocab, 0, table_stride, n, ts);
-        Stretch const so = Stretch::rows(out, outer, inner, out_outer_stride, out_inner_stride, n, os);
+        Stretch const so = Stretch::rows(out, outer, inner, n, os);
         Stretch const si = Stretch::dense(tokens, static_cast<Wide>(count) * is);
         A3B_REQUIRE(so.separate(), "rows of the output overlap");
         A3B_REQUIRE(so.apart(st) && so.apart(si), "the output overlaps the table or the tokens");
@@ -742,8 +733,8 @@ extern "C"
         int const rd = currentDevice(&props);
         if(rd != A3B_OK)
             return rd;
-        LookupArgs a{table, table_stride, {tokens, index_dtype == A3B_I64, first, static_cast<uint32_t>(vocab)}, out,
-                     {out_outer_stride, out_inner_stride}, static_cast<uint32_t>(count), static_cast<uint32_t>(inner),
+        LookupArgs a{table, table_stride, {tokens, index_dtype == A3B_I64, first, static_cast<uint32_t>(vocab)}, out.data,
+                     {out.outer_stride, out.inner_stride}, static_cast<uint32_t>(count), static_cast<uint32_t>(inner),
                      static_cast<uint32_t>(n), outer == 1, static_cast<float>(scale), 0};
         auto s = static_cast<cudaStream_t>(stream);
         return withTypes(table_dtype, out_dtype, [&](auto t, auto u)
@@ -752,7 +743,7 @@ extern "C"
             using U = decltype(u);
             constexpr int E = kLot<T, U>;
             bool const packed = n % E == 0 && rowsAligned(table, 1, vocab, 0, table_stride, ts, 16)
-                                && rowsAligned(out, outer, inner, out_outer_stride, out_inner_stride, os, 16);
+                                && rowsAligned(out.data, outer, inner, out.outer_stride, out.inner_stride, os, 16);
             return packed ? launchLookup<T, U, E>(s, props, a) : launchLookup<T, U, 1>(s, props, a);
         });
     }
@@ -766,39 +757,28 @@ extern "C"
         return planFor(props, std::min(count, most), std::min(n, most), std::min(vocab, most)).bytes;
     }
 
-    int a3b_embedding_backward(
-        a3b_stream_t stream,
-        int grad_dtype,
-        void const* grad_out,
-        uint64_t outer,
-        uint64_t inner,
-        uint64_t n,
-        int64_t grad_outer_stride,
-        int64_t grad_inner_stride,
-        int index_dtype,
-        void const* tokens,
-        int64_t first,
-        double scale,
-        int table_dtype,
-        void const* add,
-        int64_t add_stride,
-        void* grad_table,
-        uint64_t vocab,
-        int64_t table_stride,
-        void* workspace,
-        size_t workspace_bytes)
+    int a3b_embedding_backward(a3b_stream_t stream, a3b_embedding_backward_args const* args)
     {
+        A3B_REQUIRE(args, "null arguments");
+        uint64_t const outer = args->outer, inner = args->inner, n = args->n, vocab = args->vocab;
+        int64_t const first = args->first, add_stride = args->add_stride, table_stride = args->table_stride;
+        a3b_rows const& grad_out = args->grad_out;
+        void const *tokens = args->tokens, *add = args->add;
+        void *grad_table = args->grad_table, *workspace = args->workspace;
+        uint64_t const workspace_bytes = args->workspace_bytes;
+        double const scale = args->scale;
+        int const grad_dtype = args->grad_dtype, index_dtype = args->index_dtype, table_dtype = args->table_dtype;
         int const rc = checkTypes(grad_dtype, table_dtype, index_dtype, vocab, outer, inner, n, scale);
         if(rc != A3B_OK)
             return rc;
         if(vocab == 0)
             return A3B_OK;
         uint64_t const count = outer * inner;
-        A3B_REQUIRE(grad_table && (count == 0 || (grad_out && tokens)), "null gradient or tokens");
+        A3B_REQUIRE(grad_table && (count == 0 || (grad_out.data && tokens)), "null gradient or tokens");
         int const gs = rowTypeSize(grad_dtype), ts = rowTypeSize(table_dtype), is = index_dtype == A3B_I64 ? 8 : 4;
-        A3B_REQUIRE(alignedTo(gs, {grad_out}) && alignedTo(ts, {grad_table, add}) && alignedTo(is, {tokens}),
+        A3B_REQUIRE(alignedTo(gs, {grad_out.data}) && alignedTo(ts, {grad_table, add}) && alignedTo(is, {tokens}),
                     "an array is not aligned to its type");
-        Stretch const sg = Stretch::rows(count ? grad_out : nullptr, outer, inner, grad_outer_stride, grad_inner_stride, n, gs);
+        Stretch const sg = Stretch::rows(grad_out, outer, inner, n, gs);
         Stretch const so = Stretch::rows(grad_table, 1, vocab, 0, table_stride, n, ts);
         Stretch const sa = Stretch::rows(add, 1, vocab, 0, add_stride, n, ts);
         Stretch const si = Stretch::dense(tokens, static_cast<Wide>(count) * is);
@@ -824,7 +804,7 @@ extern "C"
             if(rs != A3B_OK)
                 return rs;
         }
-        SumArgs a{grad_out, {grad_outer_stride, grad_inner_stride}, keys, places,
+        SumArgs a{grad_out.data, {grad_out.outer_stride, grad_out.inner_stride}, keys, places,
                   count ? reinterpret_cast<float*>(static_cast<char*>(workspace) + p.partial) : nullptr, add, add_stride, grad_table,
                   table_stride, static_cast<uint32_t>(count), static_cast<uint32_t>(inner), static_cast<uint32_t>(n),
                   static_cast<uint32_t>(vocab), p.chunk, p.chunks, 0u, 0u, outer == 1, !inPlace, static_cast<float>(scale), 0};
@@ -833,7 +813,7 @@ extern "C"
             using T = decltype(t);
             using U = decltype(u);
             constexpr int E = kLot<T, U>;
-            bool const packed = n % E == 0 && rowsAligned(grad_out, outer, inner, grad_outer_stride, grad_inner_stride, gs, 16)
+            bool const packed = n % E == 0 && rowsAligned(grad_out.data, outer, inner, grad_out.outer_stride, grad_out.inner_stride, gs, 16)
                                 && rowsAligned(grad_table, 1, vocab, 0, table_stride, ts, 16)
                                 && rowsAligned(add, 1, vocab, 0, add_stride, ts, 16);
             return packed ? launchSum<T, U, E>(s, a) : launchSum<T, U, 1>(s, a);

@@ -61,6 +61,10 @@ namespace a3b
             s.bytes = static_cast<Wide>(n) * size;
             return s;
         }
+        static Stretch rows(a3b_rows const& r, uint64_t outer, uint64_t inner, uint64_t n, int size)
+        {
+            return rows(r.data, outer, inner, r.outer_stride, r.inner_stride, n, size);
+        }
         static Stretch dense(void const* p, Wide bytes)
         {
             Stretch s;

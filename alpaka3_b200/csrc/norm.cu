@@ -1011,32 +1011,16 @@ using namespace a3b;
 
 extern "C"
 {
-    int a3b_rms_norm(
-        a3b_stream_t stream,
-        int dtype,
-        uint64_t outer,
-        uint64_t inner,
-        uint64_t n,
-        void const* x,
-        int64_t x_outer_stride,
-        int64_t x_inner_stride,
-        void const* residual,
-        int64_t residual_outer_stride,
-        int64_t residual_inner_stride,
-        void* total,
-        int64_t total_outer_stride,
-        int64_t total_inner_stride,
-        int out_dtype,
-        void* out,
-        int64_t out_outer_stride,
-        int64_t out_inner_stride,
-        int weight_dtype,
-        void const* weight,
-        double eps,
-        float* rstd,
-        float* scales,
-        uint32_t group)
+    int a3b_rms_norm(a3b_stream_t stream, a3b_rms_norm_args const* args)
     {
+        A3B_REQUIRE(args, "null arguments");
+        uint64_t const outer = args->outer, inner = args->inner, n = args->n;
+        int const dtype = args->dtype, out_dtype = args->out_dtype, weight_dtype = args->weight_dtype;
+        a3b_rows const &x = args->x, &residual = args->residual, &total = args->total, &out = args->out;
+        void const* weight = args->weight;
+        float *rstd = args->rstd, *scales = args->scales;
+        double const eps = args->eps;
+        uint32_t const group = args->group;
         int const rc = checkShape(dtype, outer, inner, n, eps);
         if(rc != A3B_OK)
             return rc;
@@ -1047,22 +1031,22 @@ extern "C"
                     "groups of 8-bit outputs have 32, 64 or 128 elements");
         if(outer * inner == 0)
             return A3B_OK;
-        A3B_REQUIRE(x && out, "null rows or output");
-        A3B_REQUIRE(!total || residual, "a sum needs a residual");
+        A3B_REQUIRE(x.data && out.data, "null rows or output");
+        A3B_REQUIRE(!total.data || residual.data, "a sum needs a residual");
         A3B_REQUIRE(eightBits == (scales != nullptr), "scales belong to 8-bit outputs");
         int const es = rowTypeSize(dtype), os = eightBits ? 1 : es, ws = weight_dtype == A3B_F32 ? 4 : 2;
-        A3B_REQUIRE(alignedTo(es, {x, residual, total}) && alignedTo(os, {out}) && alignedTo(ws, {weight})
+        A3B_REQUIRE(alignedTo(es, {x.data, residual.data, total.data}) && alignedTo(os, {out.data}) && alignedTo(ws, {weight})
                         && alignedTo(4, {rstd, scales}),
                     "an array is not aligned to its type");
         uint64_t const rows = outer * inner, groups = group ? (n + group - 1) / group : 1;
-        Stretch const sx = Stretch::rows(x, outer, inner, x_outer_stride, x_inner_stride, n, es);
-        Stretch const sr = Stretch::rows(residual, outer, inner, residual_outer_stride, residual_inner_stride, n, es);
-        Stretch const st = Stretch::rows(total, outer, inner, total_outer_stride, total_inner_stride, n, es);
-        Stretch const so = Stretch::rows(out, outer, inner, out_outer_stride, out_inner_stride, n, os);
+        Stretch const sx = Stretch::rows(x, outer, inner, n, es);
+        Stretch const sr = Stretch::rows(residual, outer, inner, n, es);
+        Stretch const st = Stretch::rows(total, outer, inner, n, es);
+        Stretch const so = Stretch::rows(out, outer, inner, n, os);
         Stretch const sw = Stretch::dense(weight, static_cast<Wide>(n) * ws);
         Stretch const s1 = Stretch::dense(rstd, static_cast<Wide>(rows) * 4);
         Stretch const s8 = Stretch::dense(scales, static_cast<Wide>(rows) * groups * 4);
-        A3B_REQUIRE(so.separate() && (!total || st.separate()), "rows of an output overlap");
+        A3B_REQUIRE(so.separate() && (!total.data || st.separate()), "rows of an output overlap");
         for(Stretch const* w : {&so, &st})
             for(Stretch const* r : {&sx, &sr})
                 A3B_REQUIRE(w->empty() || w->sameAs(*r) || w->apart(*r),
@@ -1078,15 +1062,15 @@ extern "C"
         if(rd != A3B_OK)
             return rd;
         int const E = 16 / es;
-        auto fits = [&](void const* p, int64_t a, int64_t b, int size, int to)
-        { return !p || rowsAligned(p, outer, inner, a, b, size, to); };
-        bool const packed = n % E == 0 && fits(x, x_outer_stride, x_inner_stride, es, 16)
-                            && fits(residual, residual_outer_stride, residual_inner_stride, es, 16)
-                            && fits(total, total_outer_stride, total_inner_stride, es, 16)
-                            && fits(out, out_outer_stride, out_inner_stride, os, eightBits ? E : 16) && alignedTo(16, {weight});
+        auto fits = [&](a3b_rows const& r, int size, int to)
+        { return !r.data || rowsAligned(r.data, outer, inner, r.outer_stride, r.inner_stride, size, to); };
+        bool const packed = n % E == 0 && fits(x, es, 16)
+                            && fits(residual, es, 16)
+                            && fits(total, es, 16)
+                            && fits(out, os, eightBits ? E : 16) && alignedTo(16, {weight});
         bool const one = outer == 1;
-        NormArgs a{x, residual, total, out, {x_outer_stride, x_inner_stride}, {residual_outer_stride, residual_inner_stride},
-                   {total_outer_stride, total_inner_stride}, {out_outer_stride, out_inner_stride},
+        NormArgs a{x.data, residual.data, total.data, out.data, {x.outer_stride, x.inner_stride}, {residual.outer_stride, residual.inner_stride},
+                   {total.outer_stride, total.inner_stride}, {out.outer_stride, out.inner_stride},
                    static_cast<uint32_t>(rows), static_cast<uint32_t>(inner), static_cast<uint32_t>(n), one, weight, rstd,
                    scales, group, static_cast<uint32_t>(groups), out_dtype == A3B_E5M2, eps, static_cast<float>(eps),
                    1.f / static_cast<float>(n), eps < 0x1p-60};
@@ -1120,32 +1104,16 @@ extern "C"
         return std::max<size_t>(16, static_cast<size_t>(partialRows(props, rows)) * n * sizeof(float));
     }
 
-    int a3b_rms_norm_backward(
-        a3b_stream_t stream,
-        int dtype,
-        uint64_t outer,
-        uint64_t inner,
-        uint64_t n,
-        void const* grad_out,
-        int64_t grad_out_outer_stride,
-        int64_t grad_out_inner_stride,
-        void const* x,
-        int64_t x_outer_stride,
-        int64_t x_inner_stride,
-        void const* grad_total,
-        int64_t grad_total_outer_stride,
-        int64_t grad_total_inner_stride,
-        void* grad_x,
-        int64_t grad_x_outer_stride,
-        int64_t grad_x_inner_stride,
-        int weight_dtype,
-        void const* weight,
-        float const* rstd,
-        int grad_weight_dtype,
-        void* grad_weight,
-        void* workspace,
-        size_t workspace_bytes)
+    int a3b_rms_norm_backward(a3b_stream_t stream, a3b_rms_norm_backward_args const* args)
     {
+        A3B_REQUIRE(args, "null arguments");
+        uint64_t const outer = args->outer, inner = args->inner, n = args->n;
+        int const dtype = args->dtype, weight_dtype = args->weight_dtype, grad_weight_dtype = args->grad_weight_dtype;
+        a3b_rows const &grad_out = args->grad_out, &x = args->x, &grad_total = args->grad_total, &grad_x = args->grad_x;
+        void const* weight = args->weight;
+        float const* rstd = args->rstd;
+        void *grad_weight = args->grad_weight, *workspace = args->workspace;
+        uint64_t const workspace_bytes = args->workspace_bytes;
         int const rc = checkShape(dtype, outer, inner, n, 0.);
         if(rc != A3B_OK)
             return rc;
@@ -1162,13 +1130,13 @@ extern "C"
                 A3B_CUDA(cudaMemsetAsync(grad_weight, 0, n * static_cast<size_t>(ws), s));
             return A3B_OK;
         }
-        A3B_REQUIRE(grad_out && x && grad_x && rstd, "null rows, rstd or output");
-        A3B_REQUIRE(alignedTo(es, {grad_out, x, grad_total, grad_x}) && alignedTo(4, {rstd}), "an array is not aligned to its type");
+        A3B_REQUIRE(grad_out.data && x.data && grad_x.data && rstd, "null rows, rstd or output");
+        A3B_REQUIRE(alignedTo(es, {grad_out.data, x.data, grad_total.data, grad_x.data}) && alignedTo(4, {rstd}), "an array is not aligned to its type");
         uint64_t const rows = outer * inner;
-        Stretch const sg = Stretch::rows(grad_out, outer, inner, grad_out_outer_stride, grad_out_inner_stride, n, es);
-        Stretch const sx = Stretch::rows(x, outer, inner, x_outer_stride, x_inner_stride, n, es);
-        Stretch const st = Stretch::rows(grad_total, outer, inner, grad_total_outer_stride, grad_total_inner_stride, n, es);
-        Stretch const so = Stretch::rows(grad_x, outer, inner, grad_x_outer_stride, grad_x_inner_stride, n, es);
+        Stretch const sg = Stretch::rows(grad_out, outer, inner, n, es);
+        Stretch const sx = Stretch::rows(x, outer, inner, n, es);
+        Stretch const st = Stretch::rows(grad_total, outer, inner, n, es);
+        Stretch const so = Stretch::rows(grad_x, outer, inner, n, es);
         Stretch const sw = Stretch::dense(weight, static_cast<Wide>(n) * ws);
         Stretch const sd = Stretch::dense(grad_weight, static_cast<Wide>(n) * ws);
         Stretch const s1 = Stretch::dense(rstd, static_cast<Wide>(rows) * 4);
@@ -1191,14 +1159,15 @@ extern "C"
                                      && workspace_bytes >= a3b_rms_norm_backward_workspace(rows, n)),
                     "the workspace is missing, too small or not aligned to 16 bytes");
         int const E = 16 / es;
-        auto fits = [&](void const* p, int64_t a, int64_t b) { return !p || rowsAligned(p, outer, inner, a, b, es, 16); };
-        bool const packed = n % E == 0 && fits(grad_out, grad_out_outer_stride, grad_out_inner_stride)
-                            && fits(x, x_outer_stride, x_inner_stride)
-                            && fits(grad_total, grad_total_outer_stride, grad_total_inner_stride)
-                            && fits(grad_x, grad_x_outer_stride, grad_x_inner_stride) && alignedTo(16, {weight});
-        NormBackArgs a{grad_out, x, grad_total, grad_x, {grad_out_outer_stride, grad_out_inner_stride},
-                       {x_outer_stride, x_inner_stride}, {grad_total_outer_stride, grad_total_inner_stride},
-                       {grad_x_outer_stride, grad_x_inner_stride}, static_cast<uint32_t>(rows), static_cast<uint32_t>(inner),
+        auto fits = [&](a3b_rows const& r)
+        { return !r.data || rowsAligned(r.data, outer, inner, r.outer_stride, r.inner_stride, es, 16); };
+        bool const packed = n % E == 0 && fits(grad_out)
+                            && fits(x)
+                            && fits(grad_total)
+                            && fits(grad_x) && alignedTo(16, {weight});
+        NormBackArgs a{grad_out.data, x.data, grad_total.data, grad_x.data, {grad_out.outer_stride, grad_out.inner_stride},
+                       {x.outer_stride, x.inner_stride}, {grad_total.outer_stride, grad_total.inner_stride},
+                       {grad_x.outer_stride, grad_x.inner_stride}, static_cast<uint32_t>(rows), static_cast<uint32_t>(inner),
                        static_cast<uint32_t>(n), outer == 1, weight, rstd,
                        grad_weight ? static_cast<float*>(workspace) : nullptr};
         bool const wide = ws == 4;

@@ -612,31 +612,17 @@ using namespace a3b;
 
 extern "C"
 {
-    int a3b_verify_drafts(
-        a3b_stream_t stream,
-        int dtype,
-        uint64_t batch,
-        uint64_t length,
-        uint64_t vocab,
-        void const* logits,
-        int64_t logits_batch_stride,
-        int64_t logits_stride,
-        float const* lse,
-        double scale,
-        void const* draft_logits,
-        int64_t draft_batch_stride,
-        int64_t draft_stride,
-        float const* draft_lse,
-        double draft_scale,
-        int index_dtype,
-        void const* drafts,
-        void const* top_index,
-        float const* uniform,
-        float const* noise,
-        int64_t noise_stride,
-        void* tokens,
-        void* accepted)
+    int a3b_verify_drafts(a3b_stream_t stream, a3b_verify_drafts_args const* args)
     {
+        A3B_REQUIRE(args, "null arguments");
+        uint64_t const batch = args->batch, length = args->length, vocab = args->vocab;
+        int const dtype = args->dtype, index_dtype = args->index_dtype;
+        a3b_rows const &rows = args->logits, &draftRows = args->draft_logits;
+        void const *logits = rows.data, *draft_logits = draftRows.data, *drafts = args->drafts, *top_index = args->top_index;
+        float const *lse = args->lse, *draft_lse = args->draft_lse, *uniform = args->uniform, *noise = args->noise;
+        double const scale = args->scale, draft_scale = args->draft_scale;
+        int64_t const noise_stride = args->noise_stride;
+        void *tokens = args->tokens, *accepted = args->accepted;
         A3B_REQUIRE(rowTypeSize(dtype) != 0, "logits must be f32, f16 or bf16");
         A3B_REQUIRE(index_dtype == A3B_I32 || index_dtype == A3B_I64, "token indices must be i32 or i64");
         A3B_REQUIRE(vocab > 0, "a row needs at least one logit");
@@ -661,8 +647,8 @@ extern "C"
                     "an array is not aligned to its type");
         Wide const b = static_cast<Wide>(batch), k = static_cast<Wide>(length);
         Stretch const out = Stretch::dense(tokens, b * (k + 1) * is), count = Stretch::dense(accepted, b * is);
-        Stretch const ins[] = {Stretch::rows(logits, batch, length + 1, logits_batch_stride, logits_stride, vocab, es),
-                               Stretch::rows(draft_logits, batch, length, draft_batch_stride, draft_stride, vocab, es),
+        Stretch const ins[] = {Stretch::rows(rows, batch, length + 1, vocab, es),
+                               Stretch::rows(draftRows, batch, length, vocab, es),
                                Stretch::rows(noise, 1, batch, 0, noise_stride, vocab, 4),
                                Stretch::dense(lse, b * (k + 1) * 4),
                                Stretch::dense(draft_lse, b * k * 4),
@@ -676,12 +662,12 @@ extern "C"
         int const rd = currentDevice(&props);
         if(rd != A3B_OK)
             return rd;
-        VerifyArgs a{logits, {logits_batch_stride, logits_stride}, lse, length ? draft_logits : nullptr,
-                     {draft_batch_stride, draft_stride}, draft_lse, drafts, top_index, uniform, noise, noise_stride, tokens, accepted,
+        VerifyArgs a{logits, {rows.outer_stride, rows.inner_stride}, lse, length ? draft_logits : nullptr,
+                     {draftRows.outer_stride, draftRows.inner_stride}, draft_lse, drafts, top_index, uniform, noise, noise_stride, tokens, accepted,
                      static_cast<uint32_t>(batch), static_cast<uint32_t>(length), static_cast<uint32_t>(vocab),
                      index_dtype == A3B_I64, scale, draft_scale};
-        bool const packed = rowsAligned(logits, batch, length + 1, logits_batch_stride, logits_stride, es, 16)
-                            && (!a.draft || rowsAligned(draft_logits, batch, length, draft_batch_stride, draft_stride, es, 16))
+        bool const packed = rowsAligned(logits, batch, length + 1, rows.outer_stride, rows.inner_stride, es, 16)
+                            && (!a.draft || rowsAligned(draft_logits, batch, length, draftRows.outer_stride, draftRows.inner_stride, es, 16))
                             && rowsAligned(noise, 1, batch, 0, noise_stride, 4, 16);
         auto s = static_cast<cudaStream_t>(stream);
         if(dtype == A3B_F32)

@@ -351,13 +351,21 @@ A3B_API int a3b_clip_grads(a3b_stream_t stream, a3b_tensor_list const* list, int
 A3B_API int a3b_clip_grad_norm(a3b_stream_t stream, a3b_tensor_list const* list, int kind, double max_norm,
                                void* workspace, size_t workspace_bytes, int norm_dtype, void* norm);
 
+/* Rows of an array: row o * inner + i (o < outer, i < inner, as the call says) starts at element o * outer_stride + i *
+ * inner_stride of data and is contiguous. data null: the array is left out. */
+typedef struct a3b_rows
+{
+    void* data;
+    int64_t outer_stride;
+    int64_t inner_stride;
+} a3b_rows;
+
 /* --------------------------------------------------------------------------------- root-mean-square norm (rows) */
 
 /* Over every row of n elements: h = x + residual (rounded to dtype), r = 1 / sqrt(mean h^2 + eps), out = h * r * weight.
  * No counterpart in alpaka3: transformReduce with one result a row, and a transform with that result.
  *
- * Rows of dtype A3B_F32, A3B_F16 or A3B_BF16: row o * inner + i (o < outer, i < inner) of each array starts at element
- * o * outer_stride + i * inner_stride and is contiguous. residual: null or rows that are added; total: null or rows that
+ * Rows of dtype A3B_F32, A3B_F16 or A3B_BF16. residual: null or rows that are added; total: null or rows that
  * receive h (needs a residual). Rounded or not stored, it is the rounded h that is normed, so that a gradient which reads
  * `total` is that of what was computed. weight: n elements of dtype or A3B_F32, null: ones. rstd: null or one fp32 value a
  * row that receives r, for the gradient. The sum of squares is held in fp32, or in fp64 where that leaves fp32's range
@@ -375,12 +383,18 @@ A3B_API int a3b_clip_grad_norm(a3b_stream_t stream, a3b_tensor_list const* list,
  * are all multiples of one length that holds both (parts of one wider row). Rows of an output may not overlap. The order of
  * a row's sums follows from its length, alignment and the number of rows. At most 2^31 - 1 rows of 2^31 - 65 elements
  * (A3B_ERR_TOO_LARGE). One launch. */
-A3B_API int a3b_rms_norm(a3b_stream_t stream, int dtype, uint64_t outer, uint64_t inner, uint64_t n, void const* x,
-                         int64_t x_outer_stride, int64_t x_inner_stride, void const* residual,
-                         int64_t residual_outer_stride, int64_t residual_inner_stride, void* total,
-                         int64_t total_outer_stride, int64_t total_inner_stride, int out_dtype, void* out,
-                         int64_t out_outer_stride, int64_t out_inner_stride, int weight_dtype, void const* weight, double eps,
-                         float* rstd, float* scales, uint32_t group);
+typedef struct a3b_rms_norm_args
+{
+    uint64_t outer, inner, n;
+    a3b_rows x, residual, total, out; /* x and residual are read */
+    void const* weight;
+    float* rstd;
+    float* scales;
+    double eps; /* 0 .. 2^100 */
+    int32_t dtype, out_dtype, weight_dtype;
+    uint32_t group;
+} a3b_rms_norm_args;
+A3B_API int a3b_rms_norm(a3b_stream_t stream, a3b_rms_norm_args const* args);
 
 /* Bytes of device scratch that a3b_rms_norm_backward needs for grad_weight on the current device (any contents; nothing is
  * kept in it between calls). Calls that overlap on the GPU need one each. 0 on failure. */
@@ -394,27 +408,42 @@ A3B_API size_t a3b_rms_norm_backward_workspace(uint64_t rows, uint64_t n);
  * A3B_F32 without a weight); it needs a workspace of a3b_rms_norm_backward_workspace bytes, 16-byte aligned. All sums are
  * held in fp32 (a row's positions and the rows in a fixed order: repeated calls give the same bits) and rounded once.
  * grad_x may be grad_out, x or grad_total in place. No rows: grad_weight is set to zero. */
-A3B_API int a3b_rms_norm_backward(a3b_stream_t stream, int dtype, uint64_t outer, uint64_t inner, uint64_t n,
-                                  void const* grad_out, int64_t grad_out_outer_stride, int64_t grad_out_inner_stride,
-                                  void const* x, int64_t x_outer_stride, int64_t x_inner_stride, void const* grad_total,
-                                  int64_t grad_total_outer_stride, int64_t grad_total_inner_stride, void* grad_x,
-                                  int64_t grad_x_outer_stride, int64_t grad_x_inner_stride, int weight_dtype,
-                                  void const* weight, float const* rstd, int grad_weight_dtype, void* grad_weight,
-                                  void* workspace, size_t workspace_bytes);
+typedef struct a3b_rms_norm_backward_args
+{
+    uint64_t outer, inner, n;
+    a3b_rows grad_out, x, grad_total, grad_x; /* all but grad_x are read */
+    void const* weight;
+    float const* rstd;
+    void* grad_weight;
+    void* workspace;
+    uint64_t workspace_bytes;
+    int32_t dtype, weight_dtype, grad_weight_dtype;
+    int32_t reserved; /* 0 */
+} a3b_rms_norm_backward_args;
+A3B_API int a3b_rms_norm_backward(a3b_stream_t stream, a3b_rms_norm_backward_args const* args);
 
 /* ------------------------------------------------------------------------------- rows of a table, by tokens */
 
 /* out_i = scale * row t_i of the table, for count = outer * inner tokens t (A3B_I32 or A3B_I64, dense): a transform whose
  * input is picked by an index. The table holds the rows of the tokens [first, first + vocab), n elements each, row_stride
- * apart; a token outside it gives a row of zeros (as a table cut over ranks wants, and as -100 for padding). Row
- * o * inner + i of out starts at element o * outer_stride + i * inner_stride. Types: A3B_F32, A3B_F16 or A3B_BF16, both
+ * apart; a token outside it gives a row of zeros (as a table cut over ranks wants, and as -100 for padding). Types: A3B_F32, A3B_F16 or A3B_BF16, both
  * alike, or one of them A3B_F32; the product is formed in fp32 and rounded once. scale: any finite fp32 value. The output's
  * rows may not overlap one another, the table or the tokens (beside them in rows of steps that are all multiples of one
  * length is apart). At most 2^31 - 65 tokens, rows of the table and elements a row (A3B_ERR_TOO_LARGE; rows of more than
  * eight million elements too). One launch. */
-A3B_API int a3b_embedding(a3b_stream_t stream, int table_dtype, void const* table, uint64_t vocab, int64_t table_stride,
-                          int64_t first, int index_dtype, void const* tokens, uint64_t outer, uint64_t inner, uint64_t n,
-                          double scale, int out_dtype, void* out, int64_t out_outer_stride, int64_t out_inner_stride);
+typedef struct a3b_embedding_args
+{
+    uint64_t outer, inner, n, vocab;
+    int64_t first;
+    void const* table;
+    int64_t table_stride;
+    void const* tokens;
+    a3b_rows out;
+    double scale;
+    int32_t table_dtype, index_dtype, out_dtype;
+    int32_t reserved; /* 0 */
+} a3b_embedding_args;
+A3B_API int a3b_embedding(a3b_stream_t stream, a3b_embedding_args const* args);
 
 /* Bytes of device scratch that a3b_embedding_backward needs for `count` tokens on the current device (any contents; nothing
  * is kept in it between calls). Calls that overlap on the GPU need one each. 0 on failure. */
@@ -427,11 +456,23 @@ A3B_API size_t a3b_embedding_backward_workspace(uint64_t count, uint64_t n, uint
  * table_dtype. Sums are held in fp32 and rounded once; their order follows from count, n and vocab (and the device) alone:
  * repeated calls give the same bits. grad_out's rows may have any strides; grad_table's may not overlap. workspace: 16-byte
  * aligned, of a3b_embedding_backward_workspace bytes. grad_table and workspace lie apart from all inputs. */
-A3B_API int a3b_embedding_backward(a3b_stream_t stream, int grad_dtype, void const* grad_out, uint64_t outer, uint64_t inner,
-                                   uint64_t n, int64_t grad_outer_stride, int64_t grad_inner_stride, int index_dtype,
-                                   void const* tokens, int64_t first, double scale, int table_dtype, void const* add,
-                                   int64_t add_stride, void* grad_table, uint64_t vocab, int64_t table_stride,
-                                   void* workspace, size_t workspace_bytes);
+typedef struct a3b_embedding_backward_args
+{
+    uint64_t outer, inner, n, vocab;
+    int64_t first;
+    a3b_rows grad_out;
+    void const* tokens;
+    void const* add;
+    int64_t add_stride;
+    void* grad_table;
+    int64_t table_stride;
+    void* workspace;
+    uint64_t workspace_bytes;
+    double scale;
+    int32_t grad_dtype, index_dtype, table_dtype;
+    int32_t reserved; /* 0 */
+} a3b_embedding_backward_args;
+A3B_API int a3b_embedding_backward(a3b_stream_t stream, a3b_embedding_backward_args const* args);
 
 /* ------------------------------------------------------------------------------- verification of drafted tokens */
 
@@ -454,16 +495,26 @@ A3B_API int a3b_embedding_backward(a3b_stream_t stream, int grad_dtype, void con
  * while it equals top_index i, and the next entry follows. logits may be null if all sequences are greedy; then lse, uniform
  * and noise may be, too.
  *
- * logits: row (b, i) starts at element b * batch_stride + i * stride, likewise draft_logits; noise: row b at b *
- * noise_stride; rows are contiguous, everything else is dense. index_dtype is that of drafts, top_index, tokens and
+ * noise: row b starts at element b * noise_stride; everything else but the logits is dense. index_dtype is that of drafts, top_index, tokens and
  * accepted. scale, draft_scale: between 2^-20 and 2^20. The outputs lie apart from one another and from the inputs. One
  * launch. At most 2^31 - 1 rows of 2^31 - 65 logits (A3B_ERR_TOO_LARGE). */
-A3B_API int a3b_verify_drafts(a3b_stream_t stream, int dtype, uint64_t batch, uint64_t length, uint64_t vocab,
-                              void const* logits, int64_t logits_batch_stride, int64_t logits_stride, float const* lse,
-                              double scale, void const* draft_logits, int64_t draft_batch_stride, int64_t draft_stride,
-                              float const* draft_lse, double draft_scale, int index_dtype, void const* drafts,
-                              void const* top_index, float const* uniform, float const* noise, int64_t noise_stride,
-                              void* tokens, void* accepted);
+typedef struct a3b_verify_drafts_args
+{
+    uint64_t batch, length, vocab;
+    a3b_rows logits, draft_logits; /* read; outer: the sequence, inner: the position */
+    float const* lse;
+    float const* draft_lse;
+    double scale, draft_scale;
+    void const* drafts;
+    void const* top_index;
+    float const* uniform;
+    float const* noise;
+    int64_t noise_stride;
+    void* tokens;
+    void* accepted;
+    int32_t dtype, index_dtype;
+} a3b_verify_drafts_args;
+A3B_API int a3b_verify_drafts(a3b_stream_t stream, a3b_verify_drafts_args const* args);
 
 /* ----------------------------------------------------------------------------------------------------- nBody */
 
