@@ -116,7 +116,16 @@ namespace a3b
         {
             static constexpr int words = E == 1 ? 1 : E * static_cast<int>(sizeof(WT)) / 4;
 
-            static __device__ __forceinline__ void load(unsigned* w, WT const* p)
+            // without a weight: ones, so that the loops over elements have no branch
+            static __device__ __forceinline__ void load(unsigned* w, WT const* weight, uint32_t k)
+            {
+                if(weight)
+                    return read(w, weight + static_cast<size_t>(k) * E);
+#pragma unroll
+                for(int i = 0; i < words; ++i)
+                    w[i] = PackOf<WT>::twice(1.f);
+            }
+            static __device__ __forceinline__ void read(unsigned* w, WT const* p)
             {
                 if constexpr(E == 1)
                     Access<WT, 1>::load(w, p);
@@ -366,11 +375,11 @@ namespace a3b
             // with the row's loads under way; more than two packs' weights would cost blocks an SM
             constexpr bool early = P * W::words <= 8;
             unsigned wraw[early ? P : 1][W::words];
-            if(early && weight)
+            if(early)
 #pragma unroll
                 for(int p = 0; p < P; ++p)
                     if(uint32_t const k = p * lanes + t; k < packs)
-                        W::load(wraw[early ? p : 0], weight + static_cast<size_t>(k) * E);
+                        W::load(wraw[early ? p : 0], weight, k);
 
             float const sum = teamSum<L>(addRow<T, E, P>(a, row, live, lanes, t, raw, add), roomF);
             float const r = rootRow<T, E, P, L>(a, lanes, t, sum, raw, roomD);
@@ -382,15 +391,10 @@ namespace a3b
             {
                 uint32_t const k = p * lanes + t;
                 if constexpr(!early)
-                    if(weight)
-                        W::load(wraw[0], weight + static_cast<size_t>(k) * E);
+                    W::load(wraw[0], weight, k);
 #pragma unroll
                 for(int e = 0; e < A::pairs; ++e)
-                {
-                    y[e] = mul2(A::pair(raw[p], e), make_float2(r, r));
-                    if(weight)
-                        y[e] = mul2(y[e], W::pair(wraw[early ? p : 0], e));
-                }
+                    y[e] = mul2(mul2(A::pair(raw[p], e), make_float2(r, r)), W::pair(wraw[early ? p : 0], e));
             };
             auto largest = [&](float2 const (&y)[A::pairs])
             {
@@ -486,8 +490,8 @@ namespace a3b
                 if(in && a.residual)
                     A::load(add[q][0], static_cast<T const*>(a.residual) + a.rs.at(row, a.inner, a.one) + t * E);
             }
-            if(in && weight)
-                W::load(wraw, weight + t * E);
+            if(in)
+                W::load(wraw, weight, t);
             float sum[R];
 #pragma unroll
             for(int q = 0; q < R; ++q)
@@ -512,12 +516,7 @@ namespace a3b
                     unsigned words[A::words];
 #pragma unroll
                     for(int e = 0; e < A::pairs; ++e)
-                    {
-                        float2 y = mul2(A::pair(raw[q][0], e), make_float2(r, r));
-                        if(weight)
-                            y = mul2(y, W::pair(wraw, e));
-                        A::setPair(words, e, y);
-                    }
+                        A::setPair(words, e, mul2(mul2(A::pair(raw[q][0], e), make_float2(r, r)), W::pair(wraw, e)));
                     A::store(static_cast<T*>(a.out) + a.os.at(row, a.inner, a.one) + t * E, words);
                 }
             }
@@ -705,168 +704,145 @@ namespace a3b
             void const* weight; // may be null
             float const* rstd;
             float* partial; // one row of n sums a block; null: no gradient of the weight
+            float inverse; // 1 / n
+            uint32_t team; // threads of a team
         };
 
-        // Teams go from row to row, a lane always at the same columns, so that the weight's gradient gathers in registers;
-        // a block adds up its teams' and writes one row of partial sums. The next row's loads run under this row's sum.
+        // The block's row of partial sums from its teams', added in the teams' order: the same bits every time.
+        template<int E, int P>
+        __device__ __forceinline__ void addTeams(NormBackArgs const& a, float2 const (&dw)[P][E == 1 ? 1 : E / 2], float* sums,
+                                                 uint32_t teams, uint32_t mine, uint32_t lanes, uint32_t t)
+        {
+            float* partial = a.partial + static_cast<size_t>(blockIdx.x) * a.n;
+            float* to = teams == 1 ? partial : sums + mine * a.n;
+#pragma unroll
+            for(int p = 0; p < P; ++p)
+                if(uint32_t const k = p * lanes + t; k < a.n / E)
+#pragma unroll
+                    for(int e = 0; e < E; ++e)
+                        to[static_cast<size_t>(k) * E + e] = e % 2 ? dw[p][e / 2].y : dw[p][e / 2].x;
+            if(teams == 1)
+                return;
+            __syncthreads();
+            for(uint32_t k = threadIdx.x; k < a.n; k += blockDim.x)
+            {
+                float v = sums[k];
+#pragma unroll 4
+                for(uint32_t of = 1; of < teams; ++of)
+                    v += sums[of * a.n + k];
+                partial[k] = v;
+            }
+        }
+
+        // Teams go from row to row, a lane always at the same columns, so that the weight's gradient gathers in registers. A
+        // team is L lanes of a warp, or (L = 0) a.team threads, several in a block of up to 512, which adds up theirs and writes
+        // one row of partial sums. As in the forward pass a row is held as the words it is stored in: with 64 registers a
+        // thread two blocks of 512 share an SM, and one team's loads run under the others' sums.
         template<typename T, typename WT, int E, int P, int L>
-        __global__ void __launch_bounds__(L == 0 ? 512 : 256) rmsNormBackwardKernel(NormBackArgs a)
+        __global__ void __launch_bounds__(512, P <= 2 ? 2 : 1) rmsNormBackwardKernel(NormBackArgs a)
         {
             using A = Access<T, E>;
             using W = Weights<WT, E>;
-            constexpr bool ahead = P * A::words <= 8;
-            __shared__ float roomF[2][32];
+            constexpr bool held = P * W::words < 8; // weights in registers; more of them spill: then from L1 row by row
+            __shared__ float room[2][16];
             extern __shared__ float sums[];
-            uint32_t const lanes = L == 0 ? blockDim.x : L, t = L == 0 ? threadIdx.x : threadIdx.x % (L == 0 ? 1 : L);
-            uint32_t const perBlock = L == 0 ? 1u : 256u / (L == 0 ? 1 : L), mine = L == 0 ? 0u : threadIdx.x / (L == 0 ? 1 : L);
-            uint32_t const packs = a.n / E, step = gridDim.x * perBlock;
+            uint32_t const lanes = L > 0 ? L : a.team, mine = threadIdx.x / lanes, t = threadIdx.x - mine * lanes;
+            uint32_t const teams = blockDim.x / lanes, packs = a.n / E, step = gridDim.x * teams;
             WT const* weight = static_cast<WT const*>(a.weight);
-            unsigned wraw[ahead ? P : 1][W::words]; // held only where that leaves room; else read from L1 row by row
-            float dw[P][E];
+            unsigned wraw[held ? P : 1][W::words];
+            float2 dw[P][A::pairs];
 #pragma unroll
             for(int p = 0; p < P; ++p)
             {
-                if(uint32_t const k = p * lanes + t; ahead && weight && k < packs)
-                    W::load(wraw[ahead ? p : 0], weight + static_cast<size_t>(k) * E);
+                if(uint32_t const k = p * lanes + t; held && k < packs)
+                    W::load(wraw[held ? p : 0], weight, k);
 #pragma unroll
-                for(int e = 0; e < E; ++e)
-                    dw[p][e] = 0.f;
+                for(int e = 0; e < A::pairs; ++e)
+                    dw[p][e] = make_float2(0.f, 0.f);
             }
-            unsigned graw[P][A::words], xraw[P][A::words];
-            float r = 0.f;
-            auto load = [&](uint32_t row)
+            uint32_t row = blockIdx.x * teams + mine, turn = 0;
+            // lanes of one warp that belong to two teams make the same number of steps
+            for(uint32_t first = L > 0 ? blockIdx.x * teams : row; first < a.rows; first += step, row += step, ++turn)
             {
-                T const* g = static_cast<T const*>(a.g) + a.gs.at(row, a.inner, a.one);
-                T const* x = static_cast<T const*>(a.x) + a.xs.at(row, a.inner, a.one);
-#pragma unroll
-                for(int p = 0; p < P; ++p)
-                    if(uint32_t const k = p * lanes + t; k < packs)
-                    {
-                        A::load(graw[p], g + static_cast<size_t>(k) * E);
-                        A::load(xraw[p], x + static_cast<size_t>(k) * E);
-                    }
-                r = a.rstd[row];
-            };
-            // of access p: k = x r, g, and d = g w
-            auto terms = [&](int p, float* hat, float* g, float* d)
-            {
-                A::unpack(hat, xraw[p]);
-                A::unpack(g, graw[p]);
-                float w[E];
-                if(weight)
-                {
-                    if constexpr(ahead)
-                        W::unpack(w, wraw[p]);
-                    else
-                    {
-                        unsigned words[W::words];
-                        W::load(words, weight + static_cast<size_t>(p * lanes + t) * E);
-                        W::unpack(w, words);
-                    }
-                }
-#pragma unroll
-                for(int e = 0; e < E; ++e)
-                {
-                    hat[e] *= r;
-                    d[e] = weight ? g[e] * w[e] : g[e];
-                }
-            };
-            // all teams of a block make the same number of steps: they share the warps' shuffles
-            uint32_t row = blockIdx.x * perBlock + mine;
-            if(ahead)
-                load(row < a.rows ? row : a.rows - 1u);
-            int flip = 0;
-            for(uint32_t first = blockIdx.x * perBlock; first < a.rows; first += step, row += step)
-            {
-                bool const live = row < a.rows;
+                bool const live = L == 0 || row < a.rows;
                 uint32_t const here = live ? row : a.rows - 1u;
-                if(!ahead)
-                    load(here);
-                float hat[ahead ? P : 1][E], d[ahead ? P : 1][E];
-                float const rhere = r;
-                float c = 0.f;
-#pragma unroll
-                for(int p = 0; p < P; ++p)
-                    if(uint32_t const k = p * lanes + t; k < packs)
-                    {
-                        int const at = ahead ? p : 0;
-                        float g[E];
-                        terms(p, hat[at], g, d[at]);
-#pragma unroll
-                        for(int e = 0; e < E; ++e)
-                        {
-                            if(live)
-                                dw[p][e] = fmaf(g[e], hat[at][e], dw[p][e]);
-                            c = fmaf(d[at][e], hat[at][e], c);
-                        }
-                    }
-                unsigned traw[ahead ? P : 1][A::words];
+                T const* g = static_cast<T const*>(a.g) + a.gs.at(here, a.inner, a.one);
+                T const* x = static_cast<T const*>(a.x) + a.xs.at(here, a.inner, a.one);
                 T const* gt = a.gtotal ? static_cast<T const*>(a.gtotal) + a.ts.at(here, a.inner, a.one) : nullptr;
-                if(ahead && gt)
-#pragma unroll
-                    for(int p = 0; p < P; ++p)
-                        if(uint32_t const k = p * lanes + t; k < packs)
-                            A::load(traw[ahead ? p : 0], gt + static_cast<size_t>(k) * E);
-                if(ahead)
-                    load(row + step < a.rows ? row + step : a.rows - 1u);
-                c = teamSum<L>(c, roomF[flip]) / static_cast<float>(a.n);
-                flip ^= 1;
-                T* gx = static_cast<T*>(a.gx) + a.os.at(here, a.inner, a.one);
+                float const r = live ? a.rstd[here] : 0.f;
+                unsigned graw[P][A::words], xraw[P][A::words], traw[P][A::words];
 #pragma unroll
                 for(int p = 0; p < P; ++p)
                     if(uint32_t const k = p * lanes + t; k < packs && live)
                     {
-                        int const at = ahead ? p : 0;
-                        if constexpr(!ahead)
-                        {
-                            float g[E];
-                            terms(p, hat[at], g, d[at]);
-                            if(gt)
-                                A::load(traw[at], gt + static_cast<size_t>(k) * E);
-                        }
-#pragma unroll
-                        for(int e = 0; e < E; ++e)
-                            d[at][e] = rhere * fmaf(-hat[at][e], c, d[at][e]);
-                        unsigned raw[A::words];
-                        if(gt)
-                        {
-                            float more[E];
-                            A::unpack(more, traw[at]);
-#pragma unroll
-                            for(int e = 0; e < E; ++e)
-                                d[at][e] += more[e];
-                        }
-                        A::pack(raw, d[at]);
-                        A::store(gx + static_cast<size_t>(k) * E, raw);
+                        A::load(graw[p], g + static_cast<size_t>(k) * E);
+                        A::load(xraw[p], x + static_cast<size_t>(k) * E);
                     }
-            }
-            if(!a.partial)
-                return;
-            float* partial = a.partial + static_cast<size_t>(blockIdx.x) * a.n;
-            if constexpr(L == 0)
-            {
+                if(gt)
+#pragma unroll
+                    for(int p = 0; p < P; ++p)
+                        if(uint32_t const k = p * lanes + t; k < packs && live)
+                            A::load(traw[p], gt + static_cast<size_t>(k) * E);
+                auto weighted = [&](int p, int e) { return mul2(A::pair(graw[p], e), W::pair(wraw[held ? p : 0], e)); }; // d = g w
+                float2 c2 = make_float2(0.f, 0.f);
+#pragma unroll
+                for(int p = 0; p < P; ++p)
+                    if(uint32_t const k = p * lanes + t; k < packs && live)
+                    {
+                        if(!held)
+                            W::load(wraw[0], weight, k);
+#pragma unroll
+                        for(int e = 0; e < A::pairs; ++e)
+                        {
+                            float2 const hat = mul2(A::pair(xraw[p], e), make_float2(r, r));
+                            dw[p][e] = fma2(A::pair(graw[p], e), hat, dw[p][e]);
+                            c2 = fma2(weighted(p, e), hat, c2);
+                        }
+                    }
+                float c = c2.x + c2.y;
+                if constexpr(L > 0)
+                    c = lanesSum<L>(c);
+                else
+                {
+                    c = lanesSum<32>(c);
+                    uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = lanes / 32;
+                    if(lane == 0)
+                        room[turn & 1][warp] = c;
+                    asm volatile("bar.sync %0, %1;" ::"r"(mine + 1u), "r"(lanes) : "memory");
+                    c = lanesSum<32>(lane < warps ? room[turn & 1][mine * warps + lane] : 0.f);
+                }
+                c *= a.inverse;
+                if(!live)
+                    continue;
+                T* gx = static_cast<T*>(a.gx) + a.os.at(here, a.inner, a.one);
 #pragma unroll
                 for(int p = 0; p < P; ++p)
                     if(uint32_t const k = p * lanes + t; k < packs)
+                    {
+                        if(!held)
+                            W::load(wraw[0], weight, k);
+                        unsigned raw[A::words];
+                        float2 d[A::pairs];
 #pragma unroll
-                        for(int e = 0; e < E; ++e)
-                            partial[static_cast<size_t>(k) * E + e] = dw[p][e];
+                        for(int e = 0; e < A::pairs; ++e)
+                        {
+                            float2 const hat = mul2(A::pair(xraw[p], e), make_float2(-r, -r));
+                            d[e] = mul2(fma2(hat, make_float2(c, c), weighted(p, e)), make_float2(r, r));
+                        }
+                        if(gt)
+#pragma unroll
+                            for(int e = 0; e < A::pairs; ++e)
+                                d[e] = add2(d[e], A::pair(traw[p], e));
+#pragma unroll
+                        for(int e = 0; e < A::pairs; ++e)
+                            A::setPair(raw, e, d[e]);
+                        A::store(gx + static_cast<size_t>(k) * E, raw);
+                    }
             }
-            else
+            if(a.partial)
             {
-                for(uint32_t turn = 0; turn < perBlock; ++turn) // in the teams' order: the same bits every time
-                {
-                    if(turn == mine)
-#pragma unroll
-                        for(int p = 0; p < P; ++p)
-                            if(uint32_t const k = p * lanes + t; k < packs)
-#pragma unroll
-                                for(int e = 0; e < E; ++e)
-                                    sums[k * E + e] = turn == 0 ? dw[p][e] : sums[k * E + e] + dw[p][e];
-                    __syncthreads();
-                }
-                for(uint32_t k = threadIdx.x; k < a.n; k += 256u)
-                    partial[k] = sums[k];
+                asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); // the fold waits before it reads
+                addTeams<E, P>(a, dw, sums, teams, mine, lanes, t);
             }
         }
 
@@ -886,7 +862,7 @@ namespace a3b
 #pragma unroll 4
             for(uint32_t k = t; k < a.n; k += kLongThreads)
                 c = fmaf(toFloat(g[k]) * (weight ? toFloat(weight[k]) : 1.f), toFloat(x[k]) * r, c);
-            c = teamSum<0>(c, roomF) / static_cast<float>(a.n);
+            c = teamSum<0>(c, roomF) * a.inverse;
 #pragma unroll 4
             for(uint32_t k = t; k < a.n; k += kLongThreads)
             {
@@ -928,11 +904,12 @@ namespace a3b
         {
             __shared__ float part[32][33];
             uint32_t const lane = threadIdx.x % 32, warp = threadIdx.x / 32, k = blockIdx.x * 32 + lane;
+            asm volatile("griddepcontrol.wait;" ::: "memory");
             float s = 0.f;
             if(k < n)
-#pragma unroll 4
+#pragma unroll 10
                 for(uint32_t row = warp; row < count; row += 32)
-                    s += partial[static_cast<size_t>(row) * n + k];
+                    s += __ldcg(partial + static_cast<size_t>(row) * n + k);
             part[warp][lane] = s;
             __syncthreads();
             s = lanesSum<32>(part[lane][warp]); // now the warp has one column
@@ -940,52 +917,69 @@ namespace a3b
                 out[blockIdx.x * 32 + warp] = fromFloat<WT>(s);
         }
 
-        // Rows of partial sums at most: as many blocks as the SMs hold of the kernel above (by its launch bounds), fewer
-        // where there are fewer rows.
+        // rows of partial sums at most, whatever a call's alignment: four blocks an SM
         uint32_t partialRows(DeviceProps const* props, uint64_t rows)
         {
             return static_cast<uint32_t>(std::min<uint64_t>(rows, 4ull * static_cast<unsigned>(props->smCount)));
+        }
+
+        template<typename T, typename WT, int E, int P, int L>
+        uint32_t launchBackwardTeams(cudaStream_t stream, DeviceProps const* props, NormBackArgs a)
+        {
+            auto const sms = static_cast<uint32_t>(props->smCount);
+            a.team = L > 0 ? L : roundUp((a.n / E + P - 1) / P, 32);
+            // teams side by side in a block, unless SMs would go without
+            uint32_t const teams = std::max(1u, std::min(512 / a.team, L > 0 ? 512u / a.team : a.rows / sms));
+            uint32_t const threads = teams * a.team, resident = std::max(1u, (P <= 2 ? 1024u : 512u) / threads);
+            uint32_t const blocks = std::min({(a.rows + teams - 1) / teams, sms * resident, partialRows(props, a.rows)});
+            // a row of sums for each team: at most threads * P * E values, 32 KB
+            size_t const sums = a.partial && teams > 1 ? teams * a.n * sizeof(float) : 0;
+            rmsNormBackwardKernel<T, WT, E, P, L><<<blocks, threads, sums, stream>>>(a);
+            return blocks;
         }
 
         template<typename T, typename WT>
         int launchNormBackward(cudaStream_t stream, DeviceProps const* props, NormBackArgs const& a, bool packed, WT* gw)
         {
             constexpr int E = PackOf<T>::E;
-            uint32_t const limit = partialRows(props, a.rows);
-            uint32_t blocks = limit;
-            auto teams = [&](uint32_t lanes) { return blocks = std::min(limit, (a.rows + 256 / lanes - 1) / (256 / lanes)); };
-            size_t const room = a.partial ? a.n * sizeof(float) : 0;
             uint32_t const packs = packed ? a.n / E : a.n;
-            auto longRows = [&]
-            {
-                if(a.partial)
-                {
-                    blocks = std::min<uint32_t>(limit, 64);
-                    rmsNormWeightKernel<T><<<dim3((a.n + 31) / 32, blocks), 256, 0, stream>>>(a);
-                }
-                rmsNormBackwardLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a);
-            };
+            uint32_t blocks = 0;
             if(packed && packs <= 16)
-                rmsNormBackwardKernel<T, WT, E, 1, 16><<<teams(16), 256, room, stream>>>(a);
+                blocks = launchBackwardTeams<T, WT, E, 2, 8>(stream, props, a);
             else if(packed && packs <= 32)
-                rmsNormBackwardKernel<T, WT, E, 1, 32><<<teams(32), 256, room, stream>>>(a);
+                blocks = launchBackwardTeams<T, WT, E, 2, 16>(stream, props, a);
             else if(packed && packs <= 64)
-                rmsNormBackwardKernel<T, WT, E, 2, 32><<<teams(32), 256, room, stream>>>(a);
+                blocks = launchBackwardTeams<T, WT, E, 2, 32>(stream, props, a);
             else if(packed && packs <= 1024)
-                rmsNormBackwardKernel<T, WT, E, 2, 0><<<blocks, roundUp((packs + 1) / 2, 32), 0, stream>>>(a);
+                blocks = launchBackwardTeams<T, WT, E, 2, 0>(stream, props, a);
             else if(packed && packs <= 2048)
-                rmsNormBackwardKernel<T, WT, E, 4, 0><<<blocks, roundUp((packs + 3) / 4, 32), 0, stream>>>(a);
+                blocks = launchBackwardTeams<T, WT, E, 4, 0>(stream, props, a);
             else if(!packed && packs <= 2048)
-                rmsNormBackwardKernel<T, WT, 1, 4, 0><<<blocks, roundUp((packs + 3) / 4, 32), 0, stream>>>(a);
+                blocks = launchBackwardTeams<T, WT, 1, 4, 0>(stream, props, a);
             else if(!packed && packs <= 8192)
-                rmsNormBackwardKernel<T, WT, 1, 16, 0><<<blocks, roundUp((packs + 15) / 16, 32), 0, stream>>>(a);
+                blocks = launchBackwardTeams<T, WT, 1, 16, 0>(stream, props, a);
             else
-                longRows();
+            {
+                blocks = std::min<uint32_t>(partialRows(props, a.rows), 64);
+                if(a.partial)
+                    rmsNormWeightKernel<T><<<dim3((a.n + 31) / 32, blocks), 256, 0, stream>>>(a);
+                rmsNormBackwardLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a);
+            }
             A3B_CHECK_LAUNCH("rmsNormBackwardKernel");
             if(a.partial)
             {
-                rmsNormFoldKernel<WT><<<(a.n + 31) / 32, 1024, 0, stream>>>(a.partial, blocks, a.n, gw);
-                A3B_CHECK_LAUNCH("rmsNormFoldKernel");
+                // Its blocks may be launched while the last rows are written; they wait for the whole grid. Only this kernel
+                // follows one that signals its dependents, and it signals none.
+                cudaLaunchAttribute attribute{};
+                attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+                attribute.val.programmaticStreamSerializationAllowed = 1;
+                cudaLaunchConfig_t config{};
+                config.gridDim = dim3((a.n + 31) / 32);
+                config.blockDim = dim3(1024);
+                config.stream = stream;
+                config.attrs = &attribute;
+                config.numAttrs = 1;
+                A3B_CUDA(cudaLaunchKernelEx(&config, rmsNormFoldKernel<WT>, static_cast<float const*>(a.partial), blocks, a.n, gw));
             }
             return A3B_OK;
         }
@@ -1169,7 +1163,7 @@ extern "C"
                        {x.outer_stride, x.inner_stride}, {grad_total.outer_stride, grad_total.inner_stride},
                        {grad_x.outer_stride, grad_x.inner_stride}, static_cast<uint32_t>(rows), static_cast<uint32_t>(inner),
                        static_cast<uint32_t>(n), outer == 1, weight, rstd,
-                       grad_weight ? static_cast<float*>(workspace) : nullptr};
+                       grad_weight ? static_cast<float*>(workspace) : nullptr, 1.f / static_cast<float>(n), 0u};
         bool const wide = ws == 4;
         if(dtype == A3B_F32)
             return launchNormBackward<float, float>(s, props, a, packed, static_cast<float*>(grad_weight));
