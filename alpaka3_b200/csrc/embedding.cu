@@ -173,17 +173,19 @@ namespace a3b
 
         // ------------------------------------------------------------------------------------- sorting the tokens
         // Up to kRankMax tokens: the place of each is the number of those that come before it, by comparing all pairs. A
-        // block ranks 32 tokens, each of its warps against an eighth of the list. Quadratic, but one launch: 8192 tokens
-        // are 67 million comparisons, a few microseconds on the whole GPU.
-        constexpr uint32_t kRankMax = 8192;
+        // block ranks 32 tokens, each of its warps against an eighth of the list. Quadratic, but one short launch.
+        constexpr uint32_t kRankMax = 4096;
 
-        __global__ void __launch_bounds__(256) rankKernel(Tokens tokens, uint32_t count, uint32_t* keys, uint32_t* places)
+        __global__ void __launch_bounds__(256) rankKernel(Tokens tokens, uint32_t count, uint32_t* keys, uint32_t* places, uint32_t* runs)
         {
+            if(blockIdx.x == 0 && threadIdx.x == 0)
+                *runs = 0;
             extern __shared__ __align__(16) uint32_t all[];
             __shared__ uint32_t part[8][32];
             uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32, base = blockIdx.x * 32, i = base + lane;
             uint32_t const span = ((count + 7) / 8 + 31) / 32 * 32, low = warp * span;
             uint32_t const high = min(low + span, (count + 31) / 32 * 32);
+#pragma unroll 8
             for(uint32_t j = low + lane; j < high; j += 32) // behind the last: a key above all others
                 all[j] = j < count ? tokens(j) : 0xffffffffu;
             uint32_t const key = i < count ? tokens(i) : 0xfffffffeu;
@@ -215,9 +217,124 @@ namespace a3b
             }
         }
 
+        // Up to kClusterMax tokens: radix sort in one launch, by a cluster of eight blocks that hold the list in their shared
+        // memory; each has an eighth, each of its warps a contiguous part of that, so equal digits keep their order. A digit
+        // takes a count by every warp, one exchange of the blocks' counts and one of the tokens themselves.
+        constexpr uint32_t kClusterMax = 16384, kSortBlocks = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+        constexpr int kBins = 512;
+
+        struct ClusterSort
+        {
+            uint2 list[2][kClusterMax / kSortBlocks]; // key and place
+            uint32_t at[kSortWarps][kBins]; // counts of a warp, then where its next token of a digit goes
+            uint32_t total[kBins]; // of the block, read by the others
+            uint32_t sums[kBins / 32];
+        };
+
+        __global__ void __cluster_dims__(kSortBlocks, 1, 1) __launch_bounds__(kSortThreads)
+            clusterSortKernel(Tokens tokens, uint32_t count, int log2Each, int digits, int bits, uint32_t* keys, uint32_t* places,
+                              uint32_t* runs)
+        {
+            extern __shared__ __align__(16) unsigned char memory[];
+            auto& sh = *reinterpret_cast<ClusterSort*>(memory);
+            uint32_t const t = threadIdx.x, warp = t / 32, lane = t % 32, rank = clusterRank(), bins = 1u << bits;
+            uint32_t const own = kSortThreads << log2Each, span = own / kSortWarps; // tokens of a block and of a warp
+            if(rank == 0 && t == 0)
+                *runs = 0;
+            // A warp reads its own part in its own order, here and below.
+#pragma unroll 8
+            for(uint32_t i = lane; i < span; i += 32)
+            {
+                uint32_t const place = rank * own + warp * span + i;
+                if(place < count)
+                    sh.list[0][warp * span + i] = make_uint2(tokens(place), place);
+            }
+            uint32_t const mine = min(span, count - min(count, rank * own + warp * span)); // live tokens of this warp
+            for(int d = 0; d < digits; ++d)
+            {
+                uint2 const* from = sh.list[d & 1];
+                for(uint32_t b = lane; b < bins; b += 32)
+                    sh.at[warp][b] = 0;
+                __syncwarp();
+#pragma unroll 4
+                for(uint32_t i = lane; i < mine; i += 32)
+                    atomicAdd(&sh.at[warp][(from[warp * span + i].x >> (d * bits)) & (bins - 1u)], 1u);
+                __syncthreads();
+                // of a digit: how many of it the warps in front have, and the block
+                uint32_t all = 0;
+                if(t < bins)
+                {
+#pragma unroll 8
+                    for(uint32_t w = 0; w < kSortWarps; ++w)
+                    {
+                        uint32_t const c = sh.at[w][t];
+                        sh.at[w][t] = all;
+                        all += c;
+                    }
+                    sh.total[t] = all;
+                }
+                clusterArrive();
+                clusterWait();
+                // how many of it the blocks in front have, and all blocks; then how many smaller digits there are
+                uint32_t front = 0, v = 0;
+                if(t < bins)
+#pragma unroll
+                    for(uint32_t b = 0; b < kSortBlocks; ++b)
+                    {
+                        uint32_t const c = *inBlock(&sh.total[t], b);
+                        front += b < rank ? c : 0u;
+                        v += c;
+                    }
+                all = v;
+#pragma unroll
+                for(int step = 1; step < 32; step *= 2)
+                {
+                    uint32_t const up = __shfl_up_sync(kFullMask, v, step);
+                    if(lane >= static_cast<uint32_t>(step))
+                        v += up;
+                }
+                if(lane == 31 && warp < kBins / 32)
+                    sh.sums[warp] = v;
+                __syncthreads();
+                if(t < bins)
+                {
+                    uint32_t base = v - all + front;
+                    for(uint32_t w = 0; w < warp; ++w)
+                        base += sh.sums[w];
+#pragma unroll 8
+                    for(uint32_t w = 0; w < kSortWarps; ++w)
+                        sh.at[w][t] += base;
+                }
+                __syncthreads();
+                for(uint32_t first = 0; first < mine; first += 32)
+                {
+                    bool const live = first + lane < mine;
+                    unsigned const here = __ballot_sync(kFullMask, live);
+                    if(live)
+                    {
+                        uint2 const e = from[warp * span + first + lane];
+                        uint32_t const digit = (e.x >> (d * bits)) & (bins - 1u);
+                        unsigned const same = __match_any_sync(here, digit);
+                        uint32_t const before = __popc(same & ((1u << lane) - 1u)), to = sh.at[warp][digit] + before;
+                        __syncwarp(here);
+                        if(before == 0)
+                            sh.at[warp][digit] += __popc(same);
+                        if(d + 1 < digits)
+                            *inBlock(&sh.list[(d + 1) & 1][to & (own - 1u)], to / own) = e;
+                        else
+                            keys[to] = e.x, places[to] = e.y;
+                    }
+                    __syncwarp();
+                }
+                // the other blocks' tokens have come, and nobody reads `total` any more
+                clusterArrive();
+                clusterWait();
+            }
+        }
+
         // More tokens: radix sort, digits of at most nine bits from the lowest, three kernels a digit. A block counts and
         // later places one contiguous tile, its warps contiguous parts of it, so equal digits keep their order.
-        constexpr int kBins = 512, kTileWarps = 8;
+        constexpr int kTileWarps = 8;
 
         struct RadixArgs
         {
@@ -228,6 +345,7 @@ namespace a3b
             uint32_t* places;
             uint32_t* counts; // [bin][tile]
             uint32_t* totals; // [bin]
+            uint32_t* runs; // set to zero for the sums
             uint32_t count, tile, tiles; // tile: a multiple of 32 * kTileWarps
             int shift, bits;
             bool initial;
@@ -247,6 +365,8 @@ namespace a3b
             __shared__ uint32_t bin[kBins];
             for(uint32_t b = threadIdx.x; b < kBins; b += 256)
                 bin[b] = 0;
+            if(a.initial && blockIdx.x == 0 && threadIdx.x == 0)
+                *a.runs = 0;
             __syncthreads();
             uint32_t const low = blockIdx.x * a.tile, high = min(low + a.tile, a.count);
             for(uint32_t i = low + threadIdx.x; i < high; i += 256)
@@ -356,6 +476,7 @@ namespace a3b
             uint32_t const* keys; // sorted, `vocab` behind the last known token
             uint32_t const* places;
             float* partial; // [chunk][2][n]: the run that reaches in from the chunk before, and the one that reaches out
+            uint32_t* runs; // chunks in which a run begins that reaches out, in any order; in front of them their number
             void const* add; // may be null
             int64_t addStride;
             void* out;
@@ -367,17 +488,22 @@ namespace a3b
         };
 
         template<typename U, int E>
-        __device__ __forceinline__ void writeRow(SumArgs const& a, uint32_t row, uint32_t k, float* v)
+        __device__ __forceinline__ void loadAdd(SumArgs const& a, uint32_t row, uint32_t k, unsigned* raw)
+        {
+            Lot<U, E>::load(raw, static_cast<U const*>(a.add) + static_cast<int64_t>(row) * a.addStride + k);
+        }
+
+        // add: the words of what is added, if the call adds
+        template<typename U, int E>
+        __device__ __forceinline__ void writeRow(SumArgs const& a, uint32_t row, uint32_t k, float* v, unsigned const* add)
         {
 #pragma unroll
             for(int e = 0; e < E; ++e)
                 v[e] *= a.scale;
-            if(a.add)
+            if(add)
             {
-                unsigned raw[Lot<U, E>::words];
                 float more[E];
-                Lot<U, E>::load(raw, static_cast<U const*>(a.add) + static_cast<int64_t>(row) * a.addStride + k);
-                Lot<U, E>::unpack(more, raw);
+                Lot<U, E>::unpack(more, add);
 #pragma unroll
                 for(int e = 0; e < E; ++e)
                     v[e] += more[e];
@@ -385,21 +511,44 @@ namespace a3b
             Lot<U, E>::store(static_cast<U*>(a.out) + static_cast<int64_t>(row) * a.stride + k, v);
         }
 
-        constexpr uint32_t kFillRows = 32;
+        constexpr uint32_t kFillRows = 16;
 
         // The first blocks sum: a team has a chunk of the sorted list and E columns a lane, and loads kAhead rows before it
         // adds them. The others write the rows of tokens that do not occur.
-        template<typename T, typename U, int E>
+        template<typename T, typename U, int E, bool Add>
         __global__ void __launch_bounds__(kThreads) embeddingSumKernel(SumArgs a)
         {
-            constexpr int kAhead = 8;
+            constexpr int kAhead = 4;
             if(blockIdx.x >= a.sumBlocks)
             {
-                __shared__ bool absent[kFillRows];
+                __shared__ bool present[kFillRows];
                 uint32_t const base = (blockIdx.x - a.sumBlocks) * kFillRows, lots = a.n / E;
-                if(uint32_t const row = base + threadIdx.x; threadIdx.x < kFillRows)
+                if(threadIdx.x < kFillRows)
+                    present[threadIdx.x] = false;
+                // Where the keys of these rows begin and end in the list: both searched by all threads together, 128 parts a
+                // step (a search by halves took as long as the writing).
+                uint32_t from[2] = {0, 0}, size[2] = {a.count, a.count};
+                while(size[0] + size[1] > 0)
+#pragma unroll
+                    for(int end = 0; end < 2; ++end)
+                    {
+                        uint32_t const part = (size[end] + kThreads - 1) / kThreads;
+                        uint64_t const at = static_cast<uint64_t>(threadIdx.x + 1) * part; // the last of a part is looked at
+                        bool const below = size[end] > 0 && at <= size[end] && a.keys[from[end] + at - 1] < base + end * kFillRows;
+                        uint32_t const skip = __syncthreads_count(below) * part;
+                        size[end] = size[end] > 0 ? min(part - 1, size[end] - skip) : 0;
+                        from[end] += skip;
+                    }
+                uint32_t const lead = from[0], found = from[1] - from[0];
+                if(found <= kThreads)
                 {
-                    uint32_t low = 0, high = a.count; // the first key that is not below row
+                    if(threadIdx.x < found)
+                        present[a.keys[lead + threadIdx.x] - base] = true;
+                }
+                else if(threadIdx.x < kFillRows)
+                {
+                    uint32_t const row = base + threadIdx.x;
+                    uint32_t low = lead, high = lead + found; // the first key that is not below row
                     while(low < high)
                     {
                         uint32_t const mid = low + (high - low) / 2;
@@ -408,18 +557,21 @@ namespace a3b
                         else
                             high = mid;
                     }
-                    absent[threadIdx.x] = row < a.vocab && !(low < a.count && a.keys[low] == row);
+                    present[threadIdx.x] = low < lead + found && a.keys[low] == row;
                 }
                 __syncthreads();
-                for(uint32_t r = 0; r < kFillRows; ++r)
-                    if(absent[r])
+                for(uint32_t r = 0; r < min(kFillRows, a.vocab - base); ++r)
+                    if(!present[r])
                         for(uint32_t k = threadIdx.x; k < lots; k += kThreads)
                         {
                             float v[E];
 #pragma unroll
                             for(int e = 0; e < E; ++e)
                                 v[e] = 0.f;
-                            writeRow<U, E>(a, base + r, k * E, v);
+                            unsigned add[Lot<U, E>::words];
+                            if(Add)
+                                loadAdd<U, E>(a, base + r, k * E, add);
+                            writeRow<U, E>(a, base + r, k * E, v, Add ? add : nullptr);
                         }
                 return;
             }
@@ -431,89 +583,101 @@ namespace a3b
                 return;
             auto const c = static_cast<uint32_t>(c64);
             uint32_t const low = c * a.chunk, high = min(low + a.chunk, a.count);
-            uint32_t current = a.keys[low];
-            bool inward = low > 0 && a.keys[low - 1] == current; // the run began in an earlier chunk
+            bool inward = low > 0 && a.keys[low - 1] == a.keys[low]; // the first run began in an earlier chunk
             float sum[E];
 #pragma unroll
             for(int e = 0; e < E; ++e)
                 sum[e] = 0.f;
-            auto flush = [&](bool outward)
+            auto flush = [&](uint32_t current, bool outward, unsigned const* add)
             {
-                if(current >= a.vocab)
-                    return;
                 if(inward || outward)
                 {
+                    if(!inward && col == 0)
+                        a.runs[1 + atomicAdd(a.runs, 1u)] = c;
                     float* p = a.partial + (static_cast<size_t>(c) * 2 + (inward ? 0 : 1)) * a.n + col;
 #pragma unroll
                     for(int e = 0; e < E; ++e)
                         p[e] = sum[e];
                 }
                 else
-                    writeRow<U, E>(a, current, col, sum);
+                    writeRow<U, E>(a, current, col, sum, add);
             };
-            for(uint32_t p = low; p < high; p += kAhead)
+            // the next rows' keys and places come while these rows do
+            uint32_t next[kAhead], place[kAhead];
+            auto look = [&](uint32_t p)
             {
-                uint32_t key[kAhead];
-                unsigned raw[kAhead][Lot<T, E>::words];
 #pragma unroll
                 for(int u = 0; u < kAhead; ++u)
                 {
-                    key[u] = p + u < high ? a.keys[p + u] : a.vocab;
-                    if(key[u] < a.vocab)
-                        Lot<T, E>::load(raw[u], static_cast<T const*>(a.g) + a.gs.at(a.places[p + u], a.inner, a.one) + col);
+                    next[u] = p + u < high ? a.keys[p + u] : a.vocab;
+                    place[u] = p + u < high ? a.places[p + u] : 0u;
                 }
+            };
+            look(low);
+            for(uint32_t p = low; p < high; p += kAhead)
+            {
+                uint32_t key[kAhead + 1];
+                unsigned raw[kAhead][Lot<T, E>::words], add[Add ? kAhead : 1][Lot<U, E>::words];
+#pragma unroll
+                for(int u = 0; u < kAhead; ++u)
+                {
+                    key[u] = next[u];
+                    if(key[u] < a.vocab)
+                        Lot<T, E>::load(raw[u], static_cast<T const*>(a.g) + a.gs.at(place[u], a.inner, a.one) + col);
+                }
+                look(p + kAhead);
+                key[kAhead] = next[0]; // `vocab` behind the chunk
+                // what is added comes with a run's last row (a run that goes on into the next chunk does not need it)
+                if(Add)
+#pragma unroll
+                    for(int u = 0; u < kAhead; ++u)
+                        if(key[u] < a.vocab && key[u] != key[u + 1])
+                            loadAdd<U, E>(a, key[u], col, add[u]);
 #pragma unroll
                 for(int u = 0; u < kAhead; ++u)
                 {
                     if(key[u] >= a.vocab)
                         break; // only tokens without a row come behind
-                    if(key[u] != current)
-                    {
-                        flush(false);
-                        current = key[u];
-                        inward = false;
-#pragma unroll
-                        for(int e = 0; e < E; ++e)
-                            sum[e] = 0.f;
-                    }
                     float v[E];
                     Lot<T, E>::unpack(v, raw[u]);
 #pragma unroll
                     for(int e = 0; e < E; ++e)
                         sum[e] += v[e];
+                    if(key[u] != key[u + 1])
+                    {
+                        flush(key[u], p + u + 1 == high && high < a.count && a.keys[high] == key[u], Add ? add[Add ? u : 0] : nullptr);
+                        inward = false;
+#pragma unroll
+                        for(int e = 0; e < E; ++e)
+                            sum[e] = 0.f;
+                    }
                 }
             }
-            flush(high < a.count && a.keys[high] == current);
         }
 
-        // Joins the partial sums of a run that begins in chunk blockIdx.x and ends in a later one. Eight warps take equal
-        // parts of its chunks, a lane four columns; the parts are added in their order.
+        // Joins the partial sums of the runs that cross chunks. A block takes a run and 128 columns at a time: its eight warps
+        // have equal parts of the run's chunks, a lane four columns; the parts are added in their order.
         template<typename U, bool Packs>
         __global__ void __launch_bounds__(256) embeddingJoinKernel(SumArgs a)
         {
             __shared__ float4 part[8][32];
-            uint32_t const c = blockIdx.x, low = c * a.chunk, high = low + a.chunk; // never the last chunk
-            uint32_t const key = a.keys[high - 1];
-            if(key >= a.vocab || a.keys[high] != key)
-                return;
-            bool const whole = a.keys[low] == key; // the run fills the chunk
-            if(whole && low > 0 && a.keys[low - 1] == key)
-                return; // began earlier
-            uint32_t first = high, last = a.count; // the first place behind the run
-            while(first < last)
+            uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32, slices = (a.n + 127) / 128;
+            uint64_t const items = static_cast<uint64_t>(a.runs[0]) * slices;
+            for(uint64_t item = blockIdx.x; item < items; item += gridDim.x)
             {
-                uint32_t const mid = first + (last - first) / 2;
-                if(a.keys[mid] <= key)
-                    first = mid + 1;
-                else
-                    last = mid;
-            }
-            uint32_t const end = (first - 1) / a.chunk; // the last chunk with a part of it
-            uint32_t const parts = end - c + 1, each = (parts + 7) / 8;
-            uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-            for(uint32_t base = blockIdx.y * 128; base < a.n; base += gridDim.y * 128)
-            {
-                uint32_t const col = base + lane * 4;
+                auto const run = static_cast<uint32_t>(item / slices);
+                uint32_t const c = a.runs[1 + run], col = (static_cast<uint32_t>(item - static_cast<uint64_t>(run) * slices) * 32 + lane) * 4;
+                uint32_t const key = a.keys[(c + 1) * a.chunk]; // it reaches out: never the last chunk
+                // the chunks that begin with the run's token, 256 looked at together
+                uint32_t end = c;
+                for(bool more = true; more;)
+                {
+                    uint64_t const at = (static_cast<uint64_t>(end) + 1 + threadIdx.x) * a.chunk;
+                    int const same = __syncthreads_count(at < a.count && a.keys[at] == key);
+                    end += same;
+                    more = same == 256;
+                }
+                uint32_t const parts = end - c + 1, each = (parts + 7) / 8;
                 float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
                 for(uint32_t q = warp * each; q < min((warp + 1) * each, parts); ++q)
@@ -524,7 +688,7 @@ namespace a3b
                     {
                         if(col < a.n)
                         {
-                            float4 const v = *reinterpret_cast<float4 const*>(p);
+                            float4 const v = __ldcg(reinterpret_cast<float4 const*>(p));
                             s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
                         }
                     }
@@ -532,9 +696,8 @@ namespace a3b
 #pragma unroll
                         for(int e = 0; e < 4; ++e)
                             if(col + e < a.n)
-                                s[e] += p[e];
+                                s[e] += __ldcg(p + e);
                 }
-                __syncthreads(); // the last columns' parts have been read
                 part[warp][lane] = make_float4(s[0], s[1], s[2], s[3]);
                 __syncthreads();
                 if(warp == 0)
@@ -548,29 +711,36 @@ namespace a3b
 #pragma unroll
                     for(int e = 0; e < 4; ++e)
                         if(col + e < a.n)
-                            writeRow<U, 1>(a, key, col + e, s + e);
+                        {
+                            unsigned add[1];
+                            if(a.add)
+                                loadAdd<U, 1>(a, key, col + e, add);
+                            writeRow<U, 1>(a, key, col + e, s + e, a.add ? add : nullptr);
+                        }
                 }
+                __syncthreads(); // `part` has been read
             }
         }
 
         // ------------------------------------------------------------------------------------------ workspace
         struct Plan
         {
-            bool radix;
+            bool radix; // in several launches
             uint32_t chunk, chunks, tile, tiles;
             int digits, bits; // radix digits and bits of each
-            size_t keys, places, keys2, places2, counts, totals, partial, bytes; // offsets, and the whole
+            size_t keys, places, keys2, places2, counts, totals, runs, partial, bytes; // offsets, and the whole
         };
 
         // From sizes alone (not from alignment), so that the workspace and the order of the sums are.
         Plan planFor(DeviceProps const* props, uint64_t count, uint64_t n, uint64_t vocab)
         {
             Plan p{};
-            p.radix = count > kRankMax;
-            // About eight blocks of 128 threads an SM, each thread with eight columns; chunks of 4 to 256 positions.
+            p.radix = count > kClusterMax;
+            // About eight blocks of 128 threads an SM, each thread with eight columns; chunks of 16 to 256 positions (shorter ones
+            // leave more runs to join).
             uint64_t const perRow = std::max<uint64_t>(1, n / 8), wanted = 8ull * static_cast<unsigned>(props->smCount) * kThreads;
             uint64_t const chunk = count * perRow / wanted;
-            p.chunk = static_cast<uint32_t>(std::min<uint64_t>(256, std::max<uint64_t>(4, chunk / 4 * 4)));
+            p.chunk = static_cast<uint32_t>(std::min<uint64_t>(256, std::max<uint64_t>(16, chunk / 4 * 4)));
             p.chunks = static_cast<uint32_t>((count + p.chunk - 1) / p.chunk);
             int bits = 1;
             while(bits < 32 && (vocab >> bits) != 0) // keys are 0 .. vocab
@@ -598,28 +768,46 @@ namespace a3b
                 p.counts = take(static_cast<size_t>(kBins) * p.tiles * 4);
                 p.totals = take(kBins * 4);
             }
+            p.runs = take((static_cast<size_t>(p.chunks) + 1) * 4);
             p.partial = take(static_cast<size_t>(p.chunks) * 2 * n * 4);
             p.bytes = std::max<size_t>(at, 256);
             return p;
         }
 
-        int sortTokens(cudaStream_t stream, Plan const& p, Tokens const& tokens, uint32_t count, char* ws, uint32_t** keys,
+        int sortTokens(cudaStream_t stream, DeviceProps const* props, Plan const& p, Tokens const& tokens, uint32_t count, char* ws, uint32_t** keys,
                        uint32_t** places)
         {
             auto at = [&](size_t offset) { return reinterpret_cast<uint32_t*>(ws + offset); };
             *keys = at(p.keys);
             *places = at(p.places);
+            if(!p.radix && count > kRankMax)
+            {
+                static std::atomic<bool> ready[kMaxDevices];
+                if(!ready[props->ordinal].load(std::memory_order_relaxed))
+                {
+                    A3B_CUDA(cudaFuncSetAttribute(clusterSortKernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                  static_cast<int>(sizeof(ClusterSort))));
+                    ready[props->ordinal].store(true, std::memory_order_relaxed);
+                }
+                int log2Each = 0; // tokens of a thread
+                while((kSortBlocks * kSortThreads << log2Each) < count)
+                    ++log2Each;
+                clusterSortKernel<<<kSortBlocks, kSortThreads, sizeof(ClusterSort), stream>>>(tokens, count, log2Each, p.digits, p.bits,
+                                                                                            *keys, *places, at(p.runs));
+                A3B_CHECK_LAUNCH("clusterSortKernel");
+                return A3B_OK;
+            }
             if(!p.radix)
             {
                 uint32_t const blocks = (count + 31) / 32;
-                rankKernel<<<blocks, 256, blocks * 32 * 4, stream>>>(tokens, count, *keys, *places);
+                rankKernel<<<blocks, 256, blocks * 32 * 4, stream>>>(tokens, count, *keys, *places, at(p.runs));
                 A3B_CHECK_LAUNCH("rankKernel");
                 return A3B_OK;
             }
             uint32_t *otherKeys = at(p.keys2), *otherPlaces = at(p.places2);
             for(int d = 0; d < p.digits; ++d)
             {
-                RadixArgs a{tokens, otherKeys, otherPlaces, *keys, *places, at(p.counts), at(p.totals), count, p.tile, p.tiles,
+                RadixArgs a{tokens, otherKeys, otherPlaces, *keys, *places, at(p.counts), at(p.totals), at(p.runs), count, p.tile, p.tiles,
                             d * p.bits, p.bits, d == 0};
                 if(d > 0) // from what the digit before wrote
                 {
@@ -639,7 +827,7 @@ namespace a3b
         }
 
         template<typename T, typename U, int E>
-        int launchSum(cudaStream_t stream, SumArgs a)
+        int launchSum(cudaStream_t stream, DeviceProps const* props, SumArgs a)
         {
             uint32_t const lots = a.n / E;
             a.shift = teamShift(lots);
@@ -655,15 +843,21 @@ namespace a3b
             a.sumBlocks = static_cast<uint32_t>(sums);
             if(sums + fills == 0)
                 return A3B_OK;
-            embeddingSumKernel<T, U, E><<<static_cast<unsigned>(sums + fills), kThreads, 0, stream>>>(a);
+            auto const grid = static_cast<unsigned>(sums + fills);
+            if(a.add)
+                embeddingSumKernel<T, U, E, true><<<grid, kThreads, 0, stream>>>(a);
+            else
+                embeddingSumKernel<T, U, E, false><<<grid, kThreads, 0, stream>>>(a);
             A3B_CHECK_LAUNCH("embeddingSumKernel");
             if(a.chunks > 1)
             {
-                dim3 const grid(a.chunks - 1, std::min<uint32_t>(4, (a.n + 127) / 128));
+                // as many blocks as SMs hold, or runs and columns there can be
+                uint64_t const items = static_cast<uint64_t>(a.chunks - 1) * ((a.n + 127) / 128);
+                auto const blocks = static_cast<unsigned>(std::min<uint64_t>(8ull * static_cast<unsigned>(props->smCount), items));
                 if(a.n % 4 == 0)
-                    embeddingJoinKernel<U, true><<<grid, 256, 0, stream>>>(a);
+                    embeddingJoinKernel<U, true><<<blocks, 256, 0, stream>>>(a);
                 else
-                    embeddingJoinKernel<U, false><<<grid, 256, 0, stream>>>(a);
+                    embeddingJoinKernel<U, false><<<blocks, 256, 0, stream>>>(a);
                 A3B_CHECK_LAUNCH("embeddingJoinKernel");
             }
             return A3B_OK;
@@ -800,12 +994,13 @@ extern "C"
         if(count > 0)
         {
             Tokens const t{tokens, index_dtype == A3B_I64, first, static_cast<uint32_t>(vocab)};
-            int const rs = sortTokens(s, p, t, static_cast<uint32_t>(count), static_cast<char*>(workspace), &keys, &places);
+            int const rs = sortTokens(s, props, p, t, static_cast<uint32_t>(count), static_cast<char*>(workspace), &keys, &places);
             if(rs != A3B_OK)
                 return rs;
         }
         SumArgs a{grad_out.data, {grad_out.outer_stride, grad_out.inner_stride}, keys, places,
-                  count ? reinterpret_cast<float*>(static_cast<char*>(workspace) + p.partial) : nullptr, add, add_stride, grad_table,
+                  count ? reinterpret_cast<float*>(static_cast<char*>(workspace) + p.partial) : nullptr,
+                  count ? reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + p.runs) : nullptr, add, add_stride, grad_table,
                   table_stride, static_cast<uint32_t>(count), static_cast<uint32_t>(inner), static_cast<uint32_t>(n),
                   static_cast<uint32_t>(vocab), p.chunk, p.chunks, 0u, 0u, outer == 1, !inPlace, static_cast<float>(scale), 0};
         return withTypes(grad_dtype, table_dtype, [&](auto t, auto u)
@@ -816,7 +1011,7 @@ extern "C"
             bool const packed = n % E == 0 && rowsAligned(grad_out.data, outer, inner, grad_out.outer_stride, grad_out.inner_stride, gs, 16)
                                 && rowsAligned(grad_table, 1, vocab, 0, table_stride, ts, 16)
                                 && rowsAligned(add, 1, vocab, 0, add_stride, ts, 16);
-            return packed ? launchSum<T, U, E>(s, a) : launchSum<T, U, 1>(s, a);
+            return packed ? launchSum<T, U, E>(s, props, a) : launchSum<T, U, 1>(s, props, a);
         });
     }
 }

@@ -840,10 +840,7 @@ namespace a3b
                     }
             }
             if(a.partial)
-            {
-                asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); // the fold waits before it reads
                 addTeams<E, P>(a, dw, sums, teams, mine, lanes, t);
-            }
         }
 
         // Rows that no team holds: two passes over the row for its gradient ...
@@ -904,7 +901,6 @@ namespace a3b
         {
             __shared__ float part[32][33];
             uint32_t const lane = threadIdx.x % 32, warp = threadIdx.x / 32, k = blockIdx.x * 32 + lane;
-            asm volatile("griddepcontrol.wait;" ::: "memory");
             float s = 0.f;
             if(k < n)
 #pragma unroll 10
@@ -968,18 +964,8 @@ namespace a3b
             A3B_CHECK_LAUNCH("rmsNormBackwardKernel");
             if(a.partial)
             {
-                // Its blocks may be launched while the last rows are written; they wait for the whole grid. Only this kernel
-                // follows one that signals its dependents, and it signals none.
-                cudaLaunchAttribute attribute{};
-                attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-                attribute.val.programmaticStreamSerializationAllowed = 1;
-                cudaLaunchConfig_t config{};
-                config.gridDim = dim3((a.n + 31) / 32);
-                config.blockDim = dim3(1024);
-                config.stream = stream;
-                config.attrs = &attribute;
-                config.numAttrs = 1;
-                A3B_CUDA(cudaLaunchKernelEx(&config, rmsNormFoldKernel<WT>, static_cast<float const*>(a.partial), blocks, a.n, gw));
+                rmsNormFoldKernel<WT><<<(a.n + 31) / 32, 1024, 0, stream>>>(a.partial, blocks, a.n, gw);
+                A3B_CHECK_LAUNCH("rmsNormFoldKernel");
             }
             return A3B_OK;
         }
