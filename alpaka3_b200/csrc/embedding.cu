@@ -171,15 +171,107 @@ namespace a3b
             return A3B_OK;
         }
 
+        // ------------------------------------------------------------------------------------ rows of the gradient
+        struct SumArgs
+        {
+            void const* g;
+            RowStep gs;
+            uint32_t const* keys; // sorted, `vocab` behind the last known token
+            uint32_t const* places;
+            float* partial; // [chunk][2][n]: the run that reaches in from the chunk before, and the one that reaches out
+            uint32_t* runs; // chunks in which a run begins that reaches out, in any order; in front of them their number
+            void const* add; // may be null
+            int64_t addStride;
+            void* out;
+            int64_t stride;
+            uint32_t count, inner, n, vocab, chunk, chunks, slices, sumBlocks;
+            bool one, fill, flat; // fill: rows without a token are written; flat: they are zeros, and the table is one stretch
+            float scale;
+            int shift;
+        };
+
+        template<typename U, int E>
+        __device__ __forceinline__ void loadAdd(SumArgs const& a, uint32_t row, uint32_t k, unsigned* raw)
+        {
+            Lot<U, E>::load(raw, static_cast<U const*>(a.add) + static_cast<int64_t>(row) * a.addStride + k);
+        }
+
+        // add: the words of what is added, if the call adds
+        template<typename U, int E>
+        __device__ __forceinline__ void writeRow(SumArgs const& a, uint32_t row, uint32_t k, float* v, unsigned const* add)
+        {
+#pragma unroll
+            for(int e = 0; e < E; ++e)
+                v[e] *= a.scale;
+            if(add)
+            {
+                float more[E];
+                Lot<U, E>::unpack(more, add);
+#pragma unroll
+                for(int e = 0; e < E; ++e)
+                    v[e] += more[e];
+            }
+            Lot<U, E>::store(static_cast<U*>(a.out) + static_cast<int64_t>(row) * a.stride + k, v);
+        }
+
+        constexpr uint32_t kFillRows = 16; // rows that a block looks for
+        constexpr uint32_t kFillLots = 1024; // lots of a block that looks for none
+
+        // lot k of a row without a token: what is added, or zero
+        template<typename U, int E, bool Add>
+        __device__ __forceinline__ void fillLot(SumArgs const& a, uint32_t row, uint32_t k)
+        {
+            float v[E];
+#pragma unroll
+            for(int e = 0; e < E; ++e)
+                v[e] = 0.f;
+            unsigned add[Lot<U, E>::words];
+            if(Add)
+                loadAdd<U, E>(a, row, k * E, add);
+            writeRow<U, E>(a, row, k * E, v, Add ? add : nullptr);
+        }
+
         // ------------------------------------------------------------------------------------- sorting the tokens
         // Up to kRankMax tokens: the place of each is the number of those that come before it, by comparing all pairs. A
         // block ranks 32 tokens, each of its warps against an eighth of the list. Quadratic, but one short launch.
         constexpr uint32_t kRankMax = 4096;
 
-        __global__ void __launch_bounds__(256) rankKernel(Tokens tokens, uint32_t count, uint32_t* keys, uint32_t* places, uint32_t* runs)
+        // Where tokens are few beside the table's rows, blocks behind those that rank write every row as if its token did not
+        // occur; the sums then write over those that do. So the table is filled while the tokens are ranked, and no row needs
+        // a search (512 tokens into 32000 x 1024 fp32 27.3 us, 29.2 with the rows searched behind the sort).
+        template<typename U, int E, bool Add>
+        __global__ void __launch_bounds__(256) rankKernel(Tokens tokens, uint32_t count, uint32_t* keys, uint32_t* places, SumArgs a)
         {
+            uint32_t const ranking = (count + 31) / 32;
+            if(blockIdx.x >= ranking)
+            {
+                uint32_t const lots = a.n / E;
+                if(a.flat)
+                {
+                    // one stretch of zeros, rows of any length
+                    constexpr uint32_t per = PackOf<U>::E;
+                    uint64_t const all = static_cast<uint64_t>(a.vocab) * a.n, packs = all / per;
+                    U* out = static_cast<U*>(a.out);
+#pragma unroll
+                    for(uint32_t u = 0; u < kFillLots; u += 256)
+                    {
+                        uint64_t const i = static_cast<uint64_t>(blockIdx.x - ranking) * kFillLots + u + threadIdx.x;
+                        if(i < packs)
+                            reinterpret_cast<uint4*>(out)[i] = make_uint4(0u, 0u, 0u, 0u);
+                        else if(i == packs)
+                            for(uint64_t k = packs * per; k < all; ++k)
+                                out[k] = fromFloat<U>(0.f);
+                    }
+                    return;
+                }
+#pragma unroll
+                for(uint32_t u = 0; u < kFillLots; u += 256)
+                    if(uint32_t const i = (blockIdx.x - ranking) * kFillLots + u + threadIdx.x, row = i / lots; row < a.vocab)
+                        fillLot<U, E, Add>(a, row, i - row * lots);
+                return;
+            }
             if(blockIdx.x == 0 && threadIdx.x == 0)
-                *runs = 0;
+                *a.runs = 0;
             extern __shared__ __align__(16) uint32_t all[];
             __shared__ uint32_t part[8][32];
             uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32, base = blockIdx.x * 32, i = base + lane;
@@ -469,50 +561,6 @@ namespace a3b
         }
 
         // -------------------------------------------------------------------------------------- sums by token
-        struct SumArgs
-        {
-            void const* g;
-            RowStep gs;
-            uint32_t const* keys; // sorted, `vocab` behind the last known token
-            uint32_t const* places;
-            float* partial; // [chunk][2][n]: the run that reaches in from the chunk before, and the one that reaches out
-            uint32_t* runs; // chunks in which a run begins that reaches out, in any order; in front of them their number
-            void const* add; // may be null
-            int64_t addStride;
-            void* out;
-            int64_t stride;
-            uint32_t count, inner, n, vocab, chunk, chunks, slices, sumBlocks;
-            bool one, fill; // fill: rows without a token are written
-            float scale;
-            int shift;
-        };
-
-        template<typename U, int E>
-        __device__ __forceinline__ void loadAdd(SumArgs const& a, uint32_t row, uint32_t k, unsigned* raw)
-        {
-            Lot<U, E>::load(raw, static_cast<U const*>(a.add) + static_cast<int64_t>(row) * a.addStride + k);
-        }
-
-        // add: the words of what is added, if the call adds
-        template<typename U, int E>
-        __device__ __forceinline__ void writeRow(SumArgs const& a, uint32_t row, uint32_t k, float* v, unsigned const* add)
-        {
-#pragma unroll
-            for(int e = 0; e < E; ++e)
-                v[e] *= a.scale;
-            if(add)
-            {
-                float more[E];
-                Lot<U, E>::unpack(more, add);
-#pragma unroll
-                for(int e = 0; e < E; ++e)
-                    v[e] += more[e];
-            }
-            Lot<U, E>::store(static_cast<U*>(a.out) + static_cast<int64_t>(row) * a.stride + k, v);
-        }
-
-        constexpr uint32_t kFillRows = 16;
-
         // The first blocks sum: a team has a chunk of the sorted list and E columns a lane, and loads kAhead rows before it
         // adds them. The others write the rows of tokens that do not occur.
         template<typename T, typename U, int E, bool Add>
@@ -522,7 +570,7 @@ namespace a3b
             if(blockIdx.x >= a.sumBlocks)
             {
                 __shared__ bool present[kFillRows];
-                uint32_t const base = (blockIdx.x - a.sumBlocks) * kFillRows, lots = a.n / E;
+                uint32_t const base = (blockIdx.x - a.sumBlocks) * kFillRows;
                 if(threadIdx.x < kFillRows)
                     present[threadIdx.x] = false;
                 // Where the keys of these rows begin and end in the list: both searched by all threads together, 128 parts a
@@ -562,17 +610,8 @@ namespace a3b
                 __syncthreads();
                 for(uint32_t r = 0; r < min(kFillRows, a.vocab - base); ++r)
                     if(!present[r])
-                        for(uint32_t k = threadIdx.x; k < lots; k += kThreads)
-                        {
-                            float v[E];
-#pragma unroll
-                            for(int e = 0; e < E; ++e)
-                                v[e] = 0.f;
-                            unsigned add[Lot<U, E>::words];
-                            if(Add)
-                                loadAdd<U, E>(a, base + r, k * E, add);
-                            writeRow<U, E>(a, base + r, k * E, v, Add ? add : nullptr);
-                        }
+                        for(uint32_t k = threadIdx.x; k < a.n / E; k += kThreads)
+                            fillLot<U, E, Add>(a, base + r, k);
                 return;
             }
             uint32_t const lanes = 1u << a.shift, lane = threadIdx.x & (lanes - 1u);
@@ -780,7 +819,9 @@ namespace a3b
             auto at = [&](size_t offset) { return reinterpret_cast<uint32_t*>(ws + offset); };
             *keys = at(p.keys);
             *places = at(p.places);
-            if(!p.radix && count > kRankMax)
+            if(count <= kRankMax)
+                return A3B_OK; // with the sums
+            if(!p.radix)
             {
                 static std::atomic<bool> ready[kMaxDevices];
                 if(!ready[props->ordinal].load(std::memory_order_relaxed))
@@ -795,13 +836,6 @@ namespace a3b
                 clusterSortKernel<<<kSortBlocks, kSortThreads, sizeof(ClusterSort), stream>>>(tokens, count, log2Each, p.digits, p.bits,
                                                                                             *keys, *places, at(p.runs));
                 A3B_CHECK_LAUNCH("clusterSortKernel");
-                return A3B_OK;
-            }
-            if(!p.radix)
-            {
-                uint32_t const blocks = (count + 31) / 32;
-                rankKernel<<<blocks, 256, blocks * 32 * 4, stream>>>(tokens, count, *keys, *places, at(p.runs));
-                A3B_CHECK_LAUNCH("rankKernel");
                 return A3B_OK;
             }
             uint32_t *otherKeys = at(p.keys2), *otherPlaces = at(p.places2);
@@ -827,14 +861,27 @@ namespace a3b
         }
 
         template<typename T, typename U, int E>
-        int launchSum(cudaStream_t stream, DeviceProps const* props, SumArgs a)
+        int launchSum(cudaStream_t stream, DeviceProps const* props, SumArgs a, Tokens const& tokens, uint32_t* keys, uint32_t* places)
         {
             uint32_t const lots = a.n / E;
             a.shift = teamShift(lots);
             uint32_t const lanes = 1u << a.shift, teams = kThreads >> a.shift;
             a.slices = (lots + lanes - 1) / lanes;
             uint64_t const sums = static_cast<uint64_t>((a.chunks + teams - 1) / teams) * a.slices;
-            uint64_t const fills = a.fill ? (a.vocab + kFillRows - 1) / kFillRows : 0;
+            uint64_t fills = a.fill ? (a.vocab + kFillRows - 1) / kFillRows : 0;
+            if(a.count > 0 && a.count <= kRankMax)
+            {
+                uint32_t const ranking = (a.count + 31) / 32;
+                // at most one row in sixteen is written twice
+                uint64_t const all = a.flat ? static_cast<uint64_t>(a.vocab) * a.n / PackOf<U>::E + 1 : static_cast<uint64_t>(a.vocab) * lots;
+                bool const early = a.fill && a.count <= a.vocab / 16 && all <= static_cast<uint64_t>(UINT32_MAX) - kFillLots;
+                auto kernel = early && a.add ? rankKernel<U, E, true> : rankKernel<U, E, false>;
+                uint32_t const filling = early ? static_cast<uint32_t>((all + kFillLots - 1) / kFillLots) : 0;
+                kernel<<<ranking + filling, 256, ranking * 32 * 4, stream>>>(tokens, a.count, keys, places, a);
+                A3B_CHECK_LAUNCH("rankKernel");
+                if(early)
+                    fills = 0;
+            }
             if(sums + fills > static_cast<uint64_t>(INT_MAX))
             {
                 setError("%u tokens of %u elements are more than one launch holds", a.count, a.n);
@@ -991,10 +1038,10 @@ extern "C"
                     "the workspace is missing, too small or not aligned to 16 bytes");
         auto s = static_cast<cudaStream_t>(stream);
         uint32_t *keys = nullptr, *places = nullptr;
+        Tokens const known{tokens, index_dtype == A3B_I64, first, static_cast<uint32_t>(vocab)};
         if(count > 0)
         {
-            Tokens const t{tokens, index_dtype == A3B_I64, first, static_cast<uint32_t>(vocab)};
-            int const rs = sortTokens(s, props, p, t, static_cast<uint32_t>(count), static_cast<char*>(workspace), &keys, &places);
+            int const rs = sortTokens(s, props, p, known, static_cast<uint32_t>(count), static_cast<char*>(workspace), &keys, &places);
             if(rs != A3B_OK)
                 return rs;
         }
@@ -1002,7 +1049,8 @@ extern "C"
                   count ? reinterpret_cast<float*>(static_cast<char*>(workspace) + p.partial) : nullptr,
                   count ? reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + p.runs) : nullptr, add, add_stride, grad_table,
                   table_stride, static_cast<uint32_t>(count), static_cast<uint32_t>(inner), static_cast<uint32_t>(n),
-                  static_cast<uint32_t>(vocab), p.chunk, p.chunks, 0u, 0u, outer == 1, !inPlace, static_cast<float>(scale), 0};
+                  static_cast<uint32_t>(vocab), p.chunk, p.chunks, 0u, 0u, outer == 1, !inPlace,
+                  !add && table_stride == static_cast<int64_t>(n) && alignedTo(16, {grad_table}), static_cast<float>(scale), 0};
         return withTypes(grad_dtype, table_dtype, [&](auto t, auto u)
         {
             using T = decltype(t);
@@ -1011,7 +1059,7 @@ extern "C"
             bool const packed = n % E == 0 && rowsAligned(grad_out.data, outer, inner, grad_out.outer_stride, grad_out.inner_stride, gs, 16)
                                 && rowsAligned(grad_table, 1, vocab, 0, table_stride, ts, 16)
                                 && rowsAligned(add, 1, vocab, 0, add_stride, ts, 16);
-            return packed ? launchSum<T, U, E>(s, props, a) : launchSum<T, U, 1>(s, props, a);
+            return packed ? launchSum<T, U, E>(s, props, a, known, keys, places) : launchSum<T, U, 1>(s, props, a, known, keys, places);
         });
     }
 }

@@ -200,6 +200,51 @@ def test_sorted_and_reversed_tokens(cuda, count):
         assert torch.equal(gw.double(), summed(g, t, vocab, 1.0, None)[0])
 
 
+@pytest.mark.parametrize("pair", PAIRS)
+def test_few_tokens_of_many(cuda, pair):
+    """Few tokens beside the table's rows: the table is filled while they are sorted. One stretch or strided rows, with and
+    without packs, with and without something added; and at the counts where the way of sorting changes."""
+    from alpaka3_b200 import algo
+    source, target = pair
+    for count, vocab, n in ((1, 16, 8), (1, 17, 5), (20, 1000, 64), (20, 1001, 33), (300, 5000, 7), (62, 1000, 24), (63, 1000, 24),
+                            (4096, 70000, 8), (4097, 70000, 8), (16384, 3000, 8), (16385, 3000, 8)):
+        t = pick((count,), vocab, count, skew=count > 20, outside=count > 2)
+        g = whole_numbers((count, n), source, n)
+        want = summed(g, t, vocab, 1.0, None)[0]
+        gw = torch.full((vocab, n), 7.0, dtype=target, device="cuda")
+        algo.embedding_backward(gw, g, t)
+        assert torch.equal(gw, want.to(target)), (count, vocab, n)
+        room = torch.full((vocab + 1, n + 8), 5.0, dtype=target, device="cuda")
+        part = room[:vocab, 8 - n % 2:8 - n % 2 + n]
+        algo.embedding_backward(part, g, t)
+        assert torch.equal(part, want.to(target))
+        add = whole_numbers((vocab, n), target, 3)
+        algo.embedding_backward(part, g, t, add=add)
+        assert torch.equal(part, (want + add.double()).to(target))
+        part.fill_(5.0)
+        assert (room == 5.0).all()
+        # one stretch that begins off 16 bytes
+        flat = torch.full((vocab * n + 2,), 5.0, dtype=target, device="cuda")
+        algo.embedding_backward(flat[1:-1].view(vocab, n), g, t)
+        assert torch.equal(flat[1:-1].view(vocab, n), want.to(target)) and flat[0] == 5 and flat[-1] == 5
+
+
+def test_workspace_is_checked(cuda):
+    from alpaka3_b200 import capi
+    g, t, gw = torch.zeros(40, 64, device="cuda"), torch.zeros(40, dtype=torch.int64, device="cuda"), torch.zeros(9, 64, device="cuda")
+    size = capi.lib().a3b_embedding_backward_workspace(40, 64, 9)
+    ws = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
+
+    def call(at, bytes_):
+        return capi.lib().a3b_embedding_backward(None, capi.EMBEDDING_BACKWARD_ARGS.pack(
+            1, 40, 64, 9, 0, g.data_ptr(), 0, 64, t.data_ptr(), 0, 0, gw.data_ptr(), 64, at, bytes_, 1.0, capi.F32, capi.I64,
+            capi.F32, 0))
+    for at, bytes_ in ((0, size), (ws.data_ptr(), size - 1), (ws.data_ptr() + 8, size)):
+        assert call(at, bytes_) == capi.ERR_INVALID and "workspace" in capi.last_error()
+    assert call(ws.data_ptr(), size) == capi.OK
+    torch.cuda.synchronize()
+
+
 def test_no_tokens_and_infinities(cuda):
     from alpaka3_b200 import algo
     for n in (8, 5):

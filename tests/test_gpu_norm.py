@@ -340,6 +340,22 @@ def test_no_rows(cuda):
         assert (gw == 0).all()
 
 
+def test_workspace_is_checked(cuda):
+    from alpaka3_b200 import capi
+    x, r, gw = torch.ones(40, 64, device="cuda"), torch.ones(40, device="cuda"), torch.zeros(64, device="cuda")
+    size = capi.lib().a3b_rms_norm_backward_workspace(40, 64)
+    ws = torch.empty(size + 16, dtype=torch.uint8, device="cuda")
+
+    def call(at, bytes_):
+        rows = (x.data_ptr(), 0, 64)
+        return capi.lib().a3b_rms_norm_backward(None, capi.RMS_NORM_BACKWARD_ARGS.pack(
+            1, 40, 64, *rows, *rows, 0, 0, 0, *rows, 0, r.data_ptr(), gw.data_ptr(), at, bytes_, capi.F32, capi.F32, capi.F32, 0))
+    for at, bytes_ in ((0, size), (ws.data_ptr(), size - 1), (ws.data_ptr() + 8, size)):
+        assert call(at, bytes_) == capi.ERR_INVALID and "workspace" in capi.last_error()
+    assert call(ws.data_ptr(), size) == capi.OK
+    torch.cuda.synchronize()
+
+
 def test_streams_and_graphs(cuda):
     """Another stream than the current one; a captured call replayed on new inputs, two graphs that overlap."""
     from alpaka3_b200 import algo
