@@ -21,7 +21,7 @@ namespace a3b
 {
     namespace
     {
-        constexpr int kThreads = 256;
+        constexpr int kThreads = 512;
 
         struct VerifyArgs
         {
@@ -244,9 +244,10 @@ namespace a3b
         constexpr uint32_t kList = 1024;
 
         // This thread's lots first, first + kThreads, ...: tokens with p / noise >= least go to the list. U lots are loaded
-        // together, without conditions between the loads: 64 x 131072 bf16 takes 17.5 us with two packs together, 18.8 with
-        // one, 18.4 with three; 256 x 50257 fp32 (single tokens) 31.6 with eight, 35.9 with four, 39 with twelve (spills);
-        // stages in shared memory filled by bulk copies took 26 and 39 (a barrier a stage).
+        // together, without conditions between the loads: 64 x 131072 bf16 takes 16.3 us with two packs together, 17.1 with
+        // one (in blocks of 256 threads 17.5, 18.8, and 18.4 with three); 256 x 50257 fp32, single tokens, with eight, four
+        // and twelve 31.6, 35.9 and 39 (spills). Stages in shared memory filled by bulk copies took 26 and 39 (a barrier a
+        // stage), noise brought into L2 while the drafts are tested 5% more.
         template<typename T, int E, int U>
         __device__ __forceinline__ void scan(T const* row, float const* clock, uint32_t first, uint32_t end, Rough const& p, float least,
                                              uint32_t* list, unsigned* listed)
@@ -316,7 +317,7 @@ namespace a3b
 
         // Packed: every row of logits, draft and noise begins at 16 bytes.
         template<typename T, bool Packed>
-        __global__ void __launch_bounds__(kThreads, 4) verifyKernel(VerifyArgs a)
+        __global__ void __launch_bounds__(kThreads, 2) verifyKernel(VerifyArgs a)
         {
             constexpr int E = PackOf<T>::E, kWarps = kThreads / 32;
             __shared__ float lows[kWarps];
@@ -367,16 +368,7 @@ namespace a3b
             uint32_t const oneLow = lots * E + min(rank * onesPer, ones), oneHigh = min(oneLow + onesPer, a.vocab);
             float const* clock = a.noise + static_cast<int64_t>(b) * a.noiseStride;
             if(tid == 0)
-            {
                 founds = 0;
-                // the noise needs no decision: it comes into L2 while the drafts are tested
-                auto at16 = [&](size_t i) { return reinterpret_cast<uintptr_t>(clock + i); };
-                uintptr_t const from = (at16(Packed ? low * static_cast<size_t>(E) : oneLow) + 15) & ~uintptr_t(15);
-                uintptr_t const end = at16(Packed ? high * static_cast<size_t>(E) : oneHigh) & ~uintptr_t(15);
-                if(end > from)
-                    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from),
-                                 "r"(static_cast<unsigned>(min(end - from, uintptr_t(1) << 20))));
-            }
 
             bool refused = false;
             uint32_t const n = accepted<T>(a, b, &refused);
@@ -582,11 +574,12 @@ namespace a3b
         template<typename T>
         int launchVerify(cudaStream_t stream, DeviceProps const* props, VerifyArgs const& a, bool packed)
         {
-            // A cluster of up to eight blocks a sequence: as many as leave each thread about two packs, and fewer when the
-            // sequences alone fill the GPU (four blocks an SM).
+            // A cluster of up to eight blocks a sequence: as many as leave each thread a pack or more, and fewer when the
+            // sequences alone fill the GPU (two blocks an SM; 256 x 50256 fp32 24.6 us with one block a sequence, 30.2 with
+            // two of half the threads; 64 x 131072 bf16 with four 16.3, with eight of half the threads 16.6).
             constexpr uint32_t E = PackOf<T>::E;
             uint32_t blocks = 1;
-            uint64_t const room = 4ull * static_cast<unsigned>(props->smCount);
+            uint64_t const room = 2ull * static_cast<unsigned>(props->smCount);
             if(a.logits)
                 while(blocks < 8 && a.vocab > blocks * kThreads * E && static_cast<uint64_t>(a.batch) * blocks * 2 <= room)
                     blocks *= 2;
