@@ -596,11 +596,13 @@ def rms_norm(out, x, weight=None, residual=None, total=None, rstd=None, scales=N
     Rows of all tensors may be strided (heads of a wider product); out may be x or residual, and total may be residual or x
     (in place). For the gradient keep `total` (x without a residual) and rstd. Infinities, NaN and what may overlap: see
     a3b_rms_norm. Returns out."""
-    code, dev = _row_tensor(x, "x")
+    dtype, dev, shape = x.dtype, x.get_device(), x.shape
+    code = _LOGITS_DT.get(dtype)
+    if code is None or dev < 0 or not shape:
+        _row_tensor(x, "x")
     target = _NORM_OUT_DT.get(out.dtype)
     if target is None:
         raise TypeError(f"unsupported out dtype {out.dtype}")
-    shape, dtype = x.shape, x.dtype
     n = shape[-1]
     if out.shape != shape or out.get_device() != dev:
         raise ValueError("out must have the shape and device of x")

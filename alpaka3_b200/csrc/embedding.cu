@@ -700,12 +700,17 @@ namespace a3b
         __global__ void __launch_bounds__(256) embeddingJoinKernel(SumArgs a)
         {
             __shared__ float4 part[8][32];
-            uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32, slices = (a.n + 127) / 128;
-            uint64_t const items = static_cast<uint64_t>(a.runs[0]) * slices;
-            for(uint64_t item = blockIdx.x; item < items; item += gridDim.x)
+            uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32, slices = (a.n + 127) / 128, runs = a.runs[0];
+            uint32_t const runStep = gridDim.x / slices, sliceStep = gridDim.x % slices; // items in steps of the grid
+            for(uint32_t run = blockIdx.x / slices, slice = blockIdx.x % slices; run < runs; run += runStep, slice += sliceStep)
             {
-                auto const run = static_cast<uint32_t>(item / slices);
-                uint32_t const c = a.runs[1 + run], col = (static_cast<uint32_t>(item - static_cast<uint64_t>(run) * slices) * 32 + lane) * 4;
+                if(slice >= slices)
+                {
+                    slice -= slices;
+                    if(++run >= runs)
+                        break;
+                }
+                uint32_t const c = a.runs[1 + run], col = (slice * 32 + lane) * 4;
                 uint32_t const key = a.keys[(c + 1) * a.chunk]; // it reaches out: never the last chunk
                 // the chunks that begin with the run's token, 256 looked at together
                 uint32_t end = c;
@@ -776,10 +781,11 @@ namespace a3b
             Plan p{};
             p.radix = count > kClusterMax;
             // About eight blocks of 128 threads an SM, each thread with eight columns; chunks of 16 to 256 positions (shorter ones
-            // leave more runs to join).
+            // leave more runs to join: 4096 tokens of 257 in chunks of 8 take 21 us, of 16 18), but of 8 for few tokens, whose
+            // chunks' latency counts (512 tokens 2 us less).
             uint64_t const perRow = std::max<uint64_t>(1, n / 8), wanted = 8ull * static_cast<unsigned>(props->smCount) * kThreads;
             uint64_t const chunk = count * perRow / wanted;
-            p.chunk = static_cast<uint32_t>(std::min<uint64_t>(256, std::max<uint64_t>(16, chunk / 4 * 4)));
+            p.chunk = static_cast<uint32_t>(std::min<uint64_t>(256, std::max<uint64_t>(count < 2048 ? 8 : 16, chunk / 4 * 4)));
             p.chunks = static_cast<uint32_t>((count + p.chunk - 1) / p.chunk);
             int bits = 1;
             while(bits < 32 && (vocab >> bits) != 0) // keys are 0 .. vocab

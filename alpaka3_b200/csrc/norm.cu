@@ -170,10 +170,13 @@ namespace a3b
             return v;
         }
 
-        __device__ __forceinline__ float lanesMax(float v, int lanes)
+        // the largest of 1 << log2 neighbouring lanes (the same for the whole warp)
+        __device__ __forceinline__ float lanesMax(float v, int log2)
         {
-            for(int d = lanes / 2; d > 0; d /= 2)
-                v = maxNan(v, __shfl_xor_sync(kFullMask, v, d));
+#pragma unroll
+            for(int d = 0; d < 5; ++d)
+                if(d < log2)
+                    v = maxNan(v, __shfl_xor_sync(kFullMask, v, 1 << d));
             return v;
         }
 
@@ -199,15 +202,15 @@ namespace a3b
         __device__ __forceinline__ float teamMax(float v, float* room)
         {
             if constexpr(L > 0)
-                return lanesMax(v, L);
+                return lanesMax(v, L == 32 ? 5 : L == 16 ? 4 : 3);
             else
             {
-                v = lanesMax(v, 32);
+                v = lanesMax(v, 5);
                 unsigned const warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
                 if(lane == 0)
                     room[warp] = v;
                 __syncthreads();
-                return lanesMax(lane < warps ? room[lane] : 0.f, 32);
+                return lanesMax(lane < warps ? room[lane] : 0.f, 5);
             }
         }
 
@@ -295,6 +298,7 @@ namespace a3b
         {
             using A = Access<T, E>;
             uint32_t const packs = a.n / E;
+            T* total = a.total && live ? static_cast<T*>(a.total) + a.ts.at(row, a.inner, a.one) : nullptr;
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
             for(int p = 0; p < P; ++p)
@@ -307,8 +311,8 @@ namespace a3b
 #pragma unroll
                         for(int e = 0; e < A::pairs; ++e)
                             A::setPair(raw[p], e, add2(A::pair(raw[p], e), A::pair(add[p], e)));
-                        if(a.total && live)
-                            A::store(static_cast<T*>(a.total) + a.ts.at(row, a.inner, a.one) + static_cast<size_t>(k) * E, raw[p]);
+                        if(total)
+                            A::store(total + static_cast<size_t>(k) * E, raw[p]);
                     }
 #pragma unroll
                     for(int e = 0; e < A::pairs; ++e)
@@ -425,7 +429,7 @@ namespace a3b
                 static_assert(E > 1 && (L == 0 || L == 32), "groups lie on neighbouring lanes");
                 auto* out = static_cast<unsigned char*>(a.out) + a.os.at(row, a.inner, a.one);
                 float* scales = a.scales + static_cast<size_t>(row) * a.groups;
-                int const near = static_cast<int>(a.group) / E; // lanes of one group
+                int const near = 31 - __clz(static_cast<int>(a.group) / E); // log2 of the lanes of one group
                 float high = 0.f;
                 if(a.group == 0)
                 {
@@ -454,8 +458,13 @@ namespace a3b
                     float const scale = scaled<A::pairs>(high, a.e5m2, y);
                     if(k < packs && live)
                     {
-                        if(a.group != 0 ? k % near == 0 : k == 0)
-                            scales[a.group != 0 ? k / near : 0] = scale;
+                        if(a.group == 0)
+                        {
+                            if(k == 0)
+                                scales[0] = scale;
+                        }
+                        else if((k & ((1u << near) - 1u)) == 0)
+                            scales[k >> near] = scale;
                         unsigned w[E / 4];
 #pragma unroll
                         for(int e = 0; e < E / 4; ++e)
@@ -621,7 +630,7 @@ namespace a3b
                     v[e] = make_float2(in < a.group && k < a.n ? y(k) : 0.f, 0.f);
                     high = maxNan(high, fabsf(v[e].x));
                 }
-                float const scale = scaled(lanesMax(high, 32), a.e5m2, v);
+                float const scale = scaled(lanesMax(high, 5), a.e5m2, v);
                 if(lane == 0)
                     scales[g] = scale;
 #pragma unroll
