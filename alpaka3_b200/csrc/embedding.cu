@@ -152,12 +152,12 @@ namespace a3b
         int launchLookup(cudaStream_t stream, DeviceProps const* props, LookupArgs a)
         {
             uint32_t const lots = a.n / E;
-            a.shift = teamShift(lots);
+            // four loads under way a lane, unless that leaves SMs with few blocks
+            bool const deep = static_cast<uint64_t>(a.count) * lots >= 16ull * kThreads * static_cast<unsigned>(props->smCount);
+            uint32_t const depth = deep ? 4 : 1;
+            a.shift = teamShift((lots + depth - 1) / depth);
             uint32_t const teams = kThreads >> a.shift, lanes = 1u << a.shift;
-            uint32_t const blocks = (a.count + teams - 1) / teams;
-            // four loads under way a lane, unless that leaves SMs without a block
-            bool const deep = static_cast<uint64_t>(blocks) * ((lots + 4 * lanes - 1) / (4 * lanes)) >= 4u * static_cast<unsigned>(props->smCount);
-            uint32_t const slices = (lots + (deep ? 4 : 1) * lanes - 1) / ((deep ? 4 : 1) * lanes);
+            uint32_t const blocks = (a.count + teams - 1) / teams, slices = (lots + depth * lanes - 1) / (depth * lanes);
             if(slices > 65535)
             {
                 setError("rows of %u elements are more than one launch holds", a.n);
@@ -217,18 +217,31 @@ namespace a3b
         constexpr uint32_t kFillRows = 16; // rows that a block looks for
         constexpr uint32_t kFillLots = 1024; // lots of a block that looks for none
 
-        // lot k of a row without a token: what is added, or zero
-        template<typename U, int E, bool Add>
-        __device__ __forceinline__ void fillLot(SumArgs const& a, uint32_t row, uint32_t k)
+        // Lots of rows without a token: what is added, or zero. place(u, &row, &k) gives the thread's u-th of four; what is
+        // added is loaded for all of them first.
+        template<typename U, int E, bool Add, typename F>
+        __device__ __forceinline__ void fillLots(SumArgs const& a, F&& place)
         {
-            float v[E];
+            uint32_t row[4], k[4];
+            bool in[4];
+            unsigned add[Add ? 4 : 1][Lot<U, E>::words];
 #pragma unroll
-            for(int e = 0; e < E; ++e)
-                v[e] = 0.f;
-            unsigned add[Lot<U, E>::words];
-            if(Add)
-                loadAdd<U, E>(a, row, k * E, add);
-            writeRow<U, E>(a, row, k * E, v, Add ? add : nullptr);
+            for(int u = 0; u < 4; ++u)
+            {
+                in[u] = place(u, row + u, k + u);
+                if(Add && in[u])
+                    loadAdd<U, E>(a, row[u], k[u] * E, add[Add ? u : 0]);
+            }
+#pragma unroll
+            for(int u = 0; u < 4; ++u)
+                if(in[u])
+                {
+                    float v[E];
+#pragma unroll
+                    for(int e = 0; e < E; ++e)
+                        v[e] = 0.f;
+                    writeRow<U, E>(a, row[u], k[u] * E, v, Add ? add[Add ? u : 0] : nullptr);
+                }
         }
 
         // ------------------------------------------------------------------------------------- sorting the tokens
@@ -264,10 +277,14 @@ namespace a3b
                     }
                     return;
                 }
-#pragma unroll
-                for(uint32_t u = 0; u < kFillLots; u += 256)
-                    if(uint32_t const i = (blockIdx.x - ranking) * kFillLots + u + threadIdx.x, row = i / lots; row < a.vocab)
-                        fillLot<U, E, Add>(a, row, i - row * lots);
+                static_assert(kFillLots == 4 * 256);
+                fillLots<U, E, Add>(a, [&](int u, uint32_t* row, uint32_t* k)
+                {
+                    uint32_t const i = (blockIdx.x - ranking) * kFillLots + u * 256 + threadIdx.x;
+                    *row = i / lots;
+                    *k = i - *row * lots;
+                    return *row < a.vocab;
+                });
                 return;
             }
             if(blockIdx.x == 0 && threadIdx.x == 0)
@@ -570,7 +587,9 @@ namespace a3b
             if(blockIdx.x >= a.sumBlocks)
             {
                 __shared__ bool present[kFillRows];
-                uint32_t const base = (blockIdx.x - a.sumBlocks) * kFillRows;
+                // a block has kFillRows rows and four lots a thread of each
+                uint32_t const parts = (a.n / E + 4 * kThreads - 1) / (4 * kThreads), block = blockIdx.x - a.sumBlocks;
+                uint32_t const base = block / parts * kFillRows, first = block % parts * (4 * kThreads) + threadIdx.x;
                 if(threadIdx.x < kFillRows)
                     present[threadIdx.x] = false;
                 // Where the keys of these rows begin and end in the list: both searched by all threads together, 128 parts a
@@ -610,8 +629,12 @@ namespace a3b
                 __syncthreads();
                 for(uint32_t r = 0; r < min(kFillRows, a.vocab - base); ++r)
                     if(!present[r])
-                        for(uint32_t k = threadIdx.x; k < a.n / E; k += kThreads)
-                            fillLot<U, E, Add>(a, base + r, k);
+                        fillLots<U, E, Add>(a, [&](int u, uint32_t* row, uint32_t* k)
+                        {
+                            *row = base + r;
+                            *k = first + u * kThreads;
+                            return *k < a.n / E;
+                        });
                 return;
             }
             uint32_t const lanes = 1u << a.shift, lane = threadIdx.x & (lanes - 1u);
@@ -874,7 +897,7 @@ namespace a3b
             uint32_t const lanes = 1u << a.shift, teams = kThreads >> a.shift;
             a.slices = (lots + lanes - 1) / lanes;
             uint64_t const sums = static_cast<uint64_t>((a.chunks + teams - 1) / teams) * a.slices;
-            uint64_t fills = a.fill ? (a.vocab + kFillRows - 1) / kFillRows : 0;
+            uint64_t fills = a.fill ? static_cast<uint64_t>((a.vocab + kFillRows - 1) / kFillRows) * ((lots + 4 * kThreads - 1) / (4 * kThreads)) : 0;
             if(a.count > 0 && a.count <= kRankMax)
             {
                 uint32_t const ranking = (a.count + 31) / 32;

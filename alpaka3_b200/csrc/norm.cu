@@ -534,14 +534,19 @@ namespace a3b
         // Rows that no team holds (longer than 32768 16-bit or 16384 32-bit elements), and 8-bit outputs of rows without
         // 16-byte packs: one block a row, which goes over it two to four times, element by element; the later passes
         // find it in L2.
-        constexpr int kLongThreads = 512;
+        constexpr uint32_t kLongThreads = 1024; // at most; about eight elements a thread and pass otherwise
+
+        uint32_t longThreads(uint32_t n)
+        {
+            return std::min(kLongThreads, std::max(32u, (n / 8 + 31) / 32 * 32));
+        }
 
         template<typename T, typename WT>
         __global__ void __launch_bounds__(kLongThreads) rmsNormLongKernel(NormArgs a, int kind) // kind: 0 T, 1 8 bits
         {
             __shared__ float roomF[32], roomM[32];
             __shared__ double roomD[32];
-            uint32_t const row = blockIdx.x, t = threadIdx.x;
+            uint32_t const row = blockIdx.x, t = threadIdx.x, threads = blockDim.x;
             T const* x = static_cast<T const*>(a.x) + a.xs.at(row, a.inner, a.one);
             T const* add = a.residual ? static_cast<T const*>(a.residual) + a.rs.at(row, a.inner, a.one) : nullptr;
             T* total = a.total ? static_cast<T*>(a.total) + a.ts.at(row, a.inner, a.one) : nullptr;
@@ -555,8 +560,8 @@ namespace a3b
                 return add ? toFloat(fromFloat<T>(v + toFloat(add[k]))) : v;
             };
             float sum = 0.f;
-#pragma unroll 4
-            for(uint32_t k = t; k < a.n; k += kLongThreads)
+#pragma unroll 8
+            for(uint32_t k = t; k < a.n; k += threads)
             {
                 float v = toFloat(x[k]);
                 if(add)
@@ -573,7 +578,7 @@ namespace a3b
             if(sumLost(sum, a.tiny))
             {
                 double wide = 0.;
-                for(uint32_t k = t; k < a.n; k += kLongThreads)
+                for(uint32_t k = t; k < a.n; k += threads)
                 {
                     double const v = value(k);
                     wide = fma(v, v, wide);
@@ -593,7 +598,7 @@ namespace a3b
             {
                 T* out = static_cast<T*>(a.out) + a.os.at(row, a.inner, a.one);
 #pragma unroll 4
-                for(uint32_t k = t; k < a.n; k += kLongThreads)
+                for(uint32_t k = t; k < a.n; k += threads)
                     out[k] = fromFloat<T>(y(k));
                 return;
             }
@@ -603,11 +608,11 @@ namespace a3b
             {
                 float high = 0.f;
 #pragma unroll 4
-                for(uint32_t k = t; k < a.n; k += kLongThreads)
+                for(uint32_t k = t; k < a.n; k += threads)
                     high = maxNan(high, fabsf(y(k)));
                 high = teamMax<0>(high, roomM);
 #pragma unroll 4
-                for(uint32_t k = t; k < a.n; k += kLongThreads)
+                for(uint32_t k = t; k < a.n; k += threads)
                 {
                     float2 v[1] = {make_float2(y(k), 0.f)};
                     float const scale = scaled(high, a.e5m2, v);
@@ -619,7 +624,7 @@ namespace a3b
             }
             // a warp takes a group of 32, 64 or 128 elements
             uint32_t const warp = t / 32, lane = t % 32;
-            for(uint32_t g = warp; g < a.groups; g += kLongThreads / 32)
+            for(uint32_t g = warp; g < a.groups; g += threads / 32)
             {
                 float2 v[4];
                 float high = 0.f;
@@ -683,7 +688,7 @@ namespace a3b
                 else if(packs <= 4096)
                     rmsNormKernel<T, WT, E, 4, 0, F8><<<a.rows, roundUp((packs + 3) / 4, 32), 0, stream>>>(a);
                 else
-                    rmsNormLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a, F8);
+                    rmsNormLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a, F8);
             }
             else if constexpr(!F8)
             {
@@ -692,10 +697,10 @@ namespace a3b
                 else if(a.n <= 16384)
                     rmsNormKernel<T, WT, 1, 16, 0, false><<<a.rows, roundUp((a.n + 15) / 16, 32), 0, stream>>>(a);
                 else
-                    rmsNormLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a, 0);
+                    rmsNormLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a, 0);
             }
             else
-                rmsNormLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a, 1);
+                rmsNormLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a, 1);
             A3B_CHECK_LAUNCH("rmsNormKernel");
             return A3B_OK;
         }
@@ -857,7 +862,7 @@ namespace a3b
         __global__ void __launch_bounds__(kLongThreads) rmsNormBackwardLongKernel(NormBackArgs a)
         {
             __shared__ float roomF[32];
-            uint32_t const row = blockIdx.x, t = threadIdx.x;
+            uint32_t const row = blockIdx.x, t = threadIdx.x, threads = blockDim.x;
             T const* g = static_cast<T const*>(a.g) + a.gs.at(row, a.inner, a.one);
             T const* x = static_cast<T const*>(a.x) + a.xs.at(row, a.inner, a.one);
             T const* gt = a.gtotal ? static_cast<T const*>(a.gtotal) + a.ts.at(row, a.inner, a.one) : nullptr;
@@ -865,12 +870,12 @@ namespace a3b
             WT const* weight = static_cast<WT const*>(a.weight);
             float const r = a.rstd[row];
             float c = 0.f;
-#pragma unroll 4
-            for(uint32_t k = t; k < a.n; k += kLongThreads)
+#pragma unroll 8
+            for(uint32_t k = t; k < a.n; k += threads)
                 c = fmaf(toFloat(g[k]) * (weight ? toFloat(weight[k]) : 1.f), toFloat(x[k]) * r, c);
             c = teamSum<0>(c, roomF) * a.inverse;
-#pragma unroll 4
-            for(uint32_t k = t; k < a.n; k += kLongThreads)
+#pragma unroll 8
+            for(uint32_t k = t; k < a.n; k += threads)
             {
                 float const d = r * fmaf(-toFloat(x[k]) * r, c, toFloat(g[k]) * (weight ? toFloat(weight[k]) : 1.f));
                 gx[k] = fromFloat<T>(gt ? d + toFloat(gt[k]) : d);
@@ -965,10 +970,10 @@ namespace a3b
                 blocks = launchBackwardTeams<T, WT, 1, 16, 0>(stream, props, a);
             else
             {
-                blocks = std::min<uint32_t>(partialRows(props, a.rows), 64);
+                blocks = std::min(64u, std::max(1u, a.rows / 64)); // eight rows a warp and more
                 if(a.partial)
                     rmsNormWeightKernel<T><<<dim3((a.n + 31) / 32, blocks), 256, 0, stream>>>(a);
-                rmsNormBackwardLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a);
+                rmsNormBackwardLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a);
             }
             A3B_CHECK_LAUNCH("rmsNormBackwardKernel");
             if(a.partial)
