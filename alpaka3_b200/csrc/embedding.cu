@@ -6,7 +6,8 @@
 // stay in their order), then sums the sorted list in chunks of a fixed number of positions, whatever the tokens are: a token
 // that fills half of a batch is as well spread over the SMs as many rare ones. A run of one token within a chunk goes
 // straight to its row; one that crosses chunks leaves partial sums that a last kernel joins in order. So the bits depend on
-// the sizes alone, never on which block comes first.
+// the sizes alone, never on which block comes first. The kernels of a call follow one another by dependent launches: 65536
+// tokens 105 us in a stream, 113 without; 512 27, without 31.
 #include <algorithm>
 
 #include "layout.cuh"
@@ -256,6 +257,7 @@ namespace a3b
         __global__ void __launch_bounds__(256) rankKernel(Tokens tokens, uint32_t count, uint32_t* keys, uint32_t* places, SumArgs a)
         {
             uint32_t const ranking = (count + 31) / 32;
+            signalNext();
             if(blockIdx.x >= ranking)
             {
                 uint32_t const lots = a.n / E;
@@ -348,6 +350,7 @@ namespace a3b
             auto& sh = *reinterpret_cast<ClusterSort*>(memory);
             uint32_t const t = threadIdx.x, warp = t / 32, lane = t % 32, rank = clusterRank(), bins = 1u << bits;
             uint32_t const own = kSortThreads << log2Each, span = own / kSortWarps; // tokens of a block and of a warp
+            signalNext();
             if(rank == 0 && t == 0)
                 *runs = 0;
             // A warp reads its own part in its own order, here and below.
@@ -474,7 +477,10 @@ namespace a3b
             __shared__ uint32_t bin[kBins];
             for(uint32_t b = threadIdx.x; b < kBins; b += 256)
                 bin[b] = 0;
-            if(a.initial && blockIdx.x == 0 && threadIdx.x == 0)
+            signalNext();
+            if(!a.initial)
+                waitForPrevious();
+            else if(blockIdx.x == 0 && threadIdx.x == 0)
                 *a.runs = 0;
             __syncthreads();
             uint32_t const low = blockIdx.x * a.tile, high = min(low + a.tile, a.count);
@@ -489,6 +495,8 @@ namespace a3b
         __global__ void __launch_bounds__(128) radixScanKernel(uint32_t* counts, uint32_t* totals, uint32_t tiles, uint32_t bins)
         {
             uint32_t const b = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
+            signalNext();
+            waitForPrevious();
             if(b >= bins)
                 return;
             uint32_t* row = counts + static_cast<size_t>(b) * tiles;
@@ -519,6 +527,8 @@ namespace a3b
             uint32_t const t = threadIdx.x, warp = t / 32, lane = t % 32, bins = 1u << a.bits;
             for(uint32_t k = t; k < kTileWarps * kBins; k += 256)
                 at[k / kBins][k % kBins] = 0;
+            signalNext();
+            waitForPrevious();
             __syncthreads();
             uint32_t const span = a.tile / kTileWarps, low = min(blockIdx.x * a.tile + warp * span, a.count),
                            high = min(low + span, a.count);
@@ -584,6 +594,11 @@ namespace a3b
         __global__ void __launch_bounds__(kThreads) embeddingSumKernel(SumArgs a)
         {
             constexpr int kAhead = 4;
+            // The kernel that joins; behind many tokens its waiting blocks take the sums' place (1 us of 39 at 16384 x 1024).
+            if(a.chunks > 1 && a.count <= kRankMax)
+                signalNext();
+            if(a.count > 0)
+                waitForPrevious(); // the sort
             if(blockIdx.x >= a.sumBlocks)
             {
                 __shared__ bool present[kFillRows];
@@ -723,6 +738,7 @@ namespace a3b
         __global__ void __launch_bounds__(256) embeddingJoinKernel(SumArgs a)
         {
             __shared__ float4 part[8][32];
+            waitForPrevious();
             uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32, slices = (a.n + 127) / 128, runs = a.runs[0];
             uint32_t const runStep = gridDim.x / slices, sliceStep = gridDim.x % slices; // items in steps of the grid
             for(uint32_t run = blockIdx.x / slices, slice = blockIdx.x % slices; run < runs; run += runStep, slice += sliceStep)
@@ -879,12 +895,20 @@ namespace a3b
                     std::swap(*keys, otherKeys);
                     std::swap(*places, otherPlaces);
                 }
-                radixCountKernel<<<p.tiles, 256, 0, stream>>>(a);
-                A3B_CHECK_LAUNCH("radixCountKernel");
-                radixScanKernel<<<((1u << p.bits) + 3) / 4, 128, 0, stream>>>(a.counts, a.totals, p.tiles, 1u << p.bits);
-                A3B_CHECK_LAUNCH("radixScanKernel");
-                radixPlaceKernel<<<p.tiles, 32 * kTileWarps, 0, stream>>>(a);
-                A3B_CHECK_LAUNCH("radixPlaceKernel");
+                int rc = A3B_OK;
+                if(d > 0)
+                    rc = launchNext(stream, radixCountKernel, p.tiles, 256, 0, a);
+                else
+                {
+                    radixCountKernel<<<p.tiles, 256, 0, stream>>>(a);
+                    A3B_CHECK_LAUNCH("radixCountKernel");
+                }
+                if(rc == A3B_OK)
+                    rc = launchNext(stream, radixScanKernel, ((1u << p.bits) + 3) / 4, 128, 0, a.counts, a.totals, p.tiles, 1u << p.bits);
+                if(rc == A3B_OK)
+                    rc = launchNext(stream, radixPlaceKernel, p.tiles, 32 * kTileWarps, 0, a);
+                if(rc != A3B_OK)
+                    return rc;
             }
             return A3B_OK;
         }
@@ -920,23 +944,22 @@ namespace a3b
             if(sums + fills == 0)
                 return A3B_OK;
             auto const grid = static_cast<unsigned>(sums + fills);
-            if(a.add)
-                embeddingSumKernel<T, U, E, true><<<grid, kThreads, 0, stream>>>(a);
-            else
-                embeddingSumKernel<T, U, E, false><<<grid, kThreads, 0, stream>>>(a);
-            A3B_CHECK_LAUNCH("embeddingSumKernel");
-            if(a.chunks > 1)
+            auto kernel = a.add ? embeddingSumKernel<T, U, E, true> : embeddingSumKernel<T, U, E, false>;
+            if(a.count == 0)
+            {
+                kernel<<<grid, kThreads, 0, stream>>>(a);
+                A3B_CHECK_LAUNCH("embeddingSumKernel");
+                return A3B_OK;
+            }
+            int const rc = launchNext(stream, kernel, grid, kThreads, 0, a);
+            if(rc == A3B_OK && a.chunks > 1)
             {
                 // as many blocks as SMs hold, or runs and columns there can be
                 uint64_t const items = static_cast<uint64_t>(a.chunks - 1) * ((a.n + 127) / 128);
                 auto const blocks = static_cast<unsigned>(std::min<uint64_t>(8ull * static_cast<unsigned>(props->smCount), items));
-                if(a.n % 4 == 0)
-                    embeddingJoinKernel<U, true><<<blocks, 256, 0, stream>>>(a);
-                else
-                    embeddingJoinKernel<U, false><<<blocks, 256, 0, stream>>>(a);
-                A3B_CHECK_LAUNCH("embeddingJoinKernel");
+                return launchNext(stream, a.n % 4 == 0 ? embeddingJoinKernel<U, true> : embeddingJoinKernel<U, false>, blocks, 256, 0, a);
             }
-            return A3B_OK;
+            return rc;
         }
 
         // Calls f(T{}, U{}) for the two types; f32, f16 and bf16 with themselves, and f32 with the 16-bit ones.

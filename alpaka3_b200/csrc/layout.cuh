@@ -126,6 +126,35 @@ namespace a3b
         return true;
     }
 
+    // Launches a kernel that begins with waitForPrevious() right behind one that calls signalNext(): its blocks may start while
+    // the other's last ones run. Only for kernels of one call: the first of a call is launched in full order, and the last
+    // signals nothing, so that nothing of another call starts early.
+    template<typename... Parameters, typename... Args>
+    int launchNext(cudaStream_t stream, void (*kernel)(Parameters...), dim3 grid, unsigned threads, size_t shared, Args const&... args)
+    {
+        cudaLaunchAttribute attribute{};
+        attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attribute.val.programmaticStreamSerializationAllowed = 1;
+        cudaLaunchConfig_t config{};
+        config.gridDim = grid;
+        config.blockDim = dim3(threads);
+        config.dynamicSmemBytes = shared;
+        config.stream = stream;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        A3B_CUDA(cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(args)...));
+        return A3B_OK;
+    }
+
+    __device__ __forceinline__ void waitForPrevious()
+    {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+    }
+    __device__ __forceinline__ void signalNext()
+    {
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
+
     // bytes of an element of a floating-point type that rows may have; 0 for every other type
     inline int rowTypeSize(int dtype)
     {

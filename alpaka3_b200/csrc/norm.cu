@@ -854,7 +854,10 @@ namespace a3b
                     }
             }
             if(a.partial)
+            {
+                signalNext(); // the fold
                 addTeams<E, P>(a, dw, sums, teams, mine, lanes, t);
+            }
         }
 
         // Rows that no team holds: two passes over the row for its gradient ...
@@ -915,6 +918,7 @@ namespace a3b
         {
             __shared__ float part[32][33];
             uint32_t const lane = threadIdx.x % 32, warp = threadIdx.x / 32, k = blockIdx.x * 32 + lane;
+            waitForPrevious();
             float s = 0.f;
             if(k < n)
 #pragma unroll 10
@@ -978,8 +982,7 @@ namespace a3b
             A3B_CHECK_LAUNCH("rmsNormBackwardKernel");
             if(a.partial)
             {
-                rmsNormFoldKernel<WT><<<(a.n + 31) / 32, 1024, 0, stream>>>(a.partial, blocks, a.n, gw);
-                A3B_CHECK_LAUNCH("rmsNormFoldKernel");
+                return launchNext(stream, rmsNormFoldKernel<WT>, dim3((a.n + 31) / 32), 1024, 0, a.partial, blocks, a.n, gw);
             }
             return A3B_OK;
         }
