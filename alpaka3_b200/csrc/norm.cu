@@ -720,21 +720,35 @@ namespace a3b
             float* partial; // one row of n sums a block; null: no gradient of the weight
             float inverse; // 1 / n
             uint32_t team; // threads of a team
+            void* gw; // a single block writes the weight's gradient itself; else null
         };
 
-        // The block's row of partial sums from its teams', added in the teams' order: the same bits every time.
-        template<int E, int P>
+        // The block's row of partial sums (or the weight's gradient, if it is the only block) from its teams', added in the
+        // teams' order: the same bits every time.
+        template<typename WT, int E, int P>
         __device__ __forceinline__ void addTeams(NormBackArgs const& a, float2 const (&dw)[P][E == 1 ? 1 : E / 2], float* sums,
                                                  uint32_t teams, uint32_t mine, uint32_t lanes, uint32_t t)
         {
             float* partial = a.partial + static_cast<size_t>(blockIdx.x) * a.n;
-            float* to = teams == 1 ? partial : sums + mine * a.n;
+            auto put = [&](uint32_t k, float v)
+            {
+                if(a.gw)
+                    static_cast<WT*>(a.gw)[k] = fromFloat<WT>(v);
+                else
+                    partial[k] = v;
+            };
 #pragma unroll
             for(int p = 0; p < P; ++p)
                 if(uint32_t const k = p * lanes + t; k < a.n / E)
 #pragma unroll
                     for(int e = 0; e < E; ++e)
-                        to[static_cast<size_t>(k) * E + e] = e % 2 ? dw[p][e / 2].y : dw[p][e / 2].x;
+                    {
+                        float const v = e % 2 ? dw[p][e / 2].y : dw[p][e / 2].x;
+                        if(teams == 1)
+                            put(k * E + e, v);
+                        else
+                            sums[mine * a.n + k * E + e] = v;
+                    }
             if(teams == 1)
                 return;
             __syncthreads();
@@ -744,7 +758,7 @@ namespace a3b
 #pragma unroll 4
                 for(uint32_t of = 1; of < teams; ++of)
                     v += sums[of * a.n + k];
-                partial[k] = v;
+                put(k, v);
             }
         }
 
@@ -855,8 +869,9 @@ namespace a3b
             }
             if(a.partial)
             {
-                signalNext(); // the fold
-                addTeams<E, P>(a, dw, sums, teams, mine, lanes, t);
+                if(!a.gw)
+                    signalNext(); // the fold
+                addTeams<WT, E, P>(a, dw, sums, teams, mine, lanes, t);
             }
         }
 
@@ -937,19 +952,25 @@ namespace a3b
             return static_cast<uint32_t>(std::min<uint64_t>(rows, 4ull * static_cast<unsigned>(props->smCount)));
         }
 
+        // How many rows of partial sums the fold has to add; none when a single block wrote the weight's gradient.
         template<typename T, typename WT, int E, int P, int L>
-        uint32_t launchBackwardTeams(cudaStream_t stream, DeviceProps const* props, NormBackArgs a)
+        uint32_t launchBackwardTeams(cudaStream_t stream, DeviceProps const* props, NormBackArgs a, WT* gw)
         {
             auto const sms = static_cast<uint32_t>(props->smCount);
             a.team = L > 0 ? L : roundUp((a.n / E + P - 1) / P, 32);
-            // teams side by side in a block, unless SMs would go without
-            uint32_t const teams = std::max(1u, std::min(512 / a.team, L > 0 ? 512u / a.team : a.rows / sms));
+            // Teams side by side in a block, unless SMs would go without. Rows that one block takes in one turn are left to it: it
+            // needs no fold (1 x 4096 bf16 3.9 us, with two launches 5.6; with a second turn 6.7 against 5.7).
+            uint32_t const most = 512 / a.team;
+            bool const single = gw && a.rows <= most;
+            uint32_t const teams = std::max(1u, std::min(most, L > 0 ? most : single ? a.rows : a.rows / sms));
             uint32_t const threads = teams * a.team, resident = std::max(1u, (P <= 2 ? 1024u : 512u) / threads);
-            uint32_t const blocks = std::min({(a.rows + teams - 1) / teams, sms * resident, partialRows(props, a.rows)});
+            uint32_t const blocks
+                = single ? 1 : std::min({(a.rows + teams - 1) / teams, sms * resident, partialRows(props, a.rows)});
+            a.gw = single ? gw : nullptr;
             // a row of sums for each team: at most threads * P * E values, 32 KB
             size_t const sums = a.partial && teams > 1 ? teams * a.n * sizeof(float) : 0;
             rmsNormBackwardKernel<T, WT, E, P, L><<<blocks, threads, sums, stream>>>(a);
-            return blocks;
+            return single ? 0 : blocks;
         }
 
         template<typename T, typename WT>
@@ -959,19 +980,19 @@ namespace a3b
             uint32_t const packs = packed ? a.n / E : a.n;
             uint32_t blocks = 0;
             if(packed && packs <= 16)
-                blocks = launchBackwardTeams<T, WT, E, 2, 8>(stream, props, a);
+                blocks = launchBackwardTeams<T, WT, E, 2, 8>(stream, props, a, gw);
             else if(packed && packs <= 32)
-                blocks = launchBackwardTeams<T, WT, E, 2, 16>(stream, props, a);
+                blocks = launchBackwardTeams<T, WT, E, 2, 16>(stream, props, a, gw);
             else if(packed && packs <= 64)
-                blocks = launchBackwardTeams<T, WT, E, 2, 32>(stream, props, a);
+                blocks = launchBackwardTeams<T, WT, E, 2, 32>(stream, props, a, gw);
             else if(packed && packs <= 1024)
-                blocks = launchBackwardTeams<T, WT, E, 2, 0>(stream, props, a);
+                blocks = launchBackwardTeams<T, WT, E, 2, 0>(stream, props, a, gw);
             else if(packed && packs <= 2048)
-                blocks = launchBackwardTeams<T, WT, E, 4, 0>(stream, props, a);
+                blocks = launchBackwardTeams<T, WT, E, 4, 0>(stream, props, a, gw);
             else if(!packed && packs <= 2048)
-                blocks = launchBackwardTeams<T, WT, 1, 4, 0>(stream, props, a);
+                blocks = launchBackwardTeams<T, WT, 1, 4, 0>(stream, props, a, gw);
             else if(!packed && packs <= 8192)
-                blocks = launchBackwardTeams<T, WT, 1, 16, 0>(stream, props, a);
+                blocks = launchBackwardTeams<T, WT, 1, 16, 0>(stream, props, a, gw);
             else
             {
                 blocks = std::min(64u, std::max(1u, a.rows / 64)); // eight rows a warp and more
@@ -980,7 +1001,7 @@ namespace a3b
                 rmsNormBackwardLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a);
             }
             A3B_CHECK_LAUNCH("rmsNormBackwardKernel");
-            if(a.partial)
+            if(a.partial && blocks > 0)
             {
                 return launchNext(stream, rmsNormFoldKernel<WT>, dim3((a.n + 31) / 32), 1024, 0, a.partial, blocks, a.n, gw);
             }
@@ -1166,7 +1187,7 @@ extern "C"
                        {x.outer_stride, x.inner_stride}, {grad_total.outer_stride, grad_total.inner_stride},
                        {grad_x.outer_stride, grad_x.inner_stride}, static_cast<uint32_t>(rows), static_cast<uint32_t>(inner),
                        static_cast<uint32_t>(n), outer == 1, weight, rstd,
-                       grad_weight ? static_cast<float*>(workspace) : nullptr, 1.f / static_cast<float>(n), 0u};
+                       grad_weight ? static_cast<float*>(workspace) : nullptr, 1.f / static_cast<float>(n), 0u, nullptr};
         bool const wide = ws == 4;
         if(dtype == A3B_F32)
             return launchNormBackward<float, float>(s, props, a, packed, static_cast<float*>(grad_weight));

@@ -271,6 +271,17 @@ def test_backward_against_64_bits(cuda, dtype, n):
     check_backward(g, x, None)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [24, 100, 128, 500, 1001, 1024, 4096, 8192])
+def test_backward_of_few_rows(cuda, dtype, n):
+    """As many rows as one block takes in one turn, which then leaves no partial sums, and one fewer and more."""
+    for rows in {r + k for r in (1, 2, 4, 8, 16, 32, 64) for k in (-1, 0, 1)} - {0}:
+        x, g = make((rows, n), dtype, n + rows, 2.0), make((rows, n), dtype, n, 0.1)
+        w = make((n,), torch.float32, n).add_(1)
+        check_backward(g, x, w.to(dtype), make((rows, n), dtype, 3, 0.1))
+        check_backward(g, x, w)
+
+
 def test_many_rows(cuda):
     for n, rows, dtype in ((128, 40001, torch.bfloat16), (64, 70000, torch.float32), (1024, 5000, torch.float16),
                            (2048, 3001, torch.bfloat16), (1001, 2000, torch.float32), (35001, 600, torch.bfloat16)):
