@@ -717,14 +717,28 @@ def _token_rows(t, tokens, dev, table, tcode, name):
             _per_row(tokens, "tokens", outer * inner, dev, _INDEX_DT))
 
 
+def _lookup(table, table_name, rows, name, tokens):
+    """(device index, dtype code and row stride of the table, and what _token_rows gives) of rows, their tokens and the table"""
+    dev = table.get_device()
+    shape = table.shape
+    # The usual call, told by one question after the other; any other answer goes the long way, which also says what is wrong.
+    if len(shape) == 2 and shape[1] and rows.is_contiguous() and tokens.is_contiguous() and table.is_contiguous():
+        code, tcode, index = _LOGITS_DT.get(rows.dtype), _LOGITS_DT.get(table.dtype), _INDEX_DT.get(tokens.dtype)
+        if (code is not None and tcode is not None and index is not None and dev >= 0 and rows.get_device() == dev
+                and tokens.get_device() == dev and (code == tcode or code == capi.F32 or tcode == capi.F32)
+                and rows.shape == tokens.shape + shape[1:]):
+            n = shape[1]
+            return dev, tcode, n, code, 1, tokens.numel(), n, 0, n, index, tokens.data_ptr()
+    tcode, stride = _table(table, table_name, dev)
+    return dev, tcode, stride, *_token_rows(rows, tokens, dev, table, tcode, name)
+
+
 def embedding(out, weight, tokens, scale=1.0, first=0, stream=None):
     """out[...] = scale * weight[tokens[...] - first], one row of the table `weight` (rows, n) for each token (int64 or
     int32, contiguous, any shape; out: that shape and n). A token outside [first, first + rows) gives a row of zeros: padding
     such as -100, or the tokens of other ranks where the table is cut over ranks. Types: float32 / float16 / bfloat16, both
     alike or one of them float32. Rows may be strided. Returns out."""
-    dev = weight.get_device()
-    tcode, stride = _table(weight, "weight", dev)
-    code, outer, inner, n, so, si, index, at = _token_rows(out, tokens, dev, weight, tcode, "out")
+    dev, tcode, stride, code, outer, inner, n, so, si, index, at = _lookup(weight, "weight", out, "out", tokens)
     _call_on(dev, stream, "a3b_embedding",
              capi.EMBEDDING_ARGS.pack(outer, inner, n, weight.shape[0], first, weight.data_ptr(), stride, at, out.data_ptr(),
                                       so, si, scale, tcode, index, code, 0))
@@ -736,9 +750,8 @@ def embedding_backward(grad_weight, grad_out, tokens, scale=1.0, add=None, first
     `add`) plus scale times the sum of grad_out's rows over the places of its token. `add` has the dtype and shape of
     grad_weight (the gradient from the table's use as a head); it may be grad_weight itself, of which then only rows of
     tokens that occur are touched. The same bits in every call. Returns grad_weight."""
-    dev = grad_weight.get_device()
-    tcode, stride = _table(grad_weight, "grad_weight", dev)
-    code, outer, inner, n, so, si, index, at = _token_rows(grad_out, tokens, dev, grad_weight, tcode, "grad_out")
+    dev, tcode, stride, code, outer, inner, n, so, si, index, at = _lookup(grad_weight, "grad_weight", grad_out, "grad_out",
+                                                                           tokens)
     more = more_stride = 0
     if add is not None:
         acode, more_stride = _table(add, "add", dev)
