@@ -833,11 +833,16 @@ namespace a3b
                 else
                 {
                     c = lanesSum<32>(c);
-                    uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = lanes / 32;
-                    if(lane == 0)
-                        room[turn & 1][warp] = c;
-                    asm volatile("bar.sync %0, %1;" ::"r"(mine + 1u), "r"(lanes) : "memory");
-                    c = lanesSum<32>(lane < warps ? room[turn & 1][mine * warps + lane] : 0.f);
+                    // A team of several warps has a barrier of its own, 1 to 8 (there are 16, of which the block's is 0); one
+                    // of a single warp, up to sixteen in a block, has its sum.
+                    if(lanes > 32)
+                    {
+                        uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = lanes / 32;
+                        if(lane == 0)
+                            room[turn & 1][warp] = c;
+                        asm volatile("bar.sync %0, %1;" ::"r"(mine + 1u), "r"(lanes) : "memory");
+                        c = lanesSum<32>(lane < warps ? room[turn & 1][mine * warps + lane] : 0.f);
+                    }
                 }
                 c *= a.inverse;
                 if(!live)

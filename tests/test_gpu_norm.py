@@ -282,6 +282,19 @@ def test_backward_of_few_rows(cuda, dtype, n):
         check_backward(g, x, w)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 7, 31, 100, 126, 128])
+def test_backward_of_many_short_rows(cuda, dtype, n):
+    """Rows without packs, of one warp each, sixteen in a block: in one turn and in several."""
+    for rows in (16, 3001, 12000):
+        wide = make((rows, n + 1), dtype, n)
+        x, g = wide[:, 1:], make((rows, n), dtype, n + 1, 0.1)
+        w = make((n,), torch.float32, n).add_(1)
+        for _ in range(4):
+            check_backward(g, x, w.to(dtype), make((rows, n), dtype, 3, 0.1))
+            check_backward(g, x, w)
+
+
 def test_many_rows(cuda):
     for n, rows, dtype in ((128, 40001, torch.bfloat16), (64, 70000, torch.float32), (1024, 5000, torch.float16),
                            (2048, 3001, torch.bfloat16), (1001, 2000, torch.float32), (35001, 600, torch.bfloat16)):
