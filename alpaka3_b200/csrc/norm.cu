@@ -833,16 +833,12 @@ namespace a3b
                 else
                 {
                     c = lanesSum<32>(c);
-                    // A team of several warps has a barrier of its own, 1 to 8 (there are 16, of which the block's is 0); one
-                    // of a single warp, up to sixteen in a block, has its sum.
-                    if(lanes > 32)
-                    {
-                        uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = lanes / 32;
-                        if(lane == 0)
-                            room[turn & 1][warp] = c;
-                        asm volatile("bar.sync %0, %1;" ::"r"(mine + 1u), "r"(lanes) : "memory");
-                        c = lanesSum<32>(lane < warps ? room[turn & 1][mine * warps + lane] : 0.f);
-                    }
+                    uint32_t const warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = lanes / 32;
+                    if(lane == 0)
+                        room[turn & 1][warp] = c;
+                    // A barrier for each team, 1 to 8, since one has two warps or more (there are 16 barriers, the block's is 0).
+                    asm volatile("bar.sync %0, %1;" ::"r"(mine + 1u), "r"(lanes) : "memory");
+                    c = lanesSum<32>(lane < warps ? room[turn & 1][mine * warps + lane] : 0.f);
                 }
                 c *= a.inverse;
                 if(!live)
@@ -962,7 +958,7 @@ namespace a3b
         uint32_t launchBackwardTeams(cudaStream_t stream, DeviceProps const* props, NormBackArgs a, WT* gw)
         {
             auto const sms = static_cast<uint32_t>(props->smCount);
-            a.team = L > 0 ? L : roundUp((a.n / E + P - 1) / P, 32);
+            a.team = L > 0 ? L : std::max(64u, roundUp((a.n / E + P - 1) / P, 32)); // several warps: a barrier each
             // Teams side by side in a block, unless SMs would go without. Rows that one block takes in one turn are left to it: it
             // needs no fold (1 x 4096 bf16 3.9 us, with two launches 5.6; with a second turn 6.7 against 5.7).
             uint32_t const most = 512 / a.team;
@@ -994,6 +990,8 @@ namespace a3b
                 blocks = launchBackwardTeams<T, WT, E, 2, 0>(stream, props, a, gw);
             else if(packed && packs <= 2048)
                 blocks = launchBackwardTeams<T, WT, E, 4, 0>(stream, props, a, gw);
+            else if(!packed && packs <= 128) // a warp, without a barrier (29861 x 101 bf16 16.2 us; asking for it in the loop: 17.9)
+                blocks = launchBackwardTeams<T, WT, 1, 4, 32>(stream, props, a, gw);
             else if(!packed && packs <= 2048)
                 blocks = launchBackwardTeams<T, WT, 1, 4, 0>(stream, props, a, gw);
             else if(!packed && packs <= 8192)
