@@ -531,8 +531,146 @@ namespace a3b
             }
         }
 
-        // Rows that no team holds (longer than 32768 16-bit or 16384 32-bit elements), and 8-bit outputs of rows without
-        // 16-byte packs: one block a row, which goes over it two to four times, element by element; the later passes
+        // 8-bit outputs of rows without 16-byte packs: one block a row, in registers by single elements. A warp has Q stretches of
+        // 128 neighbouring elements, four a lane and each 32 apart, so every group of 32, 64 or 128 is one warp's. (By the long
+        // kernel below, a group at a time, 9769 x 2587 bf16 with residual took 290 us; now 95, bound by issue.)
+        template<typename T, typename WT, int Q>
+        __global__ void __launch_bounds__(1024, Q == 1 ? 2 : 1) rmsNormOddKernel(NormArgs a)
+        {
+            __shared__ float roomF[32], roomM[32];
+            __shared__ double roomD[32];
+            uint32_t const row = blockIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+            T const* x = static_cast<T const*>(a.x) + a.xs.at(row, a.inner, a.one);
+            T const* add = a.residual ? static_cast<T const*>(a.residual) + a.rs.at(row, a.inner, a.one) : nullptr;
+            T* total = add && a.total ? static_cast<T*>(a.total) + a.ts.at(row, a.inner, a.one) : nullptr;
+            WT const* weight = static_cast<WT const*>(a.weight);
+            auto at = [&](int q, int e) { return (static_cast<uint32_t>(q) * warps + warp) * 128u + static_cast<uint32_t>(e) * 32u + lane; };
+            float v[Q][4];
+#pragma unroll
+            for(int q = 0; q < Q; ++q)
+#pragma unroll
+                for(int e = 0; e < 4; ++e)
+                {
+                    uint32_t const k = at(q, e);
+                    v[q][e] = k < a.n ? toFloat(x[k]) : 0.f;
+                }
+            if(add)
+#pragma unroll
+                for(int q = 0; q < Q; ++q)
+                {
+                    float other[4];
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                    {
+                        uint32_t const k = at(q, e);
+                        other[e] = k < a.n ? toFloat(add[k]) : 0.f;
+                    }
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                    {
+                        T const h = fromFloat<T>(v[q][e] + other[e]);
+                        if(uint32_t const k = at(q, e); total && k < a.n)
+                            total[k] = h;
+                        v[q][e] = toFloat(h);
+                    }
+                }
+            float sum = 0.f;
+#pragma unroll
+            for(int q = 0; q < Q; ++q)
+#pragma unroll
+                for(int e = 0; e < 4; ++e)
+                    sum = fmaf(v[q][e], v[q][e], sum);
+            sum = teamSum<0>(sum, roomF);
+            float r;
+            if(sumLost(sum, a.tiny))
+            {
+                double wide = 0.;
+#pragma unroll
+                for(int q = 0; q < Q; ++q)
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                        wide = fma(static_cast<double>(v[q][e]), static_cast<double>(v[q][e]), wide);
+                r = rootOf(teamSum<0>(wide, roomD), a.n, a.eps);
+            }
+            else
+                r = rootOf(sum, a.inverse, a.eps32);
+            if(a.rstd && threadIdx.x == 0)
+                a.rstd[row] = r;
+            float high = 0.f;
+#pragma unroll
+            for(int q = 0; q < Q; ++q)
+            {
+                float w[4];
+#pragma unroll
+                for(int e = 0; e < 4; ++e)
+                {
+                    uint32_t const k = at(q, e);
+                    w[e] = weight && k < a.n ? toFloat(weight[k]) : 1.f;
+                }
+#pragma unroll
+                for(int e = 0; e < 4; ++e)
+                {
+                    // beyond the row zero, even where r is infinite or NaN
+                    v[q][e] = at(q, e) < a.n ? v[q][e] * r * w[e] : 0.f;
+                    high = maxNan(high, fabsf(v[q][e]));
+                }
+            }
+            auto* out = static_cast<unsigned char*>(a.out) + a.os.at(row, a.inner, a.one);
+            float* scales = a.scales + static_cast<size_t>(row) * a.groups;
+            if(a.group == 0)
+                high = teamMax<0>(high, roomM);
+#pragma unroll
+            for(int q = 0; q < Q; ++q)
+            {
+                if(at(q, 0) - lane >= a.n) // the same for the warp
+                    continue;
+                float top[4];
+                if(a.group == 0)
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                        top[e] = high;
+                else
+                {
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                        // magnitudes order as their bits do, and NaN is above infinity
+                        top[e] = __uint_as_float(__reduce_max_sync(kFullMask, __float_as_uint(fabsf(v[q][e]))));
+                    if(a.group >= 64)
+                        top[0] = top[1] = maxNan(top[0], top[1]), top[2] = top[3] = maxNan(top[2], top[3]);
+                    if(a.group == 128)
+                        top[0] = top[1] = top[2] = top[3] = maxNan(top[0], top[2]);
+                }
+                float scale[4];
+                float2 y[4];
+#pragma unroll
+                for(int e = 0; e < 4; ++e)
+                    y[e] = make_float2(v[q][e], 0.f);
+                if(a.group == 32)
+#pragma unroll
+                    for(int e = 0; e < 4; ++e)
+                        scale[e] = scaled(top[e], a.e5m2, reinterpret_cast<float2(&)[1]>(y[e]));
+                else
+#pragma unroll
+                    for(int e = 0; e < 4; e += 2)
+                        scale[e] = scale[e + 1] = scaled(top[e], a.e5m2, reinterpret_cast<float2(&)[2]>(y[e]));
+#pragma unroll
+                for(int e = 0; e < 4; ++e)
+                    if(uint32_t const k = at(q, e); k < a.n)
+                    {
+                        if(a.group == 0)
+                        {
+                            if(k == 0)
+                                scales[0] = scale[e];
+                        }
+                        else if((k & (a.group - 1u)) == 0)
+                            scales[k / 32 >> (a.group / 64)] = scale[e]; // k / group: 32, 64 or 128
+                        out[k] = static_cast<unsigned char>(eight(y[e], a.e5m2));
+                    }
+            }
+        }
+
+        // Rows that no team holds (longer than 32768 16-bit or 16384 32-bit elements; without 16-byte packs than 16384, with 8-bit
+        // outputs than 32768): one block a row, which goes over it two to four times, element by element; the later passes
         // find it in L2.
         constexpr uint32_t kLongThreads = 1024; // at most; about eight elements a thread and pass otherwise
 
@@ -700,7 +838,17 @@ namespace a3b
                     rmsNormLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a, 0);
             }
             else
-                rmsNormLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a, 1);
+            {
+                auto threads = [&](uint32_t stretches) { return (a.n + 128 * stretches - 1) / (128 * stretches) * 32; };
+                if(a.n <= 4096) // one stretch a warp, 32 registers (4000 x 4001 fp32 59 us, with two stretches 62)
+                    rmsNormOddKernel<T, WT, 1><<<a.rows, threads(1), 0, stream>>>(a);
+                else if(a.n <= 8192)
+                    rmsNormOddKernel<T, WT, 2><<<a.rows, threads(2), 0, stream>>>(a);
+                else if(a.n <= 32768)
+                    rmsNormOddKernel<T, WT, 8><<<a.rows, threads(8), 0, stream>>>(a);
+                else
+                    rmsNormLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a, 1);
+            }
             A3B_CHECK_LAUNCH("rmsNormKernel");
             return A3B_OK;
         }

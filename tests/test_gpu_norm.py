@@ -120,6 +120,32 @@ def test_eight_bits(cuda, dtype, kind, n):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", list(LARGEST))
+@pytest.mark.parametrize("n", [31, 95, 127, 129, 257, 1001, 4095, 4097, 8191, 8193, 16401, 32767, 32769])
+def test_eight_bits_without_packs(cuda, dtype, kind, n):
+    """Rows of every length at which another form takes over, and ones whose first element lies off 16 bytes; in place."""
+    for rows in (3, 50):
+        wide = make((rows, n + 1), dtype, n + rows, 1.5)
+        x, res, w = wide[:, 1:], make((rows, n), dtype, 3), make((n,), torch.float32, n).add_(1)
+        for group in (None, 32, 64, 128):
+            check_forward(x, w, None, kind, group)
+            check_forward(x, w.to(dtype), res, kind, group)
+        x[0, n // 2:] = 0
+        x[1].mul_(0)
+        a = res.clone()
+        check_forward(x, None, res, kind, 64)
+        check_forward(x, None, a, kind, 64, total=a)
+        check_forward(x, None, None, kind, 32)
+        nan = x.clone()
+        nan[2, n // 3] = math.nan
+        check_forward(nan[:2], w, None, kind, 64)
+        out, scales = torch.zeros(rows, n, dtype=kind, device="cuda"), torch.zeros(rows, -(-n // 64), device="cuda")
+        from alpaka3_b200 import algo
+        algo.rms_norm(out, nan, w, scales=scales, group=64)
+        assert torch.isnan(scales[2]).all() and torch.isnan(out[2].float()).all() and not torch.isnan(scales[:2]).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n", [64, 77, 1024, 4096, 40000])
 def test_zeros_and_empty_groups(cuda, dtype, n):
     from alpaka3_b200 import algo
