@@ -447,3 +447,32 @@ def test_streams_and_graphs(cuda):
     torch.cuda.synchronize()
     for o in outs:
         assert all(torch.equal(a, b) for a, b in zip(o, want))
+
+
+@pytest.mark.parametrize("kind", list(LARGEST))
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,shift", [(64, 0), (512, 0), (2048, 0), (16384, 0), (65536, 0), (256, 1), (4096, 1), (8192, 1), (32768, 1)])
+def test_eight_bits_next_to_a_middle(cuda, kind, dtype, n, shift):
+    """Values that lie in the middle between two of 8 bits, but for the roundings of y / s, where every unit of the scale's
+    reciprocal counts: the bits of y * (1 / s), each operation rounded to the nearest. Rows of +-1 have r = 1, so y is the
+    weight; rows begin at 16 bytes (shift 0) or not."""
+    from alpaka3_b200 import algo
+    top, bits = LARGEST[kind], torch.arange(127, device="cuda", dtype=torch.uint8).view(kind).float()
+    grid = bits[torch.isfinite(bits) & (bits > 0)]
+    middle = (grid[1:] + grid[:-1]) / 2
+    rows = 6
+    x = torch.ones(rows, n + shift, dtype=dtype, device="cuda")[:, shift:]
+    x[:, ::3] = -1
+    for seed, group in enumerate((None, 32, 64, 128)):
+        g = torch.Generator(device="cuda").manual_seed(n + seed)
+        size = min(group or n, n)
+        high = torch.rand(n // size, 1, generator=g, device="cuda") + 1
+        s = high * torch.tensor(1 / top, device="cuda")  # the rounded 1 / top
+        w = middle[torch.randint(len(middle), (n // size, size), generator=g, device="cuda")] * s
+        w[:, size // 2:size // 2 + 1] = high
+        out, scales = torch.zeros(rows, n, dtype=kind, device="cuda"), torch.zeros(rows, n // size, device="cuda")
+        rstd = torch.zeros(rows, device="cuda")
+        algo.rms_norm(out, x, w.flatten(), rstd=rstd, scales=scales, group=group, eps=0.0)
+        assert (rstd == 1).all() and torch.equal(scales, s.flatten().expand(rows, -1))
+        want = (w * (1 / s)).clamp(max=top).to(kind).float().flatten() * x.float()
+        assert torch.equal(out.float(), want)
