@@ -95,6 +95,7 @@ namespace a3b
                 float const a = (*this)(z);
                 float r;
                 asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(noise));
+                r = noise < 0.f ? NAN : r; // no part: two negative factors would make an end that nothing reaches
                 // what flushed to zero counts as up to fp32's least normal numbers
                 float const rate = a - b, wide = fmaf(off, a + b, 0x1p-125f);
                 // fmax drops NaN: an element with one takes no part
@@ -108,10 +109,19 @@ namespace a3b
             return exp(scale * static_cast<double>(z) - static_cast<double>(lse));
         }
 
+        // The scores of a row without a rate, and of one with rates but no noise they could be divided by; what can be drawn has
+        // a score of 0 or more.
+        constexpr double kNoRate = -1., kNoClock = -0.5;
+
         struct Best
         {
             double score;
             uint32_t index;
+
+            static __device__ __forceinline__ Best none()
+            {
+                return {kNoRate, UINT32_MAX};
+            }
 
             // larger, or as large and further left
             __device__ __forceinline__ void take(double s, uint32_t i)
@@ -310,7 +320,13 @@ namespace a3b
             else if(i == certain)
                 rate -= 1.;
             if(rate > 0.)
-                best->take(rate / static_cast<double>(clock[i]), i);
+            {
+                double const score = rate / static_cast<double>(clock[i]);
+                if(score >= 0.)
+                    best->take(score, i);
+                else // negative noise or NaN
+                    best->take(kNoClock, UINT32_MAX);
+            }
         }
 
         constexpr uint32_t kReach = 64;
@@ -503,7 +519,7 @@ namespace a3b
                     clusterArrive();
                     clusterWait();
                     unsigned const all = *inBlock(&founds, 0);
-                    certainly = all <= kReach;
+                    certainly = all > 0 && all <= kReach;
                     if(certainly)
                     {
                         clusterArrive(); // the first block may leave when all have read its count
@@ -516,7 +532,7 @@ namespace a3b
                             drawn = found[0];
                         else if(warp == 0)
                         {
-                            Best best{0., UINT32_MAX};
+                            Best best = Best::none();
                             for(uint32_t k = lane; k < all; k += 32)
                                 again<T>(a, row, other, clock, certain, lse, draftLse, found[k], &best);
                             drawn = warpBest(best).index;
@@ -527,7 +543,7 @@ namespace a3b
                 {
                     // Intervals say nothing (rows with nothing left, far logits, many equal quotients, noise at 0): all tokens in
                     // 64 bits.
-                    Best best{0., UINT32_MAX};
+                    Best best = Best::none();
                     for(uint32_t i = low * E + tid; i < high * E; i += kThreads)
                         again<T>(a, row, other, clock, certain, lse, draftLse, i, &best);
                     for(uint32_t i = oneLow + tid; i < oneHigh; i += kThreads)
@@ -545,16 +561,18 @@ namespace a3b
                     }
                     clusterArrive();
                     clusterWait();
-                    Best result{0., UINT32_MAX};
+                    Best result = Best::none();
                     for(unsigned r = 0; r < blocks; ++r)
                     {
                         Best const* there = inBlock(&blockBest, r);
                         result.take(there->score, there->index);
                     }
                     drawn = result.index;
+                    if(result.score > kNoRate)
+                        break; // the same in every thread of the cluster
                 }
-                if(certainly || drawn != UINT32_MAX)
-                    break; // the same in every thread of the cluster that is still here
+                if(certainly)
+                    break;
             }
             if(rank == 0 && warp == 0)
             {

@@ -488,7 +488,8 @@ A3B_API int a3b_embedding_backward(a3b_stream_t stream, a3b_embedding_backward_a
  *
  * tokens (length + 1 a sequence): the drafts that stand, the drawn token, -1 behind it; accepted: how many stand. A row with
  * nothing left (lse -infinity), a NaN or +infinity draws -1. A NaN in the draft's row refuses its draft and takes nothing
- * away. noise is positive; what is not takes no part or, at 0, wins where its rate is positive.
+ * away. noise is positive; at 0 it wins where its rate is positive, and a token whose noise is negative or NaN is not drawn
+ * (its rate still counts as one that is left: where no other is, -1 is drawn).
  *
  * Greedy sequences: top_index (null: none; length + 1 a sequence) holds the target's most likely token for every row, as
  * a3b_token_logprobs gives with one alternative. A sequence whose first entry is a token is verified greedily: draft i stands

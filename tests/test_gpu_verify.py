@@ -333,3 +333,37 @@ def test_streams_and_graphs(cuda):
                 graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
+
+
+@pytest.mark.parametrize("v", [3, 20, 5000, 40000, 131072])
+def test_noise_that_takes_no_part(cuda, v):
+    """Tokens whose noise is negative or NaN are never drawn and hide no other, whatever their rate: behind a refused draft,
+    behind drafts that all stand, and without a draft; in one block and in a cluster of blocks."""
+    for b in (1, 5):
+        for model in (True, False):
+            g = torch.Generator(device="cuda").manual_seed(v + b)
+            c = make(b, 2, v, torch.float32, 16, model=model)
+            flip = torch.rand(b, v, generator=g, device="cuda") < 0.3
+            flip[0, c["drafts"][0, 0]] = True  # what the draft took is not drawn for its sign
+            c["noise"] = torch.where(flip, -c["noise"], c["noise"])
+            nan = flip & (torch.rand(b, v, generator=g, device="cuda") < 0.2)
+            for uniform in (1.0, 0.0, None):
+                if uniform is not None:
+                    c["uniform"].fill_(uniform)
+                check(c)
+                got, want = verify({**c, "noise": c["noise"].masked_fill(nan, math.nan)}), oracle(c)
+                assert all(torch.equal(a.cpu().long(), w) for a, w in zip(got, want))
+            none = {**c, "drafts": torch.full_like(c["drafts"], -1)}
+            check(none)
+            tokens, _ = check({**none, "noise": -c["noise"].abs()})
+            assert (tokens == -1).all()
+
+
+def test_rates_without_a_clock(cuda):
+    """p = (0.2, 0.3, 0.5), and token 2 was looked up and refused."""
+    p = torch.tensor([0.2, 0.3, 0.5], device="cuda")
+    c = {"logits": p.log().expand(1, 2, 3).contiguous(), "lse": torch.zeros(1, 2, device="cuda"),
+         "drafts": torch.tensor([[2]], device="cuda"), "uniform": torch.ones(1, 1, device="cuda")}
+    for noise, token in (((1, 1, -0.1), 1), ((1, -1, -0.1), 0), ((-1, -1, 1), -1), ((-1, 1, 1), 1), ((math.nan, 1, -2), 1)):
+        tokens, accepted = verify({**c, "noise": torch.tensor([noise], device="cuda", dtype=torch.float32)})
+        assert tokens.tolist() == [[token, -1]] and accepted.item() == 0, noise
