@@ -503,7 +503,8 @@ namespace a3b
                     bar = fmaxf(bar, *inBlock(&blockLow, r));
                     useless |= *inBlock(&blockFull, r);
                 }
-                if(bar > 0.f && bar < INFINITY && !useless)
+                // Below fp32's normal numbers (large noise) a rounding is more than an interval allows for.
+                if(bar >= 0x1p-126f && bar < INFINITY && !useless)
                 {
                     // The token with this lower end has a positive rate. If no other one reaches it, it is the token, and
                     // nothing is computed again.
@@ -541,8 +542,8 @@ namespace a3b
                 }
                 if(!certainly)
                 {
-                    // Intervals say nothing (rows with nothing left, far logits, many equal quotients, noise at 0): all tokens in
-                    // 64 bits.
+                    // Intervals say nothing (rows with nothing left, far logits, many equal quotients, noise at 0 or so large that
+                    // quotients are subnormal): all tokens in 64 bits.
                     Best best = Best::none();
                     for(uint32_t i = low * E + tid; i < high * E; i += kThreads)
                         again<T>(a, row, other, clock, certain, lse, draftLse, i, &best);

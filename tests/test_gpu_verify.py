@@ -367,3 +367,15 @@ def test_rates_without_a_clock(cuda):
     for noise, token in (((1, 1, -0.1), 1), ((1, -1, -0.1), 0), ((-1, -1, 1), -1), ((-1, 1, 1), 1), ((math.nan, 1, -2), 1)):
         tokens, accepted = verify({**c, "noise": torch.tensor([noise], device="cuda", dtype=torch.float32)})
         assert tokens.tolist() == [[token, -1]] and accepted.item() == 0, noise
+
+
+@pytest.mark.parametrize("v", [1000, 5000, 50257, 131072])
+@pytest.mark.parametrize("noise", [3e38, 1e35, 1e-30])
+def test_quotients_far_from_one(cuda, v, noise):
+    """Noise of any positive size: quotients below fp32's normal numbers, which hold few digits, and large ones."""
+    c = make(20, 1, v, torch.float32, 17, model=False, spread=0.02)
+    c["noise"] = (torch.rand(20, v, device="cuda", generator=torch.Generator(device="cuda").manual_seed(v)) * 1e-3 + 1) * noise
+    c["uniform"].fill_(1.0)
+    check(c)
+    c["drafts"].fill_(-1)
+    check(c)
