@@ -914,7 +914,7 @@ namespace a3b
         }
 
         template<typename T, typename U, int E>
-        int launchSum(cudaStream_t stream, DeviceProps const* props, SumArgs a, Tokens const& tokens, uint32_t* keys, uint32_t* places)
+        int launchGradient(cudaStream_t stream, DeviceProps const* props, SumArgs a, Plan const& p, Tokens const& tokens, char* ws)
         {
             uint32_t const lots = a.n / E;
             a.shift = teamShift(lots);
@@ -922,23 +922,32 @@ namespace a3b
             a.slices = (lots + lanes - 1) / lanes;
             uint64_t const sums = static_cast<uint64_t>((a.chunks + teams - 1) / teams) * a.slices;
             uint64_t fills = a.fill ? static_cast<uint64_t>((a.vocab + kFillRows - 1) / kFillRows) * ((lots + 4 * kThreads - 1) / (4 * kThreads)) : 0;
-            if(a.count > 0 && a.count <= kRankMax)
-            {
-                uint32_t const ranking = (a.count + 31) / 32;
-                // at most one row in sixteen is written twice
-                uint64_t const all = a.flat ? static_cast<uint64_t>(a.vocab) * a.n / PackOf<U>::E + 1 : static_cast<uint64_t>(a.vocab) * lots;
-                bool const early = a.fill && a.count <= a.vocab / 16 && all <= static_cast<uint64_t>(UINT32_MAX) - kFillLots;
-                auto kernel = early && a.add ? rankKernel<U, E, true> : rankKernel<U, E, false>;
-                uint32_t const filling = early ? static_cast<uint32_t>((all + kFillLots - 1) / kFillLots) : 0;
-                kernel<<<ranking + filling, 256, ranking * 32 * 4, stream>>>(tokens, a.count, keys, places, a);
-                A3B_CHECK_LAUNCH("rankKernel");
-                if(early)
-                    fills = 0;
-            }
+            bool const ranked = a.count > 0 && a.count <= kRankMax;
+            // at most one row in sixteen is written twice
+            uint64_t const all = a.flat ? static_cast<uint64_t>(a.vocab) * a.n / PackOf<U>::E + 1 : static_cast<uint64_t>(a.vocab) * lots;
+            bool const early = ranked && a.fill && a.count <= a.vocab / 16 && all <= static_cast<uint64_t>(UINT32_MAX) - kFillLots;
+            if(early) // by the kernel that ranks
+                fills = 0;
             if(sums + fills > static_cast<uint64_t>(INT_MAX))
             {
                 setError("%u tokens of %u elements are more than one launch holds", a.count, a.n);
                 return A3B_ERR_TOO_LARGE;
+            }
+            uint32_t *keys = nullptr, *places = nullptr;
+            if(a.count > 0)
+            {
+                int const rs = sortTokens(stream, props, p, tokens, a.count, ws, &keys, &places);
+                if(rs != A3B_OK)
+                    return rs;
+                a.keys = keys, a.places = places;
+            }
+            if(ranked)
+            {
+                uint32_t const ranking = (a.count + 31) / 32;
+                auto kernel = early && a.add ? rankKernel<U, E, true> : rankKernel<U, E, false>;
+                uint32_t const filling = early ? static_cast<uint32_t>((all + kFillLots - 1) / kFillLots) : 0;
+                kernel<<<ranking + filling, 256, ranking * 32 * 4, stream>>>(tokens, a.count, keys, places, a);
+                A3B_CHECK_LAUNCH("rankKernel");
             }
             a.sumBlocks = static_cast<uint32_t>(sums);
             if(sums + fills == 0)
@@ -1089,17 +1098,11 @@ extern "C"
         A3B_REQUIRE(count == 0 || (workspace && alignedTo(16, {workspace}) && workspace_bytes >= p.bytes),
                     "the workspace is missing, too small or not aligned to 16 bytes");
         auto s = static_cast<cudaStream_t>(stream);
-        uint32_t *keys = nullptr, *places = nullptr;
         Tokens const known{tokens, index_dtype == A3B_I64, first, static_cast<uint32_t>(vocab)};
-        if(count > 0)
-        {
-            int const rs = sortTokens(s, props, p, known, static_cast<uint32_t>(count), static_cast<char*>(workspace), &keys, &places);
-            if(rs != A3B_OK)
-                return rs;
-        }
-        SumArgs a{grad_out.data, {grad_out.outer_stride, grad_out.inner_stride}, keys, places,
-                  count ? reinterpret_cast<float*>(static_cast<char*>(workspace) + p.partial) : nullptr,
-                  count ? reinterpret_cast<uint32_t*>(static_cast<char*>(workspace) + p.runs) : nullptr, add, add_stride, grad_table,
+        char* const ws = static_cast<char*>(workspace);
+        SumArgs a{grad_out.data, {grad_out.outer_stride, grad_out.inner_stride}, nullptr, nullptr,
+                  count ? reinterpret_cast<float*>(ws + p.partial) : nullptr,
+                  count ? reinterpret_cast<uint32_t*>(ws + p.runs) : nullptr, add, add_stride, grad_table,
                   table_stride, static_cast<uint32_t>(count), static_cast<uint32_t>(inner), static_cast<uint32_t>(n),
                   static_cast<uint32_t>(vocab), p.chunk, p.chunks, 0u, 0u, outer == 1, !inPlace,
                   !add && table_stride == static_cast<int64_t>(n) && alignedTo(16, {grad_table}), static_cast<float>(scale), 0};
@@ -1111,7 +1114,7 @@ extern "C"
             bool const packed = n % E == 0 && rowsAligned(grad_out.data, outer, inner, grad_out.outer_stride, grad_out.inner_stride, gs, 16)
                                 && rowsAligned(grad_table, 1, vocab, 0, table_stride, ts, 16)
                                 && rowsAligned(add, 1, vocab, 0, add_stride, ts, 16);
-            return packed ? launchSum<T, U, E>(s, props, a, known, keys, places) : launchSum<T, U, 1>(s, props, a, known, keys, places);
+            return packed ? launchGradient<T, U, E>(s, props, a, p, known, ws) : launchGradient<T, U, 1>(s, props, a, p, known, ws);
         });
     }
 }

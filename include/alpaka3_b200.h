@@ -455,7 +455,9 @@ A3B_API size_t a3b_embedding_backward_workspace(uint64_t count, uint64_t n, uint
  * rows of tokens that occur are touched. Types as in a3b_embedding: grad_out is of its out_dtype, the table of its
  * table_dtype. Sums are held in fp32 and rounded once; their order follows from count, n and vocab (and the device) alone:
  * repeated calls give the same bits. grad_out's rows may have any strides; grad_table's may not overlap. workspace: 16-byte
- * aligned, of a3b_embedding_backward_workspace bytes. grad_table and workspace lie apart from all inputs. */
+ * aligned, of a3b_embedding_backward_workspace bytes. grad_table and workspace lie apart from all inputs. A call of more
+ * blocks than one launch holds (a table of some 2^44 elements and more) is refused before anything is launched
+ * (A3B_ERR_TOO_LARGE). */
 typedef struct a3b_embedding_backward_args
 {
     uint64_t outer, inner, n, vocab;

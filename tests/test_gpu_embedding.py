@@ -309,3 +309,20 @@ def test_streams_and_graphs(cuda, count):
                 graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+def test_refusal_leaves_the_workspace(cuda):
+    """A gradient of more blocks than one launch holds is refused before anything is launched. The table (2^31 - 65 rows of
+    34816 elements) is an address that no kernel is given."""
+    from alpaka3_b200 import capi
+    n, vocab = 34816, 2**31 - 65
+    for count in (40, 9000, 40000):  # sorted with the sums, by one cluster, in several launches
+        g, t = torch.ones(1, n, device="cuda"), torch.arange(count, device="cuda")
+        size = capi.lib().a3b_embedding_backward_workspace(count, n, vocab)
+        ws = torch.full((size,), 7, dtype=torch.uint8, device="cuda")
+        rc = capi.lib().a3b_embedding_backward(None, capi.EMBEDDING_BACKWARD_ARGS.pack(
+            1, count, n, vocab, 0, g.data_ptr(), 0, 0, t.data_ptr(), 0, 0, 1 << 60, n, ws.data_ptr(), size, 1.0, capi.F32,
+            capi.I64, capi.F32, 0))
+        assert rc == capi.ERR_TOO_LARGE and "one launch" in capi.last_error()
+        torch.cuda.synchronize()
+        assert (ws == 7).all()
