@@ -430,7 +430,7 @@ A3B_API int a3b_rms_norm_backward(a3b_stream_t stream, a3b_rms_norm_backward_arg
  * alike, or one of them A3B_F32; the product is formed in fp32 and rounded once. scale: any finite fp32 value. The output's
  * rows may not overlap one another, the table or the tokens (beside them in rows of steps that are all multiples of one
  * length is apart). At most 2^31 - 65 tokens, rows of the table and elements a row (A3B_ERR_TOO_LARGE; rows of more than
- * eight million elements too). One launch. */
+ * 65535 * 512 accesses too, of one element, or of 4 or 8 where rows begin at 16 bytes and are whole packs). One launch. */
 typedef struct a3b_embedding_args
 {
     uint64_t outer, inner, n, vocab;

@@ -326,3 +326,21 @@ def test_refusal_leaves_the_workspace(cuda):
         assert rc == capi.ERR_TOO_LARGE and "one launch" in capi.last_error()
         torch.cuda.synchronize()
         assert (ws == 7).all()
+
+
+def test_longest_rows(cuda):
+    """65535 * 512 accesses a row, by single elements and by packs of four; one more is refused before anything is launched."""
+    from alpaka3_b200 import algo, capi
+    most = 65535 * 512
+    for n in (most - 1, 4 * most):
+        room = torch.arange(n, device="cuda", dtype=torch.int32).bitwise_and_(0xffff).float()
+        out = torch.zeros(2, n, device="cuda")
+        algo.embedding(out, room[None], torch.tensor([0, 1], device="cuda"), scale=2.0)
+        assert torch.equal(out[0], 2 * room) and (out[1] == 0).all()
+    for n in (most + 1, 4 * most + 4):
+        table, out = torch.ones(1, n, device="cuda"), torch.full((1, n), 7.0, device="cuda")
+        with pytest.raises(capi.A3BError, match="one launch") as e:
+            algo.embedding(out, table, torch.tensor([0], device="cuda"))
+        assert e.value.status == capi.ERR_TOO_LARGE
+        torch.cuda.synchronize()
+        assert (out == 7).all()
