@@ -374,7 +374,8 @@ typedef struct a3b_rows
  * out has dtype, or A3B_E4M3 or A3B_E5M2 with scales: groups of `group` elements of a row (32, 64 or 128, the last of a row
  * may be shorter; 0: the whole row) share the scale s = max |y| * (1 / L), L = 448 or 57344, y = h * r * weight in fp32, and
  * out = y * (1 / s) rounded to the nearest 8-bit value, at most L; both reciprocals and both products are the nearest fp32
- * values (an s below 2^-126 divides instead). scales: fp32, dense, ceil(n / group) (or 1) a row. A group of zeros has scale 0.
+ * values (an s below 2^-126 divides instead). scales: fp32, dense, ceil(n / group) (or 1) a row. A group of
+ * zeros, or one whose s rounds to 0, has scale 0 and zeros.
  *
  * NaN in a row makes its out and rstd NaN; an infinity makes rstd 0, itself NaN and the others 0. A row of zeros with eps 0
  * has rstd infinity and NaN as output. A group with a NaN has scale NaN and NaN throughout.

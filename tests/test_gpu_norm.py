@@ -476,3 +476,34 @@ def test_eight_bits_next_to_a_middle(cuda, kind, dtype, n, shift):
         assert (rstd == 1).all() and torch.equal(scales, s.flatten().expand(rows, -1))
         want = (w * (1 / s)).clamp(max=top).to(kind).float().flatten() * x.float()
         assert torch.equal(out.float(), want)
+
+
+@pytest.mark.parametrize("kind", list(LARGEST))
+@pytest.mark.parametrize("n", [256, 2048, 16384, 257, 5001, 40001])
+def test_scales_below_normal_numbers(cuda, kind, n):
+    """Weights from 1e-36 to 1e-45: every group by itself. What the kernel's fp32 steps give, subnormal numbers among them, is
+    known to the bit; where max |y| / L rounds to 0, scale and values are 0. Against the definition the scale is off by the
+    roundings of y and of itself, half of 2^-149 each, beside those of normal numbers."""
+    from alpaka3_b200 import algo
+    x, top = make((3, n), torch.float32, n), LARGEST[kind]
+    for group in (None, 32, 128):
+        for w in (1e-36, 1e-38, 1e-39, 1e-41, 1e-42, 3e-43, 3e-44, 1e-45):
+            weight = torch.full((n,), w, device="cuda")
+            if group:
+                weight[n // 2:] = 1e-30  # neighbours of another size
+            size = group or n
+            out, rstd = torch.ones(3, n, device="cuda").to(kind), torch.zeros(3, device="cuda")
+            scales = torch.ones(3, -(-n // size), device="cuda")
+            algo.rms_norm(out, x, weight, rstd=rstd, scales=scales, group=group)
+            y = x * rstd[:, None] * weight
+            parts = torch.nn.functional.pad(y, (0, -n % size)).unflatten(-1, (-1, size))
+            s = parts.abs().amax(-1) * torch.tensor(1 / top, device="cuda")
+            assert torch.equal(scales, s)
+            q = torch.where(s[..., None] < 2.0**-126, parts / s[..., None], parts * (1 / s)[..., None])
+            q = torch.where(s[..., None] == 0, torch.zeros_like(q), q).clamp(-top, top).flatten(1)[:, :n]
+            assert torch.equal(out.float(), q.to(kind).float())
+            true = definition(x, weight, None, 1e-6)[2]
+            true = torch.nn.functional.pad(true, (0, -n % size)).unflatten(-1, (-1, size)).abs().amax(-1) / top
+            close(scales, true, ((depth(n) / 2 + 7) * U * true + 2.0**-149))
+            if w < 1e-43:
+                assert (s[:, 0] == 0).all() and (out[:, :min(size, n // 2)].float() == 0).all()
