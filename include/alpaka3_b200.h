@@ -378,7 +378,9 @@ typedef struct a3b_rows
  * zeros, or one whose s rounds to 0, has scale 0 and zeros.
  *
  * NaN in a row makes its out and rstd NaN; an infinity makes rstd 0, itself NaN and the others 0. A row of zeros with eps 0
- * has rstd infinity and NaN as output. A group with a NaN has scale NaN and NaN throughout.
+ * has rstd infinity and NaN as output; one whose r is beyond fp32 (magnitudes below 2^-128 with eps 0) has rstd infinity and
+ * infinities, NaN where it is 0. A group with a NaN has scale NaN and NaN throughout; one with an infinite y has scale infinity,
+ * NaN there and 0 elsewhere.
  * An output may be an input of the same type in place (same address and strides: total = residual, out = x, ...); otherwise
  * outputs must lie apart from the inputs and from one another: wholly before or behind, or beside them in rows whose steps
  * are all multiples of one length that holds both (parts of one wider row). Rows of an output may not overlap. The order of

@@ -507,3 +507,38 @@ def test_scales_below_normal_numbers(cuda, kind, n):
             close(scales, true, ((depth(n) / 2 + 7) * U * true + 2.0**-149))
             if w < 1e-43:
                 assert (s[:, 0] == 0).all() and (out[:, :min(size, n // 2)].float() == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [8, 33, 256, 1024, 8192, 33000])
+def test_rows_whose_root_is_beyond_fp32(cuda, dtype, n):
+    """Magnitudes below 2^-128 without eps: r is infinite in fp32, and y = h r w with it; with the least eps it is not."""
+    from alpaka3_b200 import algo
+    x = make((3, n), dtype, n).clamp(-3, 3)
+    x[1] = (x[1].float() * 1e-40).to(dtype)
+    x[1, n // 2] = 0
+    out, rstd = torch.zeros_like(x), torch.zeros(3, device="cuda")
+    algo.rms_norm(out, x, rstd=rstd, eps=0.0)
+    assert rstd[1] == INF and torch.equal(torch.isnan(out[1]), x[1] == 0)
+    assert torch.isinf(out[1, x[1] != 0]).all() and torch.equal(out[1, x[1] != 0] > 0, x[1, x[1] != 0] > 0)
+    check_forward(x[::2].contiguous(), eps=0.0)
+    check_forward(x, eps=2.0**-149)
+
+
+@pytest.mark.parametrize("kind", list(LARGEST))
+@pytest.mark.parametrize("n", [64, 1000, 8192, 257, 5001, 40001])
+def test_infinite_values_of_a_group(cuda, kind, n):
+    """An infinite weight: the group's scale is infinite, its infinity NaN, what is finite 0; other groups are as without it."""
+    from alpaka3_b200 import algo
+    x, w = make((2, n), torch.float32, n), torch.ones(n, device="cuda")
+    w[n - 2] = INF
+    x[:, n - 2] = 1.0
+    for group in (None, 32):
+        size = group or n
+        out, scales = torch.ones(2, n, device="cuda").to(kind), torch.ones(2, -(-n // size), device="cuda")
+        algo.rms_norm(out, x, w, scales=scales, group=group)
+        low = (n - 2) // size * size
+        rest = torch.arange(low, min(low + size, n), device="cuda")
+        assert (scales[:, low // size] == INF).all() and torch.isnan(out[:, n - 2].float()).all()
+        assert (out.float()[:, rest[rest != n - 2]] == 0).all()
+        assert torch.isfinite(scales[:, :low // size]).all() and torch.isfinite(out.float()[:, :low]).all()
