@@ -73,43 +73,7 @@ namespace a3b
                 else
                     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
             }
-            static __device__ __forceinline__ void unpack(float* v, unsigned const* w)
-            {
-                if constexpr(E == 1)
-                    v[0] = PackOf<T>::pair(w, 0).x;
-                else
-#pragma unroll
-                    for(int k = 0; k < E / 2; ++k)
-                    {
-                        float2 const f = PackOf<T>::pair(w, k);
-                        v[2 * k] = f.x, v[2 * k + 1] = f.y;
-                    }
-            }
-            // rounded to the nearest value of T
-            static __device__ __forceinline__ void pack(unsigned* w, float const* v)
-            {
-                if constexpr(E == 1)
-                {
-                    unsigned two[2];
-                    PackOf<T>::setPair(two, 0, make_float2(v[0], 0.f));
-                    w[0] = two[0];
-                }
-                else
-#pragma unroll
-                    for(int k = 0; k < E / 2; ++k)
-                        PackOf<T>::setPair(w, k, make_float2(v[2 * k], v[2 * k + 1]));
-            }
         };
-        template<>
-        __device__ __forceinline__ void Access<float, 1>::unpack(float* v, unsigned const* w)
-        {
-            v[0] = __uint_as_float(w[0]);
-        }
-        template<>
-        __device__ __forceinline__ void Access<float, 1>::pack(unsigned* w, float const* v)
-        {
-            w[0] = __float_as_uint(v[0]);
-        }
 
         // E weights, of T or fp32, in the 16-byte words they come in
         template<typename WT, int E>
@@ -146,17 +110,6 @@ namespace a3b
                     return make_float2(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
                 else
                     return PackOf<WT>::pair(w, k);
-            }
-            static __device__ __forceinline__ void unpack(float* v, unsigned const* w)
-            {
-                if constexpr(E == 1)
-                    Access<WT, 1>::unpack(v, w);
-                else if constexpr(std::is_same_v<WT, float>)
-#pragma unroll
-                    for(int k = 0; k < E; ++k)
-                        v[k] = __uint_as_float(w[k]);
-                else
-                    Access<WT, E>::unpack(v, w);
             }
         };
 
@@ -677,12 +630,7 @@ namespace a3b
         // Rows that no team holds (longer than 32768 16-bit or 16384 32-bit elements; without 16-byte packs than 16384, with 8-bit
         // outputs than 32768): one block a row, which goes over it two to four times, element by element; the later passes
         // find it in L2.
-        constexpr uint32_t kLongThreads = 1024; // at most; about eight elements a thread and pass otherwise
-
-        uint32_t longThreads(uint32_t n)
-        {
-            return std::min(kLongThreads, std::max(32u, (n / 8 + 31) / 32 * 32));
-        }
+        constexpr uint32_t kLongThreads = 1024;
 
         template<typename T, typename WT>
         __global__ void __launch_bounds__(kLongThreads) rmsNormLongKernel(NormArgs a, int kind) // kind: 0 T, 1 8 bits
@@ -831,7 +779,7 @@ namespace a3b
                 else if(packs <= 4096)
                     rmsNormKernel<T, WT, E, 4, 0, F8><<<a.rows, roundUp((packs + 3) / 4, 32), 0, stream>>>(a);
                 else
-                    rmsNormLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a, F8);
+                    rmsNormLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a, F8);
             }
             else if constexpr(!F8)
             {
@@ -840,7 +788,7 @@ namespace a3b
                 else if(a.n <= 16384)
                     rmsNormKernel<T, WT, 1, 16, 0, false><<<a.rows, roundUp((a.n + 15) / 16, 32), 0, stream>>>(a);
                 else
-                    rmsNormLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a, 0);
+                    rmsNormLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a, 0);
             }
             else
             {
@@ -852,7 +800,7 @@ namespace a3b
                 else if(a.n <= 32768)
                     rmsNormOddKernel<T, WT, 8><<<a.rows, threads(8), 0, stream>>>(a);
                 else
-                    rmsNormLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a, 1);
+                    rmsNormLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a, 1);
             }
             A3B_CHECK_LAUNCH("rmsNormKernel");
             return A3B_OK;
@@ -1154,7 +1102,7 @@ namespace a3b
                 blocks = std::min(64u, std::max(1u, a.rows / 64)); // eight rows a warp and more
                 if(a.partial)
                     rmsNormWeightKernel<T><<<dim3((a.n + 31) / 32, blocks), 256, 0, stream>>>(a);
-                rmsNormBackwardLongKernel<T, WT><<<a.rows, longThreads(a.n), 0, stream>>>(a);
+                rmsNormBackwardLongKernel<T, WT><<<a.rows, kLongThreads, 0, stream>>>(a);
             }
             A3B_CHECK_LAUNCH("rmsNormBackwardKernel");
             if(a.partial && blocks > 0)
