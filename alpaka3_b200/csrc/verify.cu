@@ -106,7 +106,9 @@ namespace a3b
 
         __device__ __noinline__ double exactly(double scale, float z, float lse)
         {
-            return exp(scale * static_cast<double>(z) - static_cast<double>(lse));
+            // Not fused: the product has the rounding of a formula in 64-bit steps, so that far masked logits, whose product is off by
+            // more than lse is small, give its probabilities, and equal exponents are equal.
+            return exp(__dsub_rn(__dmul_rn(scale, static_cast<double>(z)), static_cast<double>(lse)));
         }
 
         // The scores of a row without a rate, and of one with rates but no noise they could be divided by; what can be drawn has

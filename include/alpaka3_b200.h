@@ -489,7 +489,7 @@ A3B_API int a3b_embedding_backward(a3b_stream_t stream, a3b_embedding_backward_a
  * (p_v - q_v)+, behind the last one that stands from the rates p_v (also where no rate is left otherwise): the token with
  * the largest rate_v / noise_v, a tie to the lowest. With uniform in [0, 1) and noise independent exponential variates the
  * tokens are distributed as if drawn from the target one by one. Comparisons and quotients are those of the formula in 64
- * bits.
+ * bits, every operation rounded by itself.
  *
  * tokens (length + 1 a sequence): the drafts that stand, the drawn token, -1 behind it; accepted: how many stand. A row with
  * nothing left (lse -infinity), a NaN or +infinity draws -1. A NaN in the draft's row refuses its draft and takes nothing

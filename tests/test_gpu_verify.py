@@ -379,3 +379,34 @@ def test_quotients_far_from_one(cuda, v, noise):
     check(c)
     c["drafts"].fill_(-1)
     check(c)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_products_are_rounded(cuda, dtype):
+    """scale * z is a 64-bit number before lse is taken from it. Token 0: its product rounds to lse itself, so p = 1 and the draft
+    leaves nothing of it; the exact product is up to 4e-12 more. So token 2 is drawn, with a rate of e^-486, e^-179 or e^-85."""
+    for scale, z in ((1.9, -40960.0), (0.7, -40960.0), (1.0 / 3, -24576.0)):
+        assert scale * z == round(scale * z)
+        c = {"logits": torch.tensor([z, -INF, z - 256], device="cuda").expand(1, 2, 3).to(dtype).contiguous(),
+             "lse": torch.full((1, 2), scale * z, device="cuda"), "drafts": torch.tensor([[1]], device="cuda"),
+             "uniform": torch.full((1, 1), 0.5, device="cuda"), "noise": torch.ones(1, 3, device="cuda"),
+             "draft_logits": torch.tensor([[[0.0, -1.0, -INF]]], device="cuda").to(dtype),
+             "draft_lse": torch.zeros(1, 1, device="cuda")}
+        tokens, _ = check(c, scale, 1.0)
+        assert tokens.tolist() == [[2, -1]]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [1.9, 0.7, 2.0**-6, 2.0**8])
+def test_masks_and_scales(cuda, dtype, scale):
+    """Rows masked by finite values, some wholly, at a scale: probabilities are those of the rounded product."""
+    g = torch.Generator(device="cuda").manual_seed(18)
+    for v in (2, 7, 27, 3000):
+        for low in (torch.finfo(dtype).min, -1e4):
+            for share in (0.5, 0.95):
+                c = make(40, 2, v, dtype, 18, True, scale, 0.9, 20.0)
+                for name, s, lse in (("logits", scale, "lse"), ("draft_logits", 0.9, "draft_lse")):
+                    c[name].masked_fill_(torch.rand(c[name].shape, generator=g, device="cuda") < share, low)
+                    c[lse] = log_sums(c[name], s)
+                check(c, scale, 0.9)
+                check({**c, "draft_logits": None, "draft_lse": None}, scale, 0.9)
