@@ -491,7 +491,8 @@ namespace a3b
 
         // 8-bit outputs of rows without 16-byte packs: one block a row, in registers by single elements. A warp has Q stretches of
         // 128 neighbouring elements, four a lane and each 32 apart, so every group of 32, 64 or 128 is one warp's. (By the long
-        // kernel below, a group at a time, 9769 x 2587 bf16 with residual took 290 us; now 95, bound by issue.)
+        // kernel below, a group at a time, 9769 x 2587 bf16 with residual took 290 us; now 92, bound by issue: 76% of the slots, DRAM
+        // at 18%.) Eight stretches (8193 to 32768 elements) do not fit 64 registers: 56 to 112 bytes a thread are in local memory.
         template<typename T, typename WT, int Q>
         __global__ void __launch_bounds__(1024, Q == 1 ? 2 : 1) rmsNormOddKernel(NormArgs a)
         {
@@ -629,7 +630,7 @@ namespace a3b
 
         // Rows that no team holds (longer than 32768 16-bit or 16384 32-bit elements; without 16-byte packs than 16384, with 8-bit
         // outputs than 32768): one block a row, which goes over it two to four times, element by element; the later passes
-        // find it in L2.
+        // find it in L2. The gradient's limits are half of that, below.
         constexpr uint32_t kLongThreads = 1024;
 
         template<typename T, typename WT>
@@ -793,7 +794,9 @@ namespace a3b
             else
             {
                 auto threads = [&](uint32_t stretches) { return (a.n + 128 * stretches - 1) / (128 * stretches) * 32; };
-                if(a.n <= 4096) // one stretch a warp, 32 registers (4000 x 4001 fp32 59 us, with two stretches 62)
+                // One stretch a warp, 32 registers: with a residual 4000 x 4001 fp32 58 us, with two stretches 61, 9769 x 2587 bf16 92 and
+                // 100; without one 50 and 44, 73 and 69.
+                if(a.n <= 4096)
                     rmsNormOddKernel<T, WT, 1><<<a.rows, threads(1), 0, stream>>>(a);
                 else if(a.n <= 8192)
                     rmsNormOddKernel<T, WT, 2><<<a.rows, threads(2), 0, stream>>>(a);
@@ -977,7 +980,8 @@ namespace a3b
             }
         }
 
-        // Rows that no team holds: two passes over the row for its gradient ...
+        // Rows that no team holds (longer than 16384 16-bit or 8192 32-bit elements; without 16-byte packs than 8192): two passes over
+        // the row for its gradient ...
         template<typename T, typename WT>
         __global__ void __launch_bounds__(kLongThreads) rmsNormBackwardLongKernel(NormBackArgs a)
         {
